@@ -96,7 +96,7 @@ def lib() -> C.CDLL:
     if not os.path.exists(LIB_PATH):
         raise ImportError(f"{LIB_PATH} is missing: build it first (python -m cdclq.build or __graft_entry__.build())")
     L = C.CDLL(LIB_PATH)
-    vp, sz, i32, u64 = C.c_void_p, C.c_size_t, C.c_int, C.c_uint64
+    vp, sz, i32, u64, i64 = C.c_void_p, C.c_size_t, C.c_int, C.c_uint64, C.c_int64
     cfgp, stp = C.POINTER(_Config), C.POINTER(_Stats)
     sig = {
         "cdclq_abi_version": ([], i32),
@@ -142,6 +142,12 @@ def lib() -> C.CDLL:
         "cdclq_dequantize_model": ([vp, C.c_char_p, C.c_char_p, i32, C.POINTER(sz)], i32),
         "cdclq_hessian_accumulate_device": ([vp, vp, vp, vp, sz, sz, vp], i32),
         "cdclq_hessian_finalize_device": ([vp, vp, sz, u64, vp], i32),
+        "cdclq_checkpoint_save_device": ([vp, vp, sz, sz, sz, i32, vp, vp, vp], i32),
+        "cdclq_checkpoint_restore_device": ([vp, vp, vp, sz, sz, i32, vp, sz, vp], i32),
+        "cdclq_vocab_work_bytes": ([sz, sz, sz, vp, sz, i32], sz),
+        "cdclq_vocab_loss_device": ([vp, vp, sz, vp, sz, sz, sz, sz, i32, vp, i64, vp, vp, vp, sz, vp], i32),
+        "cdclq_vocab_loss_backward_device": ([vp, vp, sz, vp, sz, sz, sz, sz, i32, vp, i64, vp, vp, vp, sz, vp, sz,
+                                              vp, sz, vp], i32),
         "cdclq_device_alloc": ([vp, sz, C.POINTER(vp)], i32),
         "cdclq_device_free": ([vp, vp], i32),
         "cdclq_memcpy_h2d": ([vp, vp, vp, sz], i32),
@@ -187,6 +193,8 @@ def exported_symbols() -> list[str]:
         "cdclq_rtn_layer", "cdclq_rtn_layer_device", "cdclq_proxy_loss_device", "cdclq_rel_err",
         "cdclq_rel_err_device", "cdclq_bench_run", "cdclq_quantize_model", "cdclq_dequantize_model",
         "cdclq_hessian_accumulate_device", "cdclq_hessian_finalize_device",
+        "cdclq_checkpoint_save_device", "cdclq_checkpoint_restore_device", "cdclq_vocab_work_bytes",
+        "cdclq_vocab_loss_device", "cdclq_vocab_loss_backward_device",
     ]
 
 

@@ -1,0 +1,515 @@
+// Softmax cross entropy of hidden states over a large vocabulary, without the logits in memory.
+//
+//   l_tv = x_t . w_v    lse_t = log sum_v exp l_tv    loss_t = lse_t - l_t,y(t)
+//   d_tv = g_t (exp(l_tv - lse_t) - [v = y(t)])    dx_t = sum_v d_tv w_v    dw_v = sum_t d_tv x_t
+//
+// The tokens that count (target != ignore) are packed together first: the others cost nothing and
+// what they hold reaches no result. Forward: tiles of logits on the matrix cores (mma16.h), P = the
+// vocabulary and Q = the tokens, so that a lane holds a token's logits in its registers: maximum and
+// sum of exponentials of a tile's rows take two lane exchanges, and a (maximum, sum) pair per token
+// and slab of rows is all that is stored; loss_combine joins the slabs. Gradient: pieces of the
+// vocabulary; the piece's logits are made again and turned into d (16 bits) in memory, then two
+// products give dx (f32 sums over the pieces) and the piece's rows of dw.
+//
+// d is held in the operands' 16-bit type because the matrix cores need both operands alike; it is scaled by
+// g_t / max |g| (and 2^15 in f16, whose range would lose small probabilities), both undone in f32.
+#include <hip/hip_runtime.h>
+
+#include <algorithm>
+
+#include "cdclq.h"
+#include "kernels.h"
+#include "mma16.h"
+
+namespace cdclq {
+namespace {
+
+constexpr float LOG2E = 1.4426950408889634f;
+
+// Compact list of the tokens that count, in order; zero loss and lse of the others. One workgroup.
+// info: [0] their number, [1] bits of max |g| over the finite g (backward only).
+__global__ __launch_bounds__(1024) void k_loss_tokens(const int64_t* __restrict__ y, long ignore, int t,
+                                                      const float* __restrict__ g, int* __restrict__ idx,
+                                                      int* __restrict__ pos, uint32_t* __restrict__ info,
+                                                      float* __restrict__ loss, float* __restrict__ lse) {
+  __shared__ int base;
+  __shared__ int wsum[16];
+  __shared__ float wmax[16];
+  const int lane = threadIdx.x & 63, wv = threadIdx.x >> 6;
+  if (threadIdx.x == 0) base = 0;
+  float m = 0.0f;
+  __syncthreads();
+  for (int t0 = 0; t0 < t; t0 += 1024) {
+    const int i = t0 + threadIdx.x;
+    const bool on = i < t && y[i] != ignore;
+    const uint64_t b = __builtin_amdgcn_ballot_w64(on);
+    if (lane == 0) wsum[wv] = __popcll(b);
+    __syncthreads();
+    int at = base;
+    for (int w = 0; w < wv; ++w) at += wsum[w];
+    at += __popcll(b & ((1ull << lane) - 1));
+    if (on) idx[at] = i;
+    if (i < t) {
+      if (pos) pos[i] = on ? at : -1;
+      if (!on && loss) loss[i] = 0.0f;
+      if (!on && lse) lse[i] = 0.0f;
+      if (on && g) {
+        const float a = __builtin_fabsf(g[i]);
+        if (a < __builtin_inff()) m = fmaxf(m, a);
+      }
+    }
+    __syncthreads();
+    if (threadIdx.x == 0)
+      for (int w = 0; w < 16; ++w) base += wsum[w];
+    __syncthreads();
+  }
+  for (int s = 32; s; s >>= 1) m = fmaxf(m, __shfl_xor(m, s));
+  if (lane == 0) wmax[wv] = m;
+  __syncthreads();
+  if (threadIdx.x == 0) {
+    for (int w = 0; w < 16; ++w) m = fmaxf(m, wmax[w]);
+    info[0] = base;
+    info[1] = __float_as_uint(m);
+  }
+}
+
+// Rows idx[0 .. count) of x into rows of dp elements, zeros past d; and per packed token what the tiles
+// need: its target, and for the gradient lse and the scaled weight.
+struct LossTok {
+  int target;  // -1: outside the vocabulary
+  float lse, weight;
+  int pad;
+};
+__global__ __launch_bounds__(256) void k_loss_gather(const uint16_t* __restrict__ x, long ldx, int d, int dp,
+                                                     const int* __restrict__ idx, const uint32_t* __restrict__ info,
+                                                     const int64_t* __restrict__ y, int v,
+                                                     const float* __restrict__ lse, const float* __restrict__ g,
+                                                     float gscale, uint16_t* __restrict__ xc,
+                                                     LossTok* __restrict__ tok, float* __restrict__ hit, int vec) {
+  const int i = blockIdx.x;
+  if (i >= (int)info[0]) return;
+  const int t = idx[i];
+  const uint16_t* src = x + (long)t * ldx;
+  uint16_t* dst = xc + (long)i * dp;
+  if (vec) {
+    for (int c = 8 * threadIdx.x; c < dp; c += 2048)
+      *reinterpret_cast<uint4*>(dst + c) = *reinterpret_cast<const uint4*>(src + c);
+  } else {
+    for (int c = threadIdx.x; c < dp; c += 256) dst[c] = c < d ? src[c] : (uint16_t)0;
+  }
+  if (threadIdx.x == 0) {
+    const int64_t k = y[t];
+    LossTok o;
+    o.target = k >= 0 && k < v ? (int)k : -1;
+    o.lse = lse ? lse[t] : 0.0f;
+    o.weight = 0.0f;
+    if (g) {
+      const float top = __uint_as_float(info[1]);
+      o.weight = top > 0.0f ? g[t] / top * gscale : g[t];
+      if (o.target < 0) o.weight = __builtin_nanf("");
+    }
+    o.pad = 0;
+    tok[i] = o;
+    if (hit) hit[i] = __builtin_nanf("");  // replaced by the tile that holds the target
+  }
+}
+
+// 16-bit rows of `cols` elements into rows of dp, zeros past cols (operands that the tiles cannot read)
+__global__ __launch_bounds__(256) void k_pad16(const uint16_t* __restrict__ src, long ld, int cols, int dp, long rows,
+                                               uint16_t* __restrict__ dst) {
+  const long total = rows * dp;
+  for (long i = blockIdx.x * 256l + threadIdx.x; i < total; i += gridDim.x * 256l) {
+    const long r = i / dp;
+    const int c = (int)(i - r * dp);
+    dst[i] = c < cols ? src[r * ld + c] : (uint16_t)0;
+  }
+}
+
+template <class T, int FP, int FQ, int WP, int WQ>
+__global__ __launch_bounds__(64 * WP * WQ, 2) void k_loss_tiles(const uint16_t* __restrict__ w, long ldw, int v,
+                                                                const uint16_t* __restrict__ xc, int dp,
+                                                                const uint32_t* __restrict__ info, int np, int nq,
+                                                                const LossTok* __restrict__ tok,
+                                                                float2* __restrict__ part, int ldpart,
+                                                                float* __restrict__ hit) {
+  typedef MmaTile<T, false, false, FP, FQ, WP, WQ> M;
+  __shared__ __align__(1024) uint8_t lds[M::LDS];
+  const MmaTileAt at = mma_tile_at(blockIdx.x, np, nq);
+  const int p0 = at.p * M::BP, q0 = at.q * M::BQ, count = (int)info[0];
+  if (q0 >= count) return;
+  mma_f4 acc[FP][FQ];
+  M::clear(acc);
+  M::run(lds_offset(lds), MmaOp{w, ldw, v}, MmaOp{xc, dp, count}, p0, q0, 0, dp, acc);
+  const int lane = threadIdx.x & 63;
+  const int slab = M::row(p0, 0) / (16 * FP);
+#pragma unroll
+  for (int g = 0; g < FQ; ++g) {
+    const int t = M::col(q0, g) + (lane & 15);
+    const int target = t < count ? tok[t].target : -1;
+    float m = -__builtin_inff();
+#pragma unroll
+    for (int f = 0; f < FP; ++f)
+#pragma unroll
+      for (int r = 0; r < 4; ++r) {
+        const int row = M::row(p0, f) + 4 * (lane >> 4) + r;
+        if (row >= v) acc[f][g][r] = -__builtin_inff();
+        if (row == target) hit[t] = acc[f][g][r];
+        m = fmaxf(m, acc[f][g][r]);
+      }
+    m = fmaxf(m, __shfl_xor(m, 16));
+    m = fmaxf(m, __shfl_xor(m, 32));
+    const float top = m > -__builtin_inff() ? m : 0.0f;
+    float s = 0.0f;
+#pragma unroll
+    for (int f = 0; f < FP; ++f)
+#pragma unroll
+      for (int r = 0; r < 4; ++r) s += __builtin_amdgcn_exp2f((acc[f][g][r] - top) * LOG2E);
+    s += __shfl_xor(s, 16);
+    s += __shfl_xor(s, 32);
+    if (lane < 16 && t < count) part[(long)slab * ldpart + t] = make_float2(m, s);
+  }
+}
+
+// Joins the slabs of 16 tokens: thread (token, j) takes slabs j, j + 16, ..., then 16 threads join.
+__global__ __launch_bounds__(256) void k_loss_combine(const float2* __restrict__ part, int ldpart, int nslabs,
+                                                      const uint32_t* __restrict__ info, const int* __restrict__ idx,
+                                                      const float* __restrict__ hit, float* __restrict__ loss,
+                                                      float* __restrict__ lse) {
+  const int count = (int)info[0], i = blockIdx.x * 16 + (threadIdx.x & 15), j = threadIdx.x >> 4;
+  __shared__ float2 red[256];
+  float m = -__builtin_inff(), s = 0.0f;
+  auto join = [&](float m2, float s2) {
+    const float n = fmaxf(m, m2);
+    if (n > -__builtin_inff()) {
+      s = s * __builtin_amdgcn_exp2f((m - n) * LOG2E) + s2 * __builtin_amdgcn_exp2f((m2 - n) * LOG2E);
+      m = n;
+    } else {
+      s += s2;  // nothing yet, or NaN
+    }
+  };
+  if (i < count)
+    for (int k = j; k < nslabs; k += 16) {
+      const float2 p = part[(long)k * ldpart + i];
+      join(p.x, p.y);
+    }
+  red[threadIdx.x] = make_float2(m, s);
+  __syncthreads();
+  if (j == 0 && i < count) {
+    for (int k = 1; k < 16; ++k) {
+      const float2 p = red[k * 16 + threadIdx.x];
+      join(p.x, p.y);
+    }
+    const float l = m + logf(s);
+    lse[idx[i]] = l;
+    loss[idx[i]] = l - hit[i];
+  }
+}
+
+// d of vocabulary rows [v0, v0 + 256 np) for every packed token: d[t][v - v0], ld = ldd
+template <class T, int FP, int FQ, int WP, int WQ>
+__global__ __launch_bounds__(64 * WP * WQ, 2) void k_loss_d(const uint16_t* __restrict__ w, long ldw, int v, int v0,
+                                                            const uint16_t* __restrict__ xc, int dp,
+                                                            const uint32_t* __restrict__ info, int np, int nq,
+                                                            const LossTok* __restrict__ tok, uint16_t* __restrict__ d,
+                                                            long ldd) {
+  typedef MmaTile<T, false, false, FP, FQ, WP, WQ> M;
+  __shared__ __align__(1024) uint8_t lds[M::LDS];
+  const MmaTileAt at = mma_tile_at(blockIdx.x, np, nq);
+  const int p0 = at.p * M::BP, q0 = at.q * M::BQ, count = (int)info[0];
+  if (q0 >= count) return;
+  mma_f4 acc[FP][FQ];
+  M::clear(acc);
+  M::run(lds_offset(lds), MmaOp{w + (long)v0 * ldw, ldw, v - v0}, MmaOp{xc, dp, count}, p0, q0, 0, dp, acc);
+  const int lane = threadIdx.x & 63;
+#pragma unroll
+  for (int g = 0; g < FQ; ++g) {
+    const int t = M::col(q0, g) + (lane & 15);
+    if (t >= count) continue;
+    const LossTok k = tok[t];
+#pragma unroll
+    for (int f = 0; f < FP; ++f) {
+      const int row = M::row(p0, f) + 4 * (lane >> 4);
+      float o[4];
+#pragma unroll
+      for (int r = 0; r < 4; ++r) {
+        // the difference first: it is exact where p is near 1 and p - 1 has to be right
+        const float p = __builtin_amdgcn_exp2f((acc[f][g][r] - k.lse) * LOG2E);
+        o[r] = v0 + row + r < v ? (p - (v0 + row + r == k.target ? 1.0f : 0.0f)) * k.weight : 0.0f;
+      }
+      *reinterpret_cast<uint2*>(d + (long)t * ldd + row) = make_uint2(narrow2<T>(o[0], o[1]), narrow2<T>(o[2], o[3]));
+    }
+  }
+}
+
+// dxacc[split][t][c] (+)= sum over the split's share of the piece's vocabulary of d[t][v] w[v0 + v][c]
+template <class T, int FP, int FQ, int WP, int WQ>
+__global__ __launch_bounds__(64 * WP * WQ, 2) void k_loss_dx(const uint16_t* __restrict__ w, long ldw, int dcols,
+                                                             int v0, int kpiece, int kshare,
+                                                             const uint16_t* __restrict__ d, long ldd,
+                                                             const uint32_t* __restrict__ info, int np, int nq, int t,
+                                                             int dp, int add, float* __restrict__ dxacc) {
+  typedef MmaTile<T, true, false, FP, FQ, WP, WQ> M;
+  __shared__ __align__(1024) uint8_t lds[M::LDS];
+  const int tiles = np * nq, split = blockIdx.x / tiles;
+  const MmaTileAt at = mma_tile_at(blockIdx.x - split * tiles, np, nq);
+  const int p0 = at.p * M::BP, q0 = at.q * M::BQ, count = (int)info[0];
+  if (q0 >= count) return;
+  mma_f4 acc[FP][FQ];
+  M::clear(acc);
+  M::run(lds_offset(lds), MmaOp{w + (long)v0 * ldw, ldw, dcols}, MmaOp{d, ldd, count}, p0, q0, split * kshare,
+         min(kpiece, (split + 1) * kshare), acc);
+  const int lane = threadIdx.x & 63;
+  float* out = dxacc + (long)split * t * dp;
+#pragma unroll
+  for (int g = 0; g < FQ; ++g) {
+    const int i = M::col(q0, g) + (lane & 15);
+    if (i >= count) continue;
+#pragma unroll
+    for (int f = 0; f < FP; ++f) {
+      const int c = M::row(p0, f) + 4 * (lane >> 4);
+      if (c >= dp) continue;
+      mma_f4* o = reinterpret_cast<mma_f4*>(out + (long)i * dp + c);
+      if (add) *o = *o + acc[f][g];
+      else *o = acc[f][g];
+    }
+  }
+}
+
+// dw[v0 + v][c] = top 2^-S sum_t d[t][v] xc[t][c]
+template <class T, int FP, int FQ, int WP, int WQ>
+__global__ __launch_bounds__(64 * WP * WQ, 2) void k_loss_dw(const uint16_t* __restrict__ xc, int dp, int dcols,
+                                                             const uint16_t* __restrict__ d, long ldd, int rows,
+                                                             const uint32_t* __restrict__ info, int np, int nq,
+                                                             float gscale, uint16_t* __restrict__ dw, long lddw,
+                                                             int vec) {
+  typedef MmaTile<T, true, true, FP, FQ, WP, WQ> M;
+  __shared__ __align__(1024) uint8_t lds[M::LDS];
+  const MmaTileAt at = mma_tile_at(blockIdx.x, np, nq);
+  const int p0 = at.p * M::BP, q0 = at.q * M::BQ, count = (int)info[0];
+  mma_f4 acc[FP][FQ];
+  M::clear(acc);
+  if (count > 0)
+    M::run(lds_offset(lds), MmaOp{xc, dp, dp}, MmaOp{d, ldd, (int)ldd}, p0, q0, 0, count, acc);
+  const float top = __uint_as_float(info[1]), k = (top > 0.0f ? top : 1.0f) / gscale;
+  const int lane = threadIdx.x & 63;
+#pragma unroll
+  for (int g = 0; g < FQ; ++g) {
+    const int i = M::col(q0, g) + (lane & 15);
+    if (i >= rows) continue;
+#pragma unroll
+    for (int f = 0; f < FP; ++f) {
+      const int c = M::row(p0, f) + 4 * (lane >> 4);
+      uint16_t* o = dw + (long)i * lddw + c;
+      const mma_f4 a = acc[f][g] * k;
+      if (vec) {
+        if (c < dcols) *reinterpret_cast<uint2*>(o) = make_uint2(narrow2<T>(a[0], a[1]), narrow2<T>(a[2], a[3]));
+      } else {
+#pragma unroll
+        for (int r = 0; r < 4; ++r)
+          if (c + r < dcols) o[r] = T::narrow(a[r]);
+      }
+    }
+  }
+}
+
+// dx[t] = top 2^-S sum over the splits of dxacc at the token's packed place; 0 where it does not count
+template <class T>
+__global__ __launch_bounds__(256) void k_loss_dx_out(const float* __restrict__ dxacc, int splits, int t, int d, int dp,
+                                                     const int* __restrict__ pos, const uint32_t* __restrict__ info,
+                                                     float gscale, uint16_t* __restrict__ dx, long lddx) {
+  const float top = __uint_as_float(info[1]), k = (top > 0.0f ? top : 1.0f) / gscale;
+  const long total = (long)t * dp;
+  for (long e = blockIdx.x * 256l + threadIdx.x; e * 8 < total; e += gridDim.x * 256l) {
+    const int i = (int)(e * 8 / dp), c = (int)(e * 8 - (long)i * dp), at = pos[i];
+    float s[8] = {};
+    if (at >= 0)
+      for (int j = 0; j < splits; ++j) {
+        const float* a = dxacc + ((long)j * t + at) * dp + c;
+#pragma unroll
+        for (int r = 0; r < 8; ++r) s[r] += a[r];
+      }
+    uint16_t* o = dx + (long)i * lddx + c;
+#pragma unroll
+    for (int r = 0; r < 8; ++r)
+      if (c + r < d) o[r] = T::narrow(s[r] * k);
+  }
+}
+
+inline int blocks_for(long items, int per, int most = 1 << 20) {
+  return (int)std::max(1l, std::min((items + per - 1) / per, (long)most));
+}
+
+// Calls f with the tile shape <FP, FQ, WP, WQ> for `cols` columns: 256 rows by 256, 128, 64, 32 or 16.
+// Narrow tiles read as many rows of P for fewer columns; they are taken where wide ones would compute
+// columns that nobody asked for.
+template <int FP, int FQ, int WP, int WQ>
+struct Shape {
+  static constexpr int fp = FP, fq = FQ, wp = WP, wq = WQ, bp = 16 * FP * WP, bq = 16 * FQ * WQ;
+};
+template <class F>
+hipError_t with_loss_shape(int cols, F f) {
+  if (cols > 128) return f(Shape<8, 4, 2, 4>{});
+  if (cols > 64) return f(Shape<4, 4, 4, 2>{});
+  if (cols > 32) return f(Shape<4, 2, 4, 2>{});
+  if (cols > 16) return f(Shape<2, 2, 8, 1>{});
+  return f(Shape<2, 1, 8, 1>{});
+}
+
+inline size_t up(size_t x, size_t to) { return (x + to - 1) / to * to; }
+
+}  // namespace
+
+// Workspace of the loss and its gradient, and where the parts lie in it.
+LossPlan loss_plan(long t, long d, long v, bool pad_w, bool grad) {
+  LossPlan p = {};
+  t = std::max(t, 1l);  // an empty call still writes a zero dw
+  p.dp = (int)up(d, 8);
+  size_t at = 0;
+  auto take = [&](size_t bytes) {
+    const size_t o = at;
+    at += up(bytes, 256);
+    return o;
+  };
+  p.info = take(16);
+  p.idx = take(4 * t);
+  p.pos = take(4 * t);
+  p.tok = take(sizeof(LossTok) * t);
+  p.xc = take(2 * (size_t)t * p.dp);
+  p.wpad = pad_w ? take(2 * (size_t)v * p.dp) : 0;
+  if (!grad) {
+    (void)with_loss_shape((int)t, [&](auto s) {
+      p.slab = 16 * s.fp;
+      return hipSuccess;
+    });
+    p.nslabs = (int)(up(v, 256) / p.slab);
+    p.hit = take(4 * t);
+    p.part = take(sizeof(float2) * (size_t)t * p.nslabs);
+  } else {
+    // pieces of the vocabulary: d of a piece takes at most 256 MB (about what the last-level cache
+    // keeps) and the whole vocabulary where that is less
+    const size_t rows = up(v, 256), most = std::max<size_t>(256, ((size_t)128 << 20) / t / 256 * 256);
+    p.pieces = (int)((rows + most - 1) / most);
+    p.piece = (int)up((rows + p.pieces - 1) / p.pieces, 256);
+    // a small dx is split over the vocabulary until about one round of workgroups works on it
+    int bq = 256;
+    (void)with_loss_shape((int)t, [&](auto s) {
+      bq = s.bq;
+      return hipSuccess;
+    });
+    const long tiles = (long)(up(d, 256) / 256) * (long)((t + bq - 1) / bq);
+    const long want = std::max(1l, std::min(256 / tiles, (long)p.piece / 512));
+    p.share = (int)up((p.piece + want - 1) / want, 64);
+    p.splits = (p.piece + p.share - 1) / p.share;
+    p.d = take(2 * (size_t)t * p.piece);
+    p.dxacc = take(4 * (size_t)t * p.dp * p.splits);
+  }
+  p.bytes = at;
+  return p;
+}
+
+namespace {
+
+// The packed tokens, and W where the tiles cannot read it as it is
+hipError_t prepare(hipStream_t st, const LossArgs& a, const LossPlan& p, float gscale, const uint16_t** w, long* ldw) {
+  char* ws = static_cast<char*>(a.work);
+  const bool grad = a.dx || a.dw;
+  k_loss_tokens<<<1, 1024, 0, st>>>(a.targets, a.ignore, (int)a.t, a.dloss, reinterpret_cast<int*>(ws + p.idx),
+                                    grad ? reinterpret_cast<int*>(ws + p.pos) : nullptr,
+                                    reinterpret_cast<uint32_t*>(ws + p.info), grad ? nullptr : a.loss,
+                                    grad ? nullptr : a.lse_out);
+  const int vec = a.d % 8 == 0 && a.ldx % 8 == 0 && (uintptr_t)a.x % 16 == 0;
+  if (a.t) k_loss_gather<<<(int)a.t, 256, 0, st>>>(a.x, a.ldx, (int)a.d, p.dp, reinterpret_cast<int*>(ws + p.idx),
+                                          reinterpret_cast<uint32_t*>(ws + p.info), a.targets, (int)a.v, a.lse_in,
+                                          a.dloss, gscale, reinterpret_cast<uint16_t*>(ws + p.xc),
+                                          reinterpret_cast<LossTok*>(ws + p.tok),
+                                          grad ? nullptr : reinterpret_cast<float*>(ws + p.hit), vec);
+  *w = a.w;
+  *ldw = a.ldw;
+  if (p.wpad) {
+    uint16_t* wp = reinterpret_cast<uint16_t*>(ws + p.wpad);
+    k_pad16<<<blocks_for(a.v * p.dp, 256 * 8), 256, 0, st>>>(a.w, a.ldw, (int)a.d, p.dp, a.v, wp);
+    *w = wp;
+    *ldw = p.dp;
+  }
+  return hipGetLastError();
+}
+
+template <class T>
+hipError_t forward(hipStream_t st, const LossArgs& a, const LossPlan& p) {
+  char* ws = static_cast<char*>(a.work);
+  const uint16_t* w;
+  long ldw;
+  hipError_t e = prepare(st, a, p, 1.0f, &w, &ldw);
+  if (e != hipSuccess) return e;
+  e = with_loss_shape((int)a.t, [&](auto s) {
+    typedef decltype(s) S;
+    const int np = (int)((a.v + S::bp - 1) / S::bp), nq = (int)((a.t + S::bq - 1) / S::bq);
+    k_loss_tiles<T, S::fp, S::fq, S::wp, S::wq><<<np * nq, 64 * S::wp * S::wq, 0, st>>>(
+        w, ldw, (int)a.v, reinterpret_cast<uint16_t*>(ws + p.xc), p.dp, reinterpret_cast<uint32_t*>(ws + p.info), np, nq,
+        reinterpret_cast<LossTok*>(ws + p.tok), reinterpret_cast<float2*>(ws + p.part), (int)a.t,
+        reinterpret_cast<float*>(ws + p.hit));
+    return hipGetLastError();
+  });
+  if (e != hipSuccess) return e;
+  k_loss_combine<<<(int)((a.t + 15) / 16), 256, 0, st>>>(
+      reinterpret_cast<float2*>(ws + p.part), (int)a.t, p.nslabs, reinterpret_cast<uint32_t*>(ws + p.info),
+      reinterpret_cast<int*>(ws + p.idx), reinterpret_cast<float*>(ws + p.hit), a.loss, a.lse_out);
+  return hipGetLastError();
+}
+
+template <class T>
+hipError_t backward(hipStream_t st, const LossArgs& a, const LossPlan& p) {
+  char* ws = static_cast<char*>(a.work);
+  const float gscale = T::kind == F16::kind ? 32768.0f : 1.0f;
+  const uint16_t* w;
+  long ldw;
+  hipError_t e = prepare(st, a, p, gscale, &w, &ldw);
+  if (e != hipSuccess) return e;
+  uint32_t* info = reinterpret_cast<uint32_t*>(ws + p.info);
+  uint16_t* xc = reinterpret_cast<uint16_t*>(ws + p.xc);
+  uint16_t* d = reinterpret_cast<uint16_t*>(ws + p.d);
+  float* dxacc = reinterpret_cast<float*>(ws + p.dxacc);
+  LossTok* tok = reinterpret_cast<LossTok*>(ws + p.tok);
+  const int t = (int)a.t, v = (int)a.v;
+  for (int i = 0; i < p.pieces; ++i) {
+    const int v0 = i * p.piece;
+    if (v0 >= v) break;
+    const int rows = std::min(p.piece, v - v0);
+    if (t) e = with_loss_shape(t, [&](auto s) {
+      typedef decltype(s) S;
+      const int nq = (t + S::bq - 1) / S::bq, np = (rows + S::bp - 1) / S::bp;
+      k_loss_d<T, S::fp, S::fq, S::wp, S::wq><<<np * nq, 64 * S::wp * S::wq, 0, st>>>(w, ldw, v, v0, xc, p.dp, info, np,
+                                                                                      nq, tok, d, p.piece);
+      hipError_t e1 = hipGetLastError();
+      if (e1 != hipSuccess) return e1;
+      const int npx = (p.dp + S::bp - 1) / S::bp;
+      k_loss_dx<T, S::fp, S::fq, S::wp, S::wq><<<npx * nq * p.splits, 64 * S::wp * S::wq, 0, st>>>(
+          w, ldw, p.dp, v0, rows, p.share, d, p.piece, info, npx, nq, t, p.dp, i > 0, dxacc);
+      return hipGetLastError();
+    });
+    if (e != hipSuccess) return e;
+    if (a.dw) {
+      typedef Shape<8, 4, 2, 4> S;
+      const int np = (p.dp + S::bp - 1) / S::bp, nq = (rows + S::bq - 1) / S::bq;
+      const int vec = a.lddw % 4 == 0 && a.d % 4 == 0 && (uintptr_t)a.dw % 8 == 0;
+      k_loss_dw<T, S::fp, S::fq, S::wp, S::wq><<<np * nq, 64 * S::wp * S::wq, 0, st>>>(
+          xc, p.dp, (int)a.d, d, p.piece, rows, info, np, nq, gscale, a.dw + (long)v0 * a.lddw, a.lddw, vec);
+      e = hipGetLastError();
+      if (e != hipSuccess) return e;
+    }
+  }
+  if (t) k_loss_dx_out<T><<<blocks_for((long)t * p.dp, 8 * 256), 256, 0, st>>>(
+      dxacc, p.splits, t, (int)a.d, p.dp, reinterpret_cast<int*>(ws + p.pos), info, gscale, a.dx, a.lddx);
+  return hipGetLastError();
+}
+
+}  // namespace
+
+hipError_t loss_forward(hipStream_t st, int dtype, const LossArgs& a, const LossPlan& p) {
+  return dtype == CDCLQ_DTYPE_BF16 ? forward<Bf16>(st, a, p) : forward<F16>(st, a, p);
+}
+hipError_t loss_backward(hipStream_t st, int dtype, const LossArgs& a, const LossPlan& p) {
+  return dtype == CDCLQ_DTYPE_BF16 ? backward<Bf16>(st, a, p) : backward<F16>(st, a, p);
+}
+
+}  // namespace cdclq

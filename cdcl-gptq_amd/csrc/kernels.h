@@ -264,4 +264,35 @@ hipError_t synth_perturb(hipStream_t st, uint64_t seed, uint64_t offset, size_t 
                          float* out);
 hipError_t f64_to_f32(hipStream_t st, size_t count, const double* a, float* b);
 
+// ---- k_ckpt.hip: 8-bit activation checkpoints (dtype: CDCLQ_DTYPE_F16 or _BF16). codes t x n,
+// scales t x ceil(n / 128)
+hipError_t ckpt_save(hipStream_t st, int dtype, const uint16_t* x, long ldx, long t, long n, int8_t* codes,
+                     float* scales);
+hipError_t ckpt_restore(hipStream_t st, int dtype, const int8_t* codes, const float* scales, long t, long n,
+                        uint16_t* out, long ldo);
+
+// ---- k_loss.hip: softmax cross entropy over a large vocabulary
+struct LossArgs {
+  const uint16_t* x;  // t x d, row stride ldx
+  long ldx;
+  const uint16_t* w;  // v x d, row stride ldw
+  long ldw;
+  long t, d, v;
+  const int64_t* targets;
+  int64_t ignore;
+  float *loss, *lse_out;          // forward
+  const float *lse_in, *dloss;    // gradient (dloss null: forward)
+  uint16_t *dx, *dw;              // gradient; dw may be null
+  long lddx, lddw;
+  void* work;
+};
+struct LossPlan {
+  size_t bytes, info, idx, pos, tok, xc, wpad, hit, part, d, dxacc;  // offsets into the workspace
+  int dp, slab, nslabs, pieces, piece, share, splits;
+};
+// pad_w: W's rows are not 16-byte aligned (loss_pads_w)
+LossPlan loss_plan(long t, long d, long v, bool pad_w, bool grad);
+hipError_t loss_forward(hipStream_t st, int dtype, const LossArgs& a, const LossPlan& p);
+hipError_t loss_backward(hipStream_t st, int dtype, const LossArgs& a, const LossPlan& p);
+
 }  // namespace cdclq

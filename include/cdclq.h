@@ -8,7 +8,8 @@
  * Conventions
  *  - Matrices are row-major. `*_device` entry points take pointers to device (HBM) memory of the
  *    context's GPU; the others take host memory and stage it through the device themselves.
- *  - Every call is synchronous (returns after the device work finished), like the reference.
+ *  - Every call is synchronous (returns after the device work finished), like the reference, except
+ *    those that take a stream: they enqueue their work there and return.
  *  - Status codes: CDCLQ_OK on success; on failure cdclq_last_error(ctx) holds the message. For
  *    conditions the reference reports with anyhow::bail! the text is the reference's text.
  *  - A context is thread-compatible, not thread-safe: one context per host thread and GPU.
@@ -330,6 +331,40 @@ int cdclq_quantize_model(cdclq_ctx* ctx, const cdclq_quant_opts* opts, char* rep
  * becomes `X.weight` (original column order) in `dtype` (cdclq_dtype; -1 = the header's orig_dtype,
  * else F16); other tensors pass through. *nlayers = layers expanded. */
 int cdclq_dequantize_model(cdclq_ctx* ctx, const char* input, const char* output, int dtype, size_t* nlayers);
+
+/* ---- Training and serving adapters on a packed model (no counterpart in the reference) ----
+ * These entry points enqueue their work on `stream` (a hipStream_t of the context's GPU passed as a
+ * plain pointer; NULL is the default stream) and return without waiting. All arrays are device memory,
+ * `dtype` is CDCLQ_DTYPE_F16 or CDCLQ_DTYPE_BF16 (16-bit patterns), row strides (ld*) are in elements.
+ * They allocate nothing and keep nothing between calls: scratch memory is the caller's `work` (256-byte
+ * aligned, *_work_bytes() long), free again once the stream has passed the call, so that calls on
+ * several streams need only a workspace each, and calls may be captured into a graph. Results do not
+ * depend on the launch order of workgroups: equal inputs give equal bits. */
+
+/* An activation in 8 bits: x (t x n) in blocks of 128 features, scales[t][b] = max |x| / 127 (f32),
+ * codes[t][i] = x / scale rounded to nearest, ties to even (0 where the scale is 0). A block that holds
+ * a NaN or an infinity has a NaN scale. codes t x n, scales t x ceil(n / 128), both tightly packed. */
+int cdclq_checkpoint_save_device(cdclq_ctx* ctx, const void* x, size_t ldx, size_t t, size_t n, int dtype,
+                                 int8_t* codes, float* scales, void* stream);
+/* out (t x n, dtype) = scale * code, rounded once. */
+int cdclq_checkpoint_restore_device(cdclq_ctx* ctx, const int8_t* codes, const float* scales, size_t t, size_t n,
+                                    int dtype, void* out, size_t ldo, void* stream);
+
+/* Softmax cross entropy of the logits x w^T (x t x d, w v x d) without the logits in memory:
+ * lse[t] = log sum_v exp(x_t . w_v), loss[t] = lse[t] - x_t . w_target. A token whose target is
+ * ignore_index has loss = lse = 0 and does not take part, whatever x holds there; any other target
+ * outside 0..v gives a NaN loss. */
+size_t cdclq_vocab_work_bytes(size_t t, size_t d, size_t v, const void* w, size_t ldw, int grad);
+int cdclq_vocab_loss_device(cdclq_ctx* ctx, const void* x, size_t ldx, const void* w, size_t ldw, size_t t, size_t d,
+                            size_t v, int dtype, const int64_t* targets, int64_t ignore_index, float* loss, float* lse,
+                            void* work, size_t work_bytes, void* stream);
+/* The gradient for dloss[t] = d(objective) / d(loss[t]): dx (t x d, 0 at ignored tokens) and, unless
+ * dw is NULL, dw (v x d); lse is the forward call's. With a target outside 0..v the token's dx and all
+ * of dw are NaN. grad = 1 in cdclq_vocab_work_bytes. */
+int cdclq_vocab_loss_backward_device(cdclq_ctx* ctx, const void* x, size_t ldx, const void* w, size_t ldw, size_t t,
+                                     size_t d, size_t v, int dtype, const int64_t* targets, int64_t ignore_index,
+                                     const float* lse, const float* dloss, void* dx, size_t lddx, void* dw, size_t lddw,
+                                     void* work, size_t work_bytes, void* stream);
 
 /* ---- Device memory staging for callers without their own GPU runtime binding. ---- */
 int cdclq_device_alloc(cdclq_ctx* ctx, size_t bytes, void** ptr);

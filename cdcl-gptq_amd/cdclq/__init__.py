@@ -144,6 +144,13 @@ def lib() -> C.CDLL:
         "cdclq_hessian_finalize_device": ([vp, vp, sz, u64, vp], i32),
         "cdclq_checkpoint_save_device": ([vp, vp, sz, sz, sz, i32, vp, vp, vp], i32),
         "cdclq_checkpoint_restore_device": ([vp, vp, vp, sz, sz, i32, vp, sz, vp], i32),
+        "cdclq_packed_open_device": ([vp, sz, sz, sz, vp, sz, vp, sz, vp, vp, vp, C.POINTER(vp)], i32),
+        "cdclq_packed_close": ([vp], None),
+        "cdclq_packed_bytes": ([vp], sz),
+        "cdclq_adapter_work_bytes": ([vp, vp, sz, sz, vp, vp, sz, sz, i32], sz),
+        "cdclq_adapter_linear_device": ([vp, vp, vp, sz, sz, i32, vp, vp, vp, sz, sz, vp, vp, sz, vp, vp, sz, vp], i32),
+        "cdclq_adapter_backward_device": ([vp, vp, vp, sz, sz, i32, vp, vp, vp, vp, vp, vp, sz, sz, vp, vp, sz, vp, vp,
+                                           vp, sz, vp], i32),
         "cdclq_vocab_work_bytes": ([sz, sz, sz, vp, sz, i32], sz),
         "cdclq_vocab_loss_device": ([vp, vp, sz, vp, sz, sz, sz, sz, i32, vp, i64, vp, vp, vp, sz, vp], i32),
         "cdclq_vocab_loss_backward_device": ([vp, vp, sz, vp, sz, sz, sz, sz, i32, vp, i64, vp, vp, vp, sz, vp, sz,
@@ -194,6 +201,8 @@ def exported_symbols() -> list[str]:
         "cdclq_rel_err_device", "cdclq_bench_run", "cdclq_quantize_model", "cdclq_dequantize_model",
         "cdclq_hessian_accumulate_device", "cdclq_hessian_finalize_device",
         "cdclq_checkpoint_save_device", "cdclq_checkpoint_restore_device", "cdclq_vocab_work_bytes",
+        "cdclq_packed_open_device", "cdclq_packed_close", "cdclq_packed_bytes", "cdclq_adapter_work_bytes",
+        "cdclq_adapter_linear_device", "cdclq_adapter_backward_device",
         "cdclq_vocab_loss_device", "cdclq_vocab_loss_backward_device",
     ]
 

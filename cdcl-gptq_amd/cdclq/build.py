@@ -27,6 +27,7 @@ LIB = os.path.join(PKG, "libcdclq_hip.so")
 ARCH = os.environ.get("CDCLQ_ARCH", "gfx950")
 
 SOURCES = ["k_gemm.hip", "k_gemm_wide.hip", "k_gram.hip", "k_factor.hip", "k_engine.hip", "k_repair.hip", "k_panel.hip", "k_pack.hip", "k_eval.hip", "k_ckpt.hip", "k_loss.hip",
+           "k_packed.hip", "k_adapt.hip",
            "engine.cpp", "container.cpp", "harness.cpp", "pipeline.cpp", "tune.cpp"]
 COMMON = [
     f"--offload-arch={ARCH}", "-O3", "-std=c++17", "-fPIC", "-ffp-contract=off",

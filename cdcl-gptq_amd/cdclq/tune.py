@@ -2,6 +2,8 @@
 
 The operators that a quantized model needs once its weights are frozen:
 
+  PackedLinear, Adapters                 a packed layer laid out for products; adapters A, B of one layer
+  adapter_linear / _backward             the packed projection with each token's adapter beside it
   checkpoint_save / checkpoint_restore   a layer's input kept in 8 bits until the backward pass
   vocab_loss / vocab_loss_backward       softmax cross entropy over a large vocabulary and its
                                          gradient, without the logits in memory
@@ -14,11 +16,13 @@ kind) before anything is enqueued.
 """
 from __future__ import annotations
 
+import ctypes as C
 from dataclasses import dataclass
 
+import numpy as np
 import torch
 
-from . import DTYPE_BF16, DTYPE_F16, CdclqError, Context, lib
+from . import DTYPE_BF16, DTYPE_F16, Context, lib
 
 BLOCK = 128  # features per scale of an 8-bit checkpoint
 _CODES = {torch.bfloat16: DTYPE_BF16, torch.float16: DTYPE_F16}
@@ -101,6 +105,152 @@ def checkpoint_restore(ctx: Context, ck: Checkpoint) -> torch.Tensor:
     ctx.check(lib().cdclq_checkpoint_restore_device(ctx.ptr, ck.codes.data_ptr(), ck.scales.data_ptr(), t, n,
                                                     _code(out, "out"), out.data_ptr(), n, _stream(ctx)))
     return out
+
+
+# ---------------------------------------------------------------- packed projection with adapters
+class PackedLinear:
+    """A packed (cdclq-v1) layer laid out once for products: qweight (uint8, d_out x row bytes), scales
+    (float16, or their uint16 bit patterns), qzeros (uint8), perm (int32), as torch tensors on the
+    context's GPU or as the host arrays of packed_tensors(); gbits (uint8 per group) and the group
+    size. The tensors are not needed afterwards."""
+
+    def __init__(self, ctx: Context, qweight, scales, qzeros, perm, gbits, group: int):
+        self.ptr = None
+        self.ctx = ctx
+        dev = torch.device("cuda", ctx.device)
+
+        def put(a, kinds, name):
+            if isinstance(a, np.ndarray) and a.dtype == np.uint16:
+                a = a.view(np.float16)
+            t = torch.as_tensor(a)
+            if t.dtype not in kinds:
+                raise TypeError(f"{name} is {t.dtype}, need {kinds[0]}")
+            return t.to(dev).contiguous()
+
+        qw, s16 = put(qweight, (torch.uint8,), "qweight"), put(scales, (torch.float16,), "scales")
+        qz, p32 = put(qzeros, (torch.uint8,), "qzeros"), put(perm, (torch.int32,), "perm")
+        gb = np.ascontiguousarray(gbits.cpu().numpy() if isinstance(gbits, torch.Tensor) else gbits, np.uint8)
+        if qw.dim() != 2 or p32.dim() != 1 or tuple(s16.shape) != (qw.shape[0], gb.size) or qz.shape != s16.shape:
+            raise ValueError(f"qweight {tuple(qw.shape)}, scales {tuple(s16.shape)}, qzeros {tuple(qz.shape)} and "
+                             f"{gb.size} groups do not belong together")
+        self.d_out, self.d_in = qw.shape[0], p32.shape[0]
+        torch.cuda.current_stream(dev).synchronize()
+        out = C.c_void_p()
+        ctx.check(lib().cdclq_packed_open_device(ctx.ptr, self.d_out, self.d_in, int(group), gb.ctypes.data, gb.size,
+                                                 qw.data_ptr(), qw.numel(), s16.data_ptr(), qz.data_ptr(),
+                                                 p32.data_ptr(), C.byref(out)))
+        self.ptr = out
+
+    @classmethod
+    def from_tensors(cls, ctx: Context, tensors: dict, layer: str) -> "PackedLinear":
+        """From a dict in the packed_tensors() form, or of a packed shard's tensors."""
+        def get(suffix):
+            v = tensors[f"{layer}.{suffix}"]
+            return v[1] if isinstance(v, tuple) else v
+        return cls(ctx, get("qweight"), get("scales"), get("qzeros"), get("perm"), get("gbits"),
+                   int(np.asarray(get("gsize")).ravel()[0]))
+
+    def nbytes(self) -> int:
+        """Device memory that the layer holds."""
+        return lib().cdclq_packed_bytes(self.ptr)
+
+    def close(self):
+        if getattr(self, "ptr", None):
+            lib().cdclq_packed_close(self.ptr)
+            self.ptr = None
+
+    def __del__(self):
+        try:
+            self.close()
+        except Exception:
+            pass
+
+
+class Adapters:
+    """The low-rank adapters of one layer: a (R x rank x d_in), b (R x d_out x rank), both contiguous
+    and of one 16-bit type, scaling (float32, R). Adapters of smaller rank are padded with zeros."""
+
+    def __init__(self, a: torch.Tensor, b: torch.Tensor, scaling: torch.Tensor):
+        _code(a, "a")
+        if a.dim() != 3 or b.dim() != 3 or a.shape[0] != b.shape[0] or a.shape[1] != b.shape[2]:
+            raise ValueError(f"a {tuple(a.shape)} and b {tuple(b.shape)} are not R x rank x d_in and R x d_out x rank")
+        if b.dtype != a.dtype or scaling.dtype != torch.float32:
+            raise TypeError(f"a is {a.dtype}, b {b.dtype}, scaling {scaling.dtype}; need one 16-bit type and float32")
+        if tuple(scaling.shape) != (a.shape[0],) or not (a.is_contiguous() and b.is_contiguous() and
+                                                         scaling.is_contiguous()):
+            raise ValueError("a, b and scaling (one value per adapter) must be contiguous")
+        if not (a.device == b.device == scaling.device):
+            raise ValueError("a, b and scaling are on different devices")
+        self.a, self.b, self.scaling = a, b, scaling
+        self.count, self.rank = a.shape[0], a.shape[1]
+
+
+def _adapter_args(packed: PackedLinear, x, adapters, request, name: str):
+    """(a, b, scaling, count, rank, request) addresses after checks against the layer."""
+    if adapters is None:
+        if request is not None:
+            raise ValueError("request without adapters")
+        return None, None, None, 0, 0, None
+    a = adapters.a
+    if a.device != x.device or a.dtype != x.dtype:
+        raise TypeError(f"the adapters are {a.dtype} on {a.device}, {name} is {x.dtype} on {x.device}")
+    if a.shape[2] != packed.d_in or adapters.b.shape[1] != packed.d_out:
+        raise ValueError(f"adapters of a {adapters.b.shape[1]} x {a.shape[2]} layer, the packed layer is "
+                         f"{packed.d_out} x {packed.d_in}")
+    if request is None:
+        raise ValueError("adapters need the request of each token")
+    _vector(packed.ctx, request, "request", torch.int32, x.shape[0])
+    return (a.data_ptr(), adapters.b.data_ptr(), adapters.scaling.data_ptr(), adapters.count, adapters.rank,
+            request.data_ptr())
+
+
+def adapter_linear(packed: PackedLinear, x: torch.Tensor, adapters: Adapters | None = None,
+                   request: torch.Tensor | None = None, return_low: bool = False):
+    """y (T x d_out) = x W^T with each token's adapter beside it: y_t = W x_t + scaling[q] B_q (A_q x_t),
+    q = request[t] (int32, -1: none). With return_low also low = A_q x_t (T x rank, float32), which the
+    backward pass takes."""
+    ctx = packed.ctx
+    code, ld = _code(x, "x"), _matrix(ctx, x, "x", None, None, packed.d_in)
+    t = x.shape[0]
+    a, b, s, count, rank, req = _adapter_args(packed, x, adapters, request, "x")
+    L = lib()
+    y = torch.empty(t, packed.d_out, dtype=x.dtype, device=x.device)
+    low = torch.empty(t, rank, dtype=torch.float32, device=x.device) if return_low else None
+    xp = x.data_ptr()
+    work = _work(L.cdclq_adapter_work_bytes(packed.ptr, xp, ld, t, a, b, count, rank, 0), x.device)
+    ctx.check(L.cdclq_adapter_linear_device(ctx.ptr, packed.ptr, xp, ld, t, code, a, b, s, count, rank, req,
+                                            y.data_ptr(), packed.d_out, low.data_ptr() if return_low else None,
+                                            work.data_ptr(), work.numel(), _stream(ctx)))
+    return (y, low) if return_low else y
+
+
+def adapter_linear_backward(packed: PackedLinear, dy: torch.Tensor, saved: Checkpoint | None = None,
+                            low: torch.Tensor | None = None, adapters: Adapters | None = None,
+                            request: torch.Tensor | None = None):
+    """The gradient of adapter_linear for dy (T x d_out): (dx, da, db). saved is checkpoint_save of its
+    x, low what adapter_linear returned. W is frozen. Without adapters da and db are None."""
+    ctx = packed.ctx
+    code, ld = _code(dy, "dy"), _matrix(ctx, dy, "dy", None, None, packed.d_out)
+    t = dy.shape[0]
+    a, b, s, count, rank, req = _adapter_args(packed, dy, adapters, request, "dy")
+    L = lib()
+    dx = torch.empty(t, packed.d_in, dtype=dy.dtype, device=dy.device)
+    da = db = codes = scales = lp = None
+    if rank:
+        if saved is None or low is None:
+            raise ValueError("the adapters' gradient needs the saved input and low")
+        _check_saved(ctx, saved, t, packed.d_in)
+        if _matrix(ctx, low, "low", torch.float32, t, rank) != rank:
+            raise ValueError("low must be contiguous")
+        codes, scales, lp = saved.codes.data_ptr(), saved.scales.data_ptr(), low.data_ptr()
+        da, db = torch.empty_like(adapters.a), torch.empty_like(adapters.b)
+    dyp = dy.data_ptr()
+    work = _work(L.cdclq_adapter_work_bytes(packed.ptr, dyp, ld, t, a, b, count, rank, 1), dy.device)
+    ctx.check(L.cdclq_adapter_backward_device(ctx.ptr, packed.ptr, dyp, ld, t, code, codes, scales, lp, a, b, s, count,
+                                              rank, req, dx.data_ptr(), packed.d_in, da.data_ptr() if rank else None,
+                                              db.data_ptr() if rank else None, work.data_ptr(), work.numel(),
+                                              _stream(ctx)))
+    return dx, da, db
 
 
 # ---------------------------------------------------------------- cross entropy over a vocabulary

@@ -339,22 +339,6 @@ inline int blocks_for(long items, int per, int most = 1 << 20) {
   return (int)std::max(1l, std::min((items + per - 1) / per, (long)most));
 }
 
-// Calls f with the tile shape <FP, FQ, WP, WQ> for `cols` columns: 256 rows by 256, 128, 64, 32 or 16.
-// Narrow tiles read as many rows of P for fewer columns; they are taken where wide ones would compute
-// columns that nobody asked for.
-template <int FP, int FQ, int WP, int WQ>
-struct Shape {
-  static constexpr int fp = FP, fq = FQ, wp = WP, wq = WQ, bp = 16 * FP * WP, bq = 16 * FQ * WQ;
-};
-template <class F>
-hipError_t with_loss_shape(int cols, F f) {
-  if (cols > 128) return f(Shape<8, 4, 2, 4>{});
-  if (cols > 64) return f(Shape<4, 4, 4, 2>{});
-  if (cols > 32) return f(Shape<4, 2, 4, 2>{});
-  if (cols > 16) return f(Shape<2, 2, 8, 1>{});
-  return f(Shape<2, 1, 8, 1>{});
-}
-
 inline size_t up(size_t x, size_t to) { return (x + to - 1) / to * to; }
 
 }  // namespace
@@ -377,7 +361,7 @@ LossPlan loss_plan(long t, long d, long v, bool pad_w, bool grad) {
   p.xc = take(2 * (size_t)t * p.dp);
   p.wpad = pad_w ? take(2 * (size_t)v * p.dp) : 0;
   if (!grad) {
-    (void)with_loss_shape((int)t, [&](auto s) {
+    (void)with_mma_shape(t, [&](auto s) {
       p.slab = 16 * s.fp;
       return hipSuccess;
     });
@@ -392,7 +376,7 @@ LossPlan loss_plan(long t, long d, long v, bool pad_w, bool grad) {
     p.piece = (int)up((rows + p.pieces - 1) / p.pieces, 256);
     // a small dx is split over the vocabulary until about one round of workgroups works on it
     int bq = 256;
-    (void)with_loss_shape((int)t, [&](auto s) {
+    (void)with_mma_shape(t, [&](auto s) {
       bq = s.bq;
       return hipSuccess;
     });
@@ -441,10 +425,10 @@ hipError_t forward(hipStream_t st, const LossArgs& a, const LossPlan& p) {
   long ldw;
   hipError_t e = prepare(st, a, p, 1.0f, &w, &ldw);
   if (e != hipSuccess) return e;
-  e = with_loss_shape((int)a.t, [&](auto s) {
+  e = with_mma_shape(a.t, [&](auto s) {
     typedef decltype(s) S;
     const int np = (int)((a.v + S::bp - 1) / S::bp), nq = (int)((a.t + S::bq - 1) / S::bq);
-    k_loss_tiles<T, S::fp, S::fq, S::wp, S::wq><<<np * nq, 64 * S::wp * S::wq, 0, st>>>(
+    k_loss_tiles<T, S::fp, S::fq, S::wp, S::wq><<<np * nq, S::threads, 0, st>>>(
         w, ldw, (int)a.v, reinterpret_cast<uint16_t*>(ws + p.xc), p.dp, reinterpret_cast<uint32_t*>(ws + p.info), np, nq,
         reinterpret_cast<LossTok*>(ws + p.tok), reinterpret_cast<float2*>(ws + p.part), (int)a.t,
         reinterpret_cast<float*>(ws + p.hit));
@@ -475,24 +459,24 @@ hipError_t backward(hipStream_t st, const LossArgs& a, const LossPlan& p) {
     const int v0 = i * p.piece;
     if (v0 >= v) break;
     const int rows = std::min(p.piece, v - v0);
-    if (t) e = with_loss_shape(t, [&](auto s) {
+    if (t) e = with_mma_shape(t, [&](auto s) {
       typedef decltype(s) S;
       const int nq = (t + S::bq - 1) / S::bq, np = (rows + S::bp - 1) / S::bp;
-      k_loss_d<T, S::fp, S::fq, S::wp, S::wq><<<np * nq, 64 * S::wp * S::wq, 0, st>>>(w, ldw, v, v0, xc, p.dp, info, np,
+      k_loss_d<T, S::fp, S::fq, S::wp, S::wq><<<np * nq, S::threads, 0, st>>>(w, ldw, v, v0, xc, p.dp, info, np,
                                                                                       nq, tok, d, p.piece);
       hipError_t e1 = hipGetLastError();
       if (e1 != hipSuccess) return e1;
       const int npx = (p.dp + S::bp - 1) / S::bp;
-      k_loss_dx<T, S::fp, S::fq, S::wp, S::wq><<<npx * nq * p.splits, 64 * S::wp * S::wq, 0, st>>>(
+      k_loss_dx<T, S::fp, S::fq, S::wp, S::wq><<<npx * nq * p.splits, S::threads, 0, st>>>(
           w, ldw, p.dp, v0, rows, p.share, d, p.piece, info, npx, nq, t, p.dp, i > 0, dxacc);
       return hipGetLastError();
     });
     if (e != hipSuccess) return e;
     if (a.dw) {
-      typedef Shape<8, 4, 2, 4> S;
+      typedef MmaShape<8, 4, 2, 4> S;
       const int np = (p.dp + S::bp - 1) / S::bp, nq = (rows + S::bq - 1) / S::bq;
       const int vec = a.lddw % 4 == 0 && a.d % 4 == 0 && (uintptr_t)a.dw % 8 == 0;
-      k_loss_dw<T, S::fp, S::fq, S::wp, S::wq><<<np * nq, 64 * S::wp * S::wq, 0, st>>>(
+      k_loss_dw<T, S::fp, S::fq, S::wp, S::wq><<<np * nq, S::threads, 0, st>>>(
           xc, p.dp, (int)a.d, d, p.piece, rows, info, np, nq, gscale, a.dw + (long)v0 * a.lddw, a.lddw, vec);
       e = hipGetLastError();
       if (e != hipSuccess) return e;

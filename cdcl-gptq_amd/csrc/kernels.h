@@ -295,4 +295,42 @@ LossPlan loss_plan(long t, long d, long v, bool pad_w, bool grad);
 hipError_t loss_forward(hipStream_t st, int dtype, const LossArgs& a, const LossPlan& p);
 hipError_t loss_backward(hipStream_t st, int dtype, const LossArgs& a, const LossPlan& p);
 
+// ---- k_packed.hip, k_adapt.hip: packed projection with low-rank adapters (layout: packed.h)
+struct PackedView {
+  const uint8_t* codes;    // [tile][block]
+  const uint32_t* scl;     // [tile][group][16]: f16 scale, zero point << 16
+  const uint32_t* kinfo;   // [block]: offset in the tile / 256 << 8 | run ends (bit 4 + s) | width
+  const uint32_t* grp;     // [step] its group
+  const int* col;          // [slot] original column, or -1
+  long tile_bytes;
+  int m, n, tiles, ng, nkb, bits;  // bits: the width of every block, 0 where they differ
+};
+struct AdapterArgs {
+  long t;
+  const uint16_t* x;  // forward: t x n; gradient: dy, t x m
+  long ldx;
+  const uint16_t *a, *b;  // adapters x rank x n, adapters x m x rank; null with rank 0
+  const float* scaling;
+  int adapters, rank;
+  const int* request;
+  uint16_t* y;  // forward: t x m; gradient: dx, t x n
+  long ldy;
+  float* low;  // forward: t x rank (may be null); gradient: the forward's
+  const int8_t* codes;  // gradient only: the checkpoint of x, and da, db
+  const float* scales;
+  uint16_t *da, *db;
+};
+// The container's streams into the layout: slotpos[slot] = permuted column or -1, coff / cwid its bit
+// offset and width.
+hipError_t packed_layout(hipStream_t st, const PackedView& v, int ng_in, const uint8_t* qw, long rb,
+                         const uint16_t* s16, const uint8_t* qz, const int* slotpos, const uint32_t* coff,
+                         const uint8_t* cwid, uint8_t* codes, uint32_t* scl);
+hipError_t packed_expand(hipStream_t st, int dtype, const PackedView& v, uint16_t* w16);
+size_t few_work_bytes(const PackedView& v, long t, long rank);
+hipError_t adapter_few(hipStream_t st, int dtype, const PackedView& v, const AdapterArgs& a, void* work);
+size_t wide_work_bytes(const PackedView& v, const AdapterArgs& a);
+hipError_t adapter_wide(hipStream_t st, int dtype, const PackedView& v, const AdapterArgs& a, void* work);
+size_t grad_work_bytes(const PackedView& v, const AdapterArgs& a);
+hipError_t adapter_grad(hipStream_t st, int dtype, const PackedView& v, const AdapterArgs& a, void* work);
+
 }  // namespace cdclq

@@ -222,4 +222,20 @@ __device__ __forceinline__ MmaTileAt mma_tile_at(int id, int np, int nq) {
   return {8 * band + left % wide, left / wide};
 }
 
+// Tile shapes, by the columns (tokens) there are: 256 rows by 256, 128, 64, 32 or 16. Narrow tiles read
+// as many rows of P for fewer columns; they are taken where wide ones would compute columns that
+// nobody asked for. f gets a MmaShape; its result is returned.
+template <int FP, int FQ, int WP, int WQ>
+struct MmaShape {
+  static constexpr int fp = FP, fq = FQ, wp = WP, wq = WQ, bp = 16 * FP * WP, bq = 16 * FQ * WQ, threads = 64 * WP * WQ;
+};
+template <class F>
+hipError_t with_mma_shape(long cols, F f) {
+  if (cols > 128) return f(MmaShape<8, 4, 2, 4>{});
+  if (cols > 64) return f(MmaShape<4, 4, 4, 2>{});
+  if (cols > 32) return f(MmaShape<4, 2, 4, 2>{});
+  if (cols > 16) return f(MmaShape<2, 2, 8, 1>{});
+  return f(MmaShape<2, 1, 8, 1>{});
+}
+
 }  // namespace cdclq

@@ -350,6 +350,40 @@ int cdclq_checkpoint_save_device(cdclq_ctx* ctx, const void* x, size_t ldx, size
 int cdclq_checkpoint_restore_device(cdclq_ctx* ctx, const int8_t* codes, const float* scales, size_t t, size_t n,
                                     int dtype, void* out, size_t ldo, void* stream);
 
+/* A packed layer (cdclq-v1 tensors in device memory, gbits on the host) laid out once for products with
+ * activations; the container's tensors, which have to be complete, are not needed afterwards. Opening and
+ * closing allocate, free and wait for the device. perm must be a permutation of 0..d_in. Column groups that are no multiple of 32
+ * are padded to one. cdclq_packed_bytes: device memory it holds. */
+typedef struct cdclq_packed cdclq_packed;
+int cdclq_packed_open_device(cdclq_ctx* ctx, size_t d_out, size_t d_in, size_t group, const uint8_t* gbits,
+                             size_t ngroups, const uint8_t* qweight, size_t qweight_bytes, const uint16_t* scales_f16,
+                             const uint8_t* qzeros, const int32_t* perm_i32, cdclq_packed** out);
+void cdclq_packed_close(cdclq_packed* packed);
+size_t cdclq_packed_bytes(const cdclq_packed* packed);
+
+/* y (t x d_out) = x W^T plus each token's low-rank adapter: y_t = W x_t + scaling[q] B_q (A_q x_t) with
+ * q = request[t], W the packed layer (x in the original column order), A adapters x rank x d_in, B
+ * adapters x d_out x rank (dtype), scaling f32. request[t] = -1: no adapter; any other value outside
+ * 0..adapters gives a NaN row. rank = adapters = 0 leaves the adapters out. rank <= 128; adapters of
+ * smaller rank are padded with zeros. low (t x rank f32, may be NULL) receives A_q x_t for the gradient.
+ * What a token or an adapter holds reaches no other token's or adapter's results, NaN and infinities
+ * included; a token with an infinity may get NaN where the sum is one. The workspace of more than 64
+ * tokens holds the layer in 16 bits. */
+size_t cdclq_adapter_work_bytes(const cdclq_packed* packed, const void* x, size_t ldx, size_t t, const void* a,
+                                const void* b, size_t adapters, size_t rank, int grad);
+int cdclq_adapter_linear_device(cdclq_ctx* ctx, const cdclq_packed* packed, const void* x, size_t ldx, size_t t,
+                                int dtype, const void* a, const void* b, const float* scaling, size_t adapters,
+                                size_t rank, const int32_t* request, void* y, size_t ldy, float* low, void* work,
+                                size_t work_bytes, void* stream);
+/* The gradient for dy (t x d_out): dx (t x d_in), da and db (shaped as A and B, zero for an adapter
+ * without tokens). codes / scales: the input's cdclq_checkpoint_save_device; low: the forward call's.
+ * grad = 1 in cdclq_adapter_work_bytes, with x = dy and ldx = lddy. */
+int cdclq_adapter_backward_device(cdclq_ctx* ctx, const cdclq_packed* packed, const void* dy, size_t lddy, size_t t,
+                                  int dtype, const int8_t* codes, const float* scales, const float* low, const void* a,
+                                  const void* b, const float* scaling, size_t adapters, size_t rank,
+                                  const int32_t* request, void* dx, size_t lddx, void* da, void* db, void* work,
+                                  size_t work_bytes, void* stream);
+
 /* Softmax cross entropy of the logits x w^T (x t x d, w v x d) without the logits in memory:
  * lse[t] = log sum_v exp(x_t . w_v), loss[t] = lse[t] - x_t . w_target. A token whose target is
  * ignore_index has loss = lse = 0 and does not take part, whatever x holds there; any other target

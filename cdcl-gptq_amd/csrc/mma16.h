@@ -7,10 +7,14 @@
 // v_mfma_f32_16x16x32: lane l supplies rows l & 15 at k = 8 (l >> 4) .. + 7 of both operands, and
 // register r of a result is row 4 (l >> 4) + r, column l & 15.
 //
-// Stages of 64 k are loaded straight into LDS (16 bytes a lane) in two buffers: while a stage is
-// multiplied the next one is in flight, one barrier a stage. LDS holds an operand as 16-byte granules,
-//   k contiguous:    granule g of row i at position g ^ (i & 7) of the row's 8: the 16 rows that a
-//                    16-byte read serves together then start in 8 different places of the banks;
+// Stages of 64 k (whole cache lines) are loaded straight into LDS, 16 bytes a lane, in two buffers. The
+// operands of the next 32 k are read from LDS between the MFMAs of these: Q's into a second set of
+// registers, P's each into its own place after its last use. A stage's buffer is therefore free half a
+// stage before its products end, and the loads of the stage after the next go there: they have a whole
+// stage's MFMAs to land. One barrier a stage.
+// LDS holds an operand as 16-byte granules,
+//   k contiguous:    granule g of row i at position g ^ (i >> 1 & 7) of the row's 8: the 16 rows that a
+//                    16-byte read serves together then cover all the banks once;
 //   rows contiguous: granule g of k-row k at position g ^ 2 s(k), s = (k & 3) + 4 (k >> 3 & 1), of
 //                    the row's BP / 8: read by ds_read_b64_tr_b16, which hands lane i of 16 the
 //                    column i of a 4 x 16 block, so that a block's rows start in 8 different places.
@@ -71,15 +75,17 @@ struct MmaTile {
   static constexpr int BP = 16 * FP * WP, BQ = 16 * FQ * WQ, BK = 64;
   static constexpr int STAGE = (BP + BQ) * BK * 2;  // bytes of one stage
   static constexpr int LDS = 2 * STAGE;
-  static constexpr int NP = (BP / 8 + W - 1) / W, NQ = (BQ / 8 + W - 1) / W;  // loads per wavefront and stage
+  static constexpr int GP = BP / 8, GQ = BQ / 8;  // loads of 64 granules a stage
+  static constexpr int NP = (GP + W - 1) / W, NQ = (GQ + W - 1) / W;  // ... of a wavefront, at most
   typedef typename T::v8 v8;
+  static_assert(GP % W == 0, "every wavefront loads as much of P");
   static_assert(!PS || BP >= 128, "the transposed read's swizzle spans 8 pairs of granules");
   static_assert(!QS || BQ >= 128, "the transposed read's swizzle spans 8 pairs of granules");
 
   // Where granule slot `s` of a stage comes from: its offset in k, and its address at k = k0.
   template <bool S, int B>
   static __device__ __forceinline__ int granule_k(int s) {
-    return S ? s / (B / 8) : 8 * ((s & 7) ^ ((s >> 3) & 7));
+    return S ? s / (B / 8) : 8 * ((s & 7) ^ ((s >> 4) & 7));
   }
   template <bool S, int B>
   static __device__ __forceinline__ const uint16_t* granule_at(const MmaOp& o, int r0, int k0, int s) {
@@ -111,85 +117,129 @@ struct MmaTile {
     const int lane = threadIdx.x & 63, wv = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
     const int wp = wv / WQ, wq = wv % WQ;
     if (kbeg >= kend) return;
+    const int stages = max(2, (kend - kbeg + BK - 1) / BK);
     const uint16_t *pp[NP], *pq[NQ];
 #pragma unroll
     for (int i = 0; i < NP; ++i) pp[i] = granule_at<PS, BP>(P, p0, kbeg, 64 * (wv + W * i) + lane);
 #pragma unroll
     for (int i = 0; i < NQ; ++i) pq[i] = granule_at<QS, BQ>(Q, q0, kbeg, 64 * (wv + W * i) + lane);
     const long sp = PS ? BK * P.ld : BK, sq = QS ? BK * Q.ld : BK;
-    const float* const zero = reinterpret_cast<const float*>(&mma_zero_page[0]);
+    const uint16_t* const zero = reinterpret_cast<const uint16_t*>(&mma_zero_page[0]);
+    const bool has_q = GQ % W == 0 || wv < GQ % W;  // takes part in the last load of Q
 
-    auto issue = [&](int k0, uint32_t buf) {
-      const bool whole = k0 + BK <= kend;
-#pragma unroll
-      for (int i = 0; i < NP; ++i) {
-        if (BP / 8 % W && wv + W * i >= BP / 8) break;
-        const float* src = reinterpret_cast<const float*>(pp[i]);
-        if (!whole && k0 + granule_k<PS, BP>(64 * (wv + W * i) + lane) >= kend) src = zero;
-        dma16_untracked(src, buf + 1024u * (wv + W * i));
+    // The loads of the next stage to be loaded, one at a time: 0 .. NP - 1 of P, then Q's.
+    const uint32_t to = lds + 1024u * wv;
+    auto load = [&](uint32_t buf, int i) {
+      if (i < NP) {
+        dma16_untracked(reinterpret_cast<const float*>(pp[i]), to + buf + 1024u * W * i);
         pp[i] += sp;
+      } else if (i < NP + NQ - 1 || has_q) {
+        dma16_untracked(reinterpret_cast<const float*>(pq[i - NP]), to + buf + BP * BK * 2 + 1024u * W * (i - NP));
+        pq[i - NP] += sq;
       }
+    };
+    // Before the loads of stage s: what lies past the end of k comes from the zeros.
+    auto cut = [&](int s) {
+      const int k0 = kbeg + s * BK;
+      if (k0 + BK <= kend) return;
 #pragma unroll
-      for (int i = 0; i < NQ; ++i) {
-        if (BQ / 8 % W && wv + W * i >= BQ / 8) break;
-        const float* src = reinterpret_cast<const float*>(pq[i]);
-        if (!whole && k0 + granule_k<QS, BQ>(64 * (wv + W * i) + lane) >= kend) src = zero;
-        dma16_untracked(src, buf + BP * BK * 2 + 1024u * (wv + W * i));
-        pq[i] += sq;
-      }
+      for (int i = 0; i < NP; ++i)
+        if (k0 + granule_k<PS, BP>(64 * (wv + W * i) + lane) >= kend) pp[i] = zero;
+#pragma unroll
+      for (int i = 0; i < NQ; ++i)
+        if (k0 + granule_k<QS, BQ>(64 * (wv + W * i) + lane) >= kend) pq[i] = zero;
+    };
+    auto issue = [&](int s) {
+      cut(s);
+#pragma unroll
+      for (int i = 0; i < NP + NQ; ++i) load((uint32_t)(s & 1) * STAGE, i);
     };
 
     // read addresses within a stage
     const int r = lane & 15, q = lane >> 4;
-    const uint32_t s = ((lane >> 2) & 3) | ((q & 1) << 2);
-    uint32_t ap[PS ? FP : 2], aq[QS ? FQ : 2];
+    const uint32_t sw = ((lane >> 2) & 3) | ((q & 1) << 2);
+    uint32_t ap[PS ? FP : 2], aq[QS ? FQ : 2];  // k contiguous: of the stage's halves
     if constexpr (PS) {
 #pragma unroll
       for (int f = 0; f < FP; ++f)
-        ap[f] = (8 * q + (r >> 2)) * (BP * 2) + 32 * ((uint32_t)(FP * wp + f) ^ s) + 8 * (lane & 3);
+        ap[f] = lds + (8 * q + (r >> 2)) * (BP * 2) + 32 * ((uint32_t)(FP * wp + f) ^ sw) + 8 * (lane & 3);
     } else {
 #pragma unroll
-      for (int h = 0; h < 2; ++h) ap[h] = (16 * FP * wp + r) * 128 + 16 * ((4 * h + q) ^ (r & 7));
+      for (int h = 0; h < 2; ++h) ap[h] = lds + (16 * FP * wp + r) * 128 + 16 * ((4 * h + q) ^ (r >> 1));
     }
     if constexpr (QS) {
 #pragma unroll
       for (int f = 0; f < FQ; ++f)
-        aq[f] = BP * BK * 2 + (8 * q + (r >> 2)) * (BQ * 2) + 32 * ((uint32_t)(FQ * wq + f) ^ s) + 8 * (lane & 3);
+        aq[f] = lds + BP * BK * 2 + (8 * q + (r >> 2)) * (BQ * 2) + 32 * ((uint32_t)(FQ * wq + f) ^ sw) + 8 * (lane & 3);
     } else {
 #pragma unroll
       for (int h = 0; h < 2; ++h)
-        aq[h] = BP * BK * 2 + (16 * FQ * wq + r) * 128 + 16 * ((4 * h + q) ^ (r & 7));
+        aq[h] = lds + BP * BK * 2 + (16 * FQ * wq + r) * 128 + 16 * ((4 * h + q) ^ (r >> 1));
     }
-
-    uint32_t buf = lds, other = lds + STAGE;
-    issue(kbeg, buf);
-    for (int k0 = kbeg; k0 < kend; k0 += BK) {
-      // this wavefront's part of the stage has landed and its reads of the last one are done; the
-      // barrier says so of every wavefront
-      asm volatile("s_waitcnt vmcnt(0) lgkmcnt(0)\n\ts_barrier" ::: "memory");
-      if (k0 + BK < kend) issue(k0 + BK, other);
+    // block f of half h of the stage in buffer `buf` (0 or STAGE)
+    auto read_p = [&](uint32_t buf, int h, int f) {
+      if constexpr (PS) return read_s<BP>(buf + ap[f] + 32 * h * BP * 2);
+      else return read_c(buf + ap[h] + 2048 * f);
+    };
+    auto read_q = [&](uint32_t buf, int h, int f) {
+      if constexpr (QS) return read_s<BQ>(buf + aq[f] + 32 * h * BQ * 2);
+      else return read_c(buf + aq[h] + 2048 * f);
+    };
+    v8 a[FP], even[FQ], odd[FQ];
+    // Products of 32 k while the operands of half h in `buf` are read; with LOAD the loads of a stage into
+    // `into` go out between them (at once they would fill the memory pipe and hold up what follows).
+    auto step = [&](uint32_t buf, int h, const v8(&cur)[FQ], v8(&next)[FQ], auto loads, uint32_t into) {
+      constexpr bool LOAD = decltype(loads)::value;
+      int n = 0;
+      __builtin_amdgcn_sched_barrier(0);
 #pragma unroll
-      for (int h = 0; h < 2; ++h) {
-        v8 a[FP], b[FQ];
+      for (int f = 0; f < FP; ++f) {
 #pragma unroll
-        for (int f = 0; f < FQ; ++f) {
-          if constexpr (QS) b[f] = read_s<BQ>(buf + aq[f] + 32 * h * BQ * 2);
-          else b[f] = read_c(buf + aq[h] + 2048 * f);
+        for (int g = 0; g < FQ; ++g) {
+          acc[f][g] = T::mfma(a[f], cur[g], acc[f][g]);
+          if (f == 0) {
+            next[g] = read_q(buf, h, g);
+            __builtin_amdgcn_sched_barrier(0);
+          }
         }
+        a[f] = read_p(buf, h, f);
+        if constexpr (LOAD) {
 #pragma unroll
-        for (int f = 0; f < FP; ++f) {
-          if constexpr (PS) a[f] = read_s<BP>(buf + ap[f] + 32 * h * BP * 2);
-          else a[f] = read_c(buf + ap[h] + 2048 * f);
+          for (; n < (NP + NQ) * (f + 1) / FP; ++n) load(into, n);
         }
-#pragma unroll
-        for (int f = 0; f < FP; ++f)
-#pragma unroll
-          for (int g = 0; g < FQ; ++g) acc[f][g] = T::mfma(a[f], b[g], acc[f][g]);
+        __builtin_amdgcn_sched_barrier(0);
       }
-      const uint32_t t = buf;
-      buf = other;
-      other = t;
+    };
+    constexpr std::true_type with_loads{};
+    constexpr std::false_type no_loads{};
+    issue(0);
+    issue(1);
+    if (has_q) wait_vmcnt<NP + NQ>();
+    else wait_vmcnt<NP + NQ - 1>();
+    asm volatile("s_barrier" ::: "memory");
+#pragma unroll
+    for (int g = 0; g < FQ; ++g) even[g] = read_q(0, 0, g);
+#pragma unroll
+    for (int f = 0; f < FP; ++f) a[f] = read_p(0, 0, f);
+    // this wavefront is done reading a stage and its part of the next one has landed; the barrier says so
+    // of every wavefront
+    auto turn = [&]() { asm volatile("s_waitcnt vmcnt(0) lgkmcnt(0)\n\ts_barrier" ::: "memory"); };
+    uint32_t buf = 0;
+    for (int s = 2; s < stages; ++s) {
+      step(buf, 1, even, odd, no_loads, 0u);
+      turn();
+      cut(s);
+      step(buf ^ STAGE, 0, odd, even, with_loads, buf);
+      buf ^= STAGE;
     }
+    step(buf, 1, even, odd, no_loads, 0u);
+    turn();
+    step(buf ^ STAGE, 0, odd, even, no_loads, 0u);
+    step(buf ^ STAGE, 1, even, odd, no_loads, 0u);
+#pragma unroll
+    for (int f = 0; f < FP; ++f)
+#pragma unroll
+      for (int g = 0; g < FQ; ++g) acc[f][g] = T::mfma(a[f], odd[g], acc[f][g]);
     asm volatile("s_waitcnt lgkmcnt(0)\n\ts_barrier" ::: "memory");  // the shared memory is free again
   }
   static __device__ __forceinline__ void clear(mma_f4 (&acc)[FP][FQ]) {

@@ -533,7 +533,7 @@ hipError_t shrink(hipStream_t st, const uint16_t* x, long ldx, long t, int k, co
 template <class T, bool PS>
 hipError_t wide_product(hipStream_t st, WideArgs w) {
   w.vec = w.ldo % 4 == 0 && (uintptr_t)w.out % 8 == 0;
-  return with_mma_shape(w.t, [&](auto s) {
+  return with_mma_shape(mma_pick(w.rows, w.t, w.k), [&](auto s) {
     typedef decltype(s) S;
     w.np = (w.rows + S::bp - 1) / S::bp;
     w.nq = (w.t + S::bq - 1) / S::bq;

@@ -73,45 +73,97 @@ __global__ __launch_bounds__(1024) void k_loss_tokens(const int64_t* __restrict_
   }
 }
 
-// Rows idx[0 .. count) of x into rows of dp elements, zeros past d; and per packed token what the tiles
-// need: its target, and for the gradient lse and the scaled weight.
+// What the tiles need of a packed token: its target, and for the gradient lse and the scaled weight.
 struct LossTok {
   int target;  // -1: outside the vocabulary
   float lse, weight;
   int pad;
 };
-__global__ __launch_bounds__(256) void k_loss_gather(const uint16_t* __restrict__ x, long ldx, int d, int dp,
-                                                     const int* __restrict__ idx, const uint32_t* __restrict__ info,
-                                                     const int64_t* __restrict__ y, int v,
-                                                     const float* __restrict__ lse, const float* __restrict__ g,
-                                                     float gscale, uint16_t* __restrict__ xc,
-                                                     LossTok* __restrict__ tok, float* __restrict__ hit, int vec) {
-  const int i = blockIdx.x;
-  if (i >= (int)info[0]) return;
-  const int t = idx[i];
-  const uint16_t* src = x + (long)t * ldx;
-  uint16_t* dst = xc + (long)i * dp;
-  if (vec) {
-    for (int c = 8 * threadIdx.x; c < dp; c += 2048)
+struct GatherArgs {
+  const uint16_t* x;
+  long ldx;
+  int d, dp, vec;
+  const int64_t* y;
+  int v;
+  const float *lse, *g;  // gradient
+  float gscale;
+  uint16_t* xc;
+  LossTok* tok;
+  float* hit;  // forward
+};
+// Token t as the i-th packed one: its row of x in dp elements, zeros past d, and its LossTok.
+__device__ __forceinline__ void gather_token(const GatherArgs& k, int t, int i, float top) {
+  const uint16_t* src = k.x + (long)t * k.ldx;
+  uint16_t* dst = k.xc + (long)i * k.dp;
+  if (k.vec) {
+    for (int c = 8 * threadIdx.x; c < k.dp; c += 2048)
       *reinterpret_cast<uint4*>(dst + c) = *reinterpret_cast<const uint4*>(src + c);
   } else {
-    for (int c = threadIdx.x; c < dp; c += 256) dst[c] = c < d ? src[c] : (uint16_t)0;
+    for (int c = threadIdx.x; c < k.dp; c += 256) dst[c] = c < k.d ? src[c] : (uint16_t)0;
   }
   if (threadIdx.x == 0) {
-    const int64_t k = y[t];
+    const int64_t y = k.y[t];
     LossTok o;
-    o.target = k >= 0 && k < v ? (int)k : -1;
-    o.lse = lse ? lse[t] : 0.0f;
+    o.target = y >= 0 && y < k.v ? (int)y : -1;
+    o.lse = k.lse ? k.lse[t] : 0.0f;
     o.weight = 0.0f;
-    if (g) {
-      const float top = __uint_as_float(info[1]);
-      o.weight = top > 0.0f ? g[t] / top * gscale : g[t];
+    if (k.g) {
+      o.weight = top > 0.0f ? k.g[t] / top * k.gscale : k.g[t];
       if (o.target < 0) o.weight = __builtin_nanf("");
     }
     o.pad = 0;
-    tok[i] = o;
-    if (hit) hit[i] = __builtin_nanf("");  // replaced by the tile that holds the target
+    k.tok[i] = o;
+    if (k.hit) k.hit[i] = __builtin_nanf("");  // replaced by the tile that holds the target
   }
+}
+__global__ __launch_bounds__(256) void k_loss_gather(GatherArgs k, const int* __restrict__ idx,
+                                                     const uint32_t* __restrict__ info) {
+  const int i = blockIdx.x;
+  if (i < (int)info[0]) gather_token(k, idx[i], i, __uint_as_float(info[1]));
+}
+// Both of the above in one launch for few tokens: every workgroup (one a token) counts for itself, t / 256
+// tokens a thread, which costs less than a launch up to kCountTokens.
+constexpr int kCountTokens = 2048;
+__global__ __launch_bounds__(256) void k_loss_pack(GatherArgs k, long ignore, int t, int* __restrict__ idx,
+                                                   int* __restrict__ pos, uint32_t* __restrict__ info,
+                                                   float* __restrict__ loss, float* __restrict__ lse) {
+  __shared__ int wbefore[4], wall[4];
+  __shared__ float wtop[4];
+  const int i = blockIdx.x, lane = threadIdx.x & 63, wv = threadIdx.x >> 6;
+  int before = 0, all = 0;
+  float top = 0.0f;
+  for (int j = threadIdx.x; j < t; j += 256) {
+    if (k.y[j] == ignore) continue;
+    ++all;
+    before += j < i;
+    if (k.g) {
+      const float a = __builtin_fabsf(k.g[j]);
+      if (a < __builtin_inff()) top = fmaxf(top, a);
+    }
+  }
+#pragma unroll
+  for (int s = 32; s; s >>= 1) {
+    before += __shfl_xor(before, s);
+    all += __shfl_xor(all, s);
+    top = fmaxf(top, __shfl_xor(top, s));
+  }
+  if (lane == 0) wbefore[wv] = before, wall[wv] = all, wtop[wv] = top;
+  __syncthreads();
+  before = wbefore[0] + wbefore[1] + wbefore[2] + wbefore[3];
+  all = wall[0] + wall[1] + wall[2] + wall[3];
+  top = fmaxf(fmaxf(wtop[0], wtop[1]), fmaxf(wtop[2], wtop[3]));
+  if (i == 0 && threadIdx.x == 0) {
+    info[0] = all;
+    info[1] = __float_as_uint(top);
+  }
+  const bool on = k.y[i] != ignore;
+  if (threadIdx.x == 0) {
+    if (on) idx[before] = i;
+    if (pos) pos[i] = on ? before : -1;
+    if (!on && loss) loss[i] = 0.0f;
+    if (!on && lse) lse[i] = 0.0f;
+  }
+  if (on) gather_token(k, i, before, top);
 }
 
 // 16-bit rows of `cols` elements into rows of dp, zeros past cols (operands that the tiles cannot read)
@@ -170,13 +222,14 @@ __global__ __launch_bounds__(64 * WP * WQ, 2) void k_loss_tiles(const uint16_t* 
   }
 }
 
-// Joins the slabs of 16 tokens: thread (token, j) takes slabs j, j + 16, ..., then 16 threads join.
+// Joins the slabs of 8 tokens: thread (token, j) takes slabs j, j + 32, ..., eight loads in flight.
 __global__ __launch_bounds__(256) void k_loss_combine(const float2* __restrict__ part, int ldpart, int nslabs,
                                                       const uint32_t* __restrict__ info, const int* __restrict__ idx,
                                                       const float* __restrict__ hit, float* __restrict__ loss,
                                                       float* __restrict__ lse) {
-  const int count = (int)info[0], i = blockIdx.x * 16 + (threadIdx.x & 15), j = threadIdx.x >> 4;
-  __shared__ float2 red[256];
+  const int count = (int)info[0], i = blockIdx.x * 8 + (threadIdx.x & 7), j = threadIdx.x >> 3;
+  if ((int)blockIdx.x * 8 >= count) return;
+  __shared__ float2 red[4][8];
   float m = -__builtin_inff(), s = 0.0f;
   auto join = [&](float m2, float s2) {
     const float n = fmaxf(m, m2);
@@ -187,18 +240,22 @@ __global__ __launch_bounds__(256) void k_loss_combine(const float2* __restrict__
       s += s2;  // nothing yet, or NaN
     }
   };
-  if (i < count)
-    for (int k = j; k < nslabs; k += 16) {
-      const float2 p = part[(long)k * ldpart + i];
-      join(p.x, p.y);
-    }
-  red[threadIdx.x] = make_float2(m, s);
+  const int at = min(i, count - 1);
+  for (int k = j; k < nslabs; k += 256) {
+    float2 p[8];
+#pragma unroll
+    for (int u = 0; u < 8; ++u)
+      p[u] = k + 32 * u < nslabs ? part[(long)(k + 32 * u) * ldpart + at] : make_float2(-__builtin_inff(), 0.0f);
+#pragma unroll
+    for (int u = 0; u < 8; ++u) join(p[u].x, p[u].y);
+  }
+#pragma unroll
+  for (int x = 8; x < 64; x <<= 1) join(__shfl_xor(m, x), __shfl_xor(s, x));
+  if ((threadIdx.x & 63) < 8) red[threadIdx.x >> 6][threadIdx.x & 7] = make_float2(m, s);
   __syncthreads();
   if (j == 0 && i < count) {
-    for (int k = 1; k < 16; ++k) {
-      const float2 p = red[k * 16 + threadIdx.x];
-      join(p.x, p.y);
-    }
+#pragma unroll
+    for (int w = 1; w < 4; ++w) join(red[w][threadIdx.x].x, red[w][threadIdx.x].y);
     const float l = m + logf(s);
     lse[idx[i]] = l;
     loss[idx[i]] = l - hit[i];
@@ -316,22 +373,26 @@ __global__ __launch_bounds__(64 * WP * WQ, 2) void k_loss_dw(const uint16_t* __r
 template <class T>
 __global__ __launch_bounds__(256) void k_loss_dx_out(const float* __restrict__ dxacc, int splits, int t, int d, int dp,
                                                      const int* __restrict__ pos, const uint32_t* __restrict__ info,
-                                                     float gscale, uint16_t* __restrict__ dx, long lddx) {
+                                                     float gscale, uint16_t* __restrict__ dx, long lddx, int vec) {
   const float top = __uint_as_float(info[1]), k = (top > 0.0f ? top : 1.0f) / gscale;
-  const long total = (long)t * dp;
-  for (long e = blockIdx.x * 256l + threadIdx.x; e * 8 < total; e += gridDim.x * 256l) {
-    const int i = (int)(e * 8 / dp), c = (int)(e * 8 - (long)i * dp), at = pos[i];
-    float s[8] = {};
-    if (at >= 0)
-      for (int j = 0; j < splits; ++j) {
-        const float* a = dxacc + ((long)j * t + at) * dp + c;
-#pragma unroll
-        for (int r = 0; r < 8; ++r) s[r] += a[r];
-      }
+  const long total = (long)t * dp / 4;
+  for (long e = blockIdx.x * 256l + threadIdx.x; e < total; e += gridDim.x * 256l) {
+    const int i = (int)(4 * e / dp), c = (int)(4 * e - (long)i * dp), at = pos[i];
+    mma_f4 s = {};
+    if (at >= 0) {
+      const float* a = dxacc + (long)at * dp + c;
+#pragma unroll 8
+      for (int j = 0; j < splits; ++j) s += *reinterpret_cast<const mma_f4*>(a + (long)j * t * dp);
+    }
+    s *= k;
     uint16_t* o = dx + (long)i * lddx + c;
+    if (vec) {
+      *reinterpret_cast<uint2*>(o) = make_uint2(narrow2<T>(s[0], s[1]), narrow2<T>(s[2], s[3]));
+    } else {
 #pragma unroll
-    for (int r = 0; r < 8; ++r)
-      if (c + r < d) o[r] = T::narrow(s[r] * k);
+      for (int r = 0; r < 4; ++r)
+        if (c + r < d) o[r] = T::narrow(s[r]);
+    }
   }
 }
 
@@ -361,11 +422,12 @@ LossPlan loss_plan(long t, long d, long v, bool pad_w, bool grad) {
   p.xc = take(2 * (size_t)t * p.dp);
   p.wpad = pad_w ? take(2 * (size_t)v * p.dp) : 0;
   if (!grad) {
-    (void)with_mma_shape(t, [&](auto s) {
+    p.tiles = mma_pick(v, t, p.dp);
+    (void)with_mma_shape(p.tiles, [&](auto s) {
       p.slab = 16 * s.fp;
+      p.nslabs = (int)(up(v, s.bp) / p.slab);
       return hipSuccess;
     });
-    p.nslabs = (int)(up(v, 256) / p.slab);
     p.hit = take(4 * t);
     p.part = take(sizeof(float2) * (size_t)t * p.nslabs);
   } else {
@@ -374,16 +436,17 @@ LossPlan loss_plan(long t, long d, long v, bool pad_w, bool grad) {
     const size_t rows = up(v, 256), most = std::max<size_t>(256, ((size_t)128 << 20) / t / 256 * 256);
     p.pieces = (int)((rows + most - 1) / most);
     p.piece = (int)up((rows + p.pieces - 1) / p.pieces, 256);
-    // a small dx is split over the vocabulary until about one round of workgroups works on it
-    int bq = 256;
-    (void)with_mma_shape(t, [&](auto s) {
-      bq = s.bq;
-      return hipSuccess;
-    });
-    const long tiles = (long)(up(d, 256) / 256) * (long)((t + bq - 1) / bq);
-    const long want = std::max(1l, std::min(256 / tiles, (long)p.piece / 512));
-    p.share = (int)up((p.piece + want - 1) / want, 64);
+    p.tiles = mma_pick(std::min<long>(p.piece, v), t, p.dp);
+    // a small dx is split over the vocabulary; its f32 parts are written and read at about 2100 bytes a clock
+    double best = 0;
+    for (int i = 0; i < kMmaShapes; ++i)
+      for (long n = 1; n == 1 || n <= std::min(64, p.piece / 512); n *= 2) {
+        const double c = mma_cost(p.dp, t, p.piece, i, n) + n * (8.0 / 2100) * t * p.dp;
+        if ((i == 0 && n == 1) || c < best) best = c, p.dx_tiles = i, p.splits = (int)n;
+      }
+    p.share = (int)up((p.piece + p.splits - 1) / p.splits, 64);
     p.splits = (p.piece + p.share - 1) / p.share;
+    p.dw_tiles = mma_cost(p.dp, p.piece, t, 5, 1) < mma_cost(p.dp, p.piece, t, 0, 1) ? 5 : 0;
     p.d = take(2 * (size_t)t * p.piece);
     p.dxacc = take(4 * (size_t)t * p.dp * p.splits);
   }
@@ -397,16 +460,19 @@ namespace {
 hipError_t prepare(hipStream_t st, const LossArgs& a, const LossPlan& p, float gscale, const uint16_t** w, long* ldw) {
   char* ws = static_cast<char*>(a.work);
   const bool grad = a.dx || a.dw;
-  k_loss_tokens<<<1, 1024, 0, st>>>(a.targets, a.ignore, (int)a.t, a.dloss, reinterpret_cast<int*>(ws + p.idx),
-                                    grad ? reinterpret_cast<int*>(ws + p.pos) : nullptr,
-                                    reinterpret_cast<uint32_t*>(ws + p.info), grad ? nullptr : a.loss,
-                                    grad ? nullptr : a.lse_out);
   const int vec = a.d % 8 == 0 && a.ldx % 8 == 0 && (uintptr_t)a.x % 16 == 0;
-  if (a.t) k_loss_gather<<<(int)a.t, 256, 0, st>>>(a.x, a.ldx, (int)a.d, p.dp, reinterpret_cast<int*>(ws + p.idx),
-                                          reinterpret_cast<uint32_t*>(ws + p.info), a.targets, (int)a.v, a.lse_in,
-                                          a.dloss, gscale, reinterpret_cast<uint16_t*>(ws + p.xc),
-                                          reinterpret_cast<LossTok*>(ws + p.tok),
-                                          grad ? nullptr : reinterpret_cast<float*>(ws + p.hit), vec);
+  int *idx = reinterpret_cast<int*>(ws + p.idx), *pos = grad ? reinterpret_cast<int*>(ws + p.pos) : nullptr;
+  uint32_t* info = reinterpret_cast<uint32_t*>(ws + p.info);
+  float *loss = grad ? nullptr : a.loss, *lse = grad ? nullptr : a.lse_out;
+  const GatherArgs k = {a.x, a.ldx, (int)a.d, p.dp, vec, a.targets, (int)a.v, a.lse_in, a.dloss, gscale,
+                        reinterpret_cast<uint16_t*>(ws + p.xc), reinterpret_cast<LossTok*>(ws + p.tok),
+                        grad ? nullptr : reinterpret_cast<float*>(ws + p.hit)};
+  if (a.t > 0 && a.t <= kCountTokens) {
+    k_loss_pack<<<(int)a.t, 256, 0, st>>>(k, a.ignore, (int)a.t, idx, pos, info, loss, lse);
+  } else {
+    k_loss_tokens<<<1, 1024, 0, st>>>(a.targets, a.ignore, (int)a.t, a.dloss, idx, pos, info, loss, lse);
+    if (a.t) k_loss_gather<<<(int)a.t, 256, 0, st>>>(k, idx, info);
+  }
   *w = a.w;
   *ldw = a.ldw;
   if (p.wpad) {
@@ -425,7 +491,7 @@ hipError_t forward(hipStream_t st, const LossArgs& a, const LossPlan& p) {
   long ldw;
   hipError_t e = prepare(st, a, p, 1.0f, &w, &ldw);
   if (e != hipSuccess) return e;
-  e = with_mma_shape(a.t, [&](auto s) {
+  e = with_mma_shape(p.tiles, [&](auto s) {
     typedef decltype(s) S;
     const int np = (int)((a.v + S::bp - 1) / S::bp), nq = (int)((a.t + S::bq - 1) / S::bq);
     k_loss_tiles<T, S::fp, S::fq, S::wp, S::wq><<<np * nq, S::threads, 0, st>>>(
@@ -435,7 +501,7 @@ hipError_t forward(hipStream_t st, const LossArgs& a, const LossPlan& p) {
     return hipGetLastError();
   });
   if (e != hipSuccess) return e;
-  k_loss_combine<<<(int)((a.t + 15) / 16), 256, 0, st>>>(
+  k_loss_combine<<<(int)((a.t + 7) / 8), 256, 0, st>>>(
       reinterpret_cast<float2*>(ws + p.part), (int)a.t, p.nslabs, reinterpret_cast<uint32_t*>(ws + p.info),
       reinterpret_cast<int*>(ws + p.idx), reinterpret_cast<float*>(ws + p.hit), a.loss, a.lse_out);
   return hipGetLastError();
@@ -459,31 +525,40 @@ hipError_t backward(hipStream_t st, const LossArgs& a, const LossPlan& p) {
     const int v0 = i * p.piece;
     if (v0 >= v) break;
     const int rows = std::min(p.piece, v - v0);
-    if (t) e = with_mma_shape(t, [&](auto s) {
-      typedef decltype(s) S;
-      const int nq = (t + S::bq - 1) / S::bq, np = (rows + S::bp - 1) / S::bp;
-      k_loss_d<T, S::fp, S::fq, S::wp, S::wq><<<np * nq, S::threads, 0, st>>>(w, ldw, v, v0, xc, p.dp, info, np,
-                                                                                      nq, tok, d, p.piece);
-      hipError_t e1 = hipGetLastError();
-      if (e1 != hipSuccess) return e1;
-      const int npx = (p.dp + S::bp - 1) / S::bp;
-      k_loss_dx<T, S::fp, S::fq, S::wp, S::wq><<<npx * nq * p.splits, S::threads, 0, st>>>(
-          w, ldw, p.dp, v0, rows, p.share, d, p.piece, info, npx, nq, t, p.dp, i > 0, dxacc);
-      return hipGetLastError();
-    });
-    if (e != hipSuccess) return e;
+    if (t) {
+      e = with_mma_shape(p.tiles, [&](auto s) {
+        typedef decltype(s) S;
+        const int nq = (t + S::bq - 1) / S::bq, np = (rows + S::bp - 1) / S::bp;
+        k_loss_d<T, S::fp, S::fq, S::wp, S::wq><<<np * nq, S::threads, 0, st>>>(w, ldw, v, v0, xc, p.dp, info, np, nq,
+                                                                                tok, d, p.piece);
+        return hipGetLastError();
+      });
+      if (e != hipSuccess) return e;
+      e = with_mma_shape(p.dx_tiles, [&](auto s) {
+        typedef decltype(s) S;
+        const int nq = (t + S::bq - 1) / S::bq, np = (p.dp + S::bp - 1) / S::bp;
+        k_loss_dx<T, S::fp, S::fq, S::wp, S::wq><<<np * nq * p.splits, S::threads, 0, st>>>(
+            w, ldw, p.dp, v0, rows, p.share, d, p.piece, info, np, nq, t, p.dp, i > 0, dxacc);
+        return hipGetLastError();
+      });
+      if (e != hipSuccess) return e;
+    }
     if (a.dw) {
-      typedef MmaShape<8, 4, 2, 4> S;
-      const int np = (p.dp + S::bp - 1) / S::bp, nq = (rows + S::bq - 1) / S::bq;
       const int vec = a.lddw % 4 == 0 && a.d % 4 == 0 && (uintptr_t)a.dw % 8 == 0;
-      k_loss_dw<T, S::fp, S::fq, S::wp, S::wq><<<np * nq, S::threads, 0, st>>>(
-          xc, p.dp, (int)a.d, d, p.piece, rows, info, np, nq, gscale, a.dw + (long)v0 * a.lddw, a.lddw, vec);
-      e = hipGetLastError();
+      auto go = [&](auto s) {
+        typedef decltype(s) S;
+        const int np = (p.dp + S::bp - 1) / S::bp, nq = (rows + S::bq - 1) / S::bq;
+        k_loss_dw<T, S::fp, S::fq, S::wp, S::wq><<<np * nq, S::threads, 0, st>>>(
+            xc, p.dp, (int)a.d, d, p.piece, rows, info, np, nq, gscale, a.dw + (long)v0 * a.lddw, a.lddw, vec);
+        return hipGetLastError();
+      };
+      e = p.dw_tiles == 5 ? go(MmaShape<4, 4, 2, 2>{}) : go(MmaShape<8, 4, 2, 4>{});
       if (e != hipSuccess) return e;
     }
   }
-  if (t) k_loss_dx_out<T><<<blocks_for((long)t * p.dp, 8 * 256), 256, 0, st>>>(
-      dxacc, p.splits, t, (int)a.d, p.dp, reinterpret_cast<int*>(ws + p.pos), info, gscale, a.dx, a.lddx);
+  const int vec = a.lddx % 4 == 0 && a.d % 4 == 0 && p.dp == a.d && (uintptr_t)a.dx % 8 == 0;
+  if (t) k_loss_dx_out<T><<<blocks_for((long)t * p.dp, 4 * 256), 256, 0, st>>>(
+      dxacc, p.splits, t, (int)a.d, p.dp, reinterpret_cast<int*>(ws + p.pos), info, gscale, a.dx, a.lddx, vec);
   return hipGetLastError();
 }
 

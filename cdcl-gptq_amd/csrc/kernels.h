@@ -289,6 +289,7 @@ struct LossArgs {
 struct LossPlan {
   size_t bytes, info, idx, pos, tok, xc, wpad, hit, part, d, dxacc;  // offsets into the workspace
   int dp, slab, nslabs, pieces, piece, share, splits;
+  int tiles, dx_tiles, dw_tiles;  // tile shapes (mma16.h)
 };
 // pad_w: W's rows are not 16-byte aligned (loss_pads_w)
 LossPlan loss_plan(long t, long d, long v, bool pad_w, bool grad);

@@ -5,16 +5,19 @@
 //   dA_q = sum_t u_t x^_t^T  dB_q = s_q sum_t dy_t low_t^T     (x^: the 8-bit checkpoint of x)
 //
 // W is expanded to 16 bits in the caller's workspace and multiplied by the tiles of mma16.h; it is
-// bound by those products. The low-rank terms ride along: `shrink` makes low (or u) with the rank as the
-// MFMA rows, and the product's epilogue adds B low (A^T u) to its own registers. Tokens keep their order:
-// a fragment of 16 tokens goes through the distinct adapters among them, one in all but the fragments
-// where requests meet, and a token takes only its own adapter's result, so that what another adapter
-// holds cannot reach it. low and u enter the matrix cores as the sum of two 16-bit values of a vector
-// scaled to [0.5, 1): about 16 bits of it are kept.
+// bound by those products, split in k where few tiles would leave CUs idle. The low-rank terms ride
+// along: `shrink` makes low (or u) with the rank as the MFMA rows, and the product's epilogue adds B low
+// (A^T u) to its own registers. Tokens keep their order: a fragment of 16 tokens goes through the distinct
+// adapters among them, one in all but the fragments where requests meet, and a token takes only its own
+// adapter's result, so that what another adapter holds cannot reach it. low and u enter the matrix cores as
+// the sum of two 16-bit values of a vector scaled to [0.5, 1): about 16 bits of it are kept.
 //
-// dA and dB sum over the tokens of an adapter: lists in token order, items of at most `chunk` tokens with
+// dA and dB sum over the tokens of an adapter: lists in token order, items of at most 256 tokens with
 // f32 sums of their own, joined in order (no atomics). dA reads the codes of the checkpoint, exact in
 // bf16, the scale of token and block going into u.
+//
+// Everything that waits for nothing runs in one launch (`prepare`), every last step in another (`finish`):
+// a small step is bound by launches.
 #include <hip/hip_runtime.h>
 
 #include <algorithm>
@@ -31,33 +34,53 @@ inline int blocks_for(long items, int per, int most = 1 << 20) {
   return (int)std::max(1l, std::min((items + per - 1) / per, (long)most));
 }
 
-// 16-bit rows of `cols` elements into rows of dp, zeros past cols
-__global__ __launch_bounds__(256) void k_pad_rows16(const uint16_t* __restrict__ src, long ld, int cols, int dp,
-                                                    long rows, uint16_t* __restrict__ dst) {
-  const long total = rows * dp;
-  for (long i = blockIdx.x * 256l + threadIdx.x; i < total; i += gridDim.x * 256l) {
-    const long r = i / dp;
-    const int c = (int)(i - r * dp);
-    dst[i] = c < cols ? src[r * ld + c] : (uint16_t)0;
+// ---- parts of `prepare`, each by workgroups of 256 threads, b of nb
+
+// 16-bit rows of `cols` elements into rows of dp (a multiple of 8), zeros past cols
+struct PadJob {
+  const uint16_t* src;
+  long ld;
+  int cols, dp;
+  long rows;
+  uint16_t* dst;
+};
+__device__ void pad_rows16(const PadJob& j, long b, long nb) {
+  const int per = j.dp / 8;
+  const long total = j.rows * per;
+  for (long i = b * 256 + threadIdx.x; i < total; i += nb * 256) {
+    const long r = i / per;
+    const int c = 8 * (int)(i - r * per);
+    const uint16_t* src = j.src + r * j.ld + c;
+    uint16_t v[8];
+    if (c + 8 <= j.cols) {
+      __builtin_memcpy(v, src, 16);
+    } else {
+#pragma unroll
+      for (int k = 0; k < 8; ++k) v[k] = c + k < j.cols ? src[k] : (uint16_t)0;
+    }
+    *reinterpret_cast<uint4*>(j.dst + r * j.dp + c) = *reinterpret_cast<const uint4*>(v);
   }
 }
 
-// Activations into slot order, zeros in empty slots: R rows at a time through LDS (LDS = 0: straight from
+// Activations into slot order, zeros in empty slots: `rows` of them at a time through LDS (0: straight from
 // memory, rows too long for it).
-template <int R>
-__global__ __launch_bounds__(256) void k_to_slots(PackedView v, const uint16_t* __restrict__ x, long ldx, long t,
-                                                  uint16_t* __restrict__ xp, int vec) {
-  extern __shared__ __align__(16) uint16_t rows[];
-  const long t0 = (long)blockIdx.x * (R ? R : 1);
-  const int ns = packed_slots(v), stride = (int)((v.n + 7) & ~7);
-  if constexpr (R > 0) {
-    for (int r = 0; r < R && t0 + r < t; ++r) {
-      const uint16_t* src = x + (t0 + r) * ldx;
-      if (vec) {
+struct SlotJob {
+  const uint16_t* x;
+  long ldx;
+  int t, rows, vec;
+  uint16_t* xp;
+};
+__device__ void to_slots(const PackedView& v, const SlotJob& j, uint16_t* lds, long b) {
+  const int n = j.rows ? j.rows : 1, ns = packed_slots(v), stride = (v.n + 7) & ~7;
+  const long t0 = b * n;
+  if (j.rows) {
+    for (int r = 0; r < n && t0 + r < j.t; ++r) {
+      const uint16_t* src = j.x + (t0 + r) * j.ldx;
+      if (j.vec) {
         for (int c = 8 * threadIdx.x; c < v.n; c += 2048)
-          *reinterpret_cast<uint4*>(rows + r * stride + c) = *reinterpret_cast<const uint4*>(src + c);
+          *reinterpret_cast<uint4*>(lds + r * stride + c) = *reinterpret_cast<const uint4*>(src + c);
       } else {
-        for (int c = threadIdx.x; c < v.n; c += 256) rows[r * stride + c] = src[c];
+        for (int c = threadIdx.x; c < v.n; c += 256) lds[r * stride + c] = src[c];
       }
     }
     __syncthreads();
@@ -65,81 +88,185 @@ __global__ __launch_bounds__(256) void k_to_slots(PackedView v, const uint16_t* 
   for (int s = 8 * threadIdx.x; s < ns; s += 2048) {
     const int4 c0 = *reinterpret_cast<const int4*>(v.col + s), c1 = *reinterpret_cast<const int4*>(v.col + s + 4);
     const int c[8] = {c0.x, c0.y, c0.z, c0.w, c1.x, c1.y, c1.z, c1.w};
-    for (int r = 0; r < (R ? R : 1) && t0 + r < t; ++r) {
-      const uint16_t* src = R ? rows + r * stride : x + (t0 + r) * ldx;
+    for (int r = 0; r < n && t0 + r < j.t; ++r) {
+      const uint16_t* src = j.rows ? lds + r * stride : j.x + (t0 + r) * j.ldx;
       uint32_t o[4];
 #pragma unroll
       for (int i = 0; i < 4; ++i)
         o[i] = (c[2 * i] >= 0 ? src[c[2 * i]] : 0u) | ((c[2 * i + 1] >= 0 ? (uint32_t)src[c[2 * i + 1]] : 0u) << 16);
-      *reinterpret_cast<uint4*>(xp + (t0 + r) * ns + s) = make_uint4(o[0], o[1], o[2], o[3]);
-    }
-  }
-}
-// ... and back to columns
-template <int R>
-__global__ __launch_bounds__(256) void k_from_slots(PackedView v, const uint16_t* __restrict__ xp, long t,
-                                                    uint16_t* __restrict__ x, long ldx, int vec) {
-  extern __shared__ __align__(16) uint16_t rows[];
-  const long t0 = (long)blockIdx.x * (R ? R : 1);
-  const int ns = packed_slots(v), stride = (int)((v.n + 7) & ~7);
-  for (int s = 8 * threadIdx.x; s < ns; s += 2048) {
-    const int4 c0 = *reinterpret_cast<const int4*>(v.col + s), c1 = *reinterpret_cast<const int4*>(v.col + s + 4);
-    const int c[8] = {c0.x, c0.y, c0.z, c0.w, c1.x, c1.y, c1.z, c1.w};
-    for (int r = 0; r < (R ? R : 1) && t0 + r < t; ++r) {
-      uint16_t in[8];
-      *reinterpret_cast<uint4*>(in) = *reinterpret_cast<const uint4*>(xp + (t0 + r) * ns + s);
-      uint16_t* dst = R ? rows + r * stride : x + (t0 + r) * ldx;
-#pragma unroll
-      for (int i = 0; i < 8; ++i)
-        if (c[i] >= 0) dst[c[i]] = in[i];
-    }
-  }
-  if constexpr (R > 0) {
-    __syncthreads();
-    for (int r = 0; r < R && t0 + r < t; ++r) {
-      uint16_t* dst = x + (t0 + r) * ldx;
-      if (vec) {
-        for (int c = 8 * threadIdx.x; c < v.n; c += 2048)
-          *reinterpret_cast<uint4*>(dst + c) = *reinterpret_cast<const uint4*>(rows + r * stride + c);
-      } else {
-        for (int c = threadIdx.x; c < v.n; c += 256) dst[c] = rows[r * stride + c];
-      }
+      *reinterpret_cast<uint4*>(j.xp + (t0 + r) * ns + s) = make_uint4(o[0], o[1], o[2], o[3]);
     }
   }
 }
 
 // bt[adapter][j][i] = b[adapter][i][j], rows padded to mp with zeros
-__global__ __launch_bounds__(256) void k_transpose_b(const uint16_t* __restrict__ b, int adapters, int m, int rank,
-                                                     int mp, uint16_t* __restrict__ bt) {
-  const long total = (long)adapters * mp;
-  for (long e = blockIdx.x * 256l + threadIdx.x; e < total; e += gridDim.x * 256l) {
-    const long q = e / mp;
-    const int i = (int)(e - q * mp);
-    const uint16_t* src = b + (q * m + i) * rank;
-    uint16_t* dst = bt + q * rank * mp + i;
-    for (int j = 0; j < rank; ++j) dst[(long)j * mp] = i < m ? src[j] : (uint16_t)0;
+__device__ void transpose_b(const uint16_t* src0, int adapters, int m, int rank, int mp, uint16_t* bt, long b, long nb) {
+  const int groups = (rank + 7) / 8;
+  const long total = (long)adapters * groups * mp;
+  for (long e = b * 256 + threadIdx.x; e < total; e += nb * 256) {
+    const long qg = e / mp, q = qg / groups;
+    const int i = (int)(e - qg * mp), j0 = 8 * (int)(qg - q * groups);
+    const uint16_t* src = src0 + (q * m + i) * rank + j0;
+    uint16_t* dst = bt + (q * rank + j0) * mp + i;
+    uint16_t v[8];
+    if (i < m && j0 + 8 <= rank) {
+      __builtin_memcpy(v, src, 16);
+    } else {
+#pragma unroll
+      for (int k = 0; k < 8; ++k) v[k] = i < m && j0 + k < rank ? src[k] : (uint16_t)0;
+    }
+#pragma unroll
+    for (int k = 0; k < 8; ++k)
+      if (j0 + k < rank) dst[(long)k * mp] = v[k];
   }
 }
 // at[adapter][slot][j] = a[adapter][j][column of slot], zeros in empty slots and past the rank
-__global__ __launch_bounds__(256) void k_transpose_a(PackedView v, const uint16_t* __restrict__ a, int adapters,
-                                                     int rank, int rp, uint16_t* __restrict__ at) {
-  const int ns = packed_slots(v);
-  const long total = (long)adapters * ns;
-  for (long e = blockIdx.x * 256l + threadIdx.x; e < total; e += gridDim.x * 256l) {
-    const long q = e / ns;
-    const int c = v.col[e - q * ns];
-    const uint16_t* src = a + q * rank * v.n + c;
-    for (int j = 0; j < rp; j += 8) {
-      uint32_t o[4];
+__device__ void transpose_a(const PackedView& v, const uint16_t* a, int adapters, int rank, int rp, uint16_t* at,
+                            long b, long nb) {
+  const int ns = packed_slots(v), groups = rp / 8;
+  const long total = (long)adapters * groups * ns;
+  for (long e = b * 256 + threadIdx.x; e < total; e += nb * 256) {
+    const long qg = e / ns, q = qg / groups;
+    const int s = (int)(e - qg * ns), j0 = 8 * (int)(qg - q * groups), c = v.col[s];
+    const uint16_t* src = a + (q * rank + j0) * v.n + c;
+    uint32_t o[8];
 #pragma unroll
-      for (int i = 0; i < 4; ++i) {
-        const uint32_t lo = c >= 0 && j + 2 * i < rank ? src[(long)(j + 2 * i) * v.n] : 0u;
-        const uint32_t hi = c >= 0 && j + 2 * i + 1 < rank ? src[(long)(j + 2 * i + 1) * v.n] : 0u;
-        o[i] = lo | (hi << 16);
-      }
-      *reinterpret_cast<uint4*>(at + e * rp + j) = make_uint4(o[0], o[1], o[2], o[3]);
-    }
+    for (int k = 0; k < 8; ++k) o[k] = c >= 0 && j0 + k < rank ? src[(long)k * v.n] : 0u;
+    *reinterpret_cast<uint4*>(at + (q * ns + s) * rp + j0) =
+        make_uint4(o[0] | o[1] << 16, o[2] | o[3] << 16, o[4] | o[5] << 16, o[6] | o[7] << 16);
   }
+}
+
+// Tokens of adapter q in order, list[start ..], and its items of at most 256 tokens. An adapter's items
+// begin at slot start / 256 + q, which leaves room for all of them and at most one more, marked empty.
+// of[q]: its first item and their number.
+constexpr int kItem = 256;
+struct ListJob {
+  const int* request;
+  int t, adapters, slots;
+  int* list;
+  int4* items;
+  int2* of;
+};
+__device__ void adapter_lists(const ListJob& k, int q) {
+  __shared__ int wsum[4], wbelow[4], total;
+  const int lane = threadIdx.x & 63, wv = threadIdx.x >> 6;
+  int b = 0;
+  for (int i = threadIdx.x; i < k.t; i += 256) {
+    const int r = k.request[i];
+    b += r >= 0 && r < q;
+  }
+#pragma unroll
+  for (int s = 32; s; s >>= 1) b += __shfl_xor(b, s);
+  if (lane == 0) wbelow[wv] = b;
+  if (threadIdx.x == 0) total = 0;
+  __syncthreads();
+  const int start = wbelow[0] + wbelow[1] + wbelow[2] + wbelow[3];
+  for (int t0 = 0; t0 < k.t; t0 += 256) {
+    const int i = t0 + threadIdx.x;
+    const bool on = i < k.t && k.request[i] == q;
+    const uint64_t m = __builtin_amdgcn_ballot_w64(on);
+    if (lane == 0) wsum[wv] = __popcll(m);
+    __syncthreads();
+    int at = start + total + __popcll(m & ((1ull << lane) - 1));
+    for (int w = 0; w < wv; ++w) at += wsum[w];
+    if (on) k.list[at] = i;
+    __syncthreads();
+    if (threadIdx.x == 0) total += wsum[0] + wsum[1] + wsum[2] + wsum[3];
+    __syncthreads();
+  }
+  const int n = total, first = start / kItem + q;
+  const int end = q + 1 < k.adapters ? (start + n) / kItem + q + 1 : k.slots;
+  for (int s = first + threadIdx.x; s < end; s += 256) {
+    const int at = (s - first) * kItem;
+    k.items[s] = at < n ? make_int4(q, start + at, min(kItem, n - at), 0) : make_int4(-1, 0, 0, 0);
+  }
+  if (threadIdx.x == 0) k.of[q] = make_int2(first, (n + kItem - 1) / kItem);
+}
+
+// u of few tokens: scaling B^T dy for 8 ranks of one token, a workgroup each
+struct DotJob {
+  const uint16_t* dy;
+  long ldy;
+  int t, m;
+  const uint16_t* b;
+  int rank, adapters;
+  const int* request;
+  const float* scaling;
+  float* u;  // t x rank
+};
+template <class T>
+__device__ void u_dots(const DotJob& k, int id) {
+  __shared__ float red[4][8];
+  const int groups = (k.rank + 7) / 8, tok = id / groups, j0 = 8 * (id - tok * groups);
+  const int q = k.request[tok], lane = threadIdx.x & 63, wv = threadIdx.x >> 6;
+  if (q < 0 || q >= k.adapters) {
+    if (threadIdx.x < 8 && j0 + (int)threadIdx.x < k.rank) k.u[(long)tok * k.rank + j0 + threadIdx.x] = 0.0f;
+    return;
+  }
+  const uint16_t* b = k.b + (long)q * k.m * k.rank + j0;
+  const uint16_t* dy = k.dy + (long)tok * k.ldy;
+  float s[8] = {};
+  const bool whole = j0 + 8 <= k.rank;
+#pragma unroll 4
+  for (int i = threadIdx.x; i < k.m; i += 256) {
+    uint16_t v[8];
+    const float d = T::widen(dy[i]);
+    if (whole) {
+      __builtin_memcpy(v, b + (long)i * k.rank, 16);
+    } else {
+#pragma unroll
+      for (int j = 0; j < 8; ++j) v[j] = j0 + j < k.rank ? b[(long)i * k.rank + j] : (uint16_t)0;
+    }
+#pragma unroll
+    for (int j = 0; j < 8; ++j) s[j] = __builtin_fmaf(d, T::widen(v[j]), s[j]);
+  }
+#pragma unroll
+  for (int j = 0; j < 8; ++j) {
+#pragma unroll
+    for (int x = 32; x; x >>= 1) s[j] += __shfl_xor(s[j], x);
+    if (lane == 0) red[wv][j] = s[j];
+  }
+  __syncthreads();
+  if (threadIdx.x < 8 && j0 + (int)threadIdx.x < k.rank) {
+    const int j = threadIdx.x;
+    k.u[(long)tok * k.rank + j0 + j] = k.scaling[q] * (red[0][j] + red[1][j] + red[2][j] + red[3][j]);
+  }
+}
+
+// Workgroups of each part, in this order; 0: not asked for.
+struct PrepareArgs {
+  int expand, slots, pad[3], tb, ta, lists, dots;
+  uint16_t* w16;
+  SlotJob slot;
+  PadJob pads[3];
+  const uint16_t *a, *b;
+  int adapters, rank, rp, mp;
+  uint16_t *bt, *at;
+  ListJob list;
+  DotJob dot;
+  int total() const { return expand + slots + pad[0] + pad[1] + pad[2] + tb + ta + lists + dots; }
+};
+template <class T>
+__global__ __launch_bounds__(256) void k_prepare(PackedView v, PrepareArgs k) {
+  extern __shared__ __align__(16) uint16_t lds[];
+  int b = blockIdx.x;
+  if (b < k.lists) return adapter_lists(k.list, b);
+  b -= k.lists;
+  if (b < k.dots) return u_dots<T>(k.dot, b);
+  b -= k.dots;
+  if (b < k.slots) return to_slots(v, k.slot, lds, b);
+  b -= k.slots;
+  if (b < k.expand) return packed_expand<T>(v, k.w16, b, k.expand);
+  b -= k.expand;
+#pragma unroll
+  for (int i = 0; i < 3; ++i) {
+    if (b < k.pad[i]) return pad_rows16(k.pads[i], b, k.pad[i]);
+    b -= k.pad[i];
+  }
+  if (b < k.tb) return transpose_b(k.b, k.adapters, v.m, k.rank, k.mp, k.bt, b, k.tb);
+  b -= k.tb;
+  transpose_a(v, k.a, k.adapters, k.rank, k.rp, k.at, b, k.ta);
 }
 
 // The next adapter of a fragment's tokens that is not done yet (-1: none left). q: lane's token's adapter
@@ -179,16 +306,27 @@ __global__ __launch_bounds__(512) void k_shrink(const uint16_t* __restrict__ x, 
       ar[f] = a + ((long)ad * rank + min(16 * f + (lane & 15), rank - 1)) * lda;
       acc[f] = mma_f4{};
     }
-    for (int k0 = 32 * wv; k0 < kk; k0 += 256) {
-      const int k = k0 + 8 * quad;
-      mma_u4 xv = {}, av[RF] = {};
-      if (k < kk) {
-        xv = *reinterpret_cast<const mma_u4*>(xr + k);
+    // U steps' loads in flight
+    constexpr int U = RF > 4 ? 2 : 4;
+    for (int k0 = 32 * wv; k0 < kk; k0 += 256 * U) {
+      mma_u4 xv[U], av[U][RF];
 #pragma unroll
-        for (int f = 0; f < RF; ++f) av[f] = *reinterpret_cast<const mma_u4*>(ar[f] + k);
+      for (int i = 0; i < U; ++i) {
+        const int k = k0 + 256 * i + 8 * quad;
+        xv[i] = mma_u4{};
+#pragma unroll
+        for (int f = 0; f < RF; ++f) av[i][f] = mma_u4{};
+        if (k < kk) {
+          xv[i] = *reinterpret_cast<const mma_u4*>(xr + k);
+#pragma unroll
+          for (int f = 0; f < RF; ++f) av[i][f] = *reinterpret_cast<const mma_u4*>(ar[f] + k);
+        }
       }
 #pragma unroll
-      for (int f = 0; f < RF; ++f) acc[f] = T::mfma(__builtin_bit_cast(v8, av[f]), __builtin_bit_cast(v8, xv), acc[f]);
+      for (int i = 0; i < U; ++i)
+#pragma unroll
+        for (int f = 0; f < RF; ++f)
+          acc[f] = T::mfma(__builtin_bit_cast(v8, av[i][f]), __builtin_bit_cast(v8, xv[i]), acc[f]);
     }
 #pragma unroll
     for (int f = 0; f < RF; ++f)
@@ -245,6 +383,8 @@ struct WideArgs {
   uint16_t* out;  // t x rows
   long ldo;
   int vec;
+  int splits, share;  // of k; the low-rank term goes with the first
+  float* parts;       // [split][t][rows rounded up to 4] instead of out, or null
 };
 
 // out[t][i] = sum_k W(i, k) x[t][k] + hscale_t sum_j e[q][i][j] (hl[t][j] + hl[t][rp + j])
@@ -253,16 +393,19 @@ __global__ __launch_bounds__(64 * WP * WQ, 2) void k_wide(WideArgs a) {
   typedef MmaTile<T, PS, false, FP, FQ, WP, WQ> M;
   typedef typename T::v8 v8;
   __shared__ __align__(1024) uint8_t lds[M::LDS];
-  const MmaTileAt at = mma_tile_at(blockIdx.x, a.np, a.nq);
+  const int tiles = a.np * a.nq, split = blockIdx.x / tiles;
+  const MmaTileAt at = mma_tile_at(blockIdx.x - split * tiles, a.np, a.nq);
   const int p0 = at.p * M::BP, q0 = at.q * M::BQ;
   mma_f4 acc[FP][FQ];
   M::clear(acc);
-  M::run(lds_offset(lds), MmaOp{a.w, a.ldw, a.rows}, MmaOp{a.x, a.ldx, a.t}, p0, q0, 0, a.k, acc);
+  M::run(lds_offset(lds), MmaOp{a.w, a.ldw, a.rows}, MmaOp{a.x, a.ldx, a.t}, p0, q0, split * a.share,
+         min(a.k, (split + 1) * a.share), acc);
   const int lane = threadIdx.x & 63, quad = lane >> 4;
+  const long ldp = (a.rows + 3) & ~3;
 #pragma unroll
   for (int g = 0; g < FQ; ++g) {
     const int t = M::col(q0, g) + (lane & 15);
-    if (a.e) {
+    if (a.e && split == 0) {
       const int q = t < a.t ? a.request[t] : -1;
       const bool known = q >= 0 && q < a.adapters;
       const float scale = known ? a.hscale[t] : 0.0f;
@@ -302,7 +445,9 @@ __global__ __launch_bounds__(64 * WP * WQ, 2) void k_wide(WideArgs a) {
       const int row = M::row(p0, f) + 4 * quad;
       uint16_t* o = a.out + (long)t * a.ldo + row;
       const mma_f4 c = acc[f][g];
-      if (a.vec && row + 3 < a.rows) {
+      if (a.parts) {
+        if (row < a.rows) *reinterpret_cast<mma_f4*>(a.parts + ((long)split * a.t + t) * ldp + row) = c;
+      } else if (a.vec && row + 3 < a.rows) {
         *reinterpret_cast<uint2*>(o) = make_uint2(narrow2<T>(c[0], c[1]), narrow2<T>(c[2], c[3]));
       } else {
 #pragma unroll
@@ -313,120 +458,105 @@ __global__ __launch_bounds__(64 * WP * WQ, 2) void k_wide(WideArgs a) {
   }
 }
 
-// Tokens of adapter blockIdx.x in order, list[start ..], and its items of at most `chunk` tokens. An
-// adapter's items begin at slot start / chunk + adapter, which leaves room for all of them and at most
-// one more, marked empty. first[q], count[q]: its items.
-__global__ __launch_bounds__(1024) void k_adapter_lists(const int* __restrict__ request, int t, int adapters,
-                                                        int chunk, int slots, int* __restrict__ list,
-                                                        int4* __restrict__ items, int2* __restrict__ of) {
-  __shared__ int wsum[16], below, total;
-  const int q = blockIdx.x, lane = threadIdx.x & 63, wv = threadIdx.x >> 6;
-  if (threadIdx.x == 0) below = total = 0;
-  __syncthreads();
-  int b = 0;
-  for (int i = threadIdx.x; i < t; i += 1024) {
-    const int r = request[i];
-    b += r >= 0 && r < q;
-  }
-  for (int s = 32; s; s >>= 1) b += __shfl_xor(b, s);
-  if (lane == 0) atomicAdd(&below, b);  // a sum of counts: the order does not matter
-  __syncthreads();
-  const int start = below;
-  for (int t0 = 0; t0 < t; t0 += 1024) {
-    const int i = t0 + threadIdx.x;
-    const bool on = i < t && request[i] == q;
-    const uint64_t m = __builtin_amdgcn_ballot_w64(on);
-    if (lane == 0) wsum[wv] = __popcll(m);
-    __syncthreads();
-    int at = start + total + __popcll(m & ((1ull << lane) - 1));
-    for (int w = 0; w < wv; ++w) at += wsum[w];
-    if (on) list[at] = i;
-    __syncthreads();
-    if (threadIdx.x == 0)
-      for (int w = 0; w < 16; ++w) total += wsum[w];
-    __syncthreads();
-  }
-  const int n = total, first = start / chunk + q;
-  const int end = q + 1 < adapters ? (start + n) / chunk + q + 1 : slots;
-  for (int s = first + threadIdx.x; s < end; s += 1024) {
-    const int at = (s - first) * chunk;
-    items[s] = at < n ? make_int4(q, start + at, min(chunk, n - at), 0) : make_int4(-1, 0, 0, 0);
-  }
-  if (threadIdx.x == 0) of[q] = make_int2(first, (n + chunk - 1) / chunk);
-}
-
 // part[slot][j][c] = sum over the item's tokens of l[t][j] X[t][c], j in 16 RF ranks from j0, c in 128
 // columns a wavefront. X: 8-bit codes with their scales (I8), or 16-bit values; l times scaling[q] if given.
-// A lane reads 8 neighbouring columns of 8 tokens: row i of the f-th MFMA operand is column 8 i + f.
+// A lane reads 8 neighbouring columns of 8 tokens, the next ones while these are multiplied: row i of the
+// f-th MFMA operand is column 8 i + f. The item's l lies in LDS, its token list beside it.
+struct OuterJob {
+  const void* x;
+  const float* xscale;
+  long ldx;
+  int cols, vec;
+  const float* l;
+  const float* scaling;
+  float* part;  // [slot][rp][128 * blocks of columns]
+};
 template <class T, bool I8, int RF>
-__global__ __launch_bounds__(256) void k_outer(const void* __restrict__ xs, const float* __restrict__ xscale, long ldx,
-                                               int cols, const float* __restrict__ l, int rank, int rp,
-                                               const float* __restrict__ scaling, const int* __restrict__ list,
-                                               const int4* __restrict__ items, float* __restrict__ part, int vec) {
+__device__ __forceinline__ void outer(const OuterJob& k, int colgroup, int rank, int rp, const int* list, int4 it,
+                                      int slot, int j0, float (*ll)[16 * RF + 1], int* toks) {
   typedef typename T::v8 v8;
-  const int4 it = items[blockIdx.y];
-  if (it.x < 0) return;
   const int lane = threadIdx.x & 63, wv = threadIdx.x >> 6, quad = lane >> 4;
-  const int c0 = (blockIdx.x * 4 + wv) * 128, j0 = blockIdx.z * 16 * RF;
-  if (c0 >= cols) return;
-  const int c = c0 + 8 * (lane & 15), nb = (cols + 127) / 128;
-  const float mul = scaling ? scaling[it.x] : 1.0f;
+  const float mul = k.scaling ? k.scaling[it.x] : 1.0f;
+  for (int i = threadIdx.x; i < kItem; i += 256) toks[i] = list[it.y + min(i, it.z - 1)];
+  __syncthreads();
+  // four ranks a load, half of the thread's loads in flight at once
+  constexpr int PER = 4 * RF, BATCH = PER < 8 ? PER : 8;
+  for (int e0 = 0; e0 < kItem * PER; e0 += 256 * BATCH) {
+    if (e0 / PER >= it.z) break;
+    mma_f4 v[BATCH];
+#pragma unroll
+    for (int n = 0; n < BATCH; ++n) {
+      const int e = e0 + 256 * n + threadIdx.x, i = e / PER, j = j0 + 4 * (e - i * PER);
+      v[n] = mma_f4{};
+      if (i < it.z) {
+        const float* src = k.l + (long)toks[i] * rank + j;
+        if (rank % 4 == 0) {
+          if (j < rank) v[n] = *reinterpret_cast<const mma_f4*>(src);
+        } else {
+#pragma unroll
+          for (int r = 0; r < 4; ++r)
+            if (j + r < rank) v[n][r] = src[r];
+        }
+      }
+    }
+#pragma unroll
+    for (int n = 0; n < BATCH; ++n) {
+      const int e = e0 + 256 * n + threadIdx.x, i = e / PER, j = 4 * (e - i * PER);
+#pragma unroll
+      for (int r = 0; r < 4; ++r) ll[i][j + r] = mul * v[n][r];
+    }
+  }
+  __syncthreads();
+  const int c0 = (colgroup * 4 + wv) * 128;
+  if (c0 >= k.cols) return;
+  const int c = c0 + 8 * (lane & 15), nb = (k.cols + 127) / 128;
   mma_f4 acc[8][RF];
 #pragma unroll
   for (int f = 0; f < 8; ++f)
 #pragma unroll
     for (int g = 0; g < RF; ++g) acc[f][g] = mma_f4{};
-  for (int t0 = 0; t0 < it.z; t0 += 32) {
-    int tok[8];
+  struct Raw {
+    mma_u4 h[I8 ? 1 : 8];
+    uint2 b[I8 ? 8 : 1];
+    float s[8];
+  };
+  auto load = [&](int t0, Raw& r) {
 #pragma unroll
-    for (int i = 0; i < 8; ++i) tok[i] = list[it.y + min(t0 + 8 * quad + i, it.z - 1)];
-    uint32_t xv[8][4];  // operand f, pairs of tokens
-    if constexpr (I8) {
-      uint2 raw[8];
-#pragma unroll
-      for (int i = 0; i < 8; ++i) {
-        const int8_t* src = static_cast<const int8_t*>(xs) + (long)tok[i] * ldx + c;
-        raw[i] = make_uint2(0, 0);
-        if (vec) {
-          if (c < cols) raw[i] = *reinterpret_cast<const uint2*>(src);
+    for (int i = 0; i < 8; ++i) {
+      const long tok = toks[t0 + 8 * quad + i];
+      if constexpr (I8) {
+        const int8_t* src = static_cast<const int8_t*>(k.x) + tok * k.ldx + c;
+        r.b[i] = make_uint2(0, 0);
+        if (k.vec) {
+          if (c < k.cols) r.b[i] = *reinterpret_cast<const uint2*>(src);
         } else {
           uint8_t v[8];
 #pragma unroll
-          for (int b = 0; b < 8; ++b) v[b] = c + b < cols ? (uint8_t)src[b] : (uint8_t)0;
-          raw[i] = *reinterpret_cast<uint2*>(v);
+          for (int b = 0; b < 8; ++b) v[b] = c + b < k.cols ? (uint8_t)src[b] : (uint8_t)0;
+          r.b[i] = *reinterpret_cast<uint2*>(v);
         }
+        r.s[i] = k.xscale[tok * nb + c0 / 128];
+      } else {
+        r.h[i] = mma_u4{};
+        if (c < k.cols) r.h[i] = *reinterpret_cast<const mma_u4*>(static_cast<const uint16_t*>(k.x) + tok * k.ldx + c);
       }
+    }
+  };
+  auto mul_add = [&](int t0, const Raw& r) {
+    uint32_t xv[8][4];  // operand f, pairs of tokens
 #pragma unroll
-      for (int f = 0; f < 8; ++f)
+    for (int f = 0; f < 8; ++f)
 #pragma unroll
-        for (int p = 0; p < 4; ++p) {
-          const uint32_t a = f < 4 ? raw[2 * p].x : raw[2 * p].y, b = f < 4 ? raw[2 * p + 1].x : raw[2 * p + 1].y;
+      for (int p = 0; p < 4; ++p) {
+        if constexpr (I8) {
+          const uint32_t a = f < 4 ? r.b[2 * p].x : r.b[2 * p].y, b = f < 4 ? r.b[2 * p + 1].x : r.b[2 * p + 1].y;
           xv[f][p] = narrow2<T>((float)(int8_t)(a >> (8 * (f & 3))), (float)(int8_t)(b >> (8 * (f & 3))));
+        } else {
+          xv[f][p] = __builtin_amdgcn_perm(r.h[2 * p + 1][f >> 1], r.h[2 * p][f >> 1], f & 1 ? 0x07060302u : 0x05040100u);
         }
-    } else {
-      mma_u4 raw[8];
-#pragma unroll
-      for (int i = 0; i < 8; ++i) {
-        raw[i] = mma_u4{};
-        if (c < cols) raw[i] = *reinterpret_cast<const mma_u4*>(static_cast<const uint16_t*>(xs) + (long)tok[i] * ldx + c);
       }
-#pragma unroll
-      for (int f = 0; f < 8; ++f)
-#pragma unroll
-        for (int p = 0; p < 4; ++p) {
-          const uint32_t a = raw[2 * p][f >> 1], b = raw[2 * p + 1][f >> 1];
-          xv[f][p] = __builtin_amdgcn_perm(b, a, f & 1 ? 0x07060302u : 0x05040100u);
-        }
-    }
-    float s[8];
-#pragma unroll
-    for (int i = 0; i < 8; ++i) {
-      s[i] = t0 + 8 * quad + i < it.z ? mul : 0.0f;
-      if constexpr (I8) s[i] *= xscale[(long)tok[i] * nb + c0 / 128];
-    }
 #pragma unroll
     for (int g = 0; g < RF; ++g) {
-      const int j = j0 + 16 * g + (lane & 15);
       uint32_t hi[4], lo[4];
 #pragma unroll
       for (int p = 0; p < 4; ++p) {
@@ -434,7 +564,8 @@ __global__ __launch_bounds__(256) void k_outer(const void* __restrict__ xs, cons
         uint16_t h[2];
 #pragma unroll
         for (int i = 0; i < 2; ++i) {
-          y[i] = j < rank ? s[2 * p + i] * l[(long)tok[2 * p + i] * rank + j] : 0.0f;
+          y[i] = ll[t0 + 8 * quad + 2 * p + i][16 * g + (lane & 15)];
+          if constexpr (I8) y[i] *= r.s[2 * p + i];
           h[i] = T::narrow(y[i]);
         }
         hi[p] = (uint32_t)h[0] | ((uint32_t)h[1] << 16);
@@ -449,13 +580,20 @@ __global__ __launch_bounds__(256) void k_outer(const void* __restrict__ xs, cons
         acc[f][g] = T::mfma(x, vl, acc[f][g]);
       }
     }
+  };
+  Raw now, next;
+  load(0, now);
+  for (int t0 = 0; t0 < it.z; t0 += 32) {
+    if (t0 + 32 < it.z) load(t0 + 32, next);
+    mul_add(t0, now);
+    now = next;
   }
   const long ldp = (long)nb * 128;
 #pragma unroll
   for (int g = 0; g < RF; ++g) {
     const int j = j0 + 16 * g + (lane & 15);
     if (j >= rp) continue;
-    float* o = part + ((long)blockIdx.y * rp + j) * ldp + c0;
+    float* o = k.part + ((long)slot * rp + j) * ldp + c0;
 #pragma unroll
     for (int r = 0; r < 4; ++r) {
       const int i = 8 * (4 * quad + r);
@@ -464,19 +602,153 @@ __global__ __launch_bounds__(256) void k_outer(const void* __restrict__ xs, cons
     }
   }
 }
+// dB's part (16-bit dy) in the first nb_ workgroups of x, dA's (the checkpoint) in the rest
+template <class T, int RF>
+__global__ __launch_bounds__(256, RF < 4 ? 2 : 1) void k_outer(OuterJob db, int nb_, OuterJob da, int rank, int rp,
+                                                  const int* __restrict__ list, const int4* __restrict__ items) {
+  __shared__ float ll[kItem][16 * RF + 1];
+  __shared__ int toks[kItem];
+  const int4 it = items[blockIdx.y];
+  if (it.x < 0) return;
+  if ((int)blockIdx.x < nb_) outer<T, false, RF>(db, blockIdx.x, rank, rp, list, it, blockIdx.y, blockIdx.z * 16 * RF, ll, toks);
+  else outer<Bf16, true, RF>(da, blockIdx.x - nb_, rank, rp, list, it, blockIdx.y, blockIdx.z * 16 * RF, ll, toks);
+}
 
-// Sums of an adapter's items in order, rounded once: da[q][j][c], or with ROWS db[q][c][j].
-template <class T, bool ROWS>
-__global__ __launch_bounds__(256) void k_outer_join(const float* __restrict__ part, const int2* __restrict__ of,
-                                                    int rank, int rp, int cols, long ldp, uint16_t* __restrict__ out) {
-  const int q = blockIdx.z, c = blockIdx.x * 256 + threadIdx.x;
-  if (c >= cols) return;
+// ---- parts of `finish`
+
+// Sums of an adapter's items in order, rounded once: da[q][j][c]
+struct JoinJob {
+  const float* part;
+  int cols;
+  long ldp;
+  uint16_t* out;
+};
+template <class T>
+__device__ void join_da(const JoinJob& k, const int2* of, int rank, int rp, int b) {
+  const int nc = (k.cols + 255) / 256, qj = b / nc, q = qj / rank, j = qj - q * rank;
+  const int c = (b - qj * nc) * 256 + threadIdx.x;
+  if (c >= k.cols) return;
   const int2 f = of[q];
-  for (int j = blockIdx.y; j < rank; j += gridDim.y) {
-    float s = 0.0f;
-    for (int i = 0; i < f.y; ++i) s += part[((long)(f.x + i) * rp + j) * ldp + c];
-    out[ROWS ? ((long)q * cols + c) * rank + j : ((long)q * rank + j) * cols + c] = T::narrow(s);
+  float s = 0.0f;
+#pragma unroll 4
+  for (int i = 0; i < f.y; ++i) s += k.part[((long)(f.x + i) * rp + j) * k.ldp + c];
+  k.out[((long)q * rank + j) * k.cols + c] = T::narrow(s);
+}
+// ... db[q][c][j], 8 ranks a thread
+template <class T>
+__device__ void join_db(const JoinJob& k, const int2* of, int rank, int rp, int b) {
+  const int nc = (k.cols + 255) / 256, groups = (rank + 7) / 8, qg = b / nc, q = qg / groups, j0 = 8 * (qg - q * groups);
+  const int c = (b - qg * nc) * 256 + threadIdx.x;
+  if (c >= k.cols) return;
+  const int2 f = of[q];
+  float s[8] = {};
+#pragma unroll 2
+  for (int i = 0; i < f.y; ++i)
+#pragma unroll
+    for (int j = 0; j < 8; ++j) s[j] += k.part[((long)(f.x + i) * rp + j0 + j) * k.ldp + c];
+  uint16_t* o = k.out + ((long)q * k.cols + c) * rank + j0;
+  uint32_t w[4];
+#pragma unroll
+  for (int j = 0; j < 4; ++j) w[j] = narrow2<T>(s[2 * j], s[2 * j + 1]);
+  if (j0 + 8 <= rank && rank % 8 == 0 && (uintptr_t)k.out % 16 == 0) {
+    *reinterpret_cast<uint4*>(o) = make_uint4(w[0], w[1], w[2], w[3]);
+  } else {
+#pragma unroll
+    for (int j = 0; j < 8; ++j)
+      if (j0 + j < rank) o[j] = (uint16_t)(w[j / 2] >> (16 * (j & 1)));
   }
+}
+
+// 16-bit results in slot order back to columns through LDS (as to_slots)
+struct BackJob {
+  const uint16_t* xp;
+  int t, rows, vec;
+  uint16_t* x;
+  long ldx;
+};
+__device__ void from_slots(const PackedView& v, const BackJob& j, uint16_t* lds, long b) {
+  const int n = j.rows ? j.rows : 1, ns = packed_slots(v), stride = (v.n + 7) & ~7;
+  const long t0 = b * n;
+  for (int s = 8 * threadIdx.x; s < ns; s += 2048) {
+    const int4 c0 = *reinterpret_cast<const int4*>(v.col + s), c1 = *reinterpret_cast<const int4*>(v.col + s + 4);
+    const int c[8] = {c0.x, c0.y, c0.z, c0.w, c1.x, c1.y, c1.z, c1.w};
+    for (int r = 0; r < n && t0 + r < j.t; ++r) {
+      uint16_t in[8];
+      *reinterpret_cast<uint4*>(in) = *reinterpret_cast<const uint4*>(j.xp + (t0 + r) * ns + s);
+      uint16_t* dst = j.rows ? lds + r * stride : j.x + (t0 + r) * j.ldx;
+#pragma unroll
+      for (int i = 0; i < 8; ++i)
+        if (c[i] >= 0) dst[c[i]] = in[i];
+    }
+  }
+  if (!j.rows) return;
+  __syncthreads();
+  for (int r = 0; r < n && t0 + r < j.t; ++r) {
+    uint16_t* dst = j.x + (t0 + r) * j.ldx;
+    if (j.vec) {
+      for (int c = 8 * threadIdx.x; c < v.n; c += 2048)
+        *reinterpret_cast<uint4*>(dst + c) = *reinterpret_cast<const uint4*>(lds + r * stride + c);
+    } else {
+      for (int c = threadIdx.x; c < v.n; c += 256) dst[c] = lds[r * stride + c];
+    }
+  }
+}
+
+// Results from the splits' f32 sums: out[t][c] = sum of parts[split][t][slot of c, or c], rounded once, and
+// with `a` (few tokens) A_q^T u_t added in f32 before.
+struct SumJob {
+  const float* parts;
+  int splits, t, cols;
+  long ldp;
+  const int* slot;  // of each column, null: the identity
+  const uint16_t* a;  // adapters x rank x cols
+  const float* u;
+  int rank, adapters;
+  const int* request;
+  uint16_t* out;
+  long ldo;
+};
+template <class T>
+__device__ void sum_parts(const SumJob& k, int b) {
+  const int nc = (k.cols + 255) / 256, t = b / nc, c = (b - t * nc) * 256 + threadIdx.x;
+  if (c >= k.cols) return;
+  const float* p = k.parts + (long)t * k.ldp + (k.slot ? k.slot[c] : c);
+  float s = 0.0f;
+#pragma unroll 4
+  for (int i = 0; i < k.splits; ++i) s += p[(long)i * k.t * k.ldp];
+  if (k.a) {
+    const int q = k.request[t];
+    if (q >= 0 && q < k.adapters) {
+      const uint16_t* a = k.a + (long)q * k.rank * k.cols + c;
+      const float* u = k.u + (long)t * k.rank;
+#pragma unroll 4
+      for (int j = 0; j < k.rank; ++j) s = __builtin_fmaf(T::widen(a[(long)j * k.cols]), u[j], s);
+    } else if (q != -1) {
+      s = __builtin_nanf("");  // no such adapter
+    }
+  }
+  k.out[(long)t * k.ldo + c] = T::narrow(s);
+}
+
+// Workgroups of each part; 0: not asked for.
+struct FinishArgs {
+  int nda, ndb, nback, nsum;
+  JoinJob da, db;
+  const int2* of;
+  int rank, rp;
+  BackJob back;
+  SumJob sum;
+};
+template <class T>
+__global__ __launch_bounds__(256) void k_finish(PackedView v, FinishArgs k) {
+  extern __shared__ __align__(16) uint16_t lds[];
+  int b = blockIdx.x;
+  if (b < k.nback) return from_slots(v, k.back, lds, b);
+  b -= k.nback;
+  if (b < k.nsum) return sum_parts<T>(k.sum, b);
+  b -= k.nsum;
+  if (b < k.ndb) return join_db<T>(k.db, k.of, k.rank, k.rp, b);
+  join_da<T>(k.da, k.of, k.rank, k.rp, b - k.ndb);
 }
 
 struct Arena {
@@ -494,26 +766,18 @@ struct Arena {
 inline bool aligned16(const void* p, long ld, long cols) { return (uintptr_t)p % 16 == 0 && ld % 8 == 0 && cols % 8 == 0; }
 inline int rank_pad(int rank) { return (int)up(rank, 16); }
 
-hipError_t to_slots(hipStream_t st, const PackedView& v, const uint16_t* x, long ldx, long t, uint16_t* xp) {
-  const int vec = aligned16(x, ldx, v.n);
+// Rows that to_slots / from_slots pass through 64 KB of LDS at a time, and its bytes.
+inline int slot_rows(const PackedView& v) {
   const size_t row = 2 * up(v.n, 8);
-  if (row * 4 <= 65536) k_to_slots<4><<<(int)((t + 3) / 4), 256, 4 * row, st>>>(v, x, ldx, t, xp, vec);
-  else if (row <= 65536) k_to_slots<1><<<(int)t, 256, row, st>>>(v, x, ldx, t, xp, vec);
-  else k_to_slots<0><<<(int)t, 256, 0, st>>>(v, x, ldx, t, xp, vec);
-  return hipGetLastError();
+  return row * 4 <= 65536 ? 4 : row <= 65536 ? 1 : 0;
 }
-hipError_t from_slots(hipStream_t st, const PackedView& v, const uint16_t* xp, long t, uint16_t* x, long ldx) {
-  const int vec = aligned16(x, ldx, v.n);
-  const size_t row = 2 * up(v.n, 8);
-  if (row * 4 <= 65536) k_from_slots<4><<<(int)((t + 3) / 4), 256, 4 * row, st>>>(v, xp, t, x, ldx, vec);
-  else if (row <= 65536) k_from_slots<1><<<(int)t, 256, row, st>>>(v, xp, t, x, ldx, vec);
-  else k_from_slots<0><<<(int)t, 256, 0, st>>>(v, xp, t, x, ldx, vec);
-  return hipGetLastError();
+inline size_t slot_lds(const PackedView& v) { return slot_rows(v) * 2 * up(v.n, 8); }
+inline int slot_blocks(const PackedView& v, long t) {
+  const int r = std::max(slot_rows(v), 1);
+  return (int)((t + r - 1) / r);
 }
-hipError_t pad_rows16(hipStream_t st, const uint16_t* src, long ld, long cols, long dp, long rows, uint16_t* dst) {
-  k_pad_rows16<<<blocks_for(rows * dp, 256 * 8), 256, 0, st>>>(src, ld, (int)cols, (int)dp, rows, dst);
-  return hipGetLastError();
-}
+inline int expand_blocks(const PackedView& v) { return (int)std::min(((long)v.tiles * v.nkb + 3) / 4, 1l << 16); }
+inline int pad_blocks(const PadJob& j) { return blocks_for(j.rows * (j.dp / 8), 256 * 4, 8192); }
 
 template <class T>
 hipError_t shrink(hipStream_t st, const uint16_t* x, long ldx, long t, int k, const uint16_t* a, long lda,
@@ -530,14 +794,36 @@ hipError_t shrink(hipStream_t st, const uint16_t* x, long ldx, long t, int k, co
   return go(std::integral_constant<int, 8>{});
 }
 
+// Shape and splits of a product: the f32 parts of a split one are written and read at about 4 TB/s, and
+// summing them takes a launch (4 us) unless one is there anyway.
+struct WidePlan {
+  int pick, splits, share;
+};
+WidePlan wide_plan(long rows, long t, long k, bool parts_anyway) {
+  WidePlan best = {};
+  double least = 0;
+  for (int i = 0; i < kMmaShapes; ++i)
+    for (int n = 1; n == 1 || (n <= 16 && k / n >= 256); n *= 2) {
+      const bool parts = parts_anyway || n > 1;
+      const double c = mma_cost(rows, t, k, i, n) + (parts ? n * (8.0 / 4e6) * t * rows : 0.0) +
+                       (n > 1 && !parts_anyway ? 4.0 : 0.0);
+      if ((i == 0 && n == 1) || c < least) least = c, best.pick = i, best.splits = n;
+    }
+  best.share = (int)up((k + best.splits - 1) / best.splits, 64);
+  best.splits = (int)((k + best.share - 1) / best.share);
+  return best;
+}
+
 template <class T, bool PS>
-hipError_t wide_product(hipStream_t st, WideArgs w) {
+hipError_t wide_product(hipStream_t st, const WidePlan& p, WideArgs w) {
   w.vec = w.ldo % 4 == 0 && (uintptr_t)w.out % 8 == 0;
-  return with_mma_shape(mma_pick(w.rows, w.t, w.k), [&](auto s) {
+  w.splits = p.splits;
+  w.share = p.share;
+  return with_mma_shape(p.pick, [&](auto s) {
     typedef decltype(s) S;
     w.np = (w.rows + S::bp - 1) / S::bp;
     w.nq = (w.t + S::bq - 1) / S::bq;
-    k_wide<T, PS, S::fp, S::fq, S::wp, S::wq><<<w.np * w.nq, S::threads, 0, st>>>(w);
+    k_wide<T, PS, S::fp, S::fq, S::wp, S::wq><<<w.np * w.nq * p.splits, S::threads, 0, st>>>(w);
     return hipGetLastError();
   });
 }
@@ -556,6 +842,7 @@ hipError_t wide(hipStream_t st, const PackedView& v, const AdapterArgs& a, void*
   const bool low = a.rank > 0;
   const bool pad_x = low && !aligned16(a.x, a.ldx, v.n), pad_a = low && !aligned16(a.a, v.n, v.n);
   const bool pad_b = low && (rp != a.rank || (uintptr_t)a.b % 16);
+  const WidePlan plan = wide_plan(v.m, a.t, ns, false);
   Arena m(work);
   uint16_t* w16 = m.take<uint16_t>((size_t)v.tiles * 16 * ns);
   uint16_t* xp = m.take<uint16_t>((size_t)a.t * ns);
@@ -564,27 +851,35 @@ hipError_t wide(hipStream_t st, const PackedView& v, const AdapterArgs& a, void*
   uint16_t* bpad = m.take<uint16_t>(pad_b ? (size_t)a.adapters * v.m * rp : 0);
   uint16_t* hl = m.take<uint16_t>(low ? (size_t)a.t * 2 * rp : 0);
   float* hscale = m.take<float>(low ? a.t : 0);
+  float* parts = m.take<float>(plan.splits > 1 ? (size_t)plan.splits * a.t * up(v.m, 4) : 0);
   *bytes = m.at;
   if (!run) return hipSuccess;
-  const int dtype = T::kind;
-  STEP(packed_expand(st, dtype, v, w16));
-  STEP(to_slots(st, v, a.x, a.ldx, a.t, xp));
+  PrepareArgs p = {};
+  p.expand = expand_blocks(v);
+  p.w16 = w16;
+  p.slots = slot_blocks(v, a.t);
+  p.slot = {a.x, a.ldx, (int)a.t, slot_rows(v), aligned16(a.x, a.ldx, v.n), xp};
   WideArgs w = {};
+  const uint16_t *x = a.x, *aa = a.a, *bb = a.b;
+  long ldx = a.ldx, lda = v.n;
+  if (pad_x) {
+    p.pads[0] = {a.x, a.ldx, v.n, n8, a.t, xpad};
+    p.pad[0] = pad_blocks(p.pads[0]);
+    x = xpad, ldx = n8;
+  }
+  if (pad_a) {
+    p.pads[1] = {a.a, v.n, v.n, n8, (long)a.adapters * a.rank, apad};
+    p.pad[1] = pad_blocks(p.pads[1]);
+    aa = apad, lda = n8;
+  }
+  if (pad_b) {
+    p.pads[2] = {a.b, a.rank, a.rank, rp, (long)a.adapters * v.m, bpad};
+    p.pad[2] = pad_blocks(p.pads[2]);
+    bb = bpad;
+  }
+  k_prepare<T><<<p.total(), 256, slot_lds(v), st>>>(v, p);
+  STEP(hipGetLastError());
   if (low) {
-    const uint16_t *x = a.x, *aa = a.a, *bb = a.b;
-    long ldx = a.ldx, lda = v.n;
-    if (pad_x) {
-      STEP(pad_rows16(st, a.x, a.ldx, v.n, n8, a.t, xpad));
-      x = xpad, ldx = n8;
-    }
-    if (pad_a) {
-      STEP(pad_rows16(st, a.a, v.n, v.n, n8, (long)a.adapters * a.rank, apad));
-      aa = apad, lda = n8;
-    }
-    if (pad_b) {
-      STEP(pad_rows16(st, a.b, a.rank, a.rank, rp, (long)a.adapters * v.m, bpad));
-      bb = bpad;
-    }
     STEP(shrink<T>(st, x, ldx, a.t, n8, aa, lda, a, 0, a.low, hl, hscale));
     w.e = bb;
     w.rp = rp;
@@ -596,86 +891,119 @@ hipError_t wide(hipStream_t st, const PackedView& v, const AdapterArgs& a, void*
   w.w = w16, w.ldw = ns, w.rows = v.m, w.k = ns;
   w.x = xp, w.ldx = ns, w.t = (int)a.t;
   w.out = a.y, w.ldo = a.ldy;
-  return wide_product<T, false>(st, w);
-}
-
-template <class T, bool I8>
-hipError_t outer(hipStream_t st, const void* x, const float* xscale, long ldx, int cols, const float* l,
-                 const AdapterArgs& a, const float* scaling, const int* list, const int4* items, int slots,
-                 const int2* of, float* part, int vec, uint16_t* out) {
-  const int rp = rank_pad(a.rank), nb = (cols + 127) / 128;
-  auto go = [&](auto rf) {
-    constexpr int RF = decltype(rf)::value;
-    k_outer<std::conditional_t<I8, Bf16, T>, I8, RF><<<dim3((nb + 3) / 4, slots, (rp + 16 * RF - 1) / (16 * RF)), 256, 0, st>>>(
-        x, xscale, ldx, cols, l, a.rank, rp, scaling, list, items, part, vec);
-    return hipGetLastError();
-  };
-  if (rp <= 16) STEP(go(std::integral_constant<int, 1>{}));
-  else if (rp <= 32) STEP(go(std::integral_constant<int, 2>{}));
-  else STEP(go(std::integral_constant<int, 4>{}));
-  k_outer_join<T, !I8><<<dim3((cols + 255) / 256, std::min(a.rank, 64), a.adapters), 256, 0, st>>>(part, of, a.rank, rp, cols,
-                                                                                       128l * nb, out);
+  w.parts = plan.splits > 1 ? parts : nullptr;
+  STEP((wide_product<T, false>(st, plan, w)));
+  if (!w.parts) return hipSuccess;
+  FinishArgs f = {};
+  f.sum = {parts, plan.splits, (int)a.t, v.m, (long)up(v.m, 4), nullptr, nullptr, nullptr, 0, 0, nullptr, a.y, a.ldy};
+  f.nsum = (int)(a.t * ((v.m + 255) / 256));
+  k_finish<T><<<f.nsum, 256, 0, st>>>(v, f);
   return hipGetLastError();
 }
 
+// Tokens up to which the gradient's low-rank terms are taken by dots and sums in f32.
+constexpr long kFewGrad = 64;
+
 template <class T>
 hipError_t grad(hipStream_t st, const PackedView& v, const AdapterArgs& a, void* work, bool run, size_t* bytes) {
-  const int ns = packed_slots(v), rp = rank_pad(a.rank), m8 = (int)up(v.m, 8);
-  const bool low = a.rank > 0, pad = !aligned16(a.x, a.ldx, v.m);
-  const long widest = std::max(up(v.n, 128), up(v.m, 128));
-  // items: enough of them that, with 128 columns a wavefront, the smaller side fills the GPU
-  const long narrow = std::min(up(v.n, 128), up(v.m, 128)) / 128;
-  const int chunk = (int)std::clamp<long>(up(a.t * narrow / 2048, 32), 256, 1024);
-  const int slots = (int)(a.t / chunk) + a.adapters;
+  const int ns = packed_slots(v), rp = rank_pad(a.rank), m8 = (int)up(v.m, 8), t = (int)a.t;
+  const bool low = a.rank > 0, pad = !aligned16(a.x, a.ldx, v.m), few = a.t <= kFewGrad;
+  const int slots = (int)(a.t / kItem) + a.adapters;
+  const int nbn = (v.n + 127) / 128, nbm = (v.m + 127) / 128;
+  const WidePlan plan = wide_plan(ns, a.t, v.m, few);
+  const bool parts_out = few || plan.splits > 1;
   Arena m(work);
   uint16_t* w16 = m.take<uint16_t>((size_t)v.tiles * 16 * ns);
-  uint16_t* dxp = m.take<uint16_t>((size_t)a.t * ns);
+  uint16_t* dxp = m.take<uint16_t>(parts_out ? 0 : (size_t)a.t * ns);
+  float* parts = m.take<float>(parts_out ? (size_t)plan.splits * a.t * ns : 0);
   uint16_t* dyp = m.take<uint16_t>(pad ? (size_t)a.t * m8 : 0);
-  uint16_t* bt = m.take<uint16_t>(low ? (size_t)a.adapters * a.rank * m8 : 0);
-  uint16_t* at = m.take<uint16_t>(low ? (size_t)a.adapters * ns * rp : 0);
+  uint16_t* bt = m.take<uint16_t>(low && !few ? (size_t)a.adapters * a.rank * m8 : 0);
+  uint16_t* at = m.take<uint16_t>(low && !few ? (size_t)a.adapters * ns * rp : 0);
   float* u = m.take<float>(low ? (size_t)a.t * a.rank : 0);
-  uint16_t* hl = m.take<uint16_t>(low ? (size_t)a.t * 2 * rp : 0);
-  float* hscale = m.take<float>(low ? a.t : 0);
+  uint16_t* hl = m.take<uint16_t>(low && !few ? (size_t)a.t * 2 * rp : 0);
+  float* hscale = m.take<float>(low && !few ? a.t : 0);
   int* list = m.take<int>(low ? a.t : 0);
   int4* items = m.take<int4>(low ? slots : 0);
   int2* of = m.take<int2>(low ? a.adapters : 0);
-  float* part = m.take<float>(low ? (size_t)slots * rp * widest : 0);
+  float* part_a = m.take<float>(low ? (size_t)slots * rp * nbn * 128 : 0);
+  float* part_b = m.take<float>(low ? (size_t)slots * rp * nbm * 128 : 0);
   *bytes = m.at;
   if (!run) return hipSuccess;
   const uint16_t* dy = a.x;
   long lddy = a.ldx;
-  WideArgs w = {};
-  if (a.t) {
-    STEP(packed_expand(st, T::kind, v, w16));
+  PrepareArgs p = {};
+  if (t) {
+    p.expand = expand_blocks(v);
+    p.w16 = w16;
     if (pad) {
-      STEP(pad_rows16(st, a.x, a.ldx, v.m, m8, a.t, dyp));
+      p.pads[0] = {a.x, a.ldx, v.m, m8, a.t, dyp};
+      p.pad[0] = pad_blocks(p.pads[0]);
       dy = dyp, lddy = m8;
     }
   }
   if (low) {
-    if (a.t) {
-      k_transpose_b<<<blocks_for((long)a.adapters * m8, 256), 256, 0, st>>>(a.b, a.adapters, v.m, a.rank, m8, bt);
-      k_transpose_a<<<blocks_for((long)a.adapters * ns, 256), 256, 0, st>>>(v, a.a, a.adapters, a.rank, rp, at);
-      STEP(shrink<T>(st, dy, lddy, a.t, m8, bt, m8, a, 1, u, hl, hscale));
+    p.a = a.a, p.b = a.b, p.adapters = a.adapters, p.rank = a.rank, p.rp = rp, p.mp = m8, p.bt = bt, p.at = at;
+    p.lists = a.adapters;
+    p.list = {a.request, t, a.adapters, slots, list, items, of};
+    if (t && few) {
+      p.dots = t * ((a.rank + 7) / 8);
+      p.dot = {a.x, a.ldx, t, v.m, a.b, a.rank, a.adapters, a.request, a.scaling, u};
+    } else if (t) {
+      p.tb = blocks_for((long)a.adapters * ((a.rank + 7) / 8) * m8, 256, 8192);
+      p.ta = blocks_for((long)a.adapters * (rp / 8) * ns, 256, 8192);
     }
-    k_adapter_lists<<<a.adapters, 1024, 0, st>>>(a.request, (int)a.t, a.adapters, chunk, slots, list, items, of);
-    STEP(hipGetLastError());
-    STEP((outer<T, true>(st, a.codes, a.scales, v.n, v.n, u, a, nullptr, list, items, slots, of, part,
-                         v.n % 8 == 0 && (uintptr_t)a.codes % 8 == 0, a.da)));
-    STEP((outer<T, false>(st, dy, nullptr, lddy, v.m, a.low, a, a.scaling, list, items, slots, of, part, 1, a.db)));
-    w.e = at;
-    w.rp = rp;
-    w.adapters = a.adapters;
-    w.hl = hl;
-    w.hscale = hscale;
-    w.request = a.request;
   }
-  if (!a.t) return hipSuccess;
-  w.w = w16, w.ldw = ns, w.rows = ns, w.k = v.m;
-  w.x = dy, w.ldx = lddy, w.t = (int)a.t;
-  w.out = dxp, w.ldo = ns;
-  STEP((wide_product<T, true>(st, w)));
-  return from_slots(st, v, dxp, a.t, a.y, a.ldy);
+  k_prepare<T><<<p.total(), 256, 0, st>>>(v, p);
+  STEP(hipGetLastError());
+  WideArgs w = {};
+  FinishArgs f = {};
+  if (low) {
+    if (t && !few) STEP(shrink<T>(st, dy, lddy, a.t, m8, bt, m8, a, 1, u, hl, hscale));
+    const OuterJob jb = {dy, nullptr, lddy, v.m, 1, a.low, a.scaling, part_b};
+    const OuterJob ja = {a.codes, a.scales, v.n, v.n, v.n % 8 == 0 && (uintptr_t)a.codes % 8 == 0, u, nullptr, part_a};
+    const int gb = (nbm + 3) / 4, ga = (nbn + 3) / 4;
+    auto go = [&](auto rf) {
+      constexpr int RF = decltype(rf)::value;
+      k_outer<T, RF><<<dim3(gb + ga, slots, (rp + 16 * RF - 1) / (16 * RF)), 256, 0, st>>>(jb, gb, ja, a.rank, rp, list, items);
+      return hipGetLastError();
+    };
+    if (t) {
+      if (rp <= 16) STEP(go(std::integral_constant<int, 1>{}));
+      else if (rp <= 32) STEP(go(std::integral_constant<int, 2>{}));
+      else STEP(go(std::integral_constant<int, 4>{}));
+    }
+    f.of = of;
+    f.rank = a.rank, f.rp = rp;
+    f.da = {part_a, v.n, 128l * nbn, a.da};
+    f.db = {part_b, v.m, 128l * nbm, a.db};
+    f.nda = a.adapters * a.rank * ((v.n + 255) / 256);
+    f.ndb = a.adapters * ((a.rank + 7) / 8) * ((v.m + 255) / 256);
+    if (!few) {
+      w.e = at;
+      w.rp = rp;
+      w.adapters = a.adapters;
+      w.hl = hl;
+      w.hscale = hscale;
+      w.request = a.request;
+    }
+  }
+  if (t) {
+    w.w = w16, w.ldw = ns, w.rows = ns, w.k = v.m;
+    w.x = dy, w.ldx = lddy, w.t = t;
+    w.out = dxp, w.ldo = ns;
+    w.parts = parts_out ? parts : nullptr;
+    STEP((wide_product<T, true>(st, plan, w)));
+    if (parts_out) {
+      const bool add = low && few;
+      f.sum = {parts, plan.splits, t, v.n, (long)ns, v.slot, add ? a.a : nullptr, u, a.rank, a.adapters, a.request, a.y, a.ldy};
+      f.nsum = t * ((v.n + 255) / 256);
+    } else {
+      f.back = {dxp, t, slot_rows(v), aligned16(a.y, a.ldy, v.n), a.y, a.ldy};
+      f.nback = slot_blocks(v, t);
+    }
+  }
+  k_finish<T><<<f.nda + f.ndb + f.nback + f.nsum, 256, f.nback ? slot_lds(v) : 0, st>>>(v, f);
+  return hipGetLastError();
 }
 
 }  // namespace

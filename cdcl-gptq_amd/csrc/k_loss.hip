@@ -437,11 +437,11 @@ LossPlan loss_plan(long t, long d, long v, bool pad_w, bool grad) {
     p.pieces = (int)((rows + most - 1) / most);
     p.piece = (int)up((rows + p.pieces - 1) / p.pieces, 256);
     p.tiles = mma_pick(std::min<long>(p.piece, v), t, p.dp);
-    // a small dx is split over the vocabulary; its f32 parts are written and read at about 2100 bytes a clock
+    // a small dx is split over the vocabulary; its f32 parts are written and read at about 4 TB/s
     double best = 0;
     for (int i = 0; i < kMmaShapes; ++i)
       for (long n = 1; n == 1 || n <= std::min(64, p.piece / 512); n *= 2) {
-        const double c = mma_cost(p.dp, t, p.piece, i, n) + n * (8.0 / 2100) * t * p.dp;
+        const double c = mma_cost(p.dp, t, p.piece, i, n) + n * (8.0 / 4e6) * t * p.dp;
         if ((i == 0 && n == 1) || c < best) best = c, p.dx_tiles = i, p.splits = (int)n;
       }
     p.share = (int)up((p.piece + p.splits - 1) / p.splits, 64);

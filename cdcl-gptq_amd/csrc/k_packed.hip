@@ -74,33 +74,6 @@ __global__ __launch_bounds__(256) void k_packed_scales(PackedView v, int ng_in, 
   }
 }
 
-// W in 16 bits, [tiles * 16][slots]: scale (code - zero), exact in f32, rounded once (the matrix cores
-// take both operands in the activations' type).
-template <class T>
-__global__ __launch_bounds__(256) void k_packed_expand(PackedView v, uint16_t* __restrict__ w16) {
-  const int lane = threadIdx.x & 63, q = lane >> 4, ns = packed_slots(v);
-  const long total = (long)v.tiles * v.nkb;
-  for (long id = blockIdx.x * 4l + (threadIdx.x >> 6); id < total; id += gridDim.x * 4l) {
-    const long tile = id / v.nkb;
-    const int kb = (int)(id - tile * v.nkb);
-    const uint32_t info = __builtin_amdgcn_readfirstlane(v.kinfo[kb]);
-    const int b = info & 15;
-    PackedRegs r = {};
-    packed_load<0>(v.codes + tile * v.tile_bytes + 256l * (info >> 8), lane, b, r);
-    uint16_t* out = w16 + (tile * 16 + (lane & 15)) * ns + kb * 128 + 8 * q;
-#pragma unroll
-    for (int s = 0; s < 4; ++s) {
-      const uint32_t sz = v.scl[(tile * v.ng + v.grp[4 * kb + s]) * 16 + (lane & 15)];
-      const float sc = packed_scale(sz), z = packed_zero(sz);
-      uint32_t o[4];
-#pragma unroll
-      for (int p = 0; p < 4; ++p)
-        o[p] = narrow2<T>(sc * ((float)packed_code(r, b, s, 2 * p) - z), sc * ((float)packed_code(r, b, s, 2 * p + 1) - z));
-      *reinterpret_cast<uint4*>(out + 32 * s) = make_uint4(o[0], o[1], o[2], o[3]);
-    }
-  }
-}
-
 // Activations of few tokens as MFMA operands, xf[step][fragment][lane][8], with the running sums of x
 // over a block's steps, sx[step][token]; and low = A x of every token with an adapter (0 without), one
 // wavefront per (token, rank). Workgroups below nx do the former.
@@ -376,13 +349,6 @@ hipError_t packed_layout(hipStream_t st, const PackedView& v, int ng_in, const u
   const int gy = std::min(v.tiles, 32768), gz = (v.tiles + gy - 1) / gy;
   k_packed_layout<<<dim3(v.nkb, gy, gz), 64, 0, st>>>(v, qw, rb, slotpos, coff, cwid, codes);
   k_packed_scales<<<std::min(4096, (int)(((long)v.tiles * v.ng * 16 + 255) / 256)), 256, 0, st>>>(v, ng_in, s16, qz, scl);
-  return hipGetLastError();
-}
-
-hipError_t packed_expand(hipStream_t st, int dtype, const PackedView& v, uint16_t* w16) {
-  const int grid = (int)std::min(((long)v.tiles * v.nkb + 3) / 4, 1l << 16);
-  if (dtype == CDCLQ_DTYPE_BF16) k_packed_expand<Bf16><<<grid, 256, 0, st>>>(v, w16);
-  else k_packed_expand<F16><<<grid, 256, 0, st>>>(v, w16);
   return hipGetLastError();
 }
 

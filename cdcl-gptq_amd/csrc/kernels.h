@@ -303,6 +303,7 @@ struct PackedView {
   const uint32_t* kinfo;   // [block]: offset in the tile / 256 << 8 | run ends (bit 4 + s) | width
   const uint32_t* grp;     // [step] its group
   const int* col;          // [slot] original column, or -1
+  const int* slot;         // [column] its slot
   long tile_bytes;
   int m, n, tiles, ng, nkb, bits;  // bits: the width of every block, 0 where they differ
 };
@@ -326,7 +327,6 @@ struct AdapterArgs {
 hipError_t packed_layout(hipStream_t st, const PackedView& v, int ng_in, const uint8_t* qw, long rb,
                          const uint16_t* s16, const uint8_t* qz, const int* slotpos, const uint32_t* coff,
                          const uint8_t* cwid, uint8_t* codes, uint32_t* scl);
-hipError_t packed_expand(hipStream_t st, int dtype, const PackedView& v, uint16_t* w16);
 size_t few_work_bytes(const PackedView& v, long t, long rank);
 hipError_t adapter_few(hipStream_t st, int dtype, const PackedView& v, const AdapterArgs& a, void* work);
 size_t wide_work_bytes(const PackedView& v, const AdapterArgs& a);

@@ -280,23 +280,18 @@ struct MmaShape {
   static constexpr int fp = FP, fq = FQ, wp = WP, wq = WQ, bp = 16 * FP * WP, bq = 16 * FQ * WQ, threads = 64 * WP * WQ;
 };
 
-// Clock cycles of a product of `rows` x `cols` results over k on tiles of bp x bq, `splits` ways in k: rounds
-// of tiles over 256 CUs (a CU holds two of the tiles whose stages fit its LDS twice, sharing its matrix
-// cores), each so many stages of 64 k, a stage being bound by the products (two thirds of the matrix
-// rate), by the 64 bytes a clock of the loads, or by the latency of a load. Measured on 4096 x 4096 x
-// 14336: 256 x 256 tiles 1.6 us a stage, 128 x 128 ones 0.55 us; on small products about 0.5 us a stage.
-inline double mma_cost(long rows, long cols, long k, int bp, int bq, long splits) {
-  const long tiles = ((rows + bp - 1) / bp) * ((cols + bq - 1) / bq) * splits;
-  const long stages = std::max(2l, ((k + splits - 1) / splits + 63) / 64);
-  const double work = std::max(bp * bq / 32.0 / 0.67, (bp + bq) * 2.6);
-  const long twice = (bp + bq) * 512 <= 163840 ? 2 : 1;
-  const long rounds = (tiles + 256 * twice - 1) / (256 * twice), shared = tiles > 256 ? twice : 1;
-  return rounds * (std::max(work * shared, 900.0) * stages + 6000.0);
-}
-
-// The shapes, by number, and the cheapest by mma_cost. Wide tiles read each operand less often; small ones
-// spread few results over more CUs, narrow ones compute no columns that nobody asked for.
+// The shapes, by number. Wide tiles read each operand less often; small ones spread few results over more
+// CUs, narrow ones compute no columns that nobody asked for. `us`: a tile's stage of 64 k with every CU busy,
+// measured on 4096 x 65536 results over k = 4096 (the first two narrow ones estimated); `per_cu`: the
+// workgroups that a CU's LDS holds.
 constexpr int kMmaShapes = 9;
+struct MmaShapeTime {
+  int bp, bq, per_cu;
+  double us;
+};
+constexpr MmaShapeTime kMmaTimes[kMmaShapes] = {{256, 256, 1, 1.66}, {256, 128, 1, 1.07}, {256, 64, 2, 0.55},
+                                                {256, 32, 2, 0.40},  {256, 16, 2, 0.33},  {128, 128, 2, 0.50},
+                                                {128, 64, 3, 0.31},  {128, 32, 4, 0.22},  {128, 16, 4, 0.18}};
 template <class F>
 hipError_t with_mma_shape(int pick, F f) {
   switch (pick) {
@@ -311,13 +306,16 @@ hipError_t with_mma_shape(int pick, F f) {
     default: return f(MmaShape<2, 1, 4, 1>{});
   }
 }
+// Microseconds of a product of `rows` x `cols` results over k, `splits` ways in k: rounds of tiles over 256
+// CUs, each so many stages. A stage takes at least the 0.42 us of its loads' latency, a round 4 us more for
+// its first loads and its results.
 inline double mma_cost(long rows, long cols, long k, int pick, long splits) {
-  double c = 0;
-  (void)with_mma_shape(pick, [&](auto s) {
-    c = mma_cost(rows, cols, k, s.bp, s.bq, splits);
-    return hipSuccess;
-  });
-  return c;
+  const MmaShapeTime s = kMmaTimes[pick];
+  const long tiles = ((rows + s.bp - 1) / s.bp) * ((cols + s.bq - 1) / s.bq) * splits;
+  const long stages = std::max(2l, ((k + splits - 1) / splits + 63) / 64);
+  const long rounds = (tiles + 256 * s.per_cu - 1) / (256 * s.per_cu);
+  const long shared = std::min<long>(s.per_cu, (tiles + 255) / 256);
+  return rounds * (std::max(s.us * shared, 0.42) * stages + 4.0);
 }
 inline int mma_pick(long rows, long cols, long k) {
   int best = 0;

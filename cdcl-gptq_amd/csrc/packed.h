@@ -123,4 +123,32 @@ __device__ __forceinline__ float packed_scale(uint32_t sz) {
 }
 __device__ __forceinline__ float packed_zero(uint32_t sz) { return (float)(sz >> 16); }
 
+// W in 16 bits, [tiles * 16][slots]: scale (code - zero), exact in f32, rounded once (the matrix cores
+// take both operands in the activations' type). By workgroups of 256 threads, b of nb.
+template <class T>
+__device__ void packed_expand(const PackedView& v, uint16_t* w16, long b, long nb) {
+  const int lane = threadIdx.x & 63, q = lane >> 4, ns = packed_slots(v);
+  const long total = (long)v.tiles * v.nkb;
+  for (long id = b * 4 + (threadIdx.x >> 6); id < total; id += nb * 4) {
+    const long tile = id / v.nkb;
+    const int kb = (int)(id - tile * v.nkb);
+    const uint32_t info = __builtin_amdgcn_readfirstlane(v.kinfo[kb]);
+    const int width = info & 15;
+    PackedRegs r = {};
+    packed_load<0>(v.codes + tile * v.tile_bytes + 256l * (info >> 8), lane, width, r);
+    uint16_t* out = w16 + (tile * 16 + (lane & 15)) * ns + kb * 128 + 8 * q;
+#pragma unroll
+    for (int s = 0; s < 4; ++s) {
+      const uint32_t sz = v.scl[(tile * v.ng + v.grp[4 * kb + s]) * 16 + (lane & 15)];
+      const float sc = packed_scale(sz), z = packed_zero(sz);
+      uint32_t o[4];
+#pragma unroll
+      for (int p = 0; p < 4; ++p)
+        o[p] = narrow2<T>(sc * ((float)packed_code(r, width, s, 2 * p) - z),
+                          sc * ((float)packed_code(r, width, s, 2 * p + 1) - z));
+      *reinterpret_cast<uint4*>(out + 32 * s) = make_uint4(o[0], o[1], o[2], o[3]);
+    }
+  }
+}
+
 }  // namespace cdclq

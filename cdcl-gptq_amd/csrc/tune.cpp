@@ -137,7 +137,11 @@ int open_packed(cdclq_ctx* ctx, size_t m, size_t n, size_t group, const uint8_t*
   const size_t nkb = slotpos.size() / 128;
   std::vector<uint32_t> kinfo(nkb);
   std::vector<int32_t> col(slotpos.size());
-  for (size_t i = 0; i < col.size(); ++i) col[i] = slotpos[i] < 0 ? -1 : order[slotpos[i]];
+  std::vector<int32_t> slot(n);
+  for (size_t i = 0; i < col.size(); ++i) {
+    col[i] = slotpos[i] < 0 ? -1 : order[slotpos[i]];
+    if (col[i] >= 0) slot[col[i]] = (int32_t)i;
+  }
   uint32_t at = 0;
   int bits = -1;
   for (size_t k = 0; k < nkb; ++k) {
@@ -156,8 +160,8 @@ int open_packed(cdclq_ctx* ctx, size_t m, size_t n, size_t group, const uint8_t*
   // one blob: codes, scales, then the tables
   auto up = [](size_t x) { return (x + 255) / 256 * 256; };
   const size_t codes = up((size_t)v.tiles * v.tile_bytes), scl = up((size_t)v.tiles * ng * 64);
-  const size_t tab[] = {up(4 * nkb), up(4 * grp.size()), up(4 * col.size())};
-  const size_t tables = tab[0] + tab[1] + tab[2];
+  const size_t tab[] = {up(4 * nkb), up(4 * grp.size()), up(4 * col.size()), up(4 * n)};
+  const size_t tables = tab[0] + tab[1] + tab[2] + tab[3];
   const size_t build[] = {up(4 * slotpos.size()), up(4 * n), up(n)};
   p->bytes = codes + scl + tables;
   hipError_t e = hipMalloc(&p->blob, p->bytes);
@@ -174,10 +178,12 @@ int open_packed(cdclq_ctx* ctx, size_t m, size_t n, size_t group, const uint8_t*
   v.kinfo = reinterpret_cast<uint32_t*>(t);
   v.grp = reinterpret_cast<uint32_t*>(t + tab[0]);
   v.col = reinterpret_cast<int*>(t + tab[0] + tab[1]);
+  v.slot = reinterpret_cast<int*>(t + tab[0] + tab[1] + tab[2]);
   std::vector<char> host(tables + build[0] + build[1] + build[2], 0);
   std::memcpy(host.data(), kinfo.data(), 4 * nkb);
   std::memcpy(host.data() + tab[0], grp.data(), 4 * grp.size());
   std::memcpy(host.data() + tab[0] + tab[1], col.data(), 4 * col.size());
+  std::memcpy(host.data() + tab[0] + tab[1] + tab[2], slot.data(), 4 * n);
   char* h = host.data() + tables;
   std::memcpy(h, slotpos.data(), 4 * slotpos.size());
   std::memcpy(h + build[0], coff.data(), 4 * n);

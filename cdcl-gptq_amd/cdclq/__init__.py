@@ -327,7 +327,8 @@ class Context:
         self.close()
 
     def check(self, rc: int):
-        _check(self.ptr, rc)
+        if rc != OK:
+            _check(self.ptr, rc)
 
     def clear_cache(self):
         self.check(lib().cdclq_ctx_clear_cache(self.ptr))

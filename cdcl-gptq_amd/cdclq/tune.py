@@ -22,48 +22,55 @@ from dataclasses import dataclass
 import numpy as np
 import torch
 
-from . import DTYPE_BF16, DTYPE_F16, Context, lib
+from . import DTYPE_BF16, DTYPE_F16, Context, lib as _L
 
 BLOCK = 128  # features per scale of an 8-bit checkpoint
 _CODES = {torch.bfloat16: DTYPE_BF16, torch.float16: DTYPE_F16}
 
 
+_empty = torch.empty
+_current_stream = torch._C._cuda_getCurrentRawStream  # the handle alone: a Stream object costs a microsecond
+
+
 def _code(x: torch.Tensor, name: str) -> int:
-    if x.dtype not in _CODES:
+    c = _CODES.get(x.dtype)
+    if c is None:
         raise TypeError(f"{name} is {x.dtype}, need bfloat16 or float16")
-    return _CODES[x.dtype]
+    return c
 
 
 def _matrix(ctx: Context, x: torch.Tensor, name: str, dtype=None, rows=None, cols=None) -> int:
     """Checks a 2-D tensor with contiguous rows on ctx's GPU; returns its row stride."""
-    if not x.is_cuda or x.device.index != ctx.device:
+    if x.get_device() != ctx.device:
         raise ValueError(f"{name} is on {x.device}, the context on cuda:{ctx.device}")
-    if x.dim() != 2 or (rows is not None and x.shape[0] != rows) or (cols is not None and x.shape[1] != cols):
+    shape = x.shape
+    if len(shape) != 2 or (rows is not None and shape[0] != rows) or (cols is not None and shape[1] != cols):
         want = f"{'rows' if rows is None else rows} x {'columns' if cols is None else cols}"
-        raise ValueError(f"{name} has shape {tuple(x.shape)}, need {want}")
+        raise ValueError(f"{name} has shape {tuple(shape)}, need {want}")
     if dtype is not None and x.dtype != dtype:
         raise TypeError(f"{name} is {x.dtype}, need {dtype}")
     r, c = x.stride()
-    if (c != 1 and x.shape[1] > 1) or (r < x.shape[1] and x.shape[0] > 1):
+    n = shape[1]
+    if (c != 1 and n > 1) or (r < n and shape[0] > 1):
         raise ValueError(f"{name} has strides {(r, c)}; its rows must be contiguous")
-    return max(r, x.shape[1])
+    return r if r > n else n
 
 
 def _vector(ctx: Context, x: torch.Tensor, name: str, dtype, n: int):
-    if not x.is_cuda or x.device.index != ctx.device:
+    if x.get_device() != ctx.device:
         raise ValueError(f"{name} is on {x.device}, the context on cuda:{ctx.device}")
     if x.dtype != dtype:
         raise TypeError(f"{name} is {x.dtype}, need {dtype}")
-    if tuple(x.shape) != (n,) or not x.is_contiguous():
+    if x.shape != (n,) or not x.is_contiguous():
         raise ValueError(f"{name} must be a contiguous vector of {n} values, got shape {tuple(x.shape)}")
 
 
 def _stream(ctx: Context) -> int:
-    return torch.cuda.current_stream(ctx.device).cuda_stream
+    return _current_stream(ctx.device)
 
 
 def _work(n: int, device) -> torch.Tensor:
-    return torch.empty(n, dtype=torch.uint8, device=device)
+    return _empty(n, dtype=torch.uint8, device=device)
 
 
 # ---------------------------------------------------------------- 8-bit activation checkpoints
@@ -82,9 +89,9 @@ def checkpoint_save(ctx: Context, x: torch.Tensor) -> Checkpoint:
     rounded to nearest, ties to even. A block with a NaN or an infinity is restored as NaN."""
     code, ld = _code(x, "x"), _matrix(ctx, x, "x")
     t, n = x.shape
-    codes = torch.empty(t, n, dtype=torch.int8, device=x.device)
-    scales = torch.empty(t, -(-n // BLOCK), dtype=torch.float32, device=x.device)
-    ctx.check(lib().cdclq_checkpoint_save_device(ctx.ptr, x.data_ptr(), ld, t, n, code, codes.data_ptr(),
+    codes = _empty(t, n, dtype=torch.int8, device=x.device)
+    scales = _empty(t, -(-n // BLOCK), dtype=torch.float32, device=x.device)
+    ctx.check(_L().cdclq_checkpoint_save_device(ctx.ptr, x.data_ptr(), ld, t, n, code, codes.data_ptr(),
                                                  scales.data_ptr(), _stream(ctx)))
     return Checkpoint(codes, scales, x.dtype)
 
@@ -101,8 +108,8 @@ def checkpoint_restore(ctx: Context, ck: Checkpoint) -> torch.Tensor:
     """The activation that a checkpoint holds, scale * code, in its own type."""
     _check_saved(ctx, ck)
     t, n = ck.codes.shape
-    out = torch.empty(t, n, dtype=ck.dtype, device=ck.codes.device)
-    ctx.check(lib().cdclq_checkpoint_restore_device(ctx.ptr, ck.codes.data_ptr(), ck.scales.data_ptr(), t, n,
+    out = _empty(t, n, dtype=ck.dtype, device=ck.codes.device)
+    ctx.check(_L().cdclq_checkpoint_restore_device(ctx.ptr, ck.codes.data_ptr(), ck.scales.data_ptr(), t, n,
                                                     _code(out, "out"), out.data_ptr(), n, _stream(ctx)))
     return out
 
@@ -136,7 +143,7 @@ class PackedLinear:
         self.d_out, self.d_in = qw.shape[0], p32.shape[0]
         torch.cuda.current_stream(dev).synchronize()
         out = C.c_void_p()
-        ctx.check(lib().cdclq_packed_open_device(ctx.ptr, self.d_out, self.d_in, int(group), gb.ctypes.data, gb.size,
+        ctx.check(_L().cdclq_packed_open_device(ctx.ptr, self.d_out, self.d_in, int(group), gb.ctypes.data, gb.size,
                                                  qw.data_ptr(), qw.numel(), s16.data_ptr(), qz.data_ptr(),
                                                  p32.data_ptr(), C.byref(out)))
         self.ptr = out
@@ -152,11 +159,11 @@ class PackedLinear:
 
     def nbytes(self) -> int:
         """Device memory that the layer holds."""
-        return lib().cdclq_packed_bytes(self.ptr)
+        return _L().cdclq_packed_bytes(self.ptr)
 
     def close(self):
         if getattr(self, "ptr", None):
-            lib().cdclq_packed_close(self.ptr)
+            _L().cdclq_packed_close(self.ptr)
             self.ptr = None
 
     def __del__(self):
@@ -182,7 +189,8 @@ class Adapters:
         if not (a.device == b.device == scaling.device):
             raise ValueError("a, b and scaling are on different devices")
         self.a, self.b, self.scaling = a, b, scaling
-        self.count, self.rank = a.shape[0], a.shape[1]
+        self.count, self.rank, self.d_in = a.shape
+        self.d_out = b.shape[1]
 
 
 def _adapter_args(packed: PackedLinear, x, adapters, request, name: str):
@@ -192,10 +200,10 @@ def _adapter_args(packed: PackedLinear, x, adapters, request, name: str):
             raise ValueError("request without adapters")
         return None, None, None, 0, 0, None
     a = adapters.a
-    if a.device != x.device or a.dtype != x.dtype:
+    if a.get_device() != x.get_device() or a.dtype != x.dtype:
         raise TypeError(f"the adapters are {a.dtype} on {a.device}, {name} is {x.dtype} on {x.device}")
-    if a.shape[2] != packed.d_in or adapters.b.shape[1] != packed.d_out:
-        raise ValueError(f"adapters of a {adapters.b.shape[1]} x {a.shape[2]} layer, the packed layer is "
+    if adapters.d_in != packed.d_in or adapters.d_out != packed.d_out:
+        raise ValueError(f"adapters of a {adapters.d_out} x {adapters.d_in} layer, the packed layer is "
                          f"{packed.d_out} x {packed.d_in}")
     if request is None:
         raise ValueError("adapters need the request of each token")
@@ -213,9 +221,9 @@ def adapter_linear(packed: PackedLinear, x: torch.Tensor, adapters: Adapters | N
     code, ld = _code(x, "x"), _matrix(ctx, x, "x", None, None, packed.d_in)
     t = x.shape[0]
     a, b, s, count, rank, req = _adapter_args(packed, x, adapters, request, "x")
-    L = lib()
-    y = torch.empty(t, packed.d_out, dtype=x.dtype, device=x.device)
-    low = torch.empty(t, rank, dtype=torch.float32, device=x.device) if return_low else None
+    L = _L()
+    y = _empty(t, packed.d_out, dtype=x.dtype, device=x.device)
+    low = _empty(t, rank, dtype=torch.float32, device=x.device) if return_low else None
     xp = x.data_ptr()
     work = _work(L.cdclq_adapter_work_bytes(packed.ptr, xp, ld, t, a, b, count, rank, 0), x.device)
     ctx.check(L.cdclq_adapter_linear_device(ctx.ptr, packed.ptr, xp, ld, t, code, a, b, s, count, rank, req,
@@ -233,8 +241,8 @@ def adapter_linear_backward(packed: PackedLinear, dy: torch.Tensor, saved: Check
     code, ld = _code(dy, "dy"), _matrix(ctx, dy, "dy", None, None, packed.d_out)
     t = dy.shape[0]
     a, b, s, count, rank, req = _adapter_args(packed, dy, adapters, request, "dy")
-    L = lib()
-    dx = torch.empty(t, packed.d_in, dtype=dy.dtype, device=dy.device)
+    L = _L()
+    dx = _empty(t, packed.d_in, dtype=dy.dtype, device=dy.device)
     da = db = codes = scales = lp = None
     if rank:
         if saved is None or low is None:
@@ -267,8 +275,8 @@ def vocab_loss(ctx: Context, x: torch.Tensor, w: torch.Tensor, targets: torch.Te
     weights, targets int64): (loss, lse), float32 vectors. A token whose target is ignore_index has
     loss = lse = 0 and does not take part; any other target outside 0..V gives a NaN loss."""
     code, ldx, ldw, t, d, v = _loss_args(ctx, x, w, targets)
-    L = lib()
-    out = torch.empty(2, t, dtype=torch.float32, device=x.device)
+    L = _L()
+    out = _empty(2, t, dtype=torch.float32, device=x.device)
     loss, lse = out[0], out[1]
     work = _work(L.cdclq_vocab_work_bytes(t, d, v, w.data_ptr(), ldw, 0), x.device)
     ctx.check(L.cdclq_vocab_loss_device(ctx.ptr, x.data_ptr(), ldx, w.data_ptr(), ldw, t, d, v, code,
@@ -284,9 +292,9 @@ def vocab_loss_backward(ctx: Context, x: torch.Tensor, w: torch.Tensor, targets:
     code, ldx, ldw, t, d, v = _loss_args(ctx, x, w, targets)
     _vector(ctx, lse, "lse", torch.float32, t)
     _vector(ctx, dloss, "dloss", torch.float32, t)
-    L = lib()
-    dx = torch.empty(t, d, dtype=x.dtype, device=x.device)
-    dw = torch.empty(v, d, dtype=w.dtype, device=x.device) if need_dw else None
+    L = _L()
+    dx = _empty(t, d, dtype=x.dtype, device=x.device)
+    dw = _empty(v, d, dtype=w.dtype, device=x.device) if need_dw else None
     work = _work(L.cdclq_vocab_work_bytes(t, d, v, w.data_ptr(), ldw, 1), x.device)
     ctx.check(L.cdclq_vocab_loss_backward_device(ctx.ptr, x.data_ptr(), ldx, w.data_ptr(), ldw, t, d, v, code,
                                                  targets.data_ptr(), ignore_index, lse.data_ptr(), dloss.data_ptr(),

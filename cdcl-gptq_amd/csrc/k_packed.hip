@@ -84,35 +84,35 @@ __global__ __launch_bounds__(256) void k_few_inputs(PackedView v, int nx, int nt
                                                     int adapters, const int* __restrict__ request,
                                                     float* __restrict__ low, int vec) {
   const int lane = threadIdx.x & 63, wv = threadIdx.x >> 6;
-  if ((int)blockIdx.x < nx) {
-    const int id = blockIdx.x * 4 + wv, kb = id / nt, g = id - kb * nt;
-    if (kb >= v.nkb) return;
+  if ((int)blockIdx.x < nx) {  // a block of slots and a fragment of tokens, a step each wavefront
+    __shared__ float sums[4][16];
+    const int kb = blockIdx.x / nt, g = blockIdx.x - kb * nt, step = 4 * kb + wv;
     const int tok = 16 * g + (lane & 15), q = lane >> 4;
-    float sum = 0.0f;
+    float part = 0.0f;
+    if (tok < t) {
+      const int4 c0 = *reinterpret_cast<const int4*>(v.col + 32 * step + 8 * q);
+      const int4 c1 = *reinterpret_cast<const int4*>(v.col + 32 * step + 8 * q + 4);
+      const int c[8] = {c0.x, c0.y, c0.z, c0.w, c1.x, c1.y, c1.z, c1.w};
+      const uint16_t* src = x + (long)tok * ldx;
+      uint32_t o[8];
 #pragma unroll
-    for (int s = 0; s < 4; ++s) {
-      const int step = 4 * kb + s;
-      uint16_t o[8] = {};
-      float part = 0.0f;
-      if (tok < t) {
-        const int4 c0 = *reinterpret_cast<const int4*>(v.col + 32 * step + 8 * q);
-        const int4 c1 = *reinterpret_cast<const int4*>(v.col + 32 * step + 8 * q + 4);
-        const int c[8] = {c0.x, c0.y, c0.z, c0.w, c1.x, c1.y, c1.z, c1.w};
-        const uint16_t* src = x + (long)tok * ldx;
+      for (int i = 0; i < 8; ++i) o[i] = src[max(c[i], 0)];
 #pragma unroll
-        for (int i = 0; i < 8; ++i) {
-          o[i] = c[i] >= 0 ? src[c[i]] : (uint16_t)0;
-          part += T::widen(o[i]);
-        }
-        uint32_t w[4];
-#pragma unroll
-        for (int i = 0; i < 4; ++i) w[i] = (uint32_t)o[2 * i] | ((uint32_t)o[2 * i + 1] << 16);
-        *reinterpret_cast<uint4*>(xf + ((long)(step * nt + g) * 64 + lane) * 8) = make_uint4(w[0], w[1], w[2], w[3]);
+      for (int i = 0; i < 8; ++i) {
+        if (c[i] < 0) o[i] = 0;
+        part += T::widen((uint16_t)o[i]);
       }
-      part += __shfl_xor(part, 16);
-      part += __shfl_xor(part, 32);
-      sum += part;
-      if (lane < 16) sx[step * 16 * nt + tok] = sum;
+      *reinterpret_cast<uint4*>(xf + ((long)(step * nt + g) * 64 + lane) * 8) =
+          make_uint4(o[0] | o[1] << 16, o[2] | o[3] << 16, o[4] | o[5] << 16, o[6] | o[7] << 16);
+    }
+    part += __shfl_xor(part, 16);
+    part += __shfl_xor(part, 32);
+    if (lane < 16) sums[wv][lane] = part;
+    __syncthreads();
+    if (lane < 16) {
+      float sum = sums[0][lane];
+      for (int w = 1; w <= wv; ++w) sum += sums[w][lane];
+      sx[step * 16 * nt + tok] = sum;
     }
     return;
   }
@@ -123,12 +123,23 @@ __global__ __launch_bounds__(256) void k_few_inputs(PackedView v, int nx, int nt
   if (q >= 0 && q < adapters) {
     const uint16_t *xr = x + (long)tok * ldx, *ar = a + ((long)q * rank + j) * v.n;
     if (vec) {
-      for (int c = 8 * lane; c < v.n; c += 512) {
-        uint16_t xv[8], av[8];
-        *reinterpret_cast<uint4*>(xv) = *reinterpret_cast<const uint4*>(xr + c);
-        *reinterpret_cast<uint4*>(av) = *reinterpret_cast<const uint4*>(ar + c);
+      for (int c0 = 8 * lane; c0 < v.n; c0 += 2048) {  // four steps' loads in flight
+        uint4 xv[4], av[4];
 #pragma unroll
-        for (int i = 0; i < 8; ++i) s = __builtin_fmaf(T::widen(xv[i]), T::widen(av[i]), s);
+        for (int u = 0; u < 4; ++u) {
+          const int c = c0 + 512 * u;
+          xv[u] = av[u] = make_uint4(0, 0, 0, 0);
+          if (c < v.n) {
+            xv[u] = *reinterpret_cast<const uint4*>(xr + c);
+            av[u] = *reinterpret_cast<const uint4*>(ar + c);
+          }
+        }
+#pragma unroll
+        for (int u = 0; u < 4; ++u) {
+          const uint16_t *xe = reinterpret_cast<const uint16_t*>(&xv[u]), *ae = reinterpret_cast<const uint16_t*>(&av[u]);
+#pragma unroll
+          for (int i = 0; i < 8; ++i) s = __builtin_fmaf(T::widen(xe[i]), T::widen(ae[i]), s);
+        }
       }
     } else {
       for (int c = lane; c < v.n; c += 64) s = __builtin_fmaf(T::widen(xr[c]), T::widen(ar[c]), s);
@@ -145,7 +156,7 @@ struct FewArgs {
   int t;
   const uint16_t* b;  // adapters x m x rank, null: none
   const float* scaling;
-  int adapters, rank;
+  int adapters, rank, vec;  // vec: b's rows can be read 8 ranks at a time
   const int* request;
   const float* low;
   uint16_t* y;
@@ -169,6 +180,24 @@ __global__ __launch_bounds__(64 * W) void k_packed_few(PackedView v, FewArgs k) 
     const long tile = min(tile0 + i, (long)v.tiles - 1);
     base[i] = v.codes + tile * v.tile_bytes;
     scl[i] = v.scl + tile * v.ng * 16 + 4 * (lane >> 4);
+  }
+  // The first 8 (16) ranks of B for this thread's results are asked for here: they come from HBM
+  // while the codes are worked on.
+  constexpr int OUT = (RT * 16 * 16 * NT + 64 * W - 1) / (64 * W);
+  uint4 early[OUT][2];
+  if (k.b && k.vec) {
+#pragma unroll
+    for (int i = 0; i < OUT; ++i) {
+      const int e = threadIdx.x + i * 64 * W, tok = e / (RT * 16);
+      const long row = tile0 * 16 + (e - tok * (RT * 16));
+      early[i][0] = early[i][1] = make_uint4(0, 0, 0, 0);
+      const int q = tok < k.t ? k.request[tok] : -1;
+      if (q >= 0 && q < k.adapters && row < v.m) {
+        const uint16_t* br = k.b + ((long)q * v.m + row) * k.rank;
+        early[i][0] = *reinterpret_cast<const uint4*>(br);
+        if (k.rank >= 16) early[i][1] = *reinterpret_cast<const uint4*>(br + 8);
+      }
+    }
   }
   PackedRegs next[RT] = {};
   uint32_t ninfo = 0;
@@ -281,20 +310,35 @@ __global__ __launch_bounds__(64 * W) void k_packed_few(PackedView v, FewArgs k) 
 #pragma unroll
       for (int r = 0; r < 4; ++r) red[wv][16 * i + 4 * (lane >> 4) + r][16 * g + (lane & 15)] = acc[i][g][r];
   __syncthreads();
-  for (int e = threadIdx.x; e < RT * 16 * k.t; e += 64 * W) {
-    const int tok = e / (RT * 16), i = e - tok * (RT * 16);
-    const long row = tile0 * 16 + i;
-    if (row >= v.m) continue;
+  auto dot8 = [&](const uint4& u, const float* lo) {
+    const uint16_t* b = reinterpret_cast<const uint16_t*>(&u);
+    float d = 0.0f;
+#pragma unroll
+    for (int j = 0; j < 8; ++j) d = __builtin_fmaf(T::widen(b[j]), lo[j], d);
+    return d;
+  };
+#pragma unroll
+  for (int i = 0; i < OUT; ++i) {
+    const int e = threadIdx.x + i * 64 * W, tok = e / (RT * 16), r = e - tok * (RT * 16);
+    const long row = tile0 * 16 + r;
+    if (tok >= k.t || row >= v.m) continue;
     float s = 0.0f;
 #pragma unroll
-    for (int w = 0; w < W; ++w) s += red[w][i][tok];
+    for (int w = 0; w < W; ++w) s += red[w][r][tok];
     if (k.b) {
       const int q = k.request[tok];
       if (q >= 0 && q < k.adapters) {
         const uint16_t* br = k.b + ((long)q * v.m + row) * k.rank;
         const float* lo = k.low + (long)tok * k.rank;
         float d = 0.0f;
-        for (int j = 0; j < k.rank; ++j) d = __builtin_fmaf(T::widen(br[j]), lo[j], d);
+        if (k.vec) {
+          d = dot8(early[i][0], lo);
+          if (k.rank >= 16) d += dot8(early[i][1], lo + 8);
+          for (int j = 16; j < k.rank; j += 8) d += dot8(*reinterpret_cast<const uint4*>(br + j), lo + j);
+        } else {
+#pragma unroll 4
+          for (int j = 0; j < k.rank; ++j) d = __builtin_fmaf(T::widen(br[j]), lo[j], d);
+        }
         s = __builtin_fmaf(k.scaling[q], d, s);
       } else if (q != -1) {
         s = __builtin_nanf("");  // no such adapter
@@ -306,9 +350,10 @@ __global__ __launch_bounds__(64 * W) void k_packed_few(PackedView v, FewArgs k) 
 
 template <class T, int B, int NT>
 hipError_t few_tiles(hipStream_t st, const PackedView& v, const FewArgs& k) {
-  // two row tiles share the activations' operands where one each would be far more workgroups than
-  // the CUs hold at once
-  if (v.tiles >= 1024) k_packed_few<T, B, 2, NT, 8><<<(v.tiles + 1) / 2, 512, 0, st>>>(v, k);
+  // Two row tiles share the activations' operands where that leaves two workgroups a CU (14336 rows of
+  // 4096, 32 tokens: 25 us with two, 30 with one, 26 with four); few rows take 16 wavefronts each.
+  if (v.tiles >= 512) k_packed_few<T, B, 2, NT, 8><<<(v.tiles + 1) / 2, 512, 0, st>>>(v, k);
+  else if (v.tiles <= 256) k_packed_few<T, B, 1, NT, 16><<<v.tiles, 1024, 0, st>>>(v, k);
   else k_packed_few<T, B, 1, NT, 8><<<v.tiles, 512, 0, st>>>(v, k);
   return hipGetLastError();
 }
@@ -326,12 +371,13 @@ hipError_t few(hipStream_t st, const PackedView& v, const AdapterArgs& a, void* 
   uint16_t* xf = static_cast<uint16_t*>(work);
   float* sx = reinterpret_cast<float*>(xf + (size_t)steps * nt * 512);
   float* low = a.low ? a.low : sx + (size_t)steps * nt * 16;
-  const int nx = (v.nkb * nt + 3) / 4;
+  const int nx = v.nkb * nt;
   const long nlow = a.rank ? ((long)a.t * a.rank + 3) / 4 : 0;
   const int vec = v.n % 8 == 0 && a.ldx % 8 == 0 && (uintptr_t)a.x % 16 == 0 && (uintptr_t)a.a % 16 == 0;
   k_few_inputs<T><<<(int)(nx + nlow), 256, 0, st>>>(v, nx, nt, a.x, a.ldx, (int)a.t, xf, sx, a.a, a.rank, a.adapters,
                                                     a.request, low, vec);
-  FewArgs k = {xf, sx, (int)a.t, a.rank ? a.b : nullptr, a.scaling, a.adapters, a.rank, a.request, low, a.y, a.ldy};
+  FewArgs k = {xf, sx, (int)a.t, a.rank ? a.b : nullptr, a.scaling, a.adapters, a.rank,
+               a.rank % 8 == 0 && (uintptr_t)a.b % 16 == 0, a.request, low, a.y, a.ldy};
   switch (v.bits) {
     case 2: return few_tokens<T, 2>(st, v, k);
     case 3: return few_tokens<T, 3>(st, v, k);

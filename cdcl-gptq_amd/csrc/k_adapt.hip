@@ -36,32 +36,6 @@ inline int blocks_for(long items, int per, int most = 1 << 20) {
 
 // ---- parts of `prepare`, each by workgroups of 256 threads, b of nb
 
-// 16-bit rows of `cols` elements into rows of dp (a multiple of 8), zeros past cols
-struct PadJob {
-  const uint16_t* src;
-  long ld;
-  int cols, dp;
-  long rows;
-  uint16_t* dst;
-};
-__device__ void pad_rows16(const PadJob& j, long b, long nb) {
-  const int per = j.dp / 8;
-  const long total = j.rows * per;
-  for (long i = b * 256 + threadIdx.x; i < total; i += nb * 256) {
-    const long r = i / per;
-    const int c = 8 * (int)(i - r * per);
-    const uint16_t* src = j.src + r * j.ld + c;
-    uint16_t v[8];
-    if (c + 8 <= j.cols) {
-      __builtin_memcpy(v, src, 16);
-    } else {
-#pragma unroll
-      for (int k = 0; k < 8; ++k) v[k] = c + k < j.cols ? src[k] : (uint16_t)0;
-    }
-    *reinterpret_cast<uint4*>(j.dst + r * j.dp + c) = *reinterpret_cast<const uint4*>(v);
-  }
-}
-
 // Activations into slot order, zeros in empty slots: `rows` of them at a time through LDS (0: straight from
 // memory, rows too long for it).
 struct SlotJob {
@@ -137,13 +111,13 @@ __device__ void transpose_a(const PackedView& v, const uint16_t* a, int adapters
   }
 }
 
-// Tokens of adapter q in order, list[start ..], and its items of at most 256 tokens. An adapter's items
-// begin at slot start / 256 + q, which leaves room for all of them and at most one more, marked empty.
+// Tokens of adapter q in order, list[start ..], and its items of at most `chunk` tokens. An adapter's items
+// begin at slot start / chunk + q, which leaves room for all of them and at most one more, marked empty.
 // of[q]: its first item and their number.
-constexpr int kItem = 256;
+constexpr int kItem = 256;  // tokens of an item that lie in LDS at a time; chunk is a multiple of it
 struct ListJob {
   const int* request;
-  int t, adapters, slots;
+  int t, adapters, chunk, slots;
   int* list;
   int4* items;
   int2* of;
@@ -175,13 +149,13 @@ __device__ void adapter_lists(const ListJob& k, int q) {
     if (threadIdx.x == 0) total += wsum[0] + wsum[1] + wsum[2] + wsum[3];
     __syncthreads();
   }
-  const int n = total, first = start / kItem + q;
-  const int end = q + 1 < k.adapters ? (start + n) / kItem + q + 1 : k.slots;
+  const int n = total, first = start / k.chunk + q;
+  const int end = q + 1 < k.adapters ? (start + n) / k.chunk + q + 1 : k.slots;
   for (int s = first + threadIdx.x; s < end; s += 256) {
-    const int at = (s - first) * kItem;
-    k.items[s] = at < n ? make_int4(q, start + at, min(kItem, n - at), 0) : make_int4(-1, 0, 0, 0);
+    const int at = (s - first) * k.chunk;
+    k.items[s] = at < n ? make_int4(q, start + at, min(k.chunk, n - at), 0) : make_int4(-1, 0, 0, 0);
   }
-  if (threadIdx.x == 0) k.of[q] = make_int2(first, (n + kItem - 1) / kItem);
+  if (threadIdx.x == 0) k.of[q] = make_int2(first, (n + k.chunk - 1) / k.chunk);
 }
 
 // u of few tokens: scaling B^T dy for 8 ranks of one token, a workgroup each
@@ -306,27 +280,32 @@ __global__ __launch_bounds__(512) void k_shrink(const uint16_t* __restrict__ x, 
       ar[f] = a + ((long)ad * rank + min(16 * f + (lane & 15), rank - 1)) * lda;
       acc[f] = mma_f4{};
     }
-    // U steps' loads in flight
-    constexpr int U = RF > 4 ? 2 : 4;
-    for (int k0 = 32 * wv; k0 < kk; k0 += 256 * U) {
-      mma_u4 xv[U], av[U][RF];
-#pragma unroll
-      for (int i = 0; i < U; ++i) {
-        const int k = k0 + 256 * i + 8 * quad;
-        xv[i] = mma_u4{};
-#pragma unroll
-        for (int f = 0; f < RF; ++f) av[i][f] = mma_u4{};
-        if (k < kk) {
-          xv[i] = *reinterpret_cast<const mma_u4*>(xr + k);
-#pragma unroll
-          for (int f = 0; f < RF; ++f) av[i][f] = *reinterpret_cast<const mma_u4*>(ar[f] + k);
-        }
-      }
+    // 64 k a wavefront and step, 16 of a row a lane (whole cache lines; the two operands agree on the order
+    // of k, which is all a sum needs); U steps' loads in flight
+    constexpr int U = RF > 4 ? 1 : 2;
+    for (int k0 = 64 * wv; k0 < kk; k0 += 512 * U) {
+      mma_u4 xv[U][2], av[U][2][RF];
 #pragma unroll
       for (int i = 0; i < U; ++i)
 #pragma unroll
-        for (int f = 0; f < RF; ++f)
-          acc[f] = T::mfma(__builtin_bit_cast(v8, av[i][f]), __builtin_bit_cast(v8, xv[i]), acc[f]);
+        for (int h = 0; h < 2; ++h) {
+          const int k = k0 + 512 * i + 16 * quad + 8 * h;
+          xv[i][h] = mma_u4{};
+#pragma unroll
+          for (int f = 0; f < RF; ++f) av[i][h][f] = mma_u4{};
+          if (k < kk) {
+            xv[i][h] = *reinterpret_cast<const mma_u4*>(xr + k);
+#pragma unroll
+            for (int f = 0; f < RF; ++f) av[i][h][f] = *reinterpret_cast<const mma_u4*>(ar[f] + k);
+          }
+        }
+#pragma unroll
+      for (int i = 0; i < U; ++i)
+#pragma unroll
+        for (int h = 0; h < 2; ++h)
+#pragma unroll
+          for (int f = 0; f < RF; ++f)
+            acc[f] = T::mfma(__builtin_bit_cast(v8, av[i][h][f]), __builtin_bit_cast(v8, xv[i][h]), acc[f]);
     }
 #pragma unroll
     for (int f = 0; f < RF; ++f)
@@ -382,7 +361,6 @@ struct WideArgs {
   const int* request;
   uint16_t* out;  // t x rows
   long ldo;
-  int vec;
   int splits, share;  // of k; the low-rank term goes with the first
   float* parts;       // [split][t][rows rounded up to 4] instead of out, or null
 };
@@ -439,23 +417,15 @@ __global__ __launch_bounds__(64 * WP * WQ, 2) void k_wide(WideArgs a) {
           for (int r = 0; r < 4; ++r) acc[f][g][r] = __builtin_nanf("");
       }
     }
-    if (t >= a.t) continue;
+    if (a.parts && t < a.t) {
 #pragma unroll
-    for (int f = 0; f < FP; ++f) {
-      const int row = M::row(p0, f) + 4 * quad;
-      uint16_t* o = a.out + (long)t * a.ldo + row;
-      const mma_f4 c = acc[f][g];
-      if (a.parts) {
-        if (row < a.rows) *reinterpret_cast<mma_f4*>(a.parts + ((long)split * a.t + t) * ldp + row) = c;
-      } else if (a.vec && row + 3 < a.rows) {
-        *reinterpret_cast<uint2*>(o) = make_uint2(narrow2<T>(c[0], c[1]), narrow2<T>(c[2], c[3]));
-      } else {
-#pragma unroll
-        for (int r = 0; r < 4; ++r)
-          if (row + r < a.rows) o[r] = T::narrow(c[r]);
+      for (int f = 0; f < FP; ++f) {
+        const int row = M::row(p0, f) + 4 * quad;
+        if (row < a.rows) *reinterpret_cast<mma_f4*>(a.parts + ((long)split * a.t + t) * ldp + row) = acc[f][g];
       }
     }
   }
+  if (!a.parts) M::store(lds_offset(lds), acc, p0, q0, a.rows, a.t, a.out, a.ldo);
 }
 
 // part[slot][j][c] = sum over the item's tokens of l[t][j] X[t][c], j in 16 RF ranks from j0, c in 128
@@ -466,50 +436,20 @@ struct OuterJob {
   const void* x;
   const float* xscale;
   long ldx;
-  int cols, vec;
+  int cols;
   const float* l;
   const float* scaling;
   float* part;  // [slot][rp][128 * blocks of columns]
 };
-template <class T, bool I8, int RF>
+template <class T, bool I8, bool VEC, int RF>
 __device__ __forceinline__ void outer(const OuterJob& k, int colgroup, int rank, int rp, const int* list, int4 it,
                                       int slot, int j0, float (*ll)[16 * RF + 1], int* toks) {
   typedef typename T::v8 v8;
   const int lane = threadIdx.x & 63, wv = threadIdx.x >> 6, quad = lane >> 4;
   const float mul = k.scaling ? k.scaling[it.x] : 1.0f;
-  for (int i = threadIdx.x; i < kItem; i += 256) toks[i] = list[it.y + min(i, it.z - 1)];
-  __syncthreads();
-  // four ranks a load, half of the thread's loads in flight at once
-  constexpr int PER = 4 * RF, BATCH = PER < 8 ? PER : 8;
-  for (int e0 = 0; e0 < kItem * PER; e0 += 256 * BATCH) {
-    if (e0 / PER >= it.z) break;
-    mma_f4 v[BATCH];
-#pragma unroll
-    for (int n = 0; n < BATCH; ++n) {
-      const int e = e0 + 256 * n + threadIdx.x, i = e / PER, j = j0 + 4 * (e - i * PER);
-      v[n] = mma_f4{};
-      if (i < it.z) {
-        const float* src = k.l + (long)toks[i] * rank + j;
-        if (rank % 4 == 0) {
-          if (j < rank) v[n] = *reinterpret_cast<const mma_f4*>(src);
-        } else {
-#pragma unroll
-          for (int r = 0; r < 4; ++r)
-            if (j + r < rank) v[n][r] = src[r];
-        }
-      }
-    }
-#pragma unroll
-    for (int n = 0; n < BATCH; ++n) {
-      const int e = e0 + 256 * n + threadIdx.x, i = e / PER, j = 4 * (e - i * PER);
-#pragma unroll
-      for (int r = 0; r < 4; ++r) ll[i][j + r] = mul * v[n][r];
-    }
-  }
-  __syncthreads();
-  const int c0 = (colgroup * 4 + wv) * 128;
-  if (c0 >= k.cols) return;
-  const int c = c0 + 8 * (lane & 15), nb = (k.cols + 127) / 128;
+  const int c0 = (colgroup * 4 + wv) * 128, nb = (k.cols + 127) / 128;
+  // columns past the last take part with another's values: nobody reads their sums
+  const int c = c0 + 8 * (lane & 15), cs = VEC ? min(c, ((k.cols + 7) & ~7) - 8) : c, blk = min(c0 / 128, nb - 1);
   mma_f4 acc[8][RF];
 #pragma unroll
   for (int f = 0; f < 8; ++f)
@@ -525,20 +465,18 @@ __device__ __forceinline__ void outer(const OuterJob& k, int colgroup, int rank,
     for (int i = 0; i < 8; ++i) {
       const long tok = toks[t0 + 8 * quad + i];
       if constexpr (I8) {
-        const int8_t* src = static_cast<const int8_t*>(k.x) + tok * k.ldx + c;
-        r.b[i] = make_uint2(0, 0);
-        if (k.vec) {
-          if (c < k.cols) r.b[i] = *reinterpret_cast<const uint2*>(src);
+        const int8_t* src = static_cast<const int8_t*>(k.x) + tok * k.ldx + cs;
+        if constexpr (VEC) {
+          r.b[i] = *reinterpret_cast<const uint2*>(src);
         } else {
           uint8_t v[8];
 #pragma unroll
           for (int b = 0; b < 8; ++b) v[b] = c + b < k.cols ? (uint8_t)src[b] : (uint8_t)0;
           r.b[i] = *reinterpret_cast<uint2*>(v);
         }
-        r.s[i] = k.xscale[tok * nb + c0 / 128];
+        r.s[i] = k.xscale[tok * nb + blk];
       } else {
-        r.h[i] = mma_u4{};
-        if (c < k.cols) r.h[i] = *reinterpret_cast<const mma_u4*>(static_cast<const uint16_t*>(k.x) + tok * k.ldx + c);
+        r.h[i] = *reinterpret_cast<const mma_u4*>(static_cast<const uint16_t*>(k.x) + tok * k.ldx + cs);
       }
     }
   };
@@ -581,13 +519,49 @@ __device__ __forceinline__ void outer(const OuterJob& k, int colgroup, int rank,
       }
     }
   };
-  Raw now, next;
-  load(0, now);
-  for (int t0 = 0; t0 < it.z; t0 += 32) {
-    if (t0 + 32 < it.z) load(t0 + 32, next);
-    mul_add(t0, now);
-    now = next;
+  for (int i0 = 0; i0 < it.z; i0 += kItem) {
+    const int n = min(kItem, it.z - i0);
+    if (i0) __syncthreads();
+    toks[threadIdx.x] = list[it.y + i0 + min((int)threadIdx.x, n - 1)];
+    __syncthreads();
+    // l of these tokens, 0 past the last: four ranks a load, half of the thread's loads in flight at once
+    constexpr int PER = 4 * RF, BATCH = PER < 8 ? PER : 8;
+    for (int e0 = 0; e0 < kItem * PER; e0 += 256 * BATCH) {
+      if (e0 / PER >= ((n + 31) & ~31)) break;
+      mma_f4 v[BATCH];
+#pragma unroll
+      for (int u = 0; u < BATCH; ++u) {
+        const int e = e0 + 256 * u + threadIdx.x, i = e / PER, j = j0 + 4 * (e - i * PER);
+        v[u] = mma_f4{};
+        if (i < n) {
+          const float* src = k.l + (long)toks[i] * rank + j;
+          if (rank % 4 == 0) {
+            if (j < rank) v[u] = *reinterpret_cast<const mma_f4*>(src);
+          } else {
+#pragma unroll
+            for (int r = 0; r < 4; ++r)
+              if (j + r < rank) v[u][r] = src[r];
+          }
+        }
+      }
+#pragma unroll
+      for (int u = 0; u < BATCH; ++u) {
+        const int e = e0 + 256 * u + threadIdx.x, i = e / PER, j = 4 * (e - i * PER);
+#pragma unroll
+        for (int r = 0; r < 4; ++r) ll[i][j + r] = mul * v[u][r];
+      }
+    }
+    __syncthreads();
+    if (c0 >= k.cols) continue;
+    Raw now, next;
+    load(0, now);
+    for (int t0 = 0; t0 < n; t0 += 32) {
+      load(min(t0 + 32, kItem - 32), next);
+      mul_add(t0, now);
+      now = next;
+    }
   }
+  if (c0 >= k.cols) return;
   const long ldp = (long)nb * 128;
 #pragma unroll
   for (int g = 0; g < RF; ++g) {
@@ -603,15 +577,16 @@ __device__ __forceinline__ void outer(const OuterJob& k, int colgroup, int rank,
   }
 }
 // dB's part (16-bit dy) in the first nb_ workgroups of x, dA's (the checkpoint) in the rest
-template <class T, int RF>
+template <class T, int RF, bool VECA>
 __global__ __launch_bounds__(256, RF < 4 ? 2 : 1) void k_outer(OuterJob db, int nb_, OuterJob da, int rank, int rp,
                                                   const int* __restrict__ list, const int4* __restrict__ items) {
   __shared__ float ll[kItem][16 * RF + 1];
   __shared__ int toks[kItem];
   const int4 it = items[blockIdx.y];
   if (it.x < 0) return;
-  if ((int)blockIdx.x < nb_) outer<T, false, RF>(db, blockIdx.x, rank, rp, list, it, blockIdx.y, blockIdx.z * 16 * RF, ll, toks);
-  else outer<Bf16, true, RF>(da, blockIdx.x - nb_, rank, rp, list, it, blockIdx.y, blockIdx.z * 16 * RF, ll, toks);
+  const int j0 = blockIdx.z * 16 * RF;
+  if ((int)blockIdx.x < nb_) outer<T, false, true, RF>(db, blockIdx.x, rank, rp, list, it, blockIdx.y, j0, ll, toks);
+  else outer<Bf16, true, VECA, RF>(da, blockIdx.x - nb_, rank, rp, list, it, blockIdx.y, j0, ll, toks);
 }
 
 // ---- parts of `finish`
@@ -816,7 +791,6 @@ WidePlan wide_plan(long rows, long t, long k, bool parts_anyway) {
 
 template <class T, bool PS>
 hipError_t wide_product(hipStream_t st, const WidePlan& p, WideArgs w) {
-  w.vec = w.ldo % 4 == 0 && (uintptr_t)w.out % 8 == 0;
   w.splits = p.splits;
   w.share = p.share;
   return with_mma_shape(p.pick, [&](auto s) {
@@ -901,6 +875,20 @@ hipError_t wide(hipStream_t st, const PackedView& v, const AdapterArgs& a, void*
   return hipGetLastError();
 }
 
+// Tokens of an item: long ones write fewer sums (8 bytes a column and rank, at about 5 TB/s), short ones
+// make more workgroups, of which a CU holds one (two up to rank 32); 256 tokens take one about 8 us.
+int outer_chunk(long t, int adapters, int rp, int n, int m) {
+  const long groups = ((n + 511) / 512 + (m + 511) / 512) * ((rp + 63) / 64), room = rp > 32 ? 256 : 512;
+  int best = 1;
+  double least = 0;
+  for (int c = 1; c <= 16; ++c) {
+    const long items = std::max<long>(adapters, (t + kItem * c - 1) / (kItem * c));
+    const double cost = (double)((items * groups + room - 1) / room) * (8.0 * c + 3.0) + items * rp * (8.0 / 5e6) * (n + m);
+    if (c == 1 || cost < least) least = cost, best = c;
+  }
+  return kItem * best;
+}
+
 // Tokens up to which the gradient's low-rank terms are taken by dots and sums in f32.
 constexpr long kFewGrad = 64;
 
@@ -908,8 +896,9 @@ template <class T>
 hipError_t grad(hipStream_t st, const PackedView& v, const AdapterArgs& a, void* work, bool run, size_t* bytes) {
   const int ns = packed_slots(v), rp = rank_pad(a.rank), m8 = (int)up(v.m, 8), t = (int)a.t;
   const bool low = a.rank > 0, pad = !aligned16(a.x, a.ldx, v.m), few = a.t <= kFewGrad;
-  const int slots = (int)(a.t / kItem) + a.adapters;
   const int nbn = (v.n + 127) / 128, nbm = (v.m + 127) / 128;
+  const int chunk = outer_chunk(a.t, a.adapters, rp, v.n, v.m);
+  const int slots = (int)(a.t / chunk) + a.adapters;
   const WidePlan plan = wide_plan(ns, a.t, v.m, few);
   const bool parts_out = few || plan.splits > 1;
   Arena m(work);
@@ -944,7 +933,7 @@ hipError_t grad(hipStream_t st, const PackedView& v, const AdapterArgs& a, void*
   if (low) {
     p.a = a.a, p.b = a.b, p.adapters = a.adapters, p.rank = a.rank, p.rp = rp, p.mp = m8, p.bt = bt, p.at = at;
     p.lists = a.adapters;
-    p.list = {a.request, t, a.adapters, slots, list, items, of};
+    p.list = {a.request, t, a.adapters, chunk, slots, list, items, of};
     if (t && few) {
       p.dots = t * ((a.rank + 7) / 8);
       p.dot = {a.x, a.ldx, t, v.m, a.b, a.rank, a.adapters, a.request, a.scaling, u};
@@ -959,12 +948,15 @@ hipError_t grad(hipStream_t st, const PackedView& v, const AdapterArgs& a, void*
   FinishArgs f = {};
   if (low) {
     if (t && !few) STEP(shrink<T>(st, dy, lddy, a.t, m8, bt, m8, a, 1, u, hl, hscale));
-    const OuterJob jb = {dy, nullptr, lddy, v.m, 1, a.low, a.scaling, part_b};
-    const OuterJob ja = {a.codes, a.scales, v.n, v.n, v.n % 8 == 0 && (uintptr_t)a.codes % 8 == 0, u, nullptr, part_a};
+    const OuterJob jb = {dy, nullptr, lddy, v.m, a.low, a.scaling, part_b};
+    const OuterJob ja = {a.codes, a.scales, v.n, v.n, u, nullptr, part_a};
+    const bool vec = v.n % 8 == 0 && (uintptr_t)a.codes % 8 == 0;
     const int gb = (nbm + 3) / 4, ga = (nbn + 3) / 4;
     auto go = [&](auto rf) {
       constexpr int RF = decltype(rf)::value;
-      k_outer<T, RF><<<dim3(gb + ga, slots, (rp + 16 * RF - 1) / (16 * RF)), 256, 0, st>>>(jb, gb, ja, a.rank, rp, list, items);
+      const dim3 grid(gb + ga, slots, (rp + 16 * RF - 1) / (16 * RF));
+      if (vec) k_outer<T, RF, true><<<grid, 256, 0, st>>>(jb, gb, ja, a.rank, rp, list, items);
+      else k_outer<T, RF, false><<<grid, 256, 0, st>>>(jb, gb, ja, a.rank, rp, list, items);
       return hipGetLastError();
     };
     if (t) {

@@ -82,7 +82,7 @@ struct LossTok {
 struct GatherArgs {
   const uint16_t* x;
   long ldx;
-  int d, dp, vec;
+  int d, dp;
   const int64_t* y;
   int v;
   const float *lse, *g;  // gradient
@@ -95,11 +95,15 @@ struct GatherArgs {
 __device__ __forceinline__ void gather_token(const GatherArgs& k, int t, int i, float top) {
   const uint16_t* src = k.x + (long)t * k.ldx;
   uint16_t* dst = k.xc + (long)i * k.dp;
-  if (k.vec) {
-    for (int c = 8 * threadIdx.x; c < k.dp; c += 2048)
-      *reinterpret_cast<uint4*>(dst + c) = *reinterpret_cast<const uint4*>(src + c);
-  } else {
-    for (int c = threadIdx.x; c < k.dp; c += 256) dst[c] = c < k.d ? src[c] : (uint16_t)0;
+  for (int c = 8 * threadIdx.x; c < k.dp; c += 2048) {
+    uint16_t v[8];
+    if (c + 8 <= k.d) {
+      __builtin_memcpy(v, src + c, 16);
+    } else {
+#pragma unroll
+      for (int j = 0; j < 8; ++j) v[j] = c + j < k.d ? src[c + j] : (uint16_t)0;
+    }
+    __builtin_memcpy(__builtin_assume_aligned(dst + c, 16), v, 16);
   }
   if (threadIdx.x == 0) {
     const int64_t y = k.y[t];
@@ -166,32 +170,23 @@ __global__ __launch_bounds__(256) void k_loss_pack(GatherArgs k, long ignore, in
   if (on) gather_token(k, i, before, top);
 }
 
-// 16-bit rows of `cols` elements into rows of dp, zeros past cols (operands that the tiles cannot read)
-__global__ __launch_bounds__(256) void k_pad16(const uint16_t* __restrict__ src, long ld, int cols, int dp, long rows,
-                                               uint16_t* __restrict__ dst) {
-  const long total = rows * dp;
-  for (long i = blockIdx.x * 256l + threadIdx.x; i < total; i += gridDim.x * 256l) {
-    const long r = i / dp;
-    const int c = (int)(i - r * dp);
-    dst[i] = c < cols ? src[r * ld + c] : (uint16_t)0;
-  }
-}
+__global__ __launch_bounds__(256) void k_pad16(PadJob j) { pad_rows16(j, blockIdx.x, gridDim.x); }
 
-template <class T, int FP, int FQ, int WP, int WQ>
+template <class T, int FP, int FQ, int WP, int WQ, bool U>
 __global__ __launch_bounds__(64 * WP * WQ, 2) void k_loss_tiles(const uint16_t* __restrict__ w, long ldw, int v,
                                                                 const uint16_t* __restrict__ xc, int dp,
                                                                 const uint32_t* __restrict__ info, int np, int nq,
                                                                 const LossTok* __restrict__ tok,
                                                                 float2* __restrict__ part, int ldpart,
-                                                                float* __restrict__ hit) {
-  typedef MmaTile<T, false, false, FP, FQ, WP, WQ> M;
+                                                                float* __restrict__ hit, int d) {
+  typedef MmaTile<T, false, false, FP, FQ, WP, WQ, U> M;
   __shared__ __align__(1024) uint8_t lds[M::LDS];
   const MmaTileAt at = mma_tile_at(blockIdx.x, np, nq);
   const int p0 = at.p * M::BP, q0 = at.q * M::BQ, count = (int)info[0];
   if (q0 >= count) return;
   mma_f4 acc[FP][FQ];
   M::clear(acc);
-  M::run(lds_offset(lds), MmaOp{w, ldw, v}, MmaOp{xc, dp, count}, p0, q0, 0, dp, acc);
+  M::run(lds_offset(lds), MmaOp{w, ldw, v}, MmaOp{xc, dp, count}, p0, q0, 0, U ? d : dp, acc);
   const int lane = threadIdx.x & 63;
   const int slab = M::row(p0, 0) / (16 * FP);
 #pragma unroll
@@ -222,14 +217,14 @@ __global__ __launch_bounds__(64 * WP * WQ, 2) void k_loss_tiles(const uint16_t* 
   }
 }
 
-// Joins the slabs of 8 tokens: thread (token, j) takes slabs j, j + 32, ..., eight loads in flight.
-__global__ __launch_bounds__(256) void k_loss_combine(const float2* __restrict__ part, int ldpart, int nslabs,
+// Joins the slabs of 8 tokens: thread (token, j) takes slabs j, j + 128, ..., eight loads in flight.
+__global__ __launch_bounds__(1024) void k_loss_combine(const float2* __restrict__ part, int ldpart, int nslabs,
                                                       const uint32_t* __restrict__ info, const int* __restrict__ idx,
                                                       const float* __restrict__ hit, float* __restrict__ loss,
                                                       float* __restrict__ lse) {
   const int count = (int)info[0], i = blockIdx.x * 8 + (threadIdx.x & 7), j = threadIdx.x >> 3;
   if ((int)blockIdx.x * 8 >= count) return;
-  __shared__ float2 red[4][8];
+  __shared__ float2 red[16][8];
   float m = -__builtin_inff(), s = 0.0f;
   auto join = [&](float m2, float s2) {
     const float n = fmaxf(m, m2);
@@ -241,11 +236,11 @@ __global__ __launch_bounds__(256) void k_loss_combine(const float2* __restrict__
     }
   };
   const int at = min(i, count - 1);
-  for (int k = j; k < nslabs; k += 256) {
+  for (int k = j; k < nslabs; k += 1024) {
     float2 p[8];
 #pragma unroll
     for (int u = 0; u < 8; ++u)
-      p[u] = k + 32 * u < nslabs ? part[(long)(k + 32 * u) * ldpart + at] : make_float2(-__builtin_inff(), 0.0f);
+      p[u] = k + 128 * u < nslabs ? part[(long)(k + 128 * u) * ldpart + at] : make_float2(-__builtin_inff(), 0.0f);
 #pragma unroll
     for (int u = 0; u < 8; ++u) join(p[u].x, p[u].y);
   }
@@ -255,7 +250,7 @@ __global__ __launch_bounds__(256) void k_loss_combine(const float2* __restrict__
   __syncthreads();
   if (j == 0 && i < count) {
 #pragma unroll
-    for (int w = 1; w < 4; ++w) join(red[w][threadIdx.x].x, red[w][threadIdx.x].y);
+    for (int w = 1; w < 16; ++w) join(red[w][threadIdx.x].x, red[w][threadIdx.x].y);
     const float l = m + logf(s);
     lse[idx[i]] = l;
     loss[idx[i]] = l - hit[i];
@@ -263,21 +258,22 @@ __global__ __launch_bounds__(256) void k_loss_combine(const float2* __restrict__
 }
 
 // d of vocabulary rows [v0, v0 + 256 np) for every packed token: d[t][v - v0], ld = ldd
-template <class T, int FP, int FQ, int WP, int WQ>
+template <class T, int FP, int FQ, int WP, int WQ, bool U>
 __global__ __launch_bounds__(64 * WP * WQ, 2) void k_loss_d(const uint16_t* __restrict__ w, long ldw, int v, int v0,
                                                             const uint16_t* __restrict__ xc, int dp,
                                                             const uint32_t* __restrict__ info, int np, int nq,
                                                             const LossTok* __restrict__ tok, uint16_t* __restrict__ d,
-                                                            long ldd) {
-  typedef MmaTile<T, false, false, FP, FQ, WP, WQ> M;
+                                                            long ldd, int dcols) {
+  typedef MmaTile<T, false, false, FP, FQ, WP, WQ, U> M;
   __shared__ __align__(1024) uint8_t lds[M::LDS];
   const MmaTileAt at = mma_tile_at(blockIdx.x, np, nq);
   const int p0 = at.p * M::BP, q0 = at.q * M::BQ, count = (int)info[0];
   if (q0 >= count) return;
   mma_f4 acc[FP][FQ];
   M::clear(acc);
-  M::run(lds_offset(lds), MmaOp{w + (long)v0 * ldw, ldw, v - v0}, MmaOp{xc, dp, count}, p0, q0, 0, dp, acc);
+  M::run(lds_offset(lds), MmaOp{w + (long)v0 * ldw, ldw, v - v0}, MmaOp{xc, dp, count}, p0, q0, 0, U ? dcols : dp, acc);
   const int lane = threadIdx.x & 63;
+  // from the registers: d stays in the caches, and the way through LDS costs the 256-column tiles spills
 #pragma unroll
   for (int g = 0; g < FQ; ++g) {
     const int t = M::col(q0, g) + (lane & 15);
@@ -298,36 +294,55 @@ __global__ __launch_bounds__(64 * WP * WQ, 2) void k_loss_d(const uint16_t* __re
   }
 }
 
-// dxacc[split][t][c] (+)= sum over the split's share of the piece's vocabulary of d[t][v] w[v0 + v][c]
-template <class T, int FP, int FQ, int WP, int WQ>
+// How a piece's dx is split over the vocabulary: about one round of workgroups for the tiles of the tokens
+// that count (the host knows only how many there are at most). Both the product and the sum of its parts go
+// by it. share: vocabulary entries a split.
+struct DxSplit {
+  int nq, splits, share;
+};
+__device__ __forceinline__ DxSplit dx_split(int count, int np, int bq, int piece, int round) {
+  DxSplit s;
+  s.nq = (count + bq - 1) / bq;
+  const int n = max(1, min(round / max(1, np * s.nq), piece / 512));
+  s.share = ((piece + n - 1) / n + 63) & ~63;
+  s.splits = (piece + s.share - 1) / s.share;
+  return s;
+}
+
+// dxacc[split][i][c] (+)= sum over the split's share of the piece's vocabulary of d[i][v] w[v0 + v][c], i the
+// packed token, splits nq bq tokens apart
+template <class T, int FP, int FQ, int WP, int WQ, bool U>
 __global__ __launch_bounds__(64 * WP * WQ, 2) void k_loss_dx(const uint16_t* __restrict__ w, long ldw, int dcols,
-                                                             int v0, int kpiece, int kshare,
+                                                             int v0, int kpiece, int piece, int round,
                                                              const uint16_t* __restrict__ d, long ldd,
-                                                             const uint32_t* __restrict__ info, int np, int nq, int t,
-                                                             int dp, int add, float* __restrict__ dxacc) {
-  typedef MmaTile<T, true, false, FP, FQ, WP, WQ> M;
+                                                             const uint32_t* __restrict__ info, int np, int dp,
+                                                             int add, float* __restrict__ dxacc) {
+  typedef MmaTile<T, true, false, FP, FQ, WP, WQ, U> M;
   __shared__ __align__(1024) uint8_t lds[M::LDS];
-  const int tiles = np * nq, split = blockIdx.x / tiles;
-  const MmaTileAt at = mma_tile_at(blockIdx.x - split * tiles, np, nq);
-  const int p0 = at.p * M::BP, q0 = at.q * M::BQ, count = (int)info[0];
-  if (q0 >= count) return;
+  const int count = (int)info[0];
+  const DxSplit s = dx_split(count, np, M::BQ, piece, round);
+  const int tiles = np * s.nq, split = blockIdx.x / max(1, tiles);
+  if (split >= s.splits || count == 0) return;
+  const MmaTileAt at = mma_tile_at(blockIdx.x - split * tiles, np, s.nq);
+  const int p0 = at.p * M::BP, q0 = at.q * M::BQ;
   mma_f4 acc[FP][FQ];
   M::clear(acc);
-  M::run(lds_offset(lds), MmaOp{w + (long)v0 * ldw, ldw, dcols}, MmaOp{d, ldd, count}, p0, q0, split * kshare,
-         min(kpiece, (split + 1) * kshare), acc);
+  M::run(lds_offset(lds), MmaOp{w + (long)v0 * ldw, ldw, dcols}, MmaOp{d, ldd, count}, p0, q0, split * s.share,
+         min(kpiece, (split + 1) * s.share), acc);
   const int lane = threadIdx.x & 63;
-  float* out = dxacc + (long)split * t * dp;
+  float* out = dxacc + (long)split * s.nq * M::BQ * dp;
 #pragma unroll
   for (int g = 0; g < FQ; ++g) {
     const int i = M::col(q0, g) + (lane & 15);
-    if (i >= count) continue;
+    if (i < count) {
 #pragma unroll
-    for (int f = 0; f < FP; ++f) {
-      const int c = M::row(p0, f) + 4 * (lane >> 4);
-      if (c >= dp) continue;
-      mma_f4* o = reinterpret_cast<mma_f4*>(out + (long)i * dp + c);
-      if (add) *o = *o + acc[f][g];
-      else *o = acc[f][g];
+      for (int f = 0; f < FP; ++f) {
+        const int c = M::row(p0, f) + 4 * (lane >> 4);
+        if (c >= dp) continue;
+        mma_f4* o = reinterpret_cast<mma_f4*>(out + (long)i * dp + c);
+        if (add) *o = *o + acc[f][g];
+        else *o = acc[f][g];
+      }
     }
   }
 }
@@ -337,8 +352,7 @@ template <class T, int FP, int FQ, int WP, int WQ>
 __global__ __launch_bounds__(64 * WP * WQ, 2) void k_loss_dw(const uint16_t* __restrict__ xc, int dp, int dcols,
                                                              const uint16_t* __restrict__ d, long ldd, int rows,
                                                              const uint32_t* __restrict__ info, int np, int nq,
-                                                             float gscale, uint16_t* __restrict__ dw, long lddw,
-                                                             int vec) {
+                                                             float gscale, uint16_t* __restrict__ dw, long lddw) {
   typedef MmaTile<T, true, true, FP, FQ, WP, WQ> M;
   __shared__ __align__(1024) uint8_t lds[M::LDS];
   const MmaTileAt at = mma_tile_at(blockIdx.x, np, nq);
@@ -348,41 +362,29 @@ __global__ __launch_bounds__(64 * WP * WQ, 2) void k_loss_dw(const uint16_t* __r
   if (count > 0)
     M::run(lds_offset(lds), MmaOp{xc, dp, dp}, MmaOp{d, ldd, (int)ldd}, p0, q0, 0, count, acc);
   const float top = __uint_as_float(info[1]), k = (top > 0.0f ? top : 1.0f) / gscale;
-  const int lane = threadIdx.x & 63;
 #pragma unroll
-  for (int g = 0; g < FQ; ++g) {
-    const int i = M::col(q0, g) + (lane & 15);
-    if (i >= rows) continue;
+  for (int f = 0; f < FP; ++f)
 #pragma unroll
-    for (int f = 0; f < FP; ++f) {
-      const int c = M::row(p0, f) + 4 * (lane >> 4);
-      uint16_t* o = dw + (long)i * lddw + c;
-      const mma_f4 a = acc[f][g] * k;
-      if (vec) {
-        if (c < dcols) *reinterpret_cast<uint2*>(o) = make_uint2(narrow2<T>(a[0], a[1]), narrow2<T>(a[2], a[3]));
-      } else {
-#pragma unroll
-        for (int r = 0; r < 4; ++r)
-          if (c + r < dcols) o[r] = T::narrow(a[r]);
-      }
-    }
-  }
+    for (int g = 0; g < FQ; ++g) acc[f][g] *= k;
+  M::store(lds_offset(lds), acc, p0, q0, dcols, rows, dw, lddw);
 }
 
 // dx[t] = top 2^-S sum over the splits of dxacc at the token's packed place; 0 where it does not count
 template <class T>
-__global__ __launch_bounds__(256) void k_loss_dx_out(const float* __restrict__ dxacc, int splits, int t, int d, int dp,
+__global__ __launch_bounds__(256) void k_loss_dx_out(const float* __restrict__ dxacc, int np, int bq, int piece, int round,
+                                                     int t, int d, int dp,
                                                      const int* __restrict__ pos, const uint32_t* __restrict__ info,
                                                      float gscale, uint16_t* __restrict__ dx, long lddx, int vec) {
   const float top = __uint_as_float(info[1]), k = (top > 0.0f ? top : 1.0f) / gscale;
-  const long total = (long)t * dp / 4;
+  const DxSplit sp = dx_split((int)info[0], np, bq, piece, round);
+  const long total = (long)t * dp / 4, apart = (long)sp.nq * bq * dp;
   for (long e = blockIdx.x * 256l + threadIdx.x; e < total; e += gridDim.x * 256l) {
     const int i = (int)(4 * e / dp), c = (int)(4 * e - (long)i * dp), at = pos[i];
     mma_f4 s = {};
     if (at >= 0) {
       const float* a = dxacc + (long)at * dp + c;
 #pragma unroll 8
-      for (int j = 0; j < splits; ++j) s += *reinterpret_cast<const mma_f4*>(a + (long)j * t * dp);
+      for (int j = 0; j < sp.splits; ++j) s += *reinterpret_cast<const mma_f4*>(a + j * apart);
     }
     s *= k;
     uint16_t* o = dx + (long)i * lddx + c;
@@ -398,6 +400,19 @@ __global__ __launch_bounds__(256) void k_loss_dx_out(const float* __restrict__ d
 
 inline int blocks_for(long items, int per, int most = 1 << 20) {
   return (int)std::max(1l, std::min((items + per - 1) / per, (long)most));
+}
+
+// The shapes whose P may have any alignment: those that leave registers for it, all of up to 64 columns.
+inline bool direct_shape(int pick) { return pick != 0 && pick != 1 && pick != 5; }
+constexpr int kDirectTokens = 64;
+template <class F>
+hipError_t with_loss_shape(int pick, bool direct, F f) {
+  return with_mma_shape(pick, [&](auto s) {
+    if constexpr (s.bq <= kDirectTokens) {
+      if (direct) return f(s, std::true_type{});
+    }
+    return f(s, std::false_type{});
+  });
 }
 
 inline size_t up(size_t x, size_t to) { return (x + to - 1) / to * to; }
@@ -420,9 +435,19 @@ LossPlan loss_plan(long t, long d, long v, bool pad_w, bool grad) {
   p.pos = take(4 * t);
   p.tok = take(sizeof(LossTok) * t);
   p.xc = take(2 * (size_t)t * p.dp);
-  p.wpad = pad_w ? take(2 * (size_t)v * p.dp) : 0;
+  // Rows of W that the tiles cannot load straight into LDS: few tokens read them through registers (W is
+  // what bounds them), for many a padded copy costs less.
+  p.direct = pad_w && t <= kDirectTokens;
+  auto pick_of = [&](long rows, long cols, long k) {
+    int best = -1;
+    for (int i = 0; i < kMmaShapes; ++i)
+      if (!p.direct || direct_shape(i))
+        if (best < 0 || mma_cost(rows, cols, k, i, 1) < mma_cost(rows, cols, k, best, 1)) best = i;
+    return best;
+  };
+  p.wpad = pad_w && !p.direct ? take(2 * (size_t)v * p.dp) : 0;
   if (!grad) {
-    p.tiles = mma_pick(v, t, p.dp);
+    p.tiles = pick_of(v, t, p.dp);
     (void)with_mma_shape(p.tiles, [&](auto s) {
       p.slab = 16 * s.fp;
       p.nslabs = (int)(up(v, s.bp) / p.slab);
@@ -436,19 +461,26 @@ LossPlan loss_plan(long t, long d, long v, bool pad_w, bool grad) {
     const size_t rows = up(v, 256), most = std::max<size_t>(256, ((size_t)128 << 20) / t / 256 * 256);
     p.pieces = (int)((rows + most - 1) / most);
     p.piece = (int)up((rows + p.pieces - 1) / p.pieces, 256);
-    p.tiles = mma_pick(std::min<long>(p.piece, v), t, p.dp);
-    // a small dx is split over the vocabulary; its f32 parts are written and read at about 4 TB/s
-    double best = 0;
-    for (int i = 0; i < kMmaShapes; ++i)
-      for (long n = 1; n == 1 || n <= std::min(64, p.piece / 512); n *= 2) {
-        const double c = mma_cost(p.dp, t, p.piece, i, n) + n * (8.0 / 4e6) * t * p.dp;
-        if ((i == 0 && n == 1) || c < best) best = c, p.dx_tiles = i, p.splits = (int)n;
+    p.tiles = pick_of(std::min<long>(p.piece, v), t, p.dp);
+    // a small dx is split over the vocabulary (dx_split); its f32 parts are written and read at about 4 TB/s.
+    // The transposed reads of P cost small tiles about a third more, narrow ones twice as much.
+    double best = -1;
+    for (int i = 0; i < kMmaShapes; ++i) {
+      if (p.direct && !direct_shape(i)) continue;
+      const MmaShapeTime s = kMmaTimes[i];
+      const long np = (p.dp + s.bp - 1) / s.bp, nq = (t + s.bq - 1) / s.bq, round = 256 * s.per_cu;
+      const long n = std::max(1l, std::min(round / (np * nq), (long)p.piece / 512));
+      const double c = mma_cost(p.dp, t, p.piece, i, n) * (s.bq <= 64 ? 2.0 : i ? 1.33 : 1.0) + n * (8.0 / 4e6) * t * p.dp;
+      if (best < 0 || c < best) {
+        best = c;
+        p.dx_tiles = i;
+        p.dx_round = (int)round;
+        p.dx_bytes = 4 * (size_t)p.dp * std::max<size_t>(up(t, s.bq), (size_t)(round / np) * s.bq);
       }
-    p.share = (int)up((p.piece + p.splits - 1) / p.splits, 64);
-    p.splits = (p.piece + p.share - 1) / p.share;
+    }
     p.dw_tiles = mma_cost(p.dp, p.piece, t, 5, 1) < mma_cost(p.dp, p.piece, t, 0, 1) ? 5 : 0;
     p.d = take(2 * (size_t)t * p.piece);
-    p.dxacc = take(4 * (size_t)t * p.dp * p.splits);
+    p.dxacc = take(p.dx_bytes);
   }
   p.bytes = at;
   return p;
@@ -460,11 +492,10 @@ namespace {
 hipError_t prepare(hipStream_t st, const LossArgs& a, const LossPlan& p, float gscale, const uint16_t** w, long* ldw) {
   char* ws = static_cast<char*>(a.work);
   const bool grad = a.dx || a.dw;
-  const int vec = a.d % 8 == 0 && a.ldx % 8 == 0 && (uintptr_t)a.x % 16 == 0;
   int *idx = reinterpret_cast<int*>(ws + p.idx), *pos = grad ? reinterpret_cast<int*>(ws + p.pos) : nullptr;
   uint32_t* info = reinterpret_cast<uint32_t*>(ws + p.info);
   float *loss = grad ? nullptr : a.loss, *lse = grad ? nullptr : a.lse_out;
-  const GatherArgs k = {a.x, a.ldx, (int)a.d, p.dp, vec, a.targets, (int)a.v, a.lse_in, a.dloss, gscale,
+  const GatherArgs k = {a.x, a.ldx, (int)a.d, p.dp, a.targets, (int)a.v, a.lse_in, a.dloss, gscale,
                         reinterpret_cast<uint16_t*>(ws + p.xc), reinterpret_cast<LossTok*>(ws + p.tok),
                         grad ? nullptr : reinterpret_cast<float*>(ws + p.hit)};
   if (a.t > 0 && a.t <= kCountTokens) {
@@ -477,7 +508,8 @@ hipError_t prepare(hipStream_t st, const LossArgs& a, const LossPlan& p, float g
   *ldw = a.ldw;
   if (p.wpad) {
     uint16_t* wp = reinterpret_cast<uint16_t*>(ws + p.wpad);
-    k_pad16<<<blocks_for(a.v * p.dp, 256 * 8), 256, 0, st>>>(a.w, a.ldw, (int)a.d, p.dp, a.v, wp);
+    const PadJob j = {a.w, a.ldw, (int)a.d, p.dp, a.v, wp};
+    k_pad16<<<blocks_for(a.v * (p.dp / 8), 256 * 2, 1 << 16), 256, 0, st>>>(j);
     *w = wp;
     *ldw = p.dp;
   }
@@ -491,17 +523,17 @@ hipError_t forward(hipStream_t st, const LossArgs& a, const LossPlan& p) {
   long ldw;
   hipError_t e = prepare(st, a, p, 1.0f, &w, &ldw);
   if (e != hipSuccess) return e;
-  e = with_mma_shape(p.tiles, [&](auto s) {
+  e = with_loss_shape(p.tiles, p.direct, [&](auto s, auto u) {
     typedef decltype(s) S;
     const int np = (int)((a.v + S::bp - 1) / S::bp), nq = (int)((a.t + S::bq - 1) / S::bq);
-    k_loss_tiles<T, S::fp, S::fq, S::wp, S::wq><<<np * nq, S::threads, 0, st>>>(
+    k_loss_tiles<T, S::fp, S::fq, S::wp, S::wq, decltype(u)::value><<<np * nq, S::threads, 0, st>>>(
         w, ldw, (int)a.v, reinterpret_cast<uint16_t*>(ws + p.xc), p.dp, reinterpret_cast<uint32_t*>(ws + p.info), np, nq,
         reinterpret_cast<LossTok*>(ws + p.tok), reinterpret_cast<float2*>(ws + p.part), (int)a.t,
-        reinterpret_cast<float*>(ws + p.hit));
+        reinterpret_cast<float*>(ws + p.hit), (int)a.d);
     return hipGetLastError();
   });
   if (e != hipSuccess) return e;
-  k_loss_combine<<<(int)((a.t + 7) / 8), 256, 0, st>>>(
+  k_loss_combine<<<(int)((a.t + 7) / 8), 1024, 0, st>>>(
       reinterpret_cast<float2*>(ws + p.part), (int)a.t, p.nslabs, reinterpret_cast<uint32_t*>(ws + p.info),
       reinterpret_cast<int*>(ws + p.idx), reinterpret_cast<float*>(ws + p.hit), a.loss, a.lse_out);
   return hipGetLastError();
@@ -526,30 +558,29 @@ hipError_t backward(hipStream_t st, const LossArgs& a, const LossPlan& p) {
     if (v0 >= v) break;
     const int rows = std::min(p.piece, v - v0);
     if (t) {
-      e = with_mma_shape(p.tiles, [&](auto s) {
+      e = with_loss_shape(p.tiles, p.direct, [&](auto s, auto u) {
         typedef decltype(s) S;
         const int nq = (t + S::bq - 1) / S::bq, np = (rows + S::bp - 1) / S::bp;
-        k_loss_d<T, S::fp, S::fq, S::wp, S::wq><<<np * nq, S::threads, 0, st>>>(w, ldw, v, v0, xc, p.dp, info, np, nq,
-                                                                                tok, d, p.piece);
+        k_loss_d<T, S::fp, S::fq, S::wp, S::wq, decltype(u)::value><<<np * nq, S::threads, 0, st>>>(
+            w, ldw, v, v0, xc, p.dp, info, np, nq, tok, d, p.piece, (int)a.d);
         return hipGetLastError();
       });
       if (e != hipSuccess) return e;
-      e = with_mma_shape(p.dx_tiles, [&](auto s) {
+      e = with_loss_shape(p.dx_tiles, p.direct, [&](auto s, auto u) {
         typedef decltype(s) S;
         const int nq = (t + S::bq - 1) / S::bq, np = (p.dp + S::bp - 1) / S::bp;
-        k_loss_dx<T, S::fp, S::fq, S::wp, S::wq><<<np * nq * p.splits, S::threads, 0, st>>>(
-            w, ldw, p.dp, v0, rows, p.share, d, p.piece, info, np, nq, t, p.dp, i > 0, dxacc);
+        k_loss_dx<T, S::fp, S::fq, S::wp, S::wq, decltype(u)::value><<<std::max(np * nq, p.dx_round), S::threads, 0, st>>>(
+            w, ldw, (int)a.d, v0, rows, p.piece, p.dx_round, d, p.piece, info, np, p.dp, i > 0, dxacc);
         return hipGetLastError();
       });
       if (e != hipSuccess) return e;
     }
     if (a.dw) {
-      const int vec = a.lddw % 4 == 0 && a.d % 4 == 0 && (uintptr_t)a.dw % 8 == 0;
       auto go = [&](auto s) {
         typedef decltype(s) S;
         const int np = (p.dp + S::bp - 1) / S::bp, nq = (rows + S::bq - 1) / S::bq;
         k_loss_dw<T, S::fp, S::fq, S::wp, S::wq><<<np * nq, S::threads, 0, st>>>(
-            xc, p.dp, (int)a.d, d, p.piece, rows, info, np, nq, gscale, a.dw + (long)v0 * a.lddw, a.lddw, vec);
+            xc, p.dp, (int)a.d, d, p.piece, rows, info, np, nq, gscale, a.dw + (long)v0 * a.lddw, a.lddw);
         return hipGetLastError();
       };
       e = p.dw_tiles == 5 ? go(MmaShape<4, 4, 2, 2>{}) : go(MmaShape<8, 4, 2, 4>{});
@@ -557,8 +588,12 @@ hipError_t backward(hipStream_t st, const LossArgs& a, const LossPlan& p) {
     }
   }
   const int vec = a.lddx % 4 == 0 && a.d % 4 == 0 && p.dp == a.d && (uintptr_t)a.dx % 8 == 0;
-  if (t) k_loss_dx_out<T><<<blocks_for((long)t * p.dp, 4 * 256), 256, 0, st>>>(
-      dxacc, p.splits, t, (int)a.d, p.dp, reinterpret_cast<int*>(ws + p.pos), info, gscale, a.dx, a.lddx, vec);
+  if (t) {
+    const MmaShapeTime s = kMmaTimes[p.dx_tiles];
+    k_loss_dx_out<T><<<blocks_for((long)t * p.dp, 4 * 256), 256, 0, st>>>(
+        dxacc, (p.dp + s.bp - 1) / s.bp, s.bq, p.piece, p.dx_round, t, (int)a.d, p.dp, reinterpret_cast<int*>(ws + p.pos),
+        info, gscale, a.dx, a.lddx, vec);
+  }
   return hipGetLastError();
 }
 

@@ -288,8 +288,10 @@ struct LossArgs {
 };
 struct LossPlan {
   size_t bytes, info, idx, pos, tok, xc, wpad, hit, part, d, dxacc;  // offsets into the workspace
-  int dp, slab, nslabs, pieces, piece, share, splits;
+  size_t dx_bytes;
+  int dp, slab, nslabs, pieces, piece, dx_round;
   int tiles, dx_tiles, dw_tiles;  // tile shapes (mma16.h)
+  bool direct;                    // W of any alignment, read as it is
 };
 // pad_w: W's rows are not 16-byte aligned (loss_pads_w)
 LossPlan loss_plan(long t, long d, long v, bool pad_w, bool grad);

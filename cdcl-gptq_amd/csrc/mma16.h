@@ -61,6 +61,32 @@ __device__ __forceinline__ uint32_t narrow2(float a, float b) {
   return (uint32_t)T::narrow(a) | ((uint32_t)T::narrow(b) << 16);
 }
 
+// By workgroups of 256 threads, b of nb: 16-bit rows of `cols` elements into rows of dp (a multiple of 8), zeros past cols
+struct PadJob {
+  const uint16_t* src;
+  long ld;
+  int cols, dp;
+  long rows;
+  uint16_t* dst;
+};
+__device__ inline void pad_rows16(const PadJob& j, long b, long nb) {
+  const int per = j.dp / 8;
+  const long total = j.rows * per;
+  for (long i = b * 256 + threadIdx.x; i < total; i += nb * 256) {
+    const long r = i / per;
+    const int c = 8 * (int)(i - r * per);
+    const uint16_t* src = j.src + r * j.ld + c;
+    uint16_t v[8];
+    if (c + 8 <= j.cols) {
+      __builtin_memcpy(v, src, 16);
+    } else {
+#pragma unroll
+      for (int k = 0; k < 8; ++k) v[k] = c + k < j.cols ? src[k] : (uint16_t)0;
+    }
+    *reinterpret_cast<uint4*>(j.dst + r * j.dp + c) = *reinterpret_cast<const uint4*>(v);
+  }
+}
+
 // An operand of C: `rows` rows of k values each, element (i, k) at p[i ld + k] or, rows contiguous, at
 // p[k ld + i].
 struct MmaOp {
@@ -71,7 +97,9 @@ struct MmaOp {
 
 static __device__ uint4 mma_zero_page[1];  // never written
 
-template <class T, bool PS, bool QS, int FP, int FQ, int WP, int WQ>
+// PU: P has any alignment and no padding (element-wise bounds); its granules go through registers instead of
+// straight into LDS, for which there is room in narrow tiles only.
+template <class T, bool PS, bool QS, int FP, int FQ, int WP, int WQ, bool PU = false>
 struct MmaTile {
   static constexpr int W = WP * WQ, THREADS = 64 * W;
   static constexpr int BP = 16 * FP * WP, BQ = 16 * FQ * WQ, BK = 64;
@@ -100,6 +128,12 @@ struct MmaTile {
     }
   }
 
+  // first column of a granule of a stage with the rows contiguous
+  static __device__ __forceinline__ int col_of(int s) {
+    const int k = s / (BP / 8);
+    return 8 * ((s % (BP / 8)) ^ (2 * ((k & 3) | ((k >> 1) & 4))));
+  }
+
   static __device__ __forceinline__ v8 read_c(uint32_t at) {
     return *(const __attribute__((address_space(3))) v8*)(uintptr_t)(at);
   }
@@ -126,12 +160,31 @@ struct MmaTile {
 #pragma unroll
     for (int i = 0; i < NQ; ++i) pq[i] = granule_at<QS, BQ>(Q, q0, kbeg, 64 * (wv + W * i) + lane);
     const long sp = PS ? BK * P.ld : BK, sq = QS ? BK * Q.ld : BK;
+    uint4 held[PU ? NP : 1];  // PU: a stage's granules on their way
     const uint16_t* const zero = reinterpret_cast<const uint16_t*>(&mma_zero_page[0]);
     const bool has_q = GQ % W == 0 || wv < GQ % W;  // takes part in the last load of Q
 
     // The loads of the next stage to be loaded, one at a time: 0 .. NP - 1 of P, then Q's.
     const uint32_t to = lds + 1024u * wv;
+    int kp = kbeg;  // PU: first k of the stage being loaded
     auto load = [&](uint32_t buf, int i) {
+      if constexpr (PU) {
+        if (i < NP) {
+          const int slot = 64 * (wv + W * i) + lane, k = kp + granule_k<PS, BP>(slot);
+          const int some = PS ? (k < kend ? P.rows - min(p0 + col_of(slot), (P.rows - 1) & ~7) : 0) : kend - k;
+          uint16_t v[8];
+          if (some >= 8) {
+            __builtin_memcpy(v, pp[i], 16);
+          } else {
+#pragma unroll
+            for (int e = 0; e < 8; ++e) v[e] = e < some ? pp[i][e] : (uint16_t)0;
+          }
+          __builtin_memcpy(&held[i], v, 16);
+          pp[i] += sp;
+          if (i == NP - 1) kp += BK;
+          return;
+        }
+      }
       if (i < NP) {
         dma16_untracked(reinterpret_cast<const float*>(pp[i]), to + buf + 1024u * W * i);
         pp[i] += sp;
@@ -140,12 +193,21 @@ struct MmaTile {
         pq[i - NP] += sq;
       }
     };
+    // PU: the held granules into their places
+    auto put = [&](uint32_t buf) {
+      if constexpr (PU) {
+#pragma unroll
+        for (int i = 0; i < NP; ++i)
+          *(__attribute__((address_space(3))) mma_u4*)(uintptr_t)(to + buf + 1024u * W * i + 16 * lane) =
+              mma_u4{held[i].x, held[i].y, held[i].z, held[i].w};
+      }
+    };
     // Before the loads of stage s: what lies past the end of k comes from the zeros.
     auto cut = [&](int s) {
       const int k0 = kbeg + s * BK;
       if (k0 + BK <= kend) return;
 #pragma unroll
-      for (int i = 0; i < NP; ++i)
+      for (int i = 0; i < (PU ? 0 : NP); ++i)
         if (k0 + granule_k<PS, BP>(64 * (wv + W * i) + lane) >= kend) pp[i] = zero;
 #pragma unroll
       for (int i = 0; i < NQ; ++i)
@@ -155,6 +217,7 @@ struct MmaTile {
       cut(s);
 #pragma unroll
       for (int i = 0; i < NP + NQ; ++i) load((uint32_t)(s & 1) * STAGE, i);
+      put((uint32_t)(s & 1) * STAGE);
     };
 
     // read addresses within a stage
@@ -216,7 +279,8 @@ struct MmaTile {
     constexpr std::false_type no_loads{};
     issue(0);
     issue(1);
-    if (has_q) wait_vmcnt<NP + NQ>();
+    if (PU) asm volatile("s_waitcnt vmcnt(0) lgkmcnt(0)" ::: "memory");
+    else if (has_q) wait_vmcnt<NP + NQ>();
     else wait_vmcnt<NP + NQ - 1>();
     asm volatile("s_barrier" ::: "memory");
 #pragma unroll
@@ -229,12 +293,14 @@ struct MmaTile {
     uint32_t buf = 0;
     for (int s = 2; s < stages; ++s) {
       step(buf, 1, even, odd, no_loads, 0u);
+      if (s > 2) put(buf ^ STAGE);  // stage s - 1, held since the last turn
       turn();
       cut(s);
       step(buf ^ STAGE, 0, odd, even, with_loads, buf);
       buf ^= STAGE;
     }
     step(buf, 1, even, odd, no_loads, 0u);
+    if (stages > 2) put(buf ^ STAGE);
     turn();
     step(buf ^ STAGE, 0, odd, even, no_loads, 0u);
     step(buf ^ STAGE, 1, even, odd, no_loads, 0u);
@@ -249,6 +315,42 @@ struct MmaTile {
     for (int f = 0; f < FP; ++f)
 #pragma unroll
       for (int g = 0; g < FQ; ++g) acc[f][g] = mma_f4{};
+  }
+  // out[j][i] = acc in 16 bits for the tile's columns j < qrows and rows i < prows (both counted in the
+  // whole result), whole row pieces at a time: through LDS, 16-byte granule g of column j at g ^ (j & 15), so
+  // that a wavefront's 16 columns write to different banks and 2 BP contiguous bytes go out together
+  // (straight from the registers a column's 32 bytes do). All wavefronts call it together.
+  static __device__ __forceinline__ void store(uint32_t lds, const mma_f4 (&acc)[FP][FQ], int p0, int q0, int prows,
+                                               int qrows, uint16_t* out, long ld) {
+    const int lane = threadIdx.x & 63, wv = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), quad = lane >> 4;
+    const int wp = wv / WQ, wq = wv % WQ;
+    typedef const __attribute__((address_space(3))) mma_u4* lds16;
+#pragma unroll
+    for (int g = 0; g < FQ; ++g) {
+      const int j = 16 * (FQ * wq + g) + (lane & 15);
+#pragma unroll
+      for (int f = 0; f < FP; ++f) {
+        const mma_f4 c = acc[f][g];
+        const int gran = 2 * (FP * wp + f) + (quad >> 1);
+        const uint2 v = make_uint2(narrow2<T>(c[0], c[1]), narrow2<T>(c[2], c[3]));
+        *(__attribute__((address_space(3))) uint64_t*)(uintptr_t)(lds + j * BP * 2 + 16 * (gran ^ (j & 15)) +
+                                                                  8 * (quad & 1)) = (uint64_t)v.y << 32 | v.x;
+      }
+    }
+    __syncthreads();
+    constexpr int G = BP / 8;
+#pragma unroll 4
+    for (int e = threadIdx.x; e < BQ * G; e += THREADS) {
+      const int j = e / G, g = e - j * G, i = p0 + 8 * g;
+      if (q0 + j >= qrows || i >= prows) continue;
+      const mma_u4 v = *(lds16)(uintptr_t)(lds + j * BP * 2 + 16 * (g ^ (j & 15)));
+      uint16_t* o = out + (long)(q0 + j) * ld + i;
+      if (i + 8 <= prows) {
+        __builtin_memcpy(o, &v, 16);
+      } else {
+        for (int k = 0; k < 8 && i + k < prows; ++k) o[k] = (uint16_t)(v[k >> 1] >> (16 * (k & 1)));
+      }
+    }
   }
   // first P row / Q row (result row / column) of this wavefront's block f / g; the lane's own rows are
   // row(f) + 4 (lane >> 4) + r, its column col(g) + (lane & 15)

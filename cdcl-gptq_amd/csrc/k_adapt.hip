@@ -114,6 +114,7 @@ __device__ void transpose_a(const PackedView& v, const uint16_t* a, int adapters
 // Tokens of adapter q in order, list[start ..], and its items of at most `chunk` tokens. An adapter's items
 // begin at slot start / chunk + q, which leaves room for all of them and at most one more, marked empty.
 // of[q]: its first item and their number.
+constexpr int kTile = 128;  // tokens of a tile of k_shrink_tiles
 constexpr int kItem = 256;  // tokens of an item that lie in LDS at a time; chunk is a multiple of it
 struct ListJob {
   const int* request;
@@ -121,6 +122,8 @@ struct ListJob {
   int* list;
   int4* items;
   int2* of;
+  int4* tiles;  // the same for items of kTile tokens, null: not asked for
+  int ntiles;
 };
 __device__ void adapter_lists(const ListJob& k, int q) {
   __shared__ int wsum[4], wbelow[4], total;
@@ -151,11 +154,18 @@ __device__ void adapter_lists(const ListJob& k, int q) {
   }
   const int n = total, first = start / k.chunk + q;
   const int end = q + 1 < k.adapters ? (start + n) / k.chunk + q + 1 : k.slots;
-  for (int s = first + threadIdx.x; s < end; s += 256) {
+  for (int s = first + threadIdx.x; k.items && s < end; s += 256) {
     const int at = (s - first) * k.chunk;
     k.items[s] = at < n ? make_int4(q, start + at, min(k.chunk, n - at), 0) : make_int4(-1, 0, 0, 0);
   }
-  if (threadIdx.x == 0) k.of[q] = make_int2(first, (n + k.chunk - 1) / k.chunk);
+  if (k.of && threadIdx.x == 0) k.of[q] = make_int2(first, (n + k.chunk - 1) / k.chunk);
+  if (k.tiles) {
+    const int first2 = start / kTile + q, end2 = q + 1 < k.adapters ? (start + n) / kTile + q + 1 : k.ntiles;
+    for (int s = first2 + threadIdx.x; s < end2; s += 256) {
+      const int at = (s - first2) * kTile;
+      k.tiles[s] = at < n ? make_int4(q, start + at, min(kTile, n - at), 0) : make_int4(-1, 0, 0, 0);
+    }
+  }
 }
 
 // u of few tokens: scaling B^T dy for 8 ranks of one token, a workgroup each
@@ -252,9 +262,38 @@ __device__ __forceinline__ int next_adapter(int q, uint64_t& left) {
   return a;
 }
 
+// Ranks jt, jt + 32, ... of token ot, by 32 threads: out (t x rank) = low, or scaling low with `scaled`;
+// hl[t][2 rp]: low / 2^e as two 16-bit values, hscale[t] = scaling 2^e.
+template <class T, int N>
+__device__ __forceinline__ void low_out(const float (&v)[N], int ot, int t, int rank, int rp, int adapters,
+                                        const int* request, const float* scaling, int scaled, float* out, uint16_t* hl,
+                                        float* hscale) {
+  const int jt = threadIdx.x & 31;
+  float m = 0.0f;
+#pragma unroll
+  for (int i = 0; i < N; ++i) m = fmaxf(m, __builtin_fabsf(v[i]));
+#pragma unroll
+  for (int s = 16; s; s >>= 1) m = fmaxf(m, __shfl_xor(m, s));
+  if (ot >= t) return;
+  const int rq = request[ot];
+  const float sc = rq >= 0 && rq < adapters ? scaling[rq] : 0.0f;
+  const int e = m > 0.0f && m < __builtin_inff() ? __builtin_amdgcn_frexp_expf(m) : 0;
+  if (jt == 0 && hscale) hscale[ot] = ldexpf(sc, e);
+#pragma unroll
+  for (int i = 0; i < N; ++i) {
+    const int j = jt + 32 * i;
+    if (j < rank && out) out[(long)ot * rank + j] = scaled ? sc * v[i] : v[i];
+    if (j < rp && hl) {
+      const float y = ldexpf(v[i], -e);
+      const uint16_t hi = T::narrow(y);
+      hl[(long)ot * 2 * rp + j] = hi;
+      hl[(long)ot * 2 * rp + rp + j] = T::narrow(y - T::widen(hi));
+    }
+  }
+}
+
 // low[t][j] = sum_k a[q][j][k] x[t][k] for 16 tokens a workgroup, the 8 wavefronts taking every 8th step
-// of k; out (t x rank) = low, or scaling low with `scaled`; hl[t][2 rp]: low / 2^e as two 16-bit values,
-// hscale[t] = scaling 2^e.
+// of k.
 template <class T, int RF>
 __global__ __launch_bounds__(512) void k_shrink(const uint16_t* __restrict__ x, long ldx, int t, int kk,
                                                 const uint16_t* __restrict__ a, long lda, int rank, int rp,
@@ -317,34 +356,69 @@ __global__ __launch_bounds__(512) void k_shrink(const uint16_t* __restrict__ x, 
     for (int r = 0; r < 4; ++r) red[wv][lane & 15][16 * f + 4 * quad + r] = keep[f][r];
   __syncthreads();
   // 32 threads a token
-  const int it = threadIdx.x >> 5, jt = threadIdx.x & 31, ot = blockIdx.x * 16 + it;
-  float v[(RF + 1) / 2], m = 0.0f;
+  const int it = threadIdx.x >> 5, jt = threadIdx.x & 31;
+  float v[(RF + 1) / 2];
 #pragma unroll
   for (int i = 0; i < (RF + 1) / 2; ++i) {
     const int j = jt + 32 * i;
     v[i] = 0.0f;
     if (j < rank)
       for (int w = 0; w < 8; ++w) v[i] += red[w][it][j];
-    m = fmaxf(m, __builtin_fabsf(v[i]));
   }
+  low_out<T, (RF + 1) / 2>(v, blockIdx.x * 16 + it, t, rank, rp, adapters, request, scaling, scaled, out, hl, hscale);
+}
+
+// The same for many tokens: tiles of 128 tokens of one adapter (by list) against its ranks, on the tiles of
+// mma16.h, split in k; part[split][token][rp]. The fragment loads of k_shrink touch 16 rows for 256 bytes,
+// which bounds it (4096 tokens, k = 14336, rank 64: 82 us); here a load takes 8 rows' whole lines.
+template <class T, int FP, int FQ, int WP, int WQ>
+__global__ __launch_bounds__(64 * WP * WQ, 2) void k_shrink_tiles(const uint16_t* __restrict__ x, long ldx, int kk,
+                                                                  const uint16_t* __restrict__ a, long lda, int rank,
+                                                                  int rp, const int* __restrict__ list,
+                                                                  const int4* __restrict__ tiles, int t, int share,
+                                                                  float* __restrict__ part) {
+  typedef MmaTile<T, false, false, FP, FQ, WP, WQ> M;
+  static_assert(M::BP == kTile, "a tile is an item");
+  __shared__ __align__(1024) uint8_t lds[M::LDS];
+  const int4 it = tiles[blockIdx.x];
+  if (it.x < 0) return;
+  mma_f4 acc[FP][FQ];
+  M::clear(acc);
+  M::run(lds_offset(lds), MmaOp{x, ldx, it.z, list + it.y}, MmaOp{a + (long)it.x * rank * lda, lda, rank}, 0, 0,
+         blockIdx.y * share, min(kk, ((int)blockIdx.y + 1) * share), acc);
+  const int lane = threadIdx.x & 63;
 #pragma unroll
-  for (int s = 16; s; s >>= 1) m = fmaxf(m, __shfl_xor(m, s));
-  if (ot >= t) return;
-  const int rq = request[ot];
-  const float sc = rq >= 0 && rq < adapters ? scaling[rq] : 0.0f;
-  const int e = m > 0.0f && m < __builtin_inff() ? __builtin_amdgcn_frexp_expf(m) : 0;
-  if (jt == 0 && hscale) hscale[ot] = ldexpf(sc, e);
+  for (int f = 0; f < FP; ++f)
 #pragma unroll
-  for (int i = 0; i < (RF + 1) / 2; ++i) {
-    const int j = jt + 32 * i;
-    if (j < rank && out) out[(long)ot * rank + j] = scaled ? sc * v[i] : v[i];
-    if (j < rp && hl) {
-      const float y = ldexpf(v[i], -e);
-      const uint16_t hi = T::narrow(y);
-      hl[(long)ot * 2 * rp + j] = hi;
-      hl[(long)ot * 2 * rp + rp + j] = T::narrow(y - T::widen(hi));
+    for (int r = 0; r < 4; ++r) {
+      const int i = M::row(0, f) + 4 * (lane >> 4) + r;
+      if (i >= it.z) continue;
+      float* o = part + ((long)blockIdx.y * t + list[it.y + i]) * rp;
+#pragma unroll
+      for (int g = 0; g < FQ; ++g) {
+        const int j = M::col(0, g) + (lane & 15);
+        if (j < rp) o[j] = acc[f][g][r];
+      }
     }
-  }
+}
+template <class T>
+__global__ __launch_bounds__(256) void k_shrink_sum(const float* __restrict__ part, int splits, int t, int rank, int rp,
+                                                    int adapters, const int* __restrict__ request,
+                                                    const float* __restrict__ scaling, int scaled,
+                                                    float* __restrict__ out, uint16_t* __restrict__ hl,
+                                                    float* __restrict__ hscale) {
+  const int tok = blockIdx.x * 8 + (threadIdx.x >> 5), jt = threadIdx.x & 31;
+  const int q = tok < t ? request[tok] : -1;
+  float v[4] = {};
+  if (q >= 0 && q < adapters)
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {
+      const int j = jt + 32 * i;
+      if (j < rank)
+#pragma unroll 4
+        for (int s = 0; s < splits; ++s) v[i] += part[((long)s * t + tok) * rp + j];
+    }
+  low_out<T, 4>(v, tok, t, rank, rp, adapters, request, scaling, scaled, out, hl, hscale);
 }
 
 struct WideArgs {
@@ -754,10 +828,47 @@ inline int slot_blocks(const PackedView& v, long t) {
 inline int expand_blocks(const PackedView& v) { return (int)std::min(((long)v.tiles * v.nkb + 3) / 4, 1l << 16); }
 inline int pad_blocks(const PadJob& j) { return blocks_for(j.rows * (j.dp / 8), 256 * 4, 8192); }
 
+#define STEP(expr)                       \
+  do {                                   \
+    hipError_t e_ = (expr);              \
+    if (e_ != hipSuccess) return e_;     \
+  } while (0)
+
+// How the low-rank vectors are made: k_shrink in about 82 us per 4096 tokens, 14336 of k and 5 operands of 16
+// rows; the tiles and their sum in two launches, worth it from about 20 us on.
+struct ShrinkPlan {
+  bool tiles;
+  int ntiles, splits, share;
+};
+ShrinkPlan shrink_plan(long t, long k, int adapters, int rp) {
+  ShrinkPlan p = {};
+  p.tiles = t >= 512 && 82.0 / 5 * (t / 4096.0) * (k / 14336.0) * (1 + rp / 16) > 20.0;
+  p.ntiles = (int)(t / kTile) + adapters;
+  const long n = std::max(1l, std::min(768 / std::max(1l, (t + kTile - 1) / kTile), k / 512));
+  p.share = (int)up((k + n - 1) / n, 64);
+  p.splits = (int)((k + p.share - 1) / p.share);
+  return p;
+}
 template <class T>
-hipError_t shrink(hipStream_t st, const uint16_t* x, long ldx, long t, int k, const uint16_t* a, long lda,
-                  const AdapterArgs& g, int scaled, float* out, uint16_t* hl, float* hscale) {
+hipError_t shrink(hipStream_t st, const ShrinkPlan& p, const int* list, const int4* tiles, float* part,
+                  const uint16_t* x, long ldx, long t, int k, const uint16_t* a, long lda, const AdapterArgs& g,
+                  int scaled, float* out, uint16_t* hl, float* hscale) {
   const int grid = (int)((t + 15) / 16), rp = rank_pad(g.rank);
+  if (p.tiles) {
+    auto go = [&](auto s) {
+      typedef decltype(s) S;
+      k_shrink_tiles<T, S::fp, S::fq, S::wp, S::wq><<<dim3(p.ntiles, p.splits), S::threads, 0, st>>>(
+          x, ldx, k, a, lda, g.rank, rp, list, tiles, (int)t, p.share, part);
+      return hipGetLastError();
+    };
+    if (rp <= 16) STEP(go(MmaShape<2, 1, 4, 1>{}));
+    else if (rp <= 32) STEP(go(MmaShape<2, 2, 4, 1>{}));
+    else if (rp <= 64) STEP(go(MmaShape<4, 2, 2, 2>{}));
+    else STEP(go(MmaShape<4, 4, 2, 2>{}));
+    k_shrink_sum<T><<<(int)((t + 7) / 8), 256, 0, st>>>(part, p.splits, (int)t, g.rank, rp, g.adapters, g.request,
+                                                        g.scaling, scaled, out, hl, hscale);
+    return hipGetLastError();
+  }
   auto go = [&](auto rf) {
     k_shrink<T, decltype(rf)::value><<<grid, 512, 0, st>>>(x, ldx, (int)t, k, a, lda, g.rank, rp, g.adapters, g.request,
                                                            g.scaling, scaled, out, hl, hscale);
@@ -802,12 +913,6 @@ hipError_t wide_product(hipStream_t st, const WidePlan& p, WideArgs w) {
   });
 }
 
-#define STEP(expr)                       \
-  do {                                   \
-    hipError_t e_ = (expr);              \
-    if (e_ != hipSuccess) return e_;     \
-  } while (0)
-
 // The workspace's parts are laid out by the same code that runs the steps: with `run` false only the
 // size is taken.
 template <class T>
@@ -825,6 +930,11 @@ hipError_t wide(hipStream_t st, const PackedView& v, const AdapterArgs& a, void*
   uint16_t* bpad = m.take<uint16_t>(pad_b ? (size_t)a.adapters * v.m * rp : 0);
   uint16_t* hl = m.take<uint16_t>(low ? (size_t)a.t * 2 * rp : 0);
   float* hscale = m.take<float>(low ? a.t : 0);
+  const ShrinkPlan sp = shrink_plan(a.t, n8, a.adapters, rp);
+  const bool tiled = low && sp.tiles;
+  int* list = m.take<int>(tiled ? a.t : 0);
+  int4* tiles = m.take<int4>(tiled ? sp.ntiles : 0);
+  float* lowpart = m.take<float>(tiled ? (size_t)sp.splits * a.t * rp : 0);
   float* parts = m.take<float>(plan.splits > 1 ? (size_t)plan.splits * a.t * up(v.m, 4) : 0);
   *bytes = m.at;
   if (!run) return hipSuccess;
@@ -851,10 +961,14 @@ hipError_t wide(hipStream_t st, const PackedView& v, const AdapterArgs& a, void*
     p.pad[2] = pad_blocks(p.pads[2]);
     bb = bpad;
   }
+  if (tiled) {
+    p.lists = a.adapters;
+    p.list = {a.request, (int)a.t, a.adapters, kItem, 0, list, nullptr, nullptr, tiles, sp.ntiles};
+  }
   k_prepare<T><<<p.total(), 256, slot_lds(v), st>>>(v, p);
   STEP(hipGetLastError());
   if (low) {
-    STEP(shrink<T>(st, x, ldx, a.t, n8, aa, lda, a, 0, a.low, hl, hscale));
+    STEP(shrink<T>(st, sp, list, tiles, lowpart, x, ldx, a.t, n8, aa, lda, a, 0, a.low, hl, hscale));
     w.e = bb;
     w.rp = rp;
     w.adapters = a.adapters;
@@ -914,6 +1028,10 @@ hipError_t grad(hipStream_t st, const PackedView& v, const AdapterArgs& a, void*
   int* list = m.take<int>(low ? a.t : 0);
   int4* items = m.take<int4>(low ? slots : 0);
   int2* of = m.take<int2>(low ? a.adapters : 0);
+  const ShrinkPlan sp = shrink_plan(a.t, m8, a.adapters, rp);
+  const bool tiled = low && !few && sp.tiles;
+  int4* tiles = m.take<int4>(tiled ? sp.ntiles : 0);
+  float* lowpart = m.take<float>(tiled ? (size_t)sp.splits * a.t * rp : 0);
   float* part_a = m.take<float>(low ? (size_t)slots * rp * nbn * 128 : 0);
   float* part_b = m.take<float>(low ? (size_t)slots * rp * nbm * 128 : 0);
   *bytes = m.at;
@@ -933,7 +1051,7 @@ hipError_t grad(hipStream_t st, const PackedView& v, const AdapterArgs& a, void*
   if (low) {
     p.a = a.a, p.b = a.b, p.adapters = a.adapters, p.rank = a.rank, p.rp = rp, p.mp = m8, p.bt = bt, p.at = at;
     p.lists = a.adapters;
-    p.list = {a.request, t, a.adapters, chunk, slots, list, items, of};
+    p.list = {a.request, t, a.adapters, chunk, slots, list, items, of, tiled ? tiles : nullptr, sp.ntiles};
     if (t && few) {
       p.dots = t * ((a.rank + 7) / 8);
       p.dot = {a.x, a.ldx, t, v.m, a.b, a.rank, a.adapters, a.request, a.scaling, u};
@@ -947,7 +1065,7 @@ hipError_t grad(hipStream_t st, const PackedView& v, const AdapterArgs& a, void*
   WideArgs w = {};
   FinishArgs f = {};
   if (low) {
-    if (t && !few) STEP(shrink<T>(st, dy, lddy, a.t, m8, bt, m8, a, 1, u, hl, hscale));
+    if (t && !few) STEP(shrink<T>(st, sp, list, tiles, lowpart, dy, lddy, a.t, m8, bt, m8, a, 1, u, hl, hscale));
     const OuterJob jb = {dy, nullptr, lddy, v.m, a.low, a.scaling, part_b};
     const OuterJob ja = {a.codes, a.scales, v.n, v.n, u, nullptr, part_a};
     const bool vec = v.n % 8 == 0 && (uintptr_t)a.codes % 8 == 0;

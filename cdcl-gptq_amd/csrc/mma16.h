@@ -88,11 +88,12 @@ __device__ inline void pad_rows16(const PadJob& j, long b, long nb) {
 }
 
 // An operand of C: `rows` rows of k values each, element (i, k) at p[i ld + k] or, rows contiguous, at
-// p[k ld + i].
+// p[k ld + i]. With a list (k contiguous only) row i is row list[i] of p.
 struct MmaOp {
   const uint16_t* p;
   long ld;
   int rows;
+  const int* list = nullptr;
 };
 
 static __device__ uint4 mma_zero_page[1];  // never written
@@ -124,7 +125,9 @@ struct MmaTile {
       const int g = (s % (B / 8)) ^ (2 * ((k & 3) | ((k >> 1) & 4)));
       return o.p + (long)(k0 + k) * o.ld + min(r0 + 8 * g, (o.rows - 1) & ~7);
     } else {
-      return o.p + (long)min(r0 + (s >> 3), o.rows - 1) * o.ld + k0 + granule_k<S, B>(s);
+      int row = min(r0 + (s >> 3), o.rows - 1);
+      if (o.list) row = o.list[row];
+      return o.p + (long)row * o.ld + k0 + granule_k<S, B>(s);
     }
   }
 

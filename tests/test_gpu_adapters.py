@@ -196,7 +196,10 @@ def check_backward(packed, w, ad, x, q, dy, tune, ctx):
                          [(1, 64, 128, 4, 128, 1, 8, "any"), (40, 130, 257, 3, 48, 3, 5, "any"),
                           (100, 201, 1350, 4, 128, 4, 16, "any"), (300, 512, 512, 2, 64, 2, 64, "sorted"),
                           (700, 96, 264, 4, 32, 7, 33, "any"), (1300, 128, 256, 8, 128, 1, 128, "sorted"),
-                          (65, 1001, 72, 5, 0, 40, 3, "any")])
+                          (65, 1001, 72, 5, 0, 40, 3, "any"),
+                          # long sums: the low-rank vectors by tiles of 128 tokens of one adapter
+                          (1300, 96, 8192, 4, 128, 3, 128, "any"), (1301, 8200, 100, 4, 128, 5, 120, "any"),
+                          (2100, 72, 9000, 3, 128, 2, 60, "sorted")])
 def test_gradient(ctx, tune, dtype, t, m, n, bits, group, r, rank, order):
     packed, w, _ = make_layer(ctx, tune, t + m, m, n, bits, group)
     ad = make_adapters(tune, 3, r, rank, m, n, dtype)

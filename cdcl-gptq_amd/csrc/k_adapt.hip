@@ -505,7 +505,9 @@ __global__ __launch_bounds__(64 * WP * WQ, 2) void k_wide(WideArgs a) {
 // part[slot][j][c] = sum over the item's tokens of l[t][j] X[t][c], j in 16 RF ranks from j0, c in 128
 // columns a wavefront. X: 8-bit codes with their scales (I8), or 16-bit values; l times scaling[q] if given.
 // A lane reads 8 neighbouring columns of 8 tokens, the next ones while these are multiplied: row i of the
-// f-th MFMA operand is column 8 i + f. The item's l lies in LDS, its token list beside it.
+// f-th MFMA operand is column 8 i + f. The item's l lies in LDS, its token list beside it; it enters the
+// matrix cores as the sum of two 16-bit values, in f16 divided by 2^e to keep it in range (e grows with the
+// largest l so far, the sums go along).
 struct OuterJob {
   const void* x;
   const float* xscale;
@@ -529,6 +531,8 @@ __device__ __forceinline__ void outer(const OuterJob& k, int colgroup, int rank,
   for (int f = 0; f < 8; ++f)
 #pragma unroll
     for (int g = 0; g < RF; ++g) acc[f][g] = mma_f4{};
+  int ex = -126;  // f16: the exponent that ll and the sums are divided by
+  __shared__ float wtop[4];
   struct Raw {
     mma_u4 h[I8 ? 1 : 8];
     uint2 b[I8 ? 8 : 1];
@@ -578,6 +582,7 @@ __device__ __forceinline__ void outer(const OuterJob& k, int colgroup, int rank,
         for (int i = 0; i < 2; ++i) {
           y[i] = ll[t0 + 8 * quad + 2 * p + i][16 * g + (lane & 15)];
           if constexpr (I8) y[i] *= r.s[2 * p + i];
+          if constexpr (T::kind == F16::kind) y[i] = ldexpf(y[i], -ex);
           h[i] = T::narrow(y[i]);
         }
         hi[p] = (uint32_t)h[0] | ((uint32_t)h[1] << 16);
@@ -600,6 +605,7 @@ __device__ __forceinline__ void outer(const OuterJob& k, int colgroup, int rank,
     __syncthreads();
     // l of these tokens, 0 past the last: four ranks a load, half of the thread's loads in flight at once
     constexpr int PER = 4 * RF, BATCH = PER < 8 ? PER : 8;
+    float top = 0.0f;
     for (int e0 = 0; e0 < kItem * PER; e0 += 256 * BATCH) {
       if (e0 / PER >= ((n + 31) & ~31)) break;
       mma_f4 v[BATCH];
@@ -622,10 +628,32 @@ __device__ __forceinline__ void outer(const OuterJob& k, int colgroup, int rank,
       for (int u = 0; u < BATCH; ++u) {
         const int e = e0 + 256 * u + threadIdx.x, i = e / PER, j = 4 * (e - i * PER);
 #pragma unroll
-        for (int r = 0; r < 4; ++r) ll[i][j + r] = mul * v[u][r];
+        for (int r = 0; r < 4; ++r) {
+          ll[i][j + r] = mul * v[u][r];
+          const float m = __builtin_fabsf(mul * v[u][r]);
+          if (m < __builtin_inff()) top = fmaxf(top, m);
+        }
       }
     }
+    if constexpr (T::kind == F16::kind) {
+#pragma unroll
+      for (int s = 32; s; s >>= 1) top = fmaxf(top, __shfl_xor(top, s));
+      if (lane == 0) wtop[wv] = top;
+    }
     __syncthreads();
+    if constexpr (T::kind == F16::kind) {
+      top = fmaxf(fmaxf(wtop[0], wtop[1]), fmaxf(wtop[2], wtop[3]));
+      const int to = max(ex, top > 0.0f ? __builtin_amdgcn_frexp_expf(top) : -126);
+      if (to != ex) {
+#pragma unroll
+        for (int f = 0; f < 8; ++f)
+#pragma unroll
+          for (int g = 0; g < RF; ++g)
+#pragma unroll
+            for (int r = 0; r < 4; ++r) acc[f][g][r] = ldexpf(acc[f][g][r], ex - to);
+        ex = to;
+      }
+    }
     if (c0 >= k.cols) continue;
     Raw now, next;
     load(0, now);
@@ -636,6 +664,14 @@ __device__ __forceinline__ void outer(const OuterJob& k, int colgroup, int rank,
     }
   }
   if (c0 >= k.cols) return;
+  if constexpr (T::kind == F16::kind) {
+#pragma unroll
+    for (int f = 0; f < 8; ++f)
+#pragma unroll
+      for (int g = 0; g < RF; ++g)
+#pragma unroll
+        for (int r = 0; r < 4; ++r) acc[f][g][r] = ldexpf(acc[f][g][r], ex);
+  }
   const long ldp = (long)nb * 128;
 #pragma unroll
   for (int g = 0; g < RF; ++g) {

@@ -38,8 +38,8 @@ int check_half(cdclq_ctx* ctx, int dtype) {
   return CDCLQ_OK;
 }
 
-// Sizes whose tiles and tables are counted in 32 bits.
-constexpr size_t kMaxTokens = (size_t)1 << 24, kMaxWidth = (size_t)1 << 20, kMaxVocab = (size_t)1 << 28;
+// Sizes whose tiles and tables are counted in 32 bits (and items in a grid's second dimension).
+constexpr size_t kMaxTokens = (size_t)1 << 22, kMaxWidth = (size_t)1 << 20, kMaxVocab = (size_t)1 << 24;
 
 int check_size(cdclq_ctx* ctx, const char* what, size_t got, size_t most) {
   if (got > most)

@@ -207,6 +207,20 @@ def test_gradient(ctx, tune, dtype, t, m, n, bits, group, r, rank, order):
     check_backward(packed, w, ad, normal(1, t, n, dtype=dtype), q, normal(2, t, m, dtype=dtype), tune, ctx)
 
 
+@pytest.mark.parametrize("size,factor", [(1e-4, 1), (1e4, 16)])
+def test_half_precision_gradient_of_small_and_large_low_rank_vectors(ctx, tune, size, factor):
+    """low beyond float16's range on both sides (up to 1e6, down to 1e-7): B's gradient keeps its precision
+    where its own values are in range."""
+    t, m, n, rank = 700, 96, 256, 16
+    packed, w, _ = make_layer(ctx, tune, 4, m, n, 4, 64)
+    ad = make_adapters(tune, 3, 2, rank, m, n, torch.float16)
+    ad.a.mul_(factor)
+    x = normal(1, t, n, std=size, dtype=torch.float16)
+    x[300:] *= 2.0 ** -6
+    assert torch.isfinite(x).all()
+    check_backward(packed, w, ad, x, make_request(t, t, 2, "any"), normal(2, t, m, std=1e-3, dtype=torch.float16), tune, ctx)
+
+
 def test_no_adapters_unused_adapters_and_no_tokens(ctx, tune):
     packed, w, big = make_layer(ctx, tune, 12, 90, 200, 4, 128)
     b = torch.bfloat16

@@ -815,9 +815,33 @@ __device__ void sum_parts(const SumJob& k, int b) {
   k.out[(long)t * k.ldo + c] = T::narrow(s);
 }
 
+// The same from slot order for many tokens: `rows` tokens at a time through LDS in f32 (a column's gather
+// from memory costs four times the bytes).
+template <class T>
+__device__ void sum_slots(const PackedView& v, const SumJob& k, int rows, float* lds, int b) {
+  const int ns = packed_slots(v), t0 = b * rows;
+  for (int r = 0; r < rows && t0 + r < k.t; ++r) {
+    const float* p = k.parts + (long)(t0 + r) * k.ldp;
+    for (int s = 4 * threadIdx.x; s < ns; s += 1024) {
+      const int4 c = *reinterpret_cast<const int4*>(v.col + s);
+      mma_f4 x = {};
+#pragma unroll 4
+      for (int i = 0; i < k.splits; ++i) x += *reinterpret_cast<const mma_f4*>(p + (long)i * k.t * k.ldp + s);
+      float* d = lds + r * v.n;
+      if (c.x >= 0) d[c.x] = x[0];
+      if (c.y >= 0) d[c.y] = x[1];
+      if (c.z >= 0) d[c.z] = x[2];
+      if (c.w >= 0) d[c.w] = x[3];
+    }
+  }
+  __syncthreads();
+  for (int r = 0; r < rows && t0 + r < k.t; ++r)
+    for (int c = threadIdx.x; c < v.n; c += 256) k.out[(long)(t0 + r) * k.ldo + c] = T::narrow(lds[r * v.n + c]);
+}
+
 // Workgroups of each part; 0: not asked for.
 struct FinishArgs {
-  int nda, ndb, nback, nsum;
+  int nda, ndb, nback, nsum, sum_rows;  // sum_rows: of sum_slots, 0: sum_parts
   JoinJob da, db;
   const int2* of;
   int rank, rp;
@@ -830,7 +854,10 @@ __global__ __launch_bounds__(256) void k_finish(PackedView v, FinishArgs k) {
   int b = blockIdx.x;
   if (b < k.nback) return from_slots(v, k.back, lds, b);
   b -= k.nback;
-  if (b < k.nsum) return sum_parts<T>(k.sum, b);
+  if (b < k.nsum) {
+    if (k.sum_rows) return sum_slots<T>(v, k.sum, k.sum_rows, reinterpret_cast<float*>(lds), b);
+    return sum_parts<T>(k.sum, b);
+  }
   b -= k.nsum;
   if (b < k.ndb) return join_db<T>(k.db, k.of, k.rank, k.rp, b);
   join_da<T>(k.da, k.of, k.rank, k.rp, b - k.ndb);
@@ -921,13 +948,13 @@ hipError_t shrink(hipStream_t st, const ShrinkPlan& p, const int* list, const in
 struct WidePlan {
   int pick, splits, share;
 };
-WidePlan wide_plan(long rows, long t, long k, bool parts_anyway) {
+WidePlan wide_plan(long rows, long t, long k, bool strided, bool parts_anyway) {
   WidePlan best = {};
   double least = 0;
   for (int i = 0; i < kMmaShapes; ++i)
     for (int n = 1; n == 1 || (n <= 16 && k / n >= 256); n *= 2) {
       const bool parts = parts_anyway || n > 1;
-      const double c = mma_cost(rows, t, k, i, n) + (parts ? n * (8.0 / 4e6) * t * rows : 0.0) +
+      const double c = mma_cost(rows, t, k, i, n, strided) + (parts ? n * (8.0 / 4e6) * t * rows : 0.0) +
                        (n > 1 && !parts_anyway ? 4.0 : 0.0);
       if ((i == 0 && n == 1) || c < least) least = c, best.pick = i, best.splits = n;
     }
@@ -957,7 +984,7 @@ hipError_t wide(hipStream_t st, const PackedView& v, const AdapterArgs& a, void*
   const bool low = a.rank > 0;
   const bool pad_x = low && !aligned16(a.x, a.ldx, v.n), pad_a = low && !aligned16(a.a, v.n, v.n);
   const bool pad_b = low && (rp != a.rank || (uintptr_t)a.b % 16);
-  const WidePlan plan = wide_plan(v.m, a.t, ns, false);
+  const WidePlan plan = wide_plan(v.m, a.t, ns, false, false);
   Arena m(work);
   uint16_t* w16 = m.take<uint16_t>((size_t)v.tiles * 16 * ns);
   uint16_t* xp = m.take<uint16_t>((size_t)a.t * ns);
@@ -1049,7 +1076,7 @@ hipError_t grad(hipStream_t st, const PackedView& v, const AdapterArgs& a, void*
   const int nbn = (v.n + 127) / 128, nbm = (v.m + 127) / 128;
   const int chunk = outer_chunk(a.t, a.adapters, rp, v.n, v.m);
   const int slots = (int)(a.t / chunk) + a.adapters;
-  const WidePlan plan = wide_plan(ns, a.t, v.m, few);
+  const WidePlan plan = wide_plan(ns, a.t, v.m, true, few);
   const bool parts_out = few || plan.splits > 1;
   Arena m(work);
   uint16_t* w16 = m.take<uint16_t>((size_t)v.tiles * 16 * ns);
@@ -1143,12 +1170,15 @@ hipError_t grad(hipStream_t st, const PackedView& v, const AdapterArgs& a, void*
       const bool add = low && few;
       f.sum = {parts, plan.splits, t, v.n, (long)ns, v.slot, add ? a.a : nullptr, u, a.rank, a.adapters, a.request, a.y, a.ldy};
       f.nsum = t * ((v.n + 255) / 256);
+      f.sum_rows = few ? 0 : (int)std::min<size_t>(4, 65536 / (4 * (size_t)v.n));
+      if (f.sum_rows) f.nsum = (t + f.sum_rows - 1) / f.sum_rows;
     } else {
       f.back = {dxp, t, slot_rows(v), aligned16(a.y, a.ldy, v.n), a.y, a.ldy};
       f.nback = slot_blocks(v, t);
     }
   }
-  k_finish<T><<<f.nda + f.ndb + f.nback + f.nsum, 256, f.nback ? slot_lds(v) : 0, st>>>(v, f);
+  const size_t lds = f.nback ? slot_lds(v) : 4 * (size_t)f.sum_rows * v.n;
+  k_finish<T><<<f.nda + f.ndb + f.nback + f.nsum, 256, lds, st>>>(v, f);
   return hipGetLastError();
 }
 

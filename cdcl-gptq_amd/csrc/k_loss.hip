@@ -442,7 +442,7 @@ LossPlan loss_plan(long t, long d, long v, bool pad_w, bool grad) {
     int best = -1;
     for (int i = 0; i < kMmaShapes; ++i)
       if (!p.direct || direct_shape(i))
-        if (best < 0 || mma_cost(rows, cols, k, i, 1) < mma_cost(rows, cols, k, best, 1)) best = i;
+        if (best < 0 || mma_cost(rows, cols, k, i, 1, false) < mma_cost(rows, cols, k, best, 1, false)) best = i;
     return best;
   };
   p.wpad = pad_w && !p.direct ? take(2 * (size_t)v * p.dp) : 0;
@@ -470,7 +470,7 @@ LossPlan loss_plan(long t, long d, long v, bool pad_w, bool grad) {
       const MmaShapeTime s = kMmaTimes[i];
       const long np = (p.dp + s.bp - 1) / s.bp, nq = (t + s.bq - 1) / s.bq, round = 256 * s.per_cu;
       const long n = std::max(1l, std::min(round / (np * nq), (long)p.piece / 512));
-      const double c = mma_cost(p.dp, t, p.piece, i, n) * (s.bq <= 64 ? 2.0 : i ? 1.33 : 1.0) + n * (8.0 / 4e6) * t * p.dp;
+      const double c = mma_cost(p.dp, t, p.piece, i, n, false) * (s.bq <= 64 ? 2.0 : i ? 1.33 : 1.0) + n * (8.0 / 4e6) * t * p.dp;
       if (best < 0 || c < best) {
         best = c;
         p.dx_tiles = i;
@@ -478,7 +478,7 @@ LossPlan loss_plan(long t, long d, long v, bool pad_w, bool grad) {
         p.dx_bytes = 4 * (size_t)p.dp * std::max<size_t>(up(t, s.bq), (size_t)(round / np) * s.bq);
       }
     }
-    p.dw_tiles = mma_cost(p.dp, p.piece, t, 5, 1) < mma_cost(p.dp, p.piece, t, 0, 1) ? 5 : 0;
+    p.dw_tiles = mma_cost(p.dp, p.piece, t, 5, 1, false) < mma_cost(p.dp, p.piece, t, 0, 1, false) ? 5 : 0;
     p.d = take(2 * (size_t)t * p.piece);
     p.dxacc = take(p.dx_bytes);
   }

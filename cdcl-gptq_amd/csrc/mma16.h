@@ -387,16 +387,18 @@ struct MmaShape {
 
 // The shapes, by number. Wide tiles read each operand less often; small ones spread few results over more
 // CUs, narrow ones compute no columns that nobody asked for. `us`: a tile's stage of 64 k with every CU busy,
-// measured on 4096 x 65536 results over k = 4096 (the first two narrow ones estimated); `per_cu`: the
-// workgroups that a CU's LDS holds.
+// measured on 4096 x 65536 results over k = 4096 (the narrow ones estimated); `per_cu`: the workgroups that
+// a CU's LDS holds; `alone`: a stage with few tiles in flight, which the latency of its loads and reads sets,
+// measured on 200 x 4096 results over 4096, and (P's rows contiguous) on 100 x 2688 over 6720.
 constexpr int kMmaShapes = 9;
 struct MmaShapeTime {
   int bp, bq, per_cu;
-  double us;
+  double us, alone, alone_strided;
 };
-constexpr MmaShapeTime kMmaTimes[kMmaShapes] = {{256, 256, 1, 1.66}, {256, 128, 1, 1.07}, {256, 64, 2, 0.55},
-                                                {256, 32, 2, 0.40},  {256, 16, 2, 0.33},  {128, 128, 2, 0.50},
-                                                {128, 64, 3, 0.31},  {128, 32, 4, 0.22},  {128, 16, 4, 0.18}};
+constexpr MmaShapeTime kMmaTimes[kMmaShapes] = {
+    {256, 256, 1, 1.66, 0.90, 1.15}, {256, 128, 1, 1.07, 0.65, 0.86}, {256, 64, 2, 0.55, 0.51, 0.77},
+    {256, 32, 2, 0.40, 0.50, 0.75},  {256, 16, 2, 0.33, 0.50, 0.70},  {128, 128, 2, 0.50, 0.49, 0.69},
+    {128, 64, 3, 0.31, 0.43, 0.59},  {128, 32, 4, 0.22, 0.42, 0.55},  {128, 16, 4, 0.18, 0.42, 0.55}};
 template <class F>
 hipError_t with_mma_shape(int pick, F f) {
   switch (pick) {
@@ -412,21 +414,16 @@ hipError_t with_mma_shape(int pick, F f) {
   }
 }
 // Microseconds of a product of `rows` x `cols` results over k, `splits` ways in k: rounds of tiles over 256
-// CUs, each so many stages. A stage takes at least the 0.42 us of its loads' latency, a round 4 us more for
-// its first loads and its results.
-inline double mma_cost(long rows, long cols, long k, int pick, long splits) {
+// CUs, each so many stages and 4 us more for its first loads and its results. strided: P's rows contiguous
+// (their transposed reads cost the smaller tiles a fifth).
+inline double mma_cost(long rows, long cols, long k, int pick, long splits, bool strided) {
   const MmaShapeTime s = kMmaTimes[pick];
   const long tiles = ((rows + s.bp - 1) / s.bp) * ((cols + s.bq - 1) / s.bq) * splits;
   const long stages = std::max(2l, ((k + splits - 1) / splits + 63) / 64);
   const long rounds = (tiles + 256 * s.per_cu - 1) / (256 * s.per_cu);
   const long shared = std::min<long>(s.per_cu, (tiles + 255) / 256);
-  return rounds * (std::max(s.us * shared, 0.42) * stages + 4.0);
-}
-inline int mma_pick(long rows, long cols, long k) {
-  int best = 0;
-  for (int i = 1; i < kMmaShapes; ++i)
-    if (mma_cost(rows, cols, k, i, 1) < mma_cost(rows, cols, k, best, 1)) best = i;
-  return best;
+  const double busy = s.us * shared * (strided && pick ? 1.2 : 1.0);
+  return rounds * (std::max(busy, strided ? s.alone_strided : s.alone) * stages + 4.0);
 }
 
 }  // namespace cdclq

@@ -263,28 +263,29 @@ __device__ __forceinline__ int next_adapter(int q, uint64_t& left) {
 }
 
 // Ranks jt, jt + 32, ... of token ot, by 32 threads: out (t x rank) = low, or scaling low with `scaled`;
-// hl[t][2 rp]: low / 2^e as two 16-bit values, hscale[t] = scaling 2^e.
+// hl[t][2 rp]: scaling low / 2^e as two 16-bit values, hscale[t] = 2^e; e is not below kLeastExp, where
+// f16's smallest values times its largest weights lie under half of its smallest result.
+constexpr int kLeastExp = -24;
 template <class T, int N>
 __device__ __forceinline__ void low_out(const float (&v)[N], int ot, int t, int rank, int rp, int adapters,
                                         const int* request, const float* scaling, int scaled, float* out, uint16_t* hl,
                                         float* hscale) {
-  const int jt = threadIdx.x & 31;
+  const int jt = threadIdx.x & 31, rq = request[min(ot, t - 1)];
+  const float sc = rq >= 0 && rq < adapters ? scaling[rq] : 0.0f;
   float m = 0.0f;
 #pragma unroll
-  for (int i = 0; i < N; ++i) m = fmaxf(m, __builtin_fabsf(v[i]));
+  for (int i = 0; i < N; ++i) m = fmaxf(m, __builtin_fabsf(sc * v[i]));
 #pragma unroll
   for (int s = 16; s; s >>= 1) m = fmaxf(m, __shfl_xor(m, s));
   if (ot >= t) return;
-  const int rq = request[ot];
-  const float sc = rq >= 0 && rq < adapters ? scaling[rq] : 0.0f;
-  const int e = m > 0.0f && m < __builtin_inff() ? __builtin_amdgcn_frexp_expf(m) : 0;
-  if (jt == 0 && hscale) hscale[ot] = ldexpf(sc, e);
+  const int e = m > 0.0f && m < __builtin_inff() ? max(kLeastExp, __builtin_amdgcn_frexp_expf(m)) : 0;
+  if (jt == 0 && hscale) hscale[ot] = ldexpf(1.0f, e);
 #pragma unroll
   for (int i = 0; i < N; ++i) {
     const int j = jt + 32 * i;
     if (j < rank && out) out[(long)ot * rank + j] = scaled ? sc * v[i] : v[i];
     if (j < rp && hl) {
-      const float y = ldexpf(v[i], -e);
+      const float y = ldexpf(sc * v[i], -e);
       const uint16_t hi = T::narrow(y);
       hl[(long)ot * 2 * rp + j] = hi;
       hl[(long)ot * 2 * rp + rp + j] = T::narrow(y - T::widen(hi));
@@ -454,15 +455,57 @@ __global__ __launch_bounds__(64 * WP * WQ, 2) void k_wide(WideArgs a) {
          min(a.k, (split + 1) * a.share), acc);
   const int lane = threadIdx.x & 63, quad = lane >> 4;
   const long ldp = (a.rows + 3) & ~3;
+  if (a.e && split == 0) {
+    int q[FQ];
+    float scale[FQ];
+    bool alike = true;  // every token of the wavefront has one and the same adapter, in range of f32
+    int only = 0;
 #pragma unroll
-  for (int g = 0; g < FQ; ++g) {
-    const int t = M::col(q0, g) + (lane & 15);
-    if (a.e && split == 0) {
-      const int q = t < a.t ? a.request[t] : -1;
-      const bool known = q >= 0 && q < a.adapters;
-      const float scale = known ? a.hscale[t] : 0.0f;
-      uint64_t left = __builtin_amdgcn_ballot_w64(known);
-      for (int ad = next_adapter(q, left); ad >= 0; ad = next_adapter(q, left)) {
+    for (int g = 0; g < FQ; ++g) {
+      const int t = M::col(q0, g) + (lane & 15);
+      q[g] = t < a.t ? a.request[t] : -1;
+      scale[g] = q[g] >= 0 && q[g] < a.adapters ? a.hscale[t] : 1.0f;
+      if (g == 0) only = __builtin_amdgcn_readfirstlane(q[0]);
+      alike &= __builtin_amdgcn_ballot_w64(t < a.t && !(q[g] == only && scale[g] <= 0x1p40f)) == 0;
+    }
+    alike &= only >= 0 && only < a.adapters;
+    // alike: straight onto the sums, which are divided by 2^e meanwhile: no second set of them, so all tokens
+    // at once and an adapter's rows read once. (Loops of no passes, not branches: those would copy the sums.)
+#pragma unroll
+    for (int g = 0; g < FQ; ++g) {
+      const float inv = alike ? 1.0f / scale[g] : 1.0f;
+#pragma unroll
+      for (int f = 0; f < FP; ++f) acc[f][g] *= inv;
+    }
+    const uint16_t* const e = a.e + (alike ? (long)only * a.rows * a.rp : 0);
+    const int kfs = alike ? 2 * a.rp : 0;
+    for (int kf = 0; kf < kfs; kf += 32) {
+      const int k = kf + 8 * quad, c = k < a.rp ? k : k - a.rp;
+      v8 ev[FP], h[FQ];
+#pragma unroll
+      for (int f = 0; f < FP; ++f) {
+        const uint32_t row = min(M::row(p0, f) + (lane & 15), a.rows - 1);
+        ev[f] = __builtin_bit_cast(v8, *reinterpret_cast<const mma_u4*>(e + (row * (uint32_t)a.rp + c)));
+      }
+#pragma unroll
+      for (int g = 0; g < FQ; ++g) {
+        const uint32_t t = min(M::col(q0, g) + (lane & 15), a.t - 1);
+        h[g] = __builtin_bit_cast(v8, *reinterpret_cast<const mma_u4*>(a.hl + (t * (uint32_t)(2 * a.rp) + k)));
+      }
+#pragma unroll
+      for (int f = 0; f < FP; ++f)
+#pragma unroll
+        for (int g = 0; g < FQ; ++g) acc[f][g] = T::mfma(ev[f], h[g], acc[f][g]);
+    }
+#pragma unroll
+    for (int g = 0; g < FQ; ++g) {
+      const float back = alike ? scale[g] : 1.0f;
+#pragma unroll
+      for (int f = 0; f < FP; ++f) acc[f][g] *= back;
+      const int t = M::col(q0, g) + (lane & 15);
+      const bool known = q[g] >= 0 && q[g] < a.adapters;
+      uint64_t left = alike ? 0 : __builtin_amdgcn_ballot_w64(known);
+      for (int ad = next_adapter(q[g], left); ad >= 0; ad = next_adapter(q[g], left)) {
         mma_f4 d[FP];
 #pragma unroll
         for (int f = 0; f < FP; ++f) d[f] = mma_f4{};
@@ -482,15 +525,19 @@ __global__ __launch_bounds__(64 * WP * WQ, 2) void k_wide(WideArgs a) {
         for (int f = 0; f < FP; ++f)
 #pragma unroll
           for (int r = 0; r < 4; ++r)
-            if (q == ad) acc[f][g][r] = __builtin_fmaf(scale, d[f][r], acc[f][g][r]);
+            if (q[g] == ad) acc[f][g][r] = __builtin_fmaf(scale[g], d[f][r], acc[f][g][r]);
       }
-      if (!known && q != -1) {  // no such adapter
+      if (!known && q[g] != -1) {  // no such adapter
 #pragma unroll
         for (int f = 0; f < FP; ++f)
 #pragma unroll
           for (int r = 0; r < 4; ++r) acc[f][g][r] = __builtin_nanf("");
       }
     }
+  }
+#pragma unroll
+  for (int g = 0; g < FQ; ++g) {
+    const int t = M::col(q0, g) + (lane & 15);
     if (a.parts && t < a.t) {
 #pragma unroll
       for (int f = 0; f < FP; ++f) {

@@ -266,6 +266,7 @@ __device__ __forceinline__ int next_adapter(int q, uint64_t& left) {
 // hl[t][2 rp]: scaling low / 2^e as two 16-bit values, hscale[t] = 2^e; e is not below kLeastExp, where
 // f16's smallest values times its largest weights lie under half of its smallest result.
 constexpr int kLeastExp = -24;
+constexpr float kMostScale = 0x1p40f;  // up to here sums divided by 2^e keep what counts of them
 template <class T, int N>
 __device__ __forceinline__ void low_out(const float (&v)[N], int ot, int t, int rank, int rp, int adapters,
                                         const int* request, const float* scaling, int scaled, float* out, uint16_t* hl,
@@ -458,17 +459,41 @@ __global__ __launch_bounds__(64 * WP * WQ, 2) void k_wide(WideArgs a) {
   if (a.e && split == 0) {
     int q[FQ];
     float scale[FQ];
-    bool alike = true;  // every token of the wavefront has one and the same adapter, in range of f32
-    int only = 0;
+    // alike: every token of the wavefront has one and the same adapter, or none, and 2^e is in range of f32
+    int only = -1;
 #pragma unroll
     for (int g = 0; g < FQ; ++g) {
       const int t = M::col(q0, g) + (lane & 15);
       q[g] = t < a.t ? a.request[t] : -1;
       scale[g] = q[g] >= 0 && q[g] < a.adapters ? a.hscale[t] : 1.0f;
-      if (g == 0) only = __builtin_amdgcn_readfirstlane(q[0]);
-      alike &= __builtin_amdgcn_ballot_w64(t < a.t && !(q[g] == only && scale[g] <= 0x1p40f)) == 0;
+      const uint64_t some = __builtin_amdgcn_ballot_w64(q[g] != -1);
+      if (only == -1 && some) only = __builtin_amdgcn_readlane(q[g], __builtin_ctzll(some));
     }
-    alike &= only >= 0 && only < a.adapters;
+    bool alike = only >= 0 && only < a.adapters, bare = false;
+#pragma unroll
+    for (int g = 0; g < FQ; ++g) {
+      alike &= __builtin_amdgcn_ballot_w64(q[g] != -1 && !(q[g] == only && scale[g] <= kMostScale)) == 0;
+      bare |= __builtin_amdgcn_ballot_w64(q[g] == -1 && M::col(q0, g) + (lane & 15) < a.t) != 0;
+    }
+    // A token without an adapter takes part with zeros, which infinities and NaN in the adapter's rows would
+    // turn into NaN: looked for where there is one.
+    const uint16_t* const e = a.e + (alike ? (long)only * a.rows * a.rp : 0);
+    if (alike && bare) {
+      mma_us8 top = {};
+      for (int kf = 0; kf < a.rp; kf += 32) {
+        const int k = min(kf + 8 * quad, a.rp - 8);
+#pragma unroll
+        for (int f = 0; f < FP; ++f) {
+          const uint32_t row = min(M::row(p0, f) + (lane & 15), a.rows - 1);
+          const mma_us8 v = *reinterpret_cast<const mma_us8*>(e + (row * (uint32_t)a.rp + k));
+          top = __builtin_elementwise_max(top, v & (uint16_t)0x7fff);
+        }
+      }
+      bool wild = false;
+#pragma unroll
+      for (int i = 0; i < 8; ++i) wild |= top[i] >= T::narrow(__builtin_inff());
+      alike = __builtin_amdgcn_ballot_w64(wild) == 0;
+    }
     // alike: straight onto the sums, which are divided by 2^e meanwhile: no second set of them, so all tokens
     // at once and an adapter's rows read once. (Loops of no passes, not branches: those would copy the sums.)
 #pragma unroll
@@ -477,7 +502,6 @@ __global__ __launch_bounds__(64 * WP * WQ, 2) void k_wide(WideArgs a) {
 #pragma unroll
       for (int f = 0; f < FP; ++f) acc[f][g] *= inv;
     }
-    const uint16_t* const e = a.e + (alike ? (long)only * a.rows * a.rp : 0);
     const int kfs = alike ? 2 * a.rp : 0;
     for (int kf = 0; kf < kfs; kf += 32) {
       const int k = kf + 8 * quad, c = k < a.rp ? k : k - a.rp;
@@ -505,10 +529,13 @@ __global__ __launch_bounds__(64 * WP * WQ, 2) void k_wide(WideArgs a) {
       const int t = M::col(q0, g) + (lane & 15);
       const bool known = q[g] >= 0 && q[g] < a.adapters;
       uint64_t left = alike ? 0 : __builtin_amdgcn_ballot_w64(known);
+      // the others' tokens one adapter after another, by the same operations in the same order: a token's
+      // result does not depend on its neighbours
+      const float inv = scale[g] <= kMostScale ? 1.0f / scale[g] : 0.0f;
       for (int ad = next_adapter(q[g], left); ad >= 0; ad = next_adapter(q[g], left)) {
         mma_f4 d[FP];
 #pragma unroll
-        for (int f = 0; f < FP; ++f) d[f] = mma_f4{};
+        for (int f = 0; f < FP; ++f) d[f] = acc[f][g] * inv;
         for (int kf = 0; kf < 2 * a.rp; kf += 32) {
           const int k = kf + 8 * quad, c = k < a.rp ? k : k - a.rp;
           const v8 h = __builtin_bit_cast(
@@ -525,7 +552,7 @@ __global__ __launch_bounds__(64 * WP * WQ, 2) void k_wide(WideArgs a) {
         for (int f = 0; f < FP; ++f)
 #pragma unroll
           for (int r = 0; r < 4; ++r)
-            if (q[g] == ad) acc[f][g][r] = __builtin_fmaf(scale[g], d[f][r], acc[f][g][r]);
+            if (q[g] == ad) acc[f][g][r] = __builtin_fmaf(scale[g], d[f][r], inv > 0.0f ? 0.0f : acc[f][g][r]);
       }
       if (!known && q[g] != -1) {  // no such adapter
 #pragma unroll

@@ -31,6 +31,7 @@
 namespace cdclq {
 
 typedef short mma_s4 __attribute__((ext_vector_type(4)));
+typedef uint16_t mma_us8 __attribute__((ext_vector_type(8)));
 typedef float mma_f4 __attribute__((ext_vector_type(4)));
 typedef uint32_t mma_u4 __attribute__((ext_vector_type(4)));
 

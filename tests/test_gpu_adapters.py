@@ -292,6 +292,33 @@ def test_order_of_requests_changes_no_token(ctx, tune):
         assert torch.equal(tune.adapter_linear(packed, x[p].contiguous(), ad, q[p].contiguous()), y[p])
 
 
+@pytest.mark.parametrize("t", [130, 700])
+@pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float16])
+def test_neighbours_change_no_token(ctx, tune, dtype, t):
+    """The same tokens of one adapter alone, with tokens of no adapter among them, with tokens of other
+    adapters, and with an adapter whose weights are not finite: the same bits."""
+    m, n = 300, 384
+    packed, _, _ = make_layer(ctx, tune, 6, m, n, 3, 128)
+    ad = make_adapters(tune, 2, 3, 40, m, n, dtype)
+    x = normal(1, t, n, dtype=dtype)
+    x[::7] *= 2.0 ** -9  # several exponents of the low-rank vectors
+    one = torch.zeros(t, dtype=torch.int32, device="cuda")
+    some, mixed = one.clone(), one.clone()
+    some[1::3], mixed[2::5] = -1, 1
+    y0, y1, y2 = (tune.adapter_linear(packed, x, ad, q) for q in (one, some, mixed))
+    assert torch.equal(y0[some == 0], y1[some == 0]) and torch.equal(y0[mixed == 0], y2[mixed == 0])
+    bare = tune.adapter_linear(packed, x, ad, torch.full_like(one, -1))
+    assert torch.equal(y1[some == -1], bare[some == -1])
+    sick = tune.Adapters(ad.a, ad.b.clone(), ad.scaling)
+    sick.b[0, 5], sick.b[0, 290] = float("inf"), float("nan")
+    y3 = tune.adapter_linear(packed, x, sick, some)
+    assert torch.equal(y3[some == -1], y1[some == -1])
+    fine = torch.ones(m, dtype=torch.bool, device="cuda")
+    fine[5] = fine[290] = False
+    assert torch.equal(y3[some == 0][:, fine], y1[some == 0][:, fine])
+    assert not torch.isfinite(y3[some == 0][:, ~fine]).any()
+
+
 def test_strides_and_alignment(ctx, tune):
     m, n, b = 100, 256, torch.bfloat16
     packed, _, _ = make_layer(ctx, tune, 8, m, n, 4, 128)

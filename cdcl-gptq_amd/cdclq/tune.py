@@ -7,6 +7,7 @@ The operators that a quantized model needs once its weights are frozen:
   checkpoint_save / checkpoint_restore   a layer's input kept in 8 bits until the backward pass
   vocab_loss / vocab_loss_backward       softmax cross entropy over a large vocabulary and its
                                          gradient, without the logits in memory
+  linear, cross_entropy                  the same as differentiable functions of torch's autograd
 
 Tensors are torch tensors on the context's GPU, bfloat16 or float16, with contiguous rows (any row
 stride). Every call is enqueued on torch's current stream and returns without waiting; scratch
@@ -301,3 +302,60 @@ def vocab_loss_backward(ctx: Context, x: torch.Tensor, w: torch.Tensor, targets:
                                                  dx.data_ptr(), d, dw.data_ptr() if need_dw else None, d,
                                                  work.data_ptr(), work.numel(), _stream(ctx)))
     return dx, dw
+
+
+# ---------------------------------------------------------------- as differentiable functions
+class _Linear(torch.autograd.Function):
+    @staticmethod
+    def forward(fn, x, a, b, packed, adapters, request):
+        fn.packed, fn.adapters = packed, adapters
+        if adapters is None:
+            fn.save_for_backward()
+            return adapter_linear(packed, x)
+        y, low = adapter_linear(packed, x, adapters, request, return_low=True)
+        ck = checkpoint_save(packed.ctx, x)
+        fn.dtype = x.dtype
+        fn.save_for_backward(ck.codes, ck.scales, low, request, a, b)  # a, b: changed in place would be an error
+        return y
+
+    @staticmethod
+    def backward(fn, dy):
+        dy = dy.contiguous()
+        if fn.adapters is None:
+            return adapter_linear_backward(fn.packed, dy)[0], None, None, None, None, None
+        codes, scales, low, request, _, _ = fn.saved_tensors
+        dx, da, db = adapter_linear_backward(fn.packed, dy, Checkpoint(codes, scales, fn.dtype), low, fn.adapters,
+                                             request)
+        return dx, da, db, None, None, None
+
+
+def linear(packed: PackedLinear, x: torch.Tensor, adapters: Adapters | None = None,
+           request: torch.Tensor | None = None) -> torch.Tensor:
+    """adapter_linear for autograd: gradients of x and of adapters.a and .b; between the passes x is kept
+    as an 8-bit checkpoint."""
+    return _Linear.apply(x, adapters.a if adapters else None, adapters.b if adapters else None, packed, adapters,
+                         request)
+
+
+class _CrossEntropy(torch.autograd.Function):
+    @staticmethod
+    def forward(fn, x, w, ctx, targets, ignore_index):
+        loss, lse = vocab_loss(ctx, x, w, targets, ignore_index)
+        weight = 1.0 / (targets != ignore_index).sum().clamp(min=1).float()
+        fn.save_for_backward(x, w, targets, lse, weight)
+        fn.ctx, fn.ignore_index = ctx, ignore_index
+        return loss.sum() * weight
+
+    @staticmethod
+    def backward(fn, grad):
+        x, w, targets, lse, weight = fn.saved_tensors
+        dloss = (grad * weight).float().expand(len(x)).contiguous()
+        dx, dw = vocab_loss_backward(fn.ctx, x, w, targets, lse, dloss, fn.ignore_index, fn.needs_input_grad[1])
+        return dx, dw, None, None, None
+
+
+def cross_entropy(ctx: Context, x: torch.Tensor, w: torch.Tensor, targets: torch.Tensor,
+                  ignore_index: int = -100) -> torch.Tensor:
+    """The mean of vocab_loss over the tokens that take part (0 if none does), for autograd: gradients of
+    x and, where w asks for it, of w."""
+    return _CrossEntropy.apply(x, w, ctx, targets, ignore_index)

@@ -218,41 +218,6 @@ __device__ void u_dots(const DotJob& k, int id) {
   }
 }
 
-// Workgroups of each part, in this order; 0: not asked for.
-struct PrepareArgs {
-  int expand, slots, pad[3], tb, ta, lists, dots;
-  uint16_t* w16;
-  SlotJob slot;
-  PadJob pads[3];
-  const uint16_t *a, *b;
-  int adapters, rank, rp, mp;
-  uint16_t *bt, *at;
-  ListJob list;
-  DotJob dot;
-  int total() const { return expand + slots + pad[0] + pad[1] + pad[2] + tb + ta + lists + dots; }
-};
-template <class T>
-__global__ __launch_bounds__(256) void k_prepare(PackedView v, PrepareArgs k) {
-  extern __shared__ __align__(16) uint16_t lds[];
-  int b = blockIdx.x;
-  if (b < k.lists) return adapter_lists(k.list, b);
-  b -= k.lists;
-  if (b < k.dots) return u_dots<T>(k.dot, b);
-  b -= k.dots;
-  if (b < k.slots) return to_slots(v, k.slot, lds, b);
-  b -= k.slots;
-  if (b < k.expand) return packed_expand<T>(v, k.w16, b, k.expand);
-  b -= k.expand;
-#pragma unroll
-  for (int i = 0; i < 3; ++i) {
-    if (b < k.pad[i]) return pad_rows16(k.pads[i], b, k.pad[i]);
-    b -= k.pad[i];
-  }
-  if (b < k.tb) return transpose_b(k.b, k.adapters, v.m, k.rank, k.mp, k.bt, b, k.tb);
-  b -= k.tb;
-  transpose_a(v, k.a, k.adapters, k.rank, k.rp, k.at, b, k.ta);
-}
-
 // The next adapter of a fragment's tokens that is not done yet (-1: none left). q: lane's token's adapter
 // or -1; `left`: lanes still waiting.
 __device__ __forceinline__ int next_adapter(int q, uint64_t& left) {
@@ -294,47 +259,57 @@ __device__ __forceinline__ void low_out(const float (&v)[N], int ot, int t, int 
   }
 }
 
-// low[t][j] = sum_k a[q][j][k] x[t][k] for 16 tokens a workgroup, the 8 wavefronts taking every 8th step
-// of k.
-template <class T, int RF>
-__global__ __launch_bounds__(512) void k_shrink(const uint16_t* __restrict__ x, long ldx, int t, int kk,
-                                                const uint16_t* __restrict__ a, long lda, int rank, int rp,
-                                                int adapters, const int* __restrict__ request,
-                                                const float* __restrict__ scaling, int scaled, float* __restrict__ out,
-                                                uint16_t* __restrict__ hl, float* __restrict__ hscale) {
+// low[t][j] = sum_k a[q][j][k] x[t][k] for 16 tokens a workgroup of NW wavefronts, each taking every NW-th
+// step of k.
+struct ShrinkJob {
+  const uint16_t* x;
+  long ldx;
+  int t, kk;
+  const uint16_t* a;
+  long lda;
+  int rank, rp, adapters;
+  const int* request;
+  const float* scaling;
+  int scaled;
+  float* out;  // as low_out takes them
+  uint16_t* hl;
+  float* hscale;
+};
+template <class T, int RF, int NW>
+__device__ __forceinline__ void shrink_rows(const ShrinkJob& s, int id) {
   typedef typename T::v8 v8;
-  __shared__ float red[8][16][RF * 16 + 1];
+  __shared__ float red[NW][16][RF * 16 + 1];
   const int lane = threadIdx.x & 63, wv = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), quad = lane >> 4;
-  const int tok = blockIdx.x * 16 + (lane & 15);
-  int q = tok < t ? request[tok] : -1;
-  if (q >= adapters) q = -1;
+  const int tok = id * 16 + (lane & 15);
+  int q = tok < s.t ? s.request[tok] : -1;
+  if (q >= s.adapters) q = -1;
   mma_f4 keep[RF];
 #pragma unroll
   for (int f = 0; f < RF; ++f) keep[f] = mma_f4{};
   uint64_t left = __builtin_amdgcn_ballot_w64(q >= 0);
-  const uint16_t* xr = x + (long)min(tok, t - 1) * ldx;
+  const uint16_t* xr = s.x + (long)min(tok, s.t - 1) * s.ldx;
   for (int ad = next_adapter(q, left); ad >= 0; ad = next_adapter(q, left)) {
     const uint16_t* ar[RF];
     mma_f4 acc[RF];
 #pragma unroll
     for (int f = 0; f < RF; ++f) {
-      ar[f] = a + ((long)ad * rank + min(16 * f + (lane & 15), rank - 1)) * lda;
+      ar[f] = s.a + ((long)ad * s.rank + min(16 * f + (lane & 15), s.rank - 1)) * s.lda;
       acc[f] = mma_f4{};
     }
     // 64 k a wavefront and step, 16 of a row a lane (whole cache lines; the two operands agree on the order
     // of k, which is all a sum needs); U steps' loads in flight
-    constexpr int U = RF > 4 ? 1 : 2;
-    for (int k0 = 64 * wv; k0 < kk; k0 += 512 * U) {
+    constexpr int U = RF > 4 ? 1 : 2, STEP = 64 * NW;
+    for (int k0 = 64 * wv; k0 < s.kk; k0 += STEP * U) {
       mma_u4 xv[U][2], av[U][2][RF];
 #pragma unroll
       for (int i = 0; i < U; ++i)
 #pragma unroll
         for (int h = 0; h < 2; ++h) {
-          const int k = k0 + 512 * i + 16 * quad + 8 * h;
+          const int k = k0 + STEP * i + 16 * quad + 8 * h;
           xv[i][h] = mma_u4{};
 #pragma unroll
           for (int f = 0; f < RF; ++f) av[i][h][f] = mma_u4{};
-          if (k < kk) {
+          if (k < s.kk) {
             xv[i][h] = *reinterpret_cast<const mma_u4*>(xr + k);
 #pragma unroll
             for (int f = 0; f < RF; ++f) av[i][h][f] = *reinterpret_cast<const mma_u4*>(ar[f] + k);
@@ -358,16 +333,64 @@ __global__ __launch_bounds__(512) void k_shrink(const uint16_t* __restrict__ x, 
     for (int r = 0; r < 4; ++r) red[wv][lane & 15][16 * f + 4 * quad + r] = keep[f][r];
   __syncthreads();
   // 32 threads a token
-  const int it = threadIdx.x >> 5, jt = threadIdx.x & 31;
-  float v[(RF + 1) / 2];
+  const int jt = threadIdx.x & 31;
+  for (int it = threadIdx.x >> 5; it < 16; it += 2 * NW) {
+    float v[(RF + 1) / 2];
 #pragma unroll
-  for (int i = 0; i < (RF + 1) / 2; ++i) {
-    const int j = jt + 32 * i;
-    v[i] = 0.0f;
-    if (j < rank)
-      for (int w = 0; w < 8; ++w) v[i] += red[w][it][j];
+    for (int i = 0; i < (RF + 1) / 2; ++i) {
+      const int j = jt + 32 * i;
+      v[i] = 0.0f;
+      if (j < s.rank)
+        for (int w = 0; w < NW; ++w) v[i] += red[w][it][j];
+    }
+    low_out<T, (RF + 1) / 2>(v, id * 16 + it, s.t, s.rank, s.rp, s.adapters, s.request, s.scaling, s.scaled, s.out, s.hl,
+                             s.hscale);
   }
-  low_out<T, (RF + 1) / 2>(v, blockIdx.x * 16 + it, t, rank, rp, adapters, request, scaling, scaled, out, hl, hscale);
+}
+template <class T, int RF>
+__global__ __launch_bounds__(512) void k_shrink(ShrinkJob s) {
+  shrink_rows<T, RF, 8>(s, blockIdx.x);
+}
+
+// Workgroups of each part, in this order; 0: not asked for.
+struct PrepareArgs {
+  int expand, slots, pad[3], tb, ta, lists, dots, shrink;
+  uint16_t* w16;
+  SlotJob slot;
+  PadJob pads[3];
+  const uint16_t *a, *b;
+  int adapters, rank, rp, mp;
+  uint16_t *bt, *at;
+  ListJob list;
+  DotJob dot;
+  ShrinkJob low;
+  int total() const { return expand + slots + pad[0] + pad[1] + pad[2] + tb + ta + lists + dots + shrink; }
+};
+// RF: of the low-rank vectors that are taken along (0: none)
+template <class T, int RF = 0>
+__global__ __launch_bounds__(256) void k_prepare(PackedView v, PrepareArgs k) {
+  extern __shared__ __align__(16) uint16_t lds[];
+  int b = blockIdx.x;
+  if constexpr (RF > 0) {
+    if (b < k.shrink) return shrink_rows<T, RF, 4>(k.low, b);
+    b -= k.shrink;
+  }
+  if (b < k.lists) return adapter_lists(k.list, b);
+  b -= k.lists;
+  if (b < k.dots) return u_dots<T>(k.dot, b);
+  b -= k.dots;
+  if (b < k.slots) return to_slots(v, k.slot, lds, b);
+  b -= k.slots;
+  if (b < k.expand) return packed_expand<T>(v, k.w16, b, k.expand);
+  b -= k.expand;
+#pragma unroll
+  for (int i = 0; i < 3; ++i) {
+    if (b < k.pad[i]) return pad_rows16(k.pads[i], b, k.pad[i]);
+    b -= k.pad[i];
+  }
+  if (b < k.tb) return transpose_b(k.b, k.adapters, v.m, k.rank, k.mp, k.bt, b, k.tb);
+  b -= k.tb;
+  transpose_a(v, k.a, k.adapters, k.rank, k.rp, k.at, b, k.ta);
 }
 
 // The same for many tokens: tiles of 128 tokens of one adapter (by list) against its ranks, on the tiles of
@@ -1007,8 +1030,8 @@ hipError_t shrink(hipStream_t st, const ShrinkPlan& p, const int* list, const in
     return hipGetLastError();
   }
   auto go = [&](auto rf) {
-    k_shrink<T, decltype(rf)::value><<<grid, 512, 0, st>>>(x, ldx, (int)t, k, a, lda, g.rank, rp, g.adapters, g.request,
-                                                           g.scaling, scaled, out, hl, hscale);
+    k_shrink<T, decltype(rf)::value><<<grid, 512, 0, st>>>(
+        {x, ldx, (int)t, k, a, lda, g.rank, rp, g.adapters, g.request, g.scaling, scaled, out, hl, hscale});
     return hipGetLastError();
   };
   if (rp <= 16) return go(std::integral_constant<int, 1>{});
@@ -1102,10 +1125,18 @@ hipError_t wide(hipStream_t st, const PackedView& v, const AdapterArgs& a, void*
     p.lists = a.adapters;
     p.list = {a.request, (int)a.t, a.adapters, kItem, 0, list, nullptr, nullptr, tiles, sp.ntiles};
   }
-  k_prepare<T><<<p.total(), 256, slot_lds(v), st>>>(v, p);
+  // The low-rank vectors of few ranks along with the rest, where they need nothing of it.
+  const bool along = low && !tiled && !pad_x && !pad_a && rp <= 32;
+  if (along) {
+    p.shrink = (int)((a.t + 15) / 16);
+    p.low = {x, ldx, (int)a.t, n8, aa, lda, a.rank, rp, a.adapters, a.request, a.scaling, 0, a.low, hl, hscale};
+  }
+  if (!along) k_prepare<T><<<p.total(), 256, slot_lds(v), st>>>(v, p);
+  else if (rp <= 16) k_prepare<T, 1><<<p.total(), 256, slot_lds(v), st>>>(v, p);
+  else k_prepare<T, 2><<<p.total(), 256, slot_lds(v), st>>>(v, p);
   STEP(hipGetLastError());
   if (low) {
-    STEP(shrink<T>(st, sp, list, tiles, lowpart, x, ldx, a.t, n8, aa, lda, a, 0, a.low, hl, hscale));
+    if (!along) STEP(shrink<T>(st, sp, list, tiles, lowpart, x, ldx, a.t, n8, aa, lda, a, 0, a.low, hl, hscale));
     w.e = bb;
     w.rp = rp;
     w.adapters = a.adapters;

@@ -601,6 +601,8 @@ __global__ __launch_bounds__(64 * WP * WQ, 2) void k_wide(WideArgs a) {
 
 // part[slot][j][c] = sum over the item's tokens of l[t][j] X[t][c], j in 16 RF ranks from j0, c in 128
 // columns a wavefront. X: 8-bit codes with their scales (I8), or 16-bit values; l times scaling[q] if given.
+// Two sets of four wavefronts take every other 32 tokens each (one set leaves a SIMD one wavefront, which
+// waits for its loads and its own results: rank 64 over 4096 tokens, 4096 + 14336 columns: 77 us; two: 59).
 // A lane reads 8 neighbouring columns of 8 tokens, the next ones while these are multiplied: row i of the
 // f-th MFMA operand is column 8 i + f. The item's l lies in LDS, its token list beside it; it enters the
 // matrix cores as the sum of two 16-bit values, in f16 divided by 2^e to keep it in range (e grows with the
@@ -618,7 +620,7 @@ template <class T, bool I8, bool VEC, int RF>
 __device__ __forceinline__ void outer(const OuterJob& k, int colgroup, int rank, int rp, const int* list, int4 it,
                                       int slot, int j0, float (*ll)[16 * RF + 1], int* toks) {
   typedef typename T::v8 v8;
-  const int lane = threadIdx.x & 63, wv = threadIdx.x >> 6, quad = lane >> 4;
+  const int lane = threadIdx.x & 63, wv = threadIdx.x >> 6 & 3, set = threadIdx.x >> 8, quad = lane >> 4;
   const float mul = k.scaling ? k.scaling[it.x] : 1.0f;
   const int c0 = (colgroup * 4 + wv) * 128, nb = (k.cols + 127) / 128;
   // columns past the last take part with another's values: nobody reads their sums
@@ -629,7 +631,7 @@ __device__ __forceinline__ void outer(const OuterJob& k, int colgroup, int rank,
 #pragma unroll
     for (int g = 0; g < RF; ++g) acc[f][g] = mma_f4{};
   int ex = -126;  // f16: the exponent that ll and the sums are divided by
-  __shared__ float wtop[4];
+  __shared__ float wtop[8];
   struct Raw {
     mma_u4 h[I8 ? 1 : 8];
     uint2 b[I8 ? 8 : 1];
@@ -688,27 +690,29 @@ __device__ __forceinline__ void outer(const OuterJob& k, int colgroup, int rank,
       const v8 vh = __builtin_bit_cast(v8, mma_u4{hi[0], hi[1], hi[2], hi[3]});
       const v8 vl = __builtin_bit_cast(v8, mma_u4{lo[0], lo[1], lo[2], lo[3]});
 #pragma unroll
-      for (int f = 0; f < 8; ++f) {
-        const v8 x = __builtin_bit_cast(v8, mma_u4{xv[f][0], xv[f][1], xv[f][2], xv[f][3]});
-        acc[f][g] = T::mfma(x, vh, acc[f][g]);
-        acc[f][g] = T::mfma(x, vl, acc[f][g]);
-      }
+      for (int f = 0; f < 8; ++f)
+        acc[f][g] = T::mfma(__builtin_bit_cast(v8, mma_u4{xv[f][0], xv[f][1], xv[f][2], xv[f][3]}), vh, acc[f][g]);
+#pragma unroll
+      for (int f = 0; f < 8; ++f)
+        acc[f][g] = T::mfma(__builtin_bit_cast(v8, mma_u4{xv[f][0], xv[f][1], xv[f][2], xv[f][3]}), vl, acc[f][g]);
     }
   };
   for (int i0 = 0; i0 < it.z; i0 += kItem) {
     const int n = min(kItem, it.z - i0);
     if (i0) __syncthreads();
-    toks[threadIdx.x] = list[it.y + i0 + min((int)threadIdx.x, n - 1)];
+    if (threadIdx.x < kItem) toks[threadIdx.x] = list[it.y + i0 + min((int)threadIdx.x, n - 1)];
     __syncthreads();
+    Raw now, next;
+    if (VEC && c0 < k.cols) load(32 * set, now);
     // l of these tokens, 0 past the last: four ranks a load, half of the thread's loads in flight at once
-    constexpr int PER = 4 * RF, BATCH = PER < 8 ? PER : 8;
+    constexpr int PER = 4 * RF, BATCH = PER / 2 < 4 ? PER / 2 : 4;
     float top = 0.0f;
-    for (int e0 = 0; e0 < kItem * PER; e0 += 256 * BATCH) {
-      if (e0 / PER >= ((n + 31) & ~31)) break;
+    for (int e0 = 0; e0 < kItem * PER; e0 += 512 * BATCH) {
+      if (e0 / PER >= ((n + 63) & ~63)) break;
       mma_f4 v[BATCH];
 #pragma unroll
       for (int u = 0; u < BATCH; ++u) {
-        const int e = e0 + 256 * u + threadIdx.x, i = e / PER, j = j0 + 4 * (e - i * PER);
+        const int e = e0 + 512 * u + threadIdx.x, i = e / PER, j = j0 + 4 * (e - i * PER);
         v[u] = mma_f4{};
         if (i < n) {
           const float* src = k.l + (long)toks[i] * rank + j;
@@ -723,7 +727,7 @@ __device__ __forceinline__ void outer(const OuterJob& k, int colgroup, int rank,
       }
 #pragma unroll
       for (int u = 0; u < BATCH; ++u) {
-        const int e = e0 + 256 * u + threadIdx.x, i = e / PER, j = 4 * (e - i * PER);
+        const int e = e0 + 512 * u + threadIdx.x, i = e / PER, j = 4 * (e - i * PER);
 #pragma unroll
         for (int r = 0; r < 4; ++r) {
           ll[i][j + r] = mul * v[u][r];
@@ -735,11 +739,13 @@ __device__ __forceinline__ void outer(const OuterJob& k, int colgroup, int rank,
     if constexpr (T::kind == F16::kind) {
 #pragma unroll
       for (int s = 32; s; s >>= 1) top = fmaxf(top, __shfl_xor(top, s));
-      if (lane == 0) wtop[wv] = top;
+      if (lane == 0) wtop[threadIdx.x >> 6] = top;
     }
     __syncthreads();
     if constexpr (T::kind == F16::kind) {
-      top = fmaxf(fmaxf(wtop[0], wtop[1]), fmaxf(wtop[2], wtop[3]));
+      top = wtop[0];
+#pragma unroll
+      for (int w = 1; w < 8; ++w) top = fmaxf(top, wtop[w]);
       const int to = max(ex, top > 0.0f ? __builtin_amdgcn_frexp_expf(top) : -126);
       if (to != ex) {
 #pragma unroll
@@ -752,15 +758,37 @@ __device__ __forceinline__ void outer(const OuterJob& k, int colgroup, int rank,
       }
     }
     if (c0 >= k.cols) continue;
-    Raw now, next;
-    load(0, now);
-    for (int t0 = 0; t0 < n; t0 += 32) {
-      load(min(t0 + 32, kItem - 32), next);
-      mul_add(t0, now);
-      now = next;
+    for (int t0 = 32 * set; t0 < n; t0 += 64) {
+      if constexpr (VEC) {
+        load(min(t0 + 64, kItem - 32), next);
+        mul_add(t0, now);
+        now = next;
+      } else {
+        load(t0, now);
+        mul_add(t0, now);
+      }
     }
   }
-  if (c0 >= k.cols) return;
+  // the two sets' sums together, half of them at a time
+  float* const join = &ll[0][0];
+#pragma unroll
+  for (int f0 = 0; f0 < 8; f0 += 4) {
+    __syncthreads();
+    if (set)
+#pragma unroll
+      for (int f = 0; f < 4; ++f)
+#pragma unroll
+        for (int g = 0; g < RF; ++g)
+          *reinterpret_cast<mma_f4*>(join + 4 * ((f * RF + g) * 256 + (threadIdx.x & 255))) = acc[f0 + f][g];
+    __syncthreads();
+    if (!set)
+#pragma unroll
+      for (int f = 0; f < 4; ++f)
+#pragma unroll
+        for (int g = 0; g < RF; ++g)
+          acc[f0 + f][g] += *reinterpret_cast<const mma_f4*>(join + 4 * ((f * RF + g) * 256 + threadIdx.x));
+  }
+  if (set || c0 >= k.cols) return;
   if constexpr (T::kind == F16::kind) {
 #pragma unroll
     for (int f = 0; f < 8; ++f)
@@ -785,9 +813,9 @@ __device__ __forceinline__ void outer(const OuterJob& k, int colgroup, int rank,
 }
 // dB's part (16-bit dy) in the first nb_ workgroups of x, dA's (the checkpoint) in the rest
 template <class T, int RF, bool VECA>
-__global__ __launch_bounds__(256, RF < 4 ? 2 : 1) void k_outer(OuterJob db, int nb_, OuterJob da, int rank, int rp,
+__global__ __launch_bounds__(512, 2) void k_outer(OuterJob db, int nb_, OuterJob da, int rank, int rp,
                                                   const int* __restrict__ list, const int4* __restrict__ items) {
-  __shared__ float ll[kItem][16 * RF + 1];
+  __shared__ __align__(16) float ll[kItem][16 * RF + 1];
   __shared__ int toks[kItem];
   const int4 it = items[blockIdx.y];
   if (it.x < 0) return;
@@ -1158,14 +1186,15 @@ hipError_t wide(hipStream_t st, const PackedView& v, const AdapterArgs& a, void*
 }
 
 // Tokens of an item: long ones write fewer sums (8 bytes a column and rank, at about 5 TB/s), short ones
-// make more workgroups, of which a CU holds one (two up to rank 32); 256 tokens take one about 8 us.
+// make more workgroups, of which a CU holds one (two up to rank 32); 256 tokens take one about 4 us for every
+// 16 ranks (768 tokens of 64 ranks: 59 us with the first loads and the sums' stores).
 int outer_chunk(long t, int adapters, int rp, int n, int m) {
   const long groups = ((n + 511) / 512 + (m + 511) / 512) * ((rp + 63) / 64), room = rp > 32 ? 256 : 512;
   int best = 1;
   double least = 0;
   for (int c = 1; c <= 16; ++c) {
     const long items = std::max<long>(adapters, (t + kItem * c - 1) / (kItem * c));
-    const double cost = (double)((items * groups + room - 1) / room) * (8.0 * c + 3.0) + items * rp * (8.0 / 5e6) * (n + m);
+    const double cost = (double)((items * groups + room - 1) / room) * ((1.0 + 0.25 * std::min(rp, 64)) * c + 5.0) + items * rp * (8.0 / 5e6) * (n + m);
     if (c == 1 || cost < least) least = cost, best = c;
   }
   return kItem * best;
@@ -1241,8 +1270,8 @@ hipError_t grad(hipStream_t st, const PackedView& v, const AdapterArgs& a, void*
     auto go = [&](auto rf) {
       constexpr int RF = decltype(rf)::value;
       const dim3 grid(gb + ga, slots, (rp + 16 * RF - 1) / (16 * RF));
-      if (vec) k_outer<T, RF, true><<<grid, 256, 0, st>>>(jb, gb, ja, a.rank, rp, list, items);
-      else k_outer<T, RF, false><<<grid, 256, 0, st>>>(jb, gb, ja, a.rank, rp, list, items);
+      if (vec) k_outer<T, RF, true><<<grid, 512, 0, st>>>(jb, gb, ja, a.rank, rp, list, items);
+      else k_outer<T, RF, false><<<grid, 512, 0, st>>>(jb, gb, ja, a.rank, rp, list, items);
       return hipGetLastError();
     };
     if (t) {

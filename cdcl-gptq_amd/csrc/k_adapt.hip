@@ -1013,7 +1013,10 @@ inline int slot_blocks(const PackedView& v, long t) {
   const int r = std::max(slot_rows(v), 1);
   return (int)((t + r - 1) / r);
 }
-inline int expand_blocks(const PackedView& v) { return (int)std::min(((long)v.tiles * v.nkb + 3) / 4, 1l << 16); }
+inline int expand_blocks(const PackedView& v) {
+  const long per = 4 * packed_expand_unit(v);
+  return (int)std::min(((long)v.tiles * v.nkb + per - 1) / per, 1l << 16);
+}
 inline int pad_blocks(const PadJob& j) { return blocks_for(j.rows * (j.dp / 8), 256 * 4, 8192); }
 
 #define STEP(expr)                       \
@@ -1070,16 +1073,18 @@ hipError_t shrink(hipStream_t st, const ShrinkPlan& p, const int* list, const in
 
 // Shape and splits of a product: the f32 parts of a split one are written and read at about 4 TB/s, and
 // summing them takes a launch (4 us) unless one is there anyway.
+constexpr long kCache = 200l << 20;  // expanded weights up to this many bytes are found in the last cache (256 MB)
 struct WidePlan {
   int pick, splits, share;
 };
 WidePlan wide_plan(long rows, long t, long k, bool strided, bool parts_anyway) {
+  const bool far = 2 * rows * k > kCache;
   WidePlan best = {};
   double least = 0;
   for (int i = 0; i < kMmaShapes; ++i)
     for (int n = 1; n == 1 || (n <= 16 && k / n >= 256); n *= 2) {
       const bool parts = parts_anyway || n > 1;
-      const double c = mma_cost(rows, t, k, i, n, strided) + (parts ? n * (8.0 / 4e6) * t * rows : 0.0) +
+      const double c = mma_cost(rows, t, k, i, n, strided, far) + (parts ? n * (8.0 / 4e6) * t * rows : 0.0) +
                        (n > 1 && !parts_anyway ? 4.0 : 0.0);
       if ((i == 0 && n == 1) || c < least) least = c, best.pick = i, best.splits = n;
     }

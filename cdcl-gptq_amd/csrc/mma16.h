@@ -416,15 +416,17 @@ hipError_t with_mma_shape(int pick, F f) {
 }
 // Microseconds of a product of `rows` x `cols` results over k, `splits` ways in k: rounds of tiles over 256
 // CUs, each so many stages and 4 us more for its first loads and its results. strided: P's rows contiguous
-// (their transposed reads cost the smaller tiles a fifth).
-inline double mma_cost(long rows, long cols, long k, int pick, long splits, bool strided) {
+// (their transposed reads cost the smaller tiles a fifth). far: P comes from memory, not from a cache; a stage
+// then takes 1 us at least (its loads go out one stage ahead; 218 x 13056 results over 12608).
+inline double mma_cost(long rows, long cols, long k, int pick, long splits, bool strided, bool far = false) {
   const MmaShapeTime s = kMmaTimes[pick];
   const long tiles = ((rows + s.bp - 1) / s.bp) * ((cols + s.bq - 1) / s.bq) * splits;
   const long stages = std::max(2l, ((k + splits - 1) / splits + 63) / 64);
   const long rounds = (tiles + 256 * s.per_cu - 1) / (256 * s.per_cu);
   const long shared = std::min<long>(s.per_cu, (tiles + 255) / 256);
   const double busy = s.us * shared * (strided && pick ? 1.2 : 1.0);
-  return rounds * (std::max(busy, strided ? s.alone_strided : s.alone) * stages + 4.0);
+  const double alone = std::max(strided ? s.alone_strided : s.alone, far ? 1.0 : 0.0);
+  return rounds * (std::max(busy, alone) * stages + 4.0);
 }
 
 }  // namespace cdclq

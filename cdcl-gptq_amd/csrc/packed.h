@@ -125,30 +125,51 @@ __device__ __forceinline__ float packed_zero(uint32_t sz) { return (float)(sz >>
 
 // W in 16 bits, [tiles * 16][slots]: scale (code - zero), exact in f32, rounded once (the matrix cores
 // take both operands in the activations' type). By workgroups of 256 threads, b of nb.
-template <class T>
-__device__ void packed_expand(const PackedView& v, uint16_t* w16, long b, long nb) {
+template <class T, int U>
+__device__ __forceinline__ void packed_expand_by(const PackedView& v, uint16_t* w16, long b, long nb) {
   const int lane = threadIdx.x & 63, q = lane >> 4, ns = packed_slots(v);
   const long total = (long)v.tiles * v.nkb;
-  for (long id = b * 4 + (threadIdx.x >> 6); id < total; id += nb * 4) {
-    const long tile = id / v.nkb;
-    const int kb = (int)(id - tile * v.nkb);
-    const uint32_t info = __builtin_amdgcn_readfirstlane(v.kinfo[kb]);
-    const int width = info & 15;
-    PackedRegs r = {};
-    packed_load<0>(v.codes + tile * v.tile_bytes + 256l * (info >> 8), lane, width, r);
-    uint16_t* out = w16 + (tile * 16 + (lane & 15)) * ns + kb * 128 + 8 * q;
+  for (long id0 = (b * 4 + (threadIdx.x >> 6)) * U; id0 < total; id0 += nb * 4 * U) {
+    PackedRegs r[U];
+    uint32_t sz[U][4];
+    int width[U];
+    uint16_t* out[U];
 #pragma unroll
-    for (int s = 0; s < 4; ++s) {
-      const uint32_t sz = v.scl[(tile * v.ng + v.grp[4 * kb + s]) * 16 + (lane & 15)];
-      const float sc = packed_scale(sz), z = packed_zero(sz);
-      uint32_t o[4];
+    for (int u = 0; u < U; ++u) {
+      const long id = id0 + u < total ? id0 + u : total - 1;  // the last one twice, with the same values
+      const long tile = id / v.nkb;
+      const int kb = (int)(id - tile * v.nkb);
+      const uint32_t info = __builtin_amdgcn_readfirstlane(v.kinfo[kb]);
+      width[u] = info & 15;
+      r[u] = PackedRegs{};
+      packed_load<0>(v.codes + tile * v.tile_bytes + 256l * (info >> 8), lane, width[u], r[u]);
+      out[u] = w16 + (tile * 16 + (lane & 15)) * ns + kb * 128 + 8 * q;
 #pragma unroll
-      for (int p = 0; p < 4; ++p)
-        o[p] = narrow2<T>(sc * ((float)packed_code(r, width, s, 2 * p) - z),
-                          sc * ((float)packed_code(r, width, s, 2 * p + 1) - z));
-      *reinterpret_cast<uint4*>(out + 32 * s) = make_uint4(o[0], o[1], o[2], o[3]);
+      for (int s = 0; s < 4; ++s) sz[u][s] = v.scl[(tile * v.ng + v.grp[4 * kb + s]) * 16 + (lane & 15)];
     }
+#pragma unroll
+    for (int u = 0; u < U; ++u)
+#pragma unroll
+      for (int s = 0; s < 4; ++s) {
+        const float sc = packed_scale(sz[u][s]), z = packed_zero(sz[u][s]);
+        uint32_t o[4];
+#pragma unroll
+        for (int p = 0; p < 4; ++p)
+          o[p] = narrow2<T>(sc * ((float)packed_code(r[u], width[u], s, 2 * p) - z),
+                            sc * ((float)packed_code(r[u], width[u], s, 2 * p + 1) - z));
+        *reinterpret_cast<uint4*>(out[u] + 32 * s) = make_uint4(o[0], o[1], o[2], o[3]);
+      }
   }
+}
+
+// Blocks of 128 k whose loads a wavefront issues together: one while that gives every SIMD some to hide each
+// other's waits, then more (14336 x 4096 in 4 bits: 54 us with one, 48 with two, 53
+// with four; 5632 x 2048 in 3: 15.8 with one, 17.8 with two).
+inline __host__ __device__ int packed_expand_unit(const PackedView& v) { return (long)v.tiles * v.nkb > 16384 ? 2 : 1; }
+template <class T>
+__device__ void packed_expand(const PackedView& v, uint16_t* w16, long b, long nb) {
+  if (packed_expand_unit(v) == 1) packed_expand_by<T, 1>(v, w16, b, nb);
+  else packed_expand_by<T, 2>(v, w16, b, nb);
 }
 
 }  // namespace cdclq

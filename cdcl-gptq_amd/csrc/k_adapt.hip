@@ -1205,13 +1205,15 @@ int outer_chunk(long t, int adapters, int rp, int n, int m) {
   return kItem * best;
 }
 
-// Tokens up to which the gradient's low-rank terms are taken by dots and sums in f32.
-constexpr long kFewGrad = 64;
+// The gradient's low-rank terms by dots and sums in f32, or by transposed adapters on the matrix cores: the
+// dots take no preparation but go by tokens times ranks. 4096 -> 14336, a step of 64 tokens, rank 128: 320 us
+// against 690; 128 tokens, rank 8: 161 and 195, rank 64: 322 and 340; 192 tokens, rank 64: 448 and 383.
+inline bool few_grad(const AdapterArgs& a) { return a.t <= 128 && a.t * a.rank <= 8192; }
 
 template <class T>
 hipError_t grad(hipStream_t st, const PackedView& v, const AdapterArgs& a, void* work, bool run, size_t* bytes) {
   const int ns = packed_slots(v), rp = rank_pad(a.rank), m8 = (int)up(v.m, 8), t = (int)a.t;
-  const bool low = a.rank > 0, pad = !aligned16(a.x, a.ldx, v.m), few = a.t <= kFewGrad;
+  const bool low = a.rank > 0, pad = !aligned16(a.x, a.ldx, v.m), few = few_grad(a);
   const int nbn = (v.n + 127) / 128, nbm = (v.m + 127) / 128;
   const int chunk = outer_chunk(a.t, a.adapters, rp, v.n, v.m);
   const int slots = (int)(a.t / chunk) + a.adapters;

@@ -478,7 +478,9 @@ LossPlan loss_plan(long t, long d, long v, bool pad_w, bool grad) {
         p.dx_bytes = 4 * (size_t)p.dp * std::max<size_t>(up(t, s.bq), (size_t)(round / np) * s.bq);
       }
     }
-    p.dw_tiles = mma_cost(p.dp, p.piece, t, 5, 1, false) < mma_cost(p.dp, p.piece, t, 0, 1, false) ? 5 : 0;
+    // few tokens: dw's stores are what costs, and two small tiles on a CU overlap theirs with each other's loads
+    // (62 tokens, 50001 x 1000: 36 us, large tiles 42; 64, 128256 x 4096: 363 and 370; 300: 664 and 580)
+    p.dw_tiles = t <= 192 || mma_cost(p.dp, p.piece, t, 5, 1, false) < mma_cost(p.dp, p.piece, t, 0, 1, false) ? 5 : 0;
     p.d = take(2 * (size_t)t * p.piece);
     p.dxacc = take(p.dx_bytes);
   }

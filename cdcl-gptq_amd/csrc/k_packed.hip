@@ -142,7 +142,10 @@ __global__ __launch_bounds__(256) void k_few_inputs(PackedView v, int nx, int nt
         }
       }
     } else {
-      for (int c = lane; c < v.n; c += 64) s = __builtin_fmaf(T::widen(xr[c]), T::widen(ar[c]), s);
+      for (int c0 = 8 * lane; c0 < v.n; c0 += 512)  // the same order
+#pragma unroll
+        for (int i = 0; i < 8; ++i)
+          if (c0 + i < v.n) s = __builtin_fmaf(T::widen(xr[c0 + i]), T::widen(ar[c0 + i]), s);
     }
 #pragma unroll
     for (int k = 32; k; k >>= 1) s += __shfl_xor(s, k);
@@ -153,7 +156,7 @@ __global__ __launch_bounds__(256) void k_few_inputs(PackedView v, int nx, int nt
 struct FewArgs {
   const uint16_t* xf;
   const float* sx;
-  int t;
+  int t, frags;  // of 16 tokens, in xf and sx
   const uint16_t* b;  // adapters x m x rank, null: none
   const float* scaling;
   int adapters, rank, vec;  // vec: b's rows can be read 8 ranks at a time
@@ -168,6 +171,10 @@ __global__ __launch_bounds__(64 * W) void k_packed_few(PackedView v, FewArgs k) 
   __shared__ float red[W][RT * 16][16 * NT + 1];
   const int lane = threadIdx.x & 63, wv = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
   const long tile0 = (long)blockIdx.x * RT;
+  const int first = 16 * NT * blockIdx.y, nt = k.frags, t = k.t - first;  // this workgroup's tokens
+  const int* const request = k.request + first;
+  const uint16_t* const xf = k.xf + 512l * NT * blockIdx.y;
+  const float* const sx = k.sx + first;
   mma_f4 acc[RT][NT], run[RT][NT];
 #pragma unroll
   for (int i = 0; i < RT; ++i)
@@ -191,7 +198,7 @@ __global__ __launch_bounds__(64 * W) void k_packed_few(PackedView v, FewArgs k) 
       const int e = threadIdx.x + i * 64 * W, tok = e / (RT * 16);
       const long row = tile0 * 16 + (e - tok * (RT * 16));
       early[i][0] = early[i][1] = make_uint4(0, 0, 0, 0);
-      const int q = tok < k.t ? k.request[tok] : -1;
+      const int q = tok < t ? request[tok] : -1;
       if (q >= 0 && q < k.adapters && row < v.m) {
         const uint16_t* br = k.b + ((long)q * v.m + row) * k.rank;
         early[i][0] = *reinterpret_cast<const uint4*>(br);
@@ -217,8 +224,8 @@ __global__ __launch_bounds__(64 * W) void k_packed_few(PackedView v, FewArgs k) 
 #pragma unroll
       for (int g = 0; g < NT; ++g) {
         mma_u4 u = {};
-        if (16 * g + (lane & 15) < k.t)
-          u = *reinterpret_cast<const mma_u4*>(k.xf + ((long)((4 * kb + s) * NT + g) * 64 + lane) * 8);
+        if (16 * g + (lane & 15) < t)
+          u = *reinterpret_cast<const mma_u4*>(xf + ((long)((4 * kb + s) * nt + g) * 64 + lane) * 8);
         xv[s][g] = __builtin_bit_cast(typename T::v8, u);
       }
     // scales and sums at the block's end, where a run always ends
@@ -228,7 +235,7 @@ __global__ __launch_bounds__(64 * W) void k_packed_few(PackedView v, FewArgs k) 
 #pragma unroll
     for (int i = 0; i < RT; ++i) sz3[i] = *reinterpret_cast<const mma_u4*>(scl[i] + 16 * g3);
 #pragma unroll
-    for (int g = 0; g < NT; ++g) sx3[g] = k.sx[(4 * kb + 3) * 16 * NT + 16 * g + (lane & 15)];
+    for (int g = 0; g < NT; ++g) sx3[g] = sx[(4 * kb + 3) * 16 * nt + 16 * g + (lane & 15)];
     if (kb + W < v.nkb) {
       ninfo = __builtin_amdgcn_readfirstlane(v.kinfo[kb + W]);
 #pragma unroll
@@ -264,7 +271,7 @@ __global__ __launch_bounds__(64 * W) void k_packed_few(PackedView v, FewArgs k) 
 #pragma unroll
             for (int i = 0; i < RT; ++i) sz[i] = *reinterpret_cast<const mma_u4*>(scl[i] + 16 * gi);
 #pragma unroll
-            for (int g = 0; g < NT; ++g) sum[g] = k.sx[(4 * kb + S) * 16 * NT + 16 * g + (lane & 15)];
+            for (int g = 0; g < NT; ++g) sum[g] = sx[(4 * kb + S) * 16 * nt + 16 * g + (lane & 15)];
           }
 #pragma unroll
           for (int i = 0; i < RT; ++i)
@@ -321,30 +328,33 @@ __global__ __launch_bounds__(64 * W) void k_packed_few(PackedView v, FewArgs k) 
   for (int i = 0; i < OUT; ++i) {
     const int e = threadIdx.x + i * 64 * W, tok = e / (RT * 16), r = e - tok * (RT * 16);
     const long row = tile0 * 16 + r;
-    if (tok >= k.t || row >= v.m) continue;
+    if (tok >= t || row >= v.m) continue;
     float s = 0.0f;
 #pragma unroll
     for (int w = 0; w < W; ++w) s += red[w][r][tok];
     if (k.b) {
-      const int q = k.request[tok];
+      const int q = request[tok];
       if (q >= 0 && q < k.adapters) {
         const uint16_t* br = k.b + ((long)q * v.m + row) * k.rank;
-        const float* lo = k.low + (long)tok * k.rank;
+        const float* lo = k.low + (long)(first + tok) * k.rank;
         float d = 0.0f;
         if (k.vec) {
           d = dot8(early[i][0], lo);
           if (k.rank >= 16) d += dot8(early[i][1], lo + 8);
           for (int j = 16; j < k.rank; j += 8) d += dot8(*reinterpret_cast<const uint4*>(br + j), lo + j);
         } else {
-#pragma unroll 4
-          for (int j = 0; j < k.rank; ++j) d = __builtin_fmaf(T::widen(br[j]), lo[j], d);
+          for (int j0 = 0; j0 < k.rank; j0 += 8) {  // the same order
+            float p = 0.0f;
+            for (int j = j0; j < min(j0 + 8, k.rank); ++j) p = __builtin_fmaf(T::widen(br[j]), lo[j], p);
+            d += p;
+          }
         }
         s = __builtin_fmaf(k.scaling[q], d, s);
       } else if (q != -1) {
         s = __builtin_nanf("");  // no such adapter
       }
     }
-    k.y[tok * k.ldy + row] = T::narrow(s);
+    k.y[(first + tok) * k.ldy + row] = T::narrow(s);
   }
 }
 
@@ -352,9 +362,10 @@ template <class T, int B, int NT>
 hipError_t few_tiles(hipStream_t st, const PackedView& v, const FewArgs& k) {
   // Two row tiles share the activations' operands where that leaves two workgroups a CU (14336 rows of
   // 4096, 32 tokens: 25 us with two, 30 with one, 26 with four); few rows take 16 wavefronts each.
-  if (v.tiles >= 512) k_packed_few<T, B, 2, NT, 8><<<(v.tiles + 1) / 2, 512, 0, st>>>(v, k);
-  else if (v.tiles <= 256) k_packed_few<T, B, 1, NT, 16><<<v.tiles, 1024, 0, st>>>(v, k);
-  else k_packed_few<T, B, 1, NT, 8><<<v.tiles, 512, 0, st>>>(v, k);
+  const int groups = (k.t + 16 * NT - 1) / (16 * NT);
+  if (v.tiles >= 512) k_packed_few<T, B, 2, NT, 8><<<dim3((v.tiles + 1) / 2, groups), 512, 0, st>>>(v, k);
+  else if (v.tiles <= 256) k_packed_few<T, B, 1, NT, 16><<<dim3(v.tiles, groups), 1024, 0, st>>>(v, k);
+  else k_packed_few<T, B, 1, NT, 8><<<dim3(v.tiles, groups), 512, 0, st>>>(v, k);
   return hipGetLastError();
 }
 template <class T, int B>
@@ -363,7 +374,7 @@ hipError_t few_tokens(hipStream_t st, const PackedView& v, const FewArgs& k) {
   if (k.t <= 32) return few_tiles<T, B, 2>(st, v, k);
   return few_tiles<T, B, 4>(st, v, k);
 }
-inline int few_frags(long t) { return t <= 16 ? 1 : t <= 32 ? 2 : 4; }
+inline int few_frags(long t) { return t <= 16 ? 1 : t <= 32 ? 2 : (int)((t + 63) / 64 * 4); }
 
 template <class T>
 hipError_t few(hipStream_t st, const PackedView& v, const AdapterArgs& a, void* work) {
@@ -376,7 +387,7 @@ hipError_t few(hipStream_t st, const PackedView& v, const AdapterArgs& a, void* 
   const int vec = v.n % 8 == 0 && a.ldx % 8 == 0 && (uintptr_t)a.x % 16 == 0 && (uintptr_t)a.a % 16 == 0;
   k_few_inputs<T><<<(int)(nx + nlow), 256, 0, st>>>(v, nx, nt, a.x, a.ldx, (int)a.t, xf, sx, a.a, a.rank, a.adapters,
                                                     a.request, low, vec);
-  FewArgs k = {xf, sx, (int)a.t, a.rank ? a.b : nullptr, a.scaling, a.adapters, a.rank,
+  FewArgs k = {xf, sx, (int)a.t, nt, a.rank ? a.b : nullptr, a.scaling, a.adapters, a.rank,
                a.rank % 8 == 0 && (uintptr_t)a.b % 16 == 0, a.request, low, a.y, a.ldy};
   switch (v.bits) {
     case 2: return few_tokens<T, 2>(st, v, k);

@@ -90,9 +90,11 @@ struct cdclq_packed {
 
 namespace {
 
-// Tokens up to which the packed codes are decoded in the product's registers: 64 are four MFMA column
-// fragments, the most whose sums a wavefront holds for two row tiles.
-constexpr size_t kFewTokens = 64;
+// Tokens up to which the packed codes are decoded in the product's registers, 64 at a time (the most whose sums
+// a wavefront holds for two row tiles); for more the weights are expanded to 16 bits first. 4096 -> 14336 in 4
+// bits: 128 tokens 58 us against 79 expanded, 192 84 and 90, 256 96 and 91; 4096 -> 4096 in 8: 192 50 and 51,
+// 256 65 and 52; 2048 -> 2048 in 4: 192 18 and 30.
+constexpr size_t kFewTokens = 192;
 
 int open_packed(cdclq_ctx* ctx, size_t m, size_t n, size_t group, const uint8_t* gbits, size_t ngroups,
                 const uint8_t* qweight, size_t qweight_bytes, const uint16_t* scales, const uint8_t* qzeros,

@@ -12,7 +12,11 @@
 // adapter's result, so that what another adapter holds cannot reach it. low and u enter the matrix cores as
 // the sum of two 16-bit values of a vector scaled to [0.5, 1): about 16 bits of it are kept.
 //
-// dA and dB sum over the tokens of an adapter: lists in token order, items of at most 256 tokens with
+// 4096 tokens, 4096 -> 14336, 4 bits, rank 64, bf16: forward product 425-450 us (1.1 PF, 3.5 rounds of tiles), that
+// of the gradient 340-356 (1.4 PF, one round), both bound by power where all CUs work; 2000 tokens, 2048 -> 5632:
+// 59 us. Expanding the weights and ordering the activations: 41 us (gradient) and 56 (forward), memory at 3.6 TB/s.
+//
+// dA and dB sum over the tokens of an adapter: lists in token order, items of some hundred tokens with
 // f32 sums of their own, joined in order (no atomics). dA reads the codes of the checkpoint, exact in
 // bf16, the scale of token and block going into u.
 //
@@ -395,7 +399,8 @@ __global__ __launch_bounds__(256) void k_prepare(PackedView v, PrepareArgs k) {
 
 // The same for many tokens: tiles of 128 tokens of one adapter (by list) against its ranks, on the tiles of
 // mma16.h, split in k; part[split][token][rp]. The fragment loads of k_shrink touch 16 rows for 256 bytes,
-// which bounds it (4096 tokens, k = 14336, rank 64: 82 us); here a load takes 8 rows' whole lines.
+// which bounds it (4096 tokens, k = 14336, rank 64: 82 us); here a load takes 8 rows' whole lines (41 us, and 10
+// to sum the splits; k = 4096: 15 and 5).
 template <class T, int FP, int FQ, int WP, int WQ>
 __global__ __launch_bounds__(64 * WP * WQ, 2) void k_shrink_tiles(const uint16_t* __restrict__ x, long ldx, int kk,
                                                                   const uint16_t* __restrict__ a, long lda, int rank,
@@ -941,7 +946,7 @@ __device__ void sum_parts(const SumJob& k, int b) {
 }
 
 // The same from slot order for many tokens: `rows` tokens at a time through LDS in f32 (a column's gather
-// from memory costs four times the bytes).
+// from memory costs four times the bytes: a step of 200 tokens, 4096 -> 4096, 131 us, 135 by it).
 template <class T>
 __device__ void sum_slots(const PackedView& v, const SumJob& k, int rows, float* lds, int b) {
   const int ns = packed_slots(v), t0 = b * rows;
@@ -1026,7 +1031,9 @@ inline int pad_blocks(const PadJob& j) { return blocks_for(j.rows * (j.dp / 8), 
   } while (0)
 
 // How the low-rank vectors are made: k_shrink in about 82 us per 4096 tokens, 14336 of k and 5 operands of 16
-// rows; the tiles and their sum in two launches, worth it from about 20 us on.
+// rows; the tiles and their sum in two launches, worth it from about 20 us on (training steps 4096 -> 14336 of rank 64:
+// 1024 tokens 477 us, 581 without the tiles; 4096 tokens 1019 and 1046; 640 tokens of 2048 -> 2048, rank 8, stay
+// below: 9 us in one launch).
 struct ShrinkPlan {
   bool tiles;
   int ntiles, splits, share;
@@ -1083,6 +1090,7 @@ WidePlan wide_plan(long rows, long t, long k, bool strided, bool parts_anyway) {
   double least = 0;
   for (int i = 0; i < kMmaShapes; ++i)
     for (int n = 1; n == 1 || (n <= 16 && k / n >= 256); n *= 2) {
+      if (!strided && kMmaTimes[i].bq == 16) continue;  // the forward product has more tokens
       const bool parts = parts_anyway || n > 1;
       const double c = mma_cost(rows, t, k, i, n, strided, far) + (parts ? n * (8.0 / 4e6) * t * rows : 0.0) +
                        (n > 1 && !parts_anyway ? 4.0 : 0.0);
@@ -1099,10 +1107,13 @@ hipError_t wide_product(hipStream_t st, const WidePlan& p, WideArgs w) {
   w.share = p.share;
   return with_mma_shape(p.pick, [&](auto s) {
     typedef decltype(s) S;
-    w.np = (w.rows + S::bp - 1) / S::bp;
-    w.nq = (w.t + S::bq - 1) / S::bq;
-    k_wide<T, PS, S::fp, S::fq, S::wp, S::wq><<<w.np * w.nq * p.splits, S::threads, 0, st>>>(w);
-    return hipGetLastError();
+    if constexpr (PS || S::bq > 16) {
+      w.np = (w.rows + S::bp - 1) / S::bp;
+      w.nq = (w.t + S::bq - 1) / S::bq;
+      k_wide<T, PS, S::fp, S::fq, S::wp, S::wq><<<w.np * w.nq * p.splits, S::threads, 0, st>>>(w);
+      return hipGetLastError();
+    }
+    return hipErrorInvalidConfiguration;
   });
 }
 
@@ -1158,7 +1169,9 @@ hipError_t wide(hipStream_t st, const PackedView& v, const AdapterArgs& a, void*
     p.lists = a.adapters;
     p.list = {a.request, (int)a.t, a.adapters, kItem, 0, list, nullptr, nullptr, tiles, sp.ntiles};
   }
-  // The low-rank vectors of few ranks along with the rest, where they need nothing of it.
+  // The low-rank vectors of few ranks along with the rest, where they need nothing of it (2000 tokens, 2048 ->
+  // 5632: 75 us, 80 in a launch of their own; 4096 tokens, 4096 -> 4096: 145 and 152). Of more ranks their registers
+  // would leave the other parts few wavefronts.
   const bool along = low && !tiled && !pad_x && !pad_a && rp <= 32;
   if (along) {
     p.shrink = (int)((a.t + 15) / 16);

@@ -13,6 +13,11 @@
 //
 // d is held in the operands' 16-bit type because the matrix cores need both operands alike; it is scaled by
 // g_t / max |g| (and 2^15 in f16, whose range would lose small probabilities), both undone in f32.
+//
+// The products bound it, and those by the card's power where they are large (matrix cores busy 65-70% at
+// 1.6-1.9 GHz; the library's product: 1.34-1.40 PF). d = 4096, vocabulary 128256, bf16: forward of 2048 tokens
+// 1.66 ms (1.30 PF); gradient of 4096 tokens, a tenth ignored, in four pieces: d 829 us, dx 722, dw 748 each (1.17,
+// 1.36, 1.31 PF of the tiles' work), joining dx 30 us.
 #include <hip/hip_runtime.h>
 
 #include <algorithm>
@@ -126,7 +131,8 @@ __global__ __launch_bounds__(256) void k_loss_gather(GatherArgs k, const int* __
   if (i < (int)info[0]) gather_token(k, idx[i], i, __uint_as_float(info[1]));
 }
 // Both of the above in one launch for few tokens: every workgroup (one a token) counts for itself, t / 256
-// tokens a thread, which costs less than a launch up to kCountTokens.
+// tokens a thread, which costs less than a launch up to kCountTokens (a forward call over 8000 x 1024: 256 tokens
+// 21.6 us, 23.8 in two launches; 2048 tokens 46.7 and 48.6; 4096 tokens 86.7 and 83.4).
 constexpr int kCountTokens = 2048;
 __global__ __launch_bounds__(256) void k_loss_pack(GatherArgs k, long ignore, int t, int* __restrict__ idx,
                                                    int* __restrict__ pos, uint32_t* __restrict__ info,
@@ -403,7 +409,7 @@ inline int blocks_for(long items, int per, int most = 1 << 20) {
 }
 
 // The shapes whose P may have any alignment: those that leave registers for it, all of up to 64 columns.
-inline bool direct_shape(int pick) { return pick != 0 && pick != 1 && pick != 5; }
+inline bool direct_shape(int pick) { return kMmaTimes[pick].bq <= 64; }
 constexpr int kDirectTokens = 64;
 template <class F>
 hipError_t with_loss_shape(int pick, bool direct, F f) {
@@ -436,7 +442,8 @@ LossPlan loss_plan(long t, long d, long v, bool pad_w, bool grad) {
   p.tok = take(sizeof(LossTok) * t);
   p.xc = take(2 * (size_t)t * p.dp);
   // Rows of W that the tiles cannot load straight into LDS: few tokens read them through registers (W is
-  // what bounds them), for many a padded copy costs less.
+  // what bounds them), for many a padded copy costs less (both gradients of 64 tokens, 50001 x 1001: 176 us, 203
+  // with a copy; 32000 x 4097: 353 and 429).
   p.direct = pad_w && t <= kDirectTokens;
   auto pick_of = [&](long rows, long cols, long k) {
     int best = -1;
@@ -480,7 +487,7 @@ LossPlan loss_plan(long t, long d, long v, bool pad_w, bool grad) {
     }
     // few tokens: dw's stores are what costs, and two small tiles on a CU overlap theirs with each other's loads
     // (62 tokens, 50001 x 1000: 36 us, large tiles 42; 64, 128256 x 4096: 363 and 370; 300: 664 and 580)
-    p.dw_tiles = t <= 192 || mma_cost(p.dp, p.piece, t, 5, 1, false) < mma_cost(p.dp, p.piece, t, 0, 1, false) ? 5 : 0;
+    p.dw_tiles = t <= 192 || mma_cost(p.dp, p.piece, t, 4, 1, false) < mma_cost(p.dp, p.piece, t, 0, 1, false) ? 4 : 0;
     p.d = take(2 * (size_t)t * p.piece);
     p.dxacc = take(p.dx_bytes);
   }
@@ -585,7 +592,7 @@ hipError_t backward(hipStream_t st, const LossArgs& a, const LossPlan& p) {
             xc, p.dp, (int)a.d, d, p.piece, rows, info, np, nq, gscale, a.dw + (long)v0 * a.lddw, a.lddw);
         return hipGetLastError();
       };
-      e = p.dw_tiles == 5 ? go(MmaShape<4, 4, 2, 2>{}) : go(MmaShape<8, 4, 2, 4>{});
+      e = p.dw_tiles == 4 ? go(MmaShape<4, 4, 2, 2>{}) : go(MmaShape<8, 4, 2, 4>{});
       if (e != hipSuccess) return e;
     }
   }

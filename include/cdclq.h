@@ -367,7 +367,7 @@ size_t cdclq_packed_bytes(const cdclq_packed* packed);
  * 0..adapters gives a NaN row. rank = adapters = 0 leaves the adapters out. rank <= 128; adapters of
  * smaller rank are padded with zeros. low (t x rank f32, may be NULL) receives A_q x_t for the gradient.
  * What a token or an adapter holds reaches no other token's or adapter's results, NaN and infinities
- * included; a token with an infinity may get NaN where the sum is one. The workspace of more than 64
+ * included; a token with an infinity may get NaN where the sum is one. The workspace of more than 192
  * tokens holds the layer in 16 bits. */
 size_t cdclq_adapter_work_bytes(const cdclq_packed* packed, const void* x, size_t ldx, size_t t, const void* a,
                                 const void* b, size_t adapters, size_t rank, int grad);

@@ -234,7 +234,7 @@ __device__ __forceinline__ int next_adapter(int q, uint64_t& left) {
 // Ranks jt, jt + 32, ... of token ot, by 32 threads: out (t x rank) = low, or scaling low with `scaled`;
 // hl[t][2 rp]: scaling low / 2^e as two 16-bit values, hscale[t] = 2^e; e is not below kLeastExp, where
 // f16's smallest values times its largest weights lie under half of its smallest result.
-constexpr int kLeastExp = -24;
+constexpr int kLeastExp = -24, kMostExp = 120;  // 2^120 and a value of up to 2^8 stay finite
 constexpr float kMostScale = 0x1p40f;  // up to here sums divided by 2^e keep what counts of them
 template <class T, int N>
 __device__ __forceinline__ void low_out(const float (&v)[N], int ot, int t, int rank, int rp, int adapters,
@@ -248,7 +248,7 @@ __device__ __forceinline__ void low_out(const float (&v)[N], int ot, int t, int 
 #pragma unroll
   for (int s = 16; s; s >>= 1) m = fmaxf(m, __shfl_xor(m, s));
   if (ot >= t) return;
-  const int e = m > 0.0f && m < __builtin_inff() ? max(kLeastExp, __builtin_amdgcn_frexp_expf(m)) : 0;
+  const int e = m > 0.0f && m < __builtin_inff() ? min(max(kLeastExp, __builtin_amdgcn_frexp_expf(m)), kMostExp) : 0;
   if (jt == 0 && hscale) hscale[ot] = ldexpf(1.0f, e);
 #pragma unroll
   for (int i = 0; i < N; ++i) {

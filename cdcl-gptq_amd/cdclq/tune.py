@@ -217,7 +217,8 @@ def adapter_linear(packed: PackedLinear, x: torch.Tensor, adapters: Adapters | N
                    request: torch.Tensor | None = None, return_low: bool = False):
     """y (T x d_out) = x W^T with each token's adapter beside it: y_t = W x_t + scaling[q] B_q (A_q x_t),
     q = request[t] (int32, -1: none). With return_low also low = A_q x_t (T x rank, float32), which the
-    backward pass takes."""
+    backward pass takes. The requests may come in any order; calls of more than 192 tokens and the backward
+    pass are faster when the tokens of an adapter stand together."""
     ctx = packed.ctx
     code, ld = _code(x, "x"), _matrix(ctx, x, "x", None, None, packed.d_in)
     t = x.shape[0]

@@ -477,7 +477,7 @@ LossPlan loss_plan(long t, long d, long v, bool pad_w, bool grad) {
       const MmaShapeTime s = kMmaTimes[i];
       const long np = (p.dp + s.bp - 1) / s.bp, nq = (t + s.bq - 1) / s.bq, round = 256 * s.per_cu;
       const long n = std::max(1l, std::min(round / (np * nq), (long)p.piece / 512));
-      const double c = mma_cost(p.dp, t, p.piece, i, n, false) * (s.bq <= 64 ? 2.0 : i ? 1.33 : 1.0) + n * (8.0 / 4e6) * t * p.dp;
+      const double c = mma_cost(p.dp, t, p.piece, i, n, false) * (s.bq <= 64 ? 2.0 : s.bp < 256 ? 1.33 : 1.0) + n * (8.0 / 4e6) * t * p.dp;
       if (best < 0 || c < best) {
         best = c;
         p.dx_tiles = i;

@@ -395,7 +395,9 @@ struct MmaShape {
 // measured on 4096 x 65536 results over k = 4096 (the narrow ones estimated); `per_cu`: the workgroups that
 // a CU's LDS holds; `alone`: a stage with few tiles in flight, which the latency of its loads and reads sets,
 // measured on 200 x 4096 results over 4096, and (P's rows contiguous) on 100 x 2688 over 6720.
-constexpr int kMmaShapes = 8;
+// 256 x 192 beside 256 x 256: where the latter leave CUs idle (2000 x 5632 over 2048: 50 us, 59; but 4096 x 14336
+// over 4096: 464, 450).
+constexpr int kMmaShapes = 9;
 struct MmaShapeTime {
   int bp, bq, per_cu;
   double us, alone, alone_strided;
@@ -403,7 +405,8 @@ struct MmaShapeTime {
 constexpr MmaShapeTime kMmaTimes[kMmaShapes] = {
     {256, 256, 1, 1.66, 0.90, 1.15}, {256, 64, 2, 0.55, 0.51, 0.77},
     {256, 32, 2, 0.40, 0.50, 0.75},  {256, 16, 2, 0.33, 0.50, 0.70},  {128, 128, 2, 0.50, 0.49, 0.69},
-    {128, 64, 3, 0.31, 0.43, 0.59},  {128, 32, 4, 0.22, 0.42, 0.55},  {128, 16, 4, 0.18, 0.42, 0.55}};
+    {128, 64, 3, 0.31, 0.43, 0.59},  {128, 32, 4, 0.22, 0.42, 0.55},  {128, 16, 4, 0.18, 0.42, 0.55},
+    {256, 192, 1, 1.40, 0.78, 1.00}};
 template <class F>
 hipError_t with_mma_shape(int pick, F f) {
   switch (pick) {
@@ -414,7 +417,8 @@ hipError_t with_mma_shape(int pick, F f) {
     case 4: return f(MmaShape<4, 4, 2, 2>{});
     case 5: return f(MmaShape<4, 2, 2, 2>{});
     case 6: return f(MmaShape<2, 2, 4, 1>{});
-    default: return f(MmaShape<2, 1, 4, 1>{});
+    case 7: return f(MmaShape<2, 1, 4, 1>{});
+    default: return f(MmaShape<8, 3, 2, 4>{});
   }
 }
 // Microseconds of a product of `rows` x `cols` results over k, `splits` ways in k: rounds of tiles over 256

@@ -14,7 +14,7 @@
 //
 // 4096 tokens, 4096 -> 14336, 4 bits, rank 64, bf16: forward product 425-450 us (1.1 PF, 3.5 rounds of tiles), that
 // of the gradient 340-356 (1.4 PF, one round), both bound by power where all CUs work; 2000 tokens, 2048 -> 5632:
-// 59 us. Expanding the weights and ordering the activations: 41 us (gradient) and 56 (forward), memory at 3.6 TB/s.
+// 50 us. Expanding the weights and ordering the activations: 41 us (gradient) and 56 (forward), memory at 3.6 TB/s.
 //
 // dA and dB sum over the tokens of an adapter: lists in token order, items of some hundred tokens with
 // f32 sums of their own, joined in order (no atomics). dA reads the codes of the checkpoint, exact in
@@ -1170,7 +1170,7 @@ hipError_t wide(hipStream_t st, const PackedView& v, const AdapterArgs& a, void*
     p.list = {a.request, (int)a.t, a.adapters, kItem, 0, list, nullptr, nullptr, tiles, sp.ntiles};
   }
   // The low-rank vectors of few ranks along with the rest, where they need nothing of it (2000 tokens, 2048 ->
-  // 5632: 75 us, 80 in a launch of their own; 4096 tokens, 4096 -> 4096: 145 and 152). Of more ranks their registers
+  // 5632: 5 us less than with a launch of their own; 4096 tokens, 4096 -> 4096: 145 us and 152). Of more ranks their registers
   // would leave the other parts few wavefronts.
   const bool along = low && !tiled && !pad_x && !pad_a && rp <= 32;
   if (along) {

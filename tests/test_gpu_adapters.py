@@ -4,7 +4,8 @@ definition in 64 bits.
 Tolerances: u is the unit roundoff of the 16-bit type (2^-8 for bfloat16, 2^-11 for float16), f32 2^-24.
 A sum of k exact products in f32 is off by at most k 2^-24 sum |.|. Up to 64 tokens the weights are exact
 (2^b + code, of at most 34 times the size of code - zero, and sum x are summed instead); beyond, each
-weight is rounded to 16 bits (u). The low-rank vectors lose at most 2^-15 of their largest element."""
+weight is rounded to 16 bits (u); from 65 to 192 tokens the first form runs under the second's bound. The
+low-rank vectors lose at most 2^-15 of their largest element."""
 import numpy as np
 import pytest
 import torch
@@ -290,6 +291,38 @@ def test_order_of_requests_changes_no_token(ctx, tune):
         y = tune.adapter_linear(packed, x, ad, q)
         p = torch.randperm(t, generator=rng(1), device="cuda")
         assert torch.equal(tune.adapter_linear(packed, x[p].contiguous(), ad, q[p].contiguous()), y[p])
+
+
+@pytest.mark.parametrize("bits,group", [(2, 64), (3, 128), (4, 128), (8, 32), (5, 48), (1, 17), (6, 0), (7, 128)])
+@pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float16])
+def test_expanded_widths_and_groups(ctx, tune, dtype, bits, group):
+    m, n = 203, 393
+    for lead in (0, 2):
+        packed, w, big = make_layer(ctx, tune, bits * 100 + group, m, n, bits, group, lead if group else 0)
+        ad = make_adapters(tune, 5, 3, 8, m, n, dtype)
+        x = normal(4, 210, n, dtype=dtype)
+        check_forward(packed, w, big, ad, x, make_request(3, 210, 3, "sorted"), tune)
+
+
+@pytest.mark.parametrize("rank", [1, 7, 16, 17, 33, 64, 100, 128])
+@pytest.mark.parametrize("order", ["any", "sorted"])
+def test_expanded_ranks(ctx, tune, rank, order):
+    m, n, t = 290, 512, 1100
+    packed, w, big = make_layer(ctx, tune, rank, m, n, 4, 128)
+    for dtype in (torch.bfloat16, torch.float16):
+        ad = make_adapters(tune, rank, 4, rank, m, n, dtype)
+        check_forward(packed, w, big, ad, normal(2, t, n, dtype=dtype), make_request(t, t, 4, order), tune)
+
+
+@pytest.mark.parametrize("t", [127, 128, 129, 191, 192, 193])
+@pytest.mark.parametrize("rank", [4, 64, 128])
+def test_token_counts_where_the_form_changes(ctx, tune, t, rank):
+    m, n, b = 150, 264, torch.bfloat16
+    packed, w, big = make_layer(ctx, tune, t, m, n, 4, 128)
+    ad = make_adapters(tune, 3, 3, rank, m, n, b)
+    x, q = normal(1, t, n, dtype=b), make_request(t, t, 3, "any")
+    check_forward(packed, w, big, ad, x, q, tune)
+    check_backward(packed, w, ad, x, q, normal(2, t, m, dtype=b), tune, ctx)
 
 
 @pytest.mark.parametrize("t", [130, 700])

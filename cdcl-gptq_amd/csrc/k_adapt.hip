@@ -865,8 +865,8 @@ __device__ void join_db(const JoinJob& k, const int2* of, int rank, int rp, int 
   uint32_t w[4];
 #pragma unroll
   for (int j = 0; j < 4; ++j) w[j] = narrow2<T>(s[2 * j], s[2 * j + 1]);
-  if (j0 + 8 <= rank && rank % 8 == 0 && (uintptr_t)k.out % 16 == 0) {
-    *reinterpret_cast<uint4*>(o) = make_uint4(w[0], w[1], w[2], w[3]);
+  if (j0 + 8 <= rank) {
+    __builtin_memcpy(o, w, 16);  // any alignment
   } else {
 #pragma unroll
     for (int j = 0; j < 8; ++j)

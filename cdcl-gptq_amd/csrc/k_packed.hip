@@ -346,11 +346,16 @@ __global__ __launch_bounds__(64 * W) void k_packed_few(PackedView v, FewArgs k) 
           if (k.rank >= 16) d += dot8(early[i][1], lo + 8);
           for (int j = 16; j < k.rank; j += 8) d += dot8(*reinterpret_cast<const uint4*>(br + j), lo + j);
         } else {
-          for (int j0 = 0; j0 < k.rank; j0 += 8) {  // the same order
-            float p = 0.0f;
-            for (int j = j0; j < min(j0 + 8, k.rank); ++j) p = __builtin_fmaf(T::widen(br[j]), lo[j], p);
-            d += p;
+          int j0 = 0;  // the same order
+#pragma unroll 4
+          for (; j0 + 8 <= k.rank; j0 += 8) {
+            uint4 u;
+            __builtin_memcpy(&u, br + j0, 16);
+            d += dot8(u, lo + j0);
           }
+          float p = 0.0f;
+          for (int j = j0; j < k.rank; ++j) p = __builtin_fmaf(T::widen(br[j]), lo[j], p);
+          d += p;
         }
         s = __builtin_fmaf(k.scaling[q], d, s);
       } else if (q != -1) {

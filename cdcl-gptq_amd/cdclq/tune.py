@@ -22,6 +22,7 @@ from dataclasses import dataclass
 
 import numpy as np
 import torch
+from torch.autograd.function import once_differentiable
 
 from . import DTYPE_BF16, DTYPE_F16, Context, lib as _L
 
@@ -320,6 +321,7 @@ class _Linear(torch.autograd.Function):
         return y
 
     @staticmethod
+    @once_differentiable
     def backward(fn, dy):
         dy = dy.contiguous()
         if fn.adapters is None:
@@ -332,8 +334,8 @@ class _Linear(torch.autograd.Function):
 
 def linear(packed: PackedLinear, x: torch.Tensor, adapters: Adapters | None = None,
            request: torch.Tensor | None = None) -> torch.Tensor:
-    """adapter_linear for autograd: gradients of x and of adapters.a and .b; between the passes x is kept
-    as an 8-bit checkpoint."""
+    """adapter_linear for autograd: gradients of x and of adapters.a and .b, of first order only; between the
+    passes x is kept as an 8-bit checkpoint."""
     return _Linear.apply(x, adapters.a if adapters else None, adapters.b if adapters else None, packed, adapters,
                          request)
 
@@ -348,6 +350,7 @@ class _CrossEntropy(torch.autograd.Function):
         return loss.sum() * weight
 
     @staticmethod
+    @once_differentiable
     def backward(fn, grad):
         x, w, targets, lse, weight = fn.saved_tensors
         dloss = (grad * weight).float().expand(len(x)).contiguous()
@@ -357,6 +360,6 @@ class _CrossEntropy(torch.autograd.Function):
 
 def cross_entropy(ctx: Context, x: torch.Tensor, w: torch.Tensor, targets: torch.Tensor,
                   ignore_index: int = -100) -> torch.Tensor:
-    """The mean of vocab_loss over the tokens that take part (0 if none does), for autograd: gradients of
-    x and, where w asks for it, of w."""
+    """The mean of vocab_loss over the tokens that take part (0 if none does), for autograd: gradients (of
+    first order only) of x and, where w asks for it, of w."""
     return _CrossEntropy.apply(x, w, ctx, targets, ignore_index)

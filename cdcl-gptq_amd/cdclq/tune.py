@@ -22,7 +22,6 @@ from dataclasses import dataclass
 
 import numpy as np
 import torch
-from torch.autograd.function import once_differentiable
 
 from . import DTYPE_BF16, DTYPE_F16, Context, lib as _L
 
@@ -307,6 +306,18 @@ def vocab_loss_backward(ctx: Context, x: torch.Tensor, w: torch.Tensor, targets:
 
 
 # ---------------------------------------------------------------- as differentiable functions
+def _first_order(backward):
+    """A backward pass that has no gradient of its own and refuses to take part in a graph (create_graph). Its
+    results would count there as constants and lose terms without a word; an error tied to them, as torch's
+    once_differentiable makes, is reached only where the graph happens to lead through it."""
+    def run(fn, *grads):
+        if torch.is_grad_enabled():
+            raise RuntimeError("cdclq.tune: linear and cross_entropy have gradients of first order only "
+                               "(create_graph is not supported)")
+        return backward(fn, *grads)
+    return run
+
+
 class _Linear(torch.autograd.Function):
     @staticmethod
     def forward(fn, x, a, b, packed, adapters, request):
@@ -321,7 +332,7 @@ class _Linear(torch.autograd.Function):
         return y
 
     @staticmethod
-    @once_differentiable
+    @_first_order
     def backward(fn, dy):
         dy = dy.contiguous()
         if fn.adapters is None:
@@ -350,7 +361,7 @@ class _CrossEntropy(torch.autograd.Function):
         return loss.sum() * weight
 
     @staticmethod
-    @once_differentiable
+    @_first_order
     def backward(fn, grad):
         x, w, targets, lse, weight = fn.saved_tensors
         dloss = (grad * weight).float().expand(len(x)).contiguous()

@@ -320,35 +320,39 @@ def _first_order(backward):
 
 class _Linear(torch.autograd.Function):
     @staticmethod
-    def forward(fn, x, a, b, packed, adapters, request):
-        fn.packed, fn.adapters = packed, adapters
+    def forward(fn, x, a, b, scaling, packed, adapters, request):
+        fn.packed, fn.has_adapters = packed, adapters is not None
         if adapters is None:
             fn.save_for_backward()
             return adapter_linear(packed, x)
         y, low = adapter_linear(packed, x, adapters, request, return_low=True)
         ck = checkpoint_save(packed.ctx, x)
         fn.dtype = x.dtype
-        fn.save_for_backward(ck.codes, ck.scales, low, request, a, b)  # a, b: changed in place would be an error
+        fn.save_for_backward(ck.codes, ck.scales, low, request, a, b, scaling)
         return y
 
     @staticmethod
     @_first_order
     def backward(fn, dy):
         dy = dy.contiguous()
-        if fn.adapters is None:
-            return adapter_linear_backward(fn.packed, dy)[0], None, None, None, None, None
-        codes, scales, low, request, _, _ = fn.saved_tensors
-        dx, da, db = adapter_linear_backward(fn.packed, dy, Checkpoint(codes, scales, fn.dtype), low, fn.adapters,
-                                             request)
-        return dx, da, db, None, None, None
+        if not fn.has_adapters:
+            return adapter_linear_backward(fn.packed, dy)[0], None, None, None, None, None, None
+        # the operands of the forward call, whatever the Adapters hold by now; changed in place is an error here
+        codes, scales, low, request, a, b, scaling = fn.saved_tensors
+        dx, da, db = adapter_linear_backward(fn.packed, dy, Checkpoint(codes, scales, fn.dtype), low,
+                                             Adapters(a, b, scaling), request)
+        return dx, da, db, None, None, None, None
 
 
 def linear(packed: PackedLinear, x: torch.Tensor, adapters: Adapters | None = None,
            request: torch.Tensor | None = None) -> torch.Tensor:
     """adapter_linear for autograd: gradients of x and of adapters.a and .b, of first order only; between the
-    passes x is kept as an 8-bit checkpoint."""
-    return _Linear.apply(x, adapters.a if adapters else None, adapters.b if adapters else None, packed, adapters,
-                         request)
+    passes x is kept as an 8-bit checkpoint. scaling is a constant."""
+    if adapters is None:
+        return _Linear.apply(x, None, None, None, packed, None, request)
+    if adapters.scaling.requires_grad and torch.is_grad_enabled():
+        raise ValueError("scaling asks for a gradient; linear has none for it")
+    return _Linear.apply(x, adapters.a, adapters.b, adapters.scaling, packed, adapters, request)
 
 
 class _CrossEntropy(torch.autograd.Function):

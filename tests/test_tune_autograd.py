@@ -114,3 +114,35 @@ def test_second_order_is_refused(calls):
             torch.autograd.grad(f().sum(), x, create_graph=True)
         (g,) = torch.autograd.grad(f().sum(), x)
         assert torch.isfinite(g).all() and g.any()
+
+
+@pytest.mark.parametrize("what", ["a", "b", "scaling"])
+def test_operands_changed_in_place_are_refused(calls, what):
+    layer, x, ad, q = case()
+    y = tune.linear(layer, x, ad, q)
+    with torch.no_grad():
+        getattr(ad, what).mul_(3.0)
+    with pytest.raises(RuntimeError, match="modified by an inplace operation"):
+        y.sum().backward()
+
+
+@pytest.mark.parametrize("what", ["a", "b", "scaling"])
+def test_operands_replaced_do_not_reach_the_gradient(calls, what):
+    """Another tensor put into the Adapters between the passes: the gradient is of what y was made with."""
+    layer, x, ad, q = case()
+    x = x.requires_grad_()
+    a, b = ad.a, ad.b
+    want = torch.autograd.grad(wanted(layer, x, a, b, ad.scaling, q).sum(), (x, a, b))
+    y = tune.linear(layer, x, ad, q)
+    setattr(ad, what, (getattr(ad, what).detach() * 3.0).requires_grad_(what != "scaling"))
+    for g, w in zip(torch.autograd.grad(y.sum(), (x, a, b)), want):
+        assert torch.allclose(g, w, atol=1e-5)
+
+
+def test_a_scaling_that_asks_for_a_gradient_is_refused(calls):
+    layer, x, ad, q = case()
+    ad.scaling.requires_grad_()
+    with pytest.raises(ValueError, match="scaling"):
+        tune.linear(layer, x, ad, q)
+    with torch.no_grad():  # no gradient is asked for
+        assert torch.allclose(tune.linear(layer, x, ad, q), wanted(layer, x, ad.a, ad.b, ad.scaling, q), atol=1e-5)

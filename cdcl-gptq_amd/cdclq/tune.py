@@ -324,7 +324,7 @@ class _Linear(torch.autograd.Function):
         fn.packed, fn.has_adapters = packed, adapters is not None
         if adapters is None:
             fn.save_for_backward()
-            return adapter_linear(packed, x)
+            return adapter_linear(packed, x, None, request)
         y, low = adapter_linear(packed, x, adapters, request, return_low=True)
         ck = checkpoint_save(packed.ctx, x)
         fn.dtype = x.dtype

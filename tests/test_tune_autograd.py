@@ -146,3 +146,11 @@ def test_a_scaling_that_asks_for_a_gradient_is_refused(calls):
         tune.linear(layer, x, ad, q)
     with torch.no_grad():  # no gradient is asked for
         assert torch.allclose(tune.linear(layer, x, ad, q), wanted(layer, x, ad.a, ad.b, ad.scaling, q), atol=1e-5)
+
+
+def test_a_request_without_adapters_is_refused(monkeypatch):
+    """As adapter_linear refuses it (before anything reaches the library)."""
+    layer, x, _, q = case()
+    monkeypatch.setattr(tune, "_matrix", lambda *_: 6)
+    with pytest.raises(ValueError, match="request without adapters"):
+        tune.linear(layer, x.bfloat16(), None, q)

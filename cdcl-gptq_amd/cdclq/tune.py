@@ -348,9 +348,12 @@ def linear(packed: PackedLinear, x: torch.Tensor, adapters: Adapters | None = No
            request: torch.Tensor | None = None) -> torch.Tensor:
     """adapter_linear for autograd: gradients of x and of adapters.a and .b, of first order only; between the
     passes x is kept as an 8-bit checkpoint. scaling is a constant."""
+    wanted = (x,) if adapters is None else (x, adapters.a, adapters.b, adapters.scaling)
+    if not (torch.is_grad_enabled() and any(t.requires_grad for t in wanted)):
+        return adapter_linear(packed, x, adapters, request)  # no checkpoint, no low
     if adapters is None:
         return _Linear.apply(x, None, None, None, packed, None, request)
-    if adapters.scaling.requires_grad and torch.is_grad_enabled():
+    if adapters.scaling.requires_grad:
         raise ValueError("scaling asks for a gradient; linear has none for it")
     return _Linear.apply(x, adapters.a, adapters.b, adapters.scaling, packed, adapters, request)
 

@@ -154,3 +154,16 @@ def test_a_request_without_adapters_is_refused(monkeypatch):
     monkeypatch.setattr(tune, "_matrix", lambda *_: 6)
     with pytest.raises(ValueError, match="request without adapters"):
         tune.linear(layer, x.bfloat16(), None, q)
+
+
+def test_nothing_is_kept_where_no_gradient_is_asked_for(calls):
+    layer, x, ad, q = case()
+    want = wanted(layer, x, ad.a, ad.b, ad.scaling, q).detach()
+    with torch.no_grad():
+        assert torch.allclose(tune.linear(layer, x, ad, q), want, atol=1e-5)
+    assert not calls
+    layer, x, ad, q = case(grad=False)
+    assert torch.allclose(tune.linear(layer, x, ad, q), want, atol=1e-5) and not calls
+    layer, x, ad, q = case()
+    tune.linear(layer, x, ad, q)
+    assert len(calls) == 1

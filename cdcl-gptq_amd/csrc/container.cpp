@@ -36,7 +36,7 @@ std::string check_layout(size_t d_in, size_t group, const uint8_t* gbits, size_t
   if (d_in == 0) return "";
   if (d_in > kMaxDin) return "d_in " + std::to_string(d_in) + " exceeds this build's limit of 131072 columns";
   if (group == 0) return "group size must be > 0";
-  const size_t used = (d_in + group - 1) / group;
+  const size_t used = d_in / group + (d_in % group != 0);  // group may be as large as size_t goes
   if (ngroups < used)
     return "ngroups " + std::to_string(ngroups) + " is smaller than ceil(d_in / group) = " + std::to_string(used);
   if (need_widths) {
@@ -90,7 +90,7 @@ struct LayoutDev {
 // widths, which then build nothing either (every call ends with a stream synchronisation, so no
 // kernel still reads it when it is replaced).
 int upload_layout(cdclq_ctx* ctx, size_t n, size_t g, const uint8_t* gbits, LayoutDev* D) {
-  const size_t used = (n + g - 1) / g, wpr = (row_bytes_of(n, g, gbits) + 3) / 4;
+  const size_t used = n / g + (n % g != 0), wpr = (row_bytes_of(n, g, gbits) + 3) / 4;
   const size_t a = ((n + 1) * 4 + 255) & ~(size_t)255;
   const size_t b = (wpr * 4 + 255) & ~(size_t)255;
   const size_t c = ((n + 7) / 8 * 4 + 255) & ~(size_t)255;
@@ -149,6 +149,7 @@ int pack_device(cdclq_ctx* ctx, size_t d_out, size_t n, size_t g, const uint8_t*
   if (d_out == 0 || n == 0) return CDCLQ_OK;
   const std::string why = check_layout(n, g, gbits, ng, true);
   if (!why.empty()) return fail(ctx, CDCLQ_INVALID_ARG, why);
+  g = std::min(g, n);  // one group holds all; kernels take it in 32 bits
   if (!codes || !scales || !zeros || !perm || !qweight || !s16 || !qz || !p32)
     return fail(ctx, CDCLQ_INVALID_ARG, "null buffer argument");
   const size_t rb = row_bytes_of(n, g, gbits);
@@ -213,6 +214,7 @@ int dequant_packed_device(cdclq_ctx* ctx, size_t d_out, size_t n, size_t g, cons
   if (d_out == 0 || n == 0) return CDCLQ_OK;
   const std::string why = check_layout(n, g, gbits, ng, true);
   if (!why.empty()) return fail(ctx, CDCLQ_INVALID_ARG, why);
+  g = std::min(g, n);  // one group holds all; kernels take it in 32 bits
   if (!qweight || !s16 || !qz || !p32 || !out) return fail(ctx, CDCLQ_INVALID_ARG, "null buffer argument");
   const size_t rb = row_bytes_of(n, g, gbits);
   if (qweight_bytes < d_out * rb)
@@ -238,6 +240,7 @@ int dequant_layer_device(cdclq_ctx* ctx, size_t d_out, size_t n, size_t g, size_
   if (d_out == 0 || n == 0) return CDCLQ_OK;
   const std::string why = check_layout(n, g, nullptr, ng, false);
   if (!why.empty()) return fail(ctx, CDCLQ_INVALID_ARG, why);
+  g = std::min(g, n);
   if (!codes || !scales || !zeros || !perm || !out) return fail(ctx, CDCLQ_INVALID_ARG, "null buffer argument");
   HIPCK(hipSetDevice(ctx->device));
   uint32_t* cdesc;

@@ -1,0 +1,39 @@
+"""GPU tests of what cdclq.tune and the container calls beside it take and refuse at the ends of their ranges:
+layouts that do not fit their tensors, views of one row, sizes whose launches pass 2^32 work-items."""
+import numpy as np
+import pytest
+import torch
+
+import cdclq
+from tests.test_gpu_adapters import make_adapters, make_layer, make_request, normal
+
+pytestmark = pytest.mark.gpu
+
+
+@pytest.fixture(scope="module")
+def ctx():
+    c = cdclq.Context(0)
+    yield c
+    c.close()
+
+
+@pytest.fixture(scope="module")
+def tune():
+    from cdclq import tune
+    return tune
+
+
+def test_the_largest_group_is_one_group_of_any_width(ctx):
+    """A group of 2^64 - 1 (a signed caller's -1) over layers of one shape and several widths: the tables of one
+    are not taken for the next."""
+    n, m = 40, 6
+    r = np.random.default_rng(1)
+    for bits in (4, 8, 3):
+        ql = cdclq.QLayer(m, n, n, np.arange(n, dtype=np.uint32), np.array([bits], np.uint8),
+                          r.integers(0, 1 << bits, (m, n)).astype(np.uint8), np.ones((m, 1), np.float32),
+                          np.zeros((m, 1), np.float32))
+        qw, s16, qz, p32 = cdclq.pack_layer(ctx, ql)
+        got = cdclq.dequantize_packed(ctx, qw, s16, qz, p32, ql.gbits, (1 << 64) - 1)
+        assert np.array_equal(got, ql.codes.astype(np.float32))
+        assert np.array_equal(cdclq.dequantize_layer(ctx, cdclq.QLayer(m, n, (1 << 64) - 1, ql.perm, ql.gbits, ql.codes,
+                                                                       ql.scales, ql.zeros)), got)

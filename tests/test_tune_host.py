@@ -39,3 +39,12 @@ def test_null_handles_are_refused():
     assert L.cdclq_packed_open_device(None, 1, 8, 8, 0, 1, 0, 8, 0, 0, 0, None) == cdclq.INVALID_ARG
     L.cdclq_packed_close(None)
     assert L.cdclq_packed_bytes(None) == 0
+
+
+def test_widths_are_checked_for_any_group_size():
+    """d_in + group - 1 passes the end of size_t: the widths were not looked at (-1 of a signed caller)."""
+    assert cdclq.row_bytes(10, (1 << 64) - 1, [4]) == cdclq.row_bytes(10, 10, [4]) == 5
+    for group in (10, 1 << 40, (1 << 64) - 9, (1 << 64) - 1):
+        for gbits in ([9], [0], []):
+            with pytest.raises(cdclq.CdclqError):
+                cdclq.row_bytes(10, group, gbits)

@@ -581,6 +581,16 @@ def row_bytes(n: int, g: int, gbits) -> int:
     return out.value
 
 
+def check_row_width(width: int, n: int, g: int, gbits):
+    """Refuses qweight rows wider than the layout's (a layout of another layer, rows padded for alignment): the
+    library takes the rows one after another and would read one into the next. Rows that are too short, and
+    layouts that are none, it reports itself."""
+    gbits = np.ascontiguousarray(gbits, np.uint8)
+    out = C.c_size_t()
+    if n and lib().cdclq_row_bytes(n, g, gbits.ctypes.data, gbits.size, C.byref(out)) == OK and width > out.value:
+        raise CdclqError(INVALID_ARG, f"qweight has rows of {width} bytes, the layout's take {out.value}")
+
+
 def pack_layer(ctx: Context, ql: QLayer):
     """QLayer::pack + io::packed_tensors (src/quant.rs:207-214, src/io.rs:244-264) on the GPU:
     (qweight u8 [d_out, row_bytes], scales f16 bits u16 [d_out, ng], qzeros u8 [d_out, ng],
@@ -626,6 +636,7 @@ def dequantize_packed(ctx: Context, qweight, scales_f16, qzeros, perm_i32, gbits
     p32 = np.ascontiguousarray(perm_i32, np.int32)
     gbits = np.ascontiguousarray(gbits, np.uint8)
     d_out, d_in = qweight.shape[0], p32.size
+    check_row_width(qweight.size // d_out if d_out else 0, d_in, group, gbits)
     out = np.zeros((d_out, d_in), _DTYPE_NP.get(dt, np.float32))
     ctx.check(lib().cdclq_dequantize_packed(ctx.ptr, d_out, d_in, group, gbits.ctypes.data, gbits.size,
                                             qweight.ctypes.data, qweight.size, s16.ctypes.data, qz.ctypes.data,

@@ -23,7 +23,7 @@ from dataclasses import dataclass
 import numpy as np
 import torch
 
-from . import DTYPE_BF16, DTYPE_F16, Context, lib as _L
+from . import DTYPE_BF16, DTYPE_F16, Context, check_row_width, lib as _L
 
 BLOCK = 128  # features per scale of an 8-bit checkpoint
 _CODES = {torch.bfloat16: DTYPE_BF16, torch.float16: DTYPE_F16}
@@ -142,6 +142,7 @@ class PackedLinear:
             raise ValueError(f"qweight {tuple(qw.shape)}, scales {tuple(s16.shape)}, qzeros {tuple(qz.shape)} and "
                              f"{gb.size} groups do not belong together")
         self.d_out, self.d_in = qw.shape[0], p32.shape[0]
+        check_row_width(qw.shape[1], self.d_in, int(group), gb)
         torch.cuda.current_stream(dev).synchronize()
         out = C.c_void_p()
         ctx.check(_L().cdclq_packed_open_device(ctx.ptr, self.d_out, self.d_in, int(group), gb.ctypes.data, gb.size,

@@ -37,3 +37,19 @@ def test_the_largest_group_is_one_group_of_any_width(ctx):
         assert np.array_equal(got, ql.codes.astype(np.float32))
         assert np.array_equal(cdclq.dequantize_layer(ctx, cdclq.QLayer(m, n, (1 << 64) - 1, ql.perm, ql.gbits, ql.codes,
                                                                        ql.scales, ql.zeros)), got)
+
+
+@pytest.mark.parametrize("extra", [1, 8, -1])
+def test_rows_of_another_width_are_refused(ctx, tune, extra):
+    """qweight rows wider than the layout's (a layout of another layer, rows padded for alignment) are not read
+    one into the next."""
+    ql = cdclq.QLayer(6, 64, 32, np.arange(64, dtype=np.uint32), np.array([4, 3], np.uint8),
+                      np.random.default_rng(1).integers(0, 8, (6, 64)).astype(np.uint8), np.ones((6, 2), np.float32),
+                      np.zeros((6, 2), np.float32))
+    qw, s16, qz, p32 = cdclq.pack_layer(ctx, ql)
+    tune.PackedLinear(ctx, qw, s16, qz, p32, ql.gbits, 32).close()
+    wrong = np.zeros((6, qw.shape[1] + extra), np.uint8)
+    with pytest.raises(cdclq.CdclqError, match="qweight"):
+        tune.PackedLinear(ctx, wrong, s16, qz, p32, ql.gbits, 32)
+    with pytest.raises(cdclq.CdclqError, match="qweight"):
+        cdclq.dequantize_packed(ctx, wrong, s16, qz, p32, ql.gbits, 32)

@@ -98,11 +98,11 @@ def checkpoint_save(ctx: Context, x: torch.Tensor) -> Checkpoint:
 
 
 def _check_saved(ctx: Context, ck: Checkpoint, rows=None, cols=None):
-    if _matrix(ctx, ck.codes, "codes", torch.int8, rows, cols) != ck.codes.shape[1]:
-        raise ValueError("codes must be contiguous")
+    _matrix(ctx, ck.codes, "codes", torch.int8, rows, cols)
     t, n = ck.codes.shape
-    if _matrix(ctx, ck.scales, "scales", torch.float32, t, -(-n // BLOCK)) != ck.scales.shape[1]:
-        raise ValueError("scales must be contiguous")
+    _matrix(ctx, ck.scales, "scales", torch.float32, t, -(-n // BLOCK))
+    if not (ck.codes.is_contiguous() and ck.scales.is_contiguous()):
+        raise ValueError("codes and scales must be contiguous")
 
 
 def checkpoint_restore(ctx: Context, ck: Checkpoint) -> torch.Tensor:
@@ -251,7 +251,8 @@ def adapter_linear_backward(packed: PackedLinear, dy: torch.Tensor, saved: Check
         if saved is None or low is None:
             raise ValueError("the adapters' gradient needs the saved input and low")
         _check_saved(ctx, saved, t, packed.d_in)
-        if _matrix(ctx, low, "low", torch.float32, t, rank) != rank:
+        _matrix(ctx, low, "low", torch.float32, t, rank)
+        if not low.is_contiguous():
             raise ValueError("low must be contiguous")
         codes, scales, lp = saved.codes.data_ptr(), saved.scales.data_ptr(), low.data_ptr()
         da, db = torch.empty_like(adapters.a), torch.empty_like(adapters.b)

@@ -53,3 +53,28 @@ def test_rows_of_another_width_are_refused(ctx, tune, extra):
         tune.PackedLinear(ctx, wrong, s16, qz, p32, ql.gbits, 32)
     with pytest.raises(cdclq.CdclqError, match="qweight"):
         cdclq.dequantize_packed(ctx, wrong, s16, qz, p32, ql.gbits, 32)
+
+
+def test_views_of_one_row_are_contiguous(ctx, tune):
+    """One token's row of larger tensors (its stride is of no meaning): low and a checkpoint of it are taken."""
+    m, n, rank = 48, 256, 8
+    packed, _, _ = make_layer(ctx, tune, 3, m, n, 4, 128)
+    ad = make_adapters(tune, 2, 2, rank, m, n, torch.bfloat16)
+    q = torch.ones(1, dtype=torch.int32, device="cuda")
+    x, dy = normal(1, 1, n, dtype=torch.bfloat16), normal(2, 1, m, dtype=torch.bfloat16)
+    low = tune.adapter_linear(packed, x, ad, q, return_low=True)[1]
+    ck = tune.checkpoint_save(ctx, x)
+    want = tune.adapter_linear_backward(packed, dy, ck, low, ad, q)
+
+    def row(z):
+        out = torch.zeros(1, z.shape[1] + 24, dtype=z.dtype, device="cuda")[:, : z.shape[1]].copy_(z)
+        assert out.is_contiguous() and out.stride(0) > out.shape[1]
+        return out
+
+    ck2 = tune.Checkpoint(row(ck.codes), row(ck.scales), ck.dtype)
+    assert torch.equal(tune.checkpoint_restore(ctx, ck2), tune.checkpoint_restore(ctx, ck))
+    for a, b in zip(tune.adapter_linear_backward(packed, dy, ck2, row(low), ad, q), want):
+        assert torch.equal(a, b)
+    two = torch.zeros(2, n + 8, dtype=torch.int8, device="cuda")[:, :n]
+    with pytest.raises(ValueError, match="contiguous"):
+        tune.checkpoint_restore(ctx, tune.Checkpoint(two, torch.zeros(2, 2, device="cuda"), torch.bfloat16))

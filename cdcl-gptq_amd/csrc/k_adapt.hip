@@ -977,11 +977,13 @@ struct FinishArgs {
   int rank, rp;
   BackJob back;
   SumJob sum;
+  __host__ __device__ int total() const { return nda + ndb + nback + nsum; }
 };
 template <class T>
 __global__ __launch_bounds__(256) void k_finish(PackedView v, FinishArgs k) {
   extern __shared__ __align__(16) uint16_t lds[];
-  int b = blockIdx.x;
+  int b = blockIdx.x + blockIdx.y * gridDim.x;
+  if (b >= k.total()) return;
   if (b < k.nback) return from_slots(v, k.back, lds, b);
   b -= k.nback;
   if (b < k.nsum) {
@@ -1199,7 +1201,7 @@ hipError_t wide(hipStream_t st, const PackedView& v, const AdapterArgs& a, void*
   FinishArgs f = {};
   f.sum = {parts, plan.splits, (int)a.t, v.m, (long)up(v.m, 4), nullptr, nullptr, nullptr, 0, 0, nullptr, a.y, a.ldy};
   f.nsum = (int)(a.t * ((v.m + 255) / 256));
-  k_finish<T><<<f.nsum, 256, 0, st>>>(v, f);
+  k_finish<T><<<launch_grid(f.total()), 256, 0, st>>>(v, f);
   return hipGetLastError();
 }
 
@@ -1332,7 +1334,7 @@ hipError_t grad(hipStream_t st, const PackedView& v, const AdapterArgs& a, void*
     }
   }
   const size_t lds = f.nback ? slot_lds(v) : 4 * (size_t)f.sum_rows * v.n;
-  k_finish<T><<<f.nda + f.ndb + f.nback + f.nsum, 256, lds, st>>>(v, f);
+  k_finish<T><<<launch_grid(f.total()), 256, lds, st>>>(v, f);
   return hipGetLastError();
 }
 

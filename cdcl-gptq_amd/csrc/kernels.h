@@ -264,6 +264,13 @@ hipError_t synth_perturb(hipStream_t st, uint64_t seed, uint64_t offset, size_t 
                          float* out);
 hipError_t f64_to_f32(hipStream_t st, size_t count, const double* a, float* b);
 
+// Workgroups along x, from 2^20 on along y as well: a launch of 2^32 work-items along x runs only what passes that,
+// without an error. A kernel's workgroup is blockIdx.x + blockIdx.y * gridDim.x; those past the last return.
+inline dim3 launch_grid(long blocks) {
+  const long x = blocks < (1l << 20) ? blocks : 1l << 20;
+  return dim3((unsigned)x, (unsigned)((blocks + x - 1) / x));
+}
+
 // ---- k_ckpt.hip: 8-bit activation checkpoints (dtype: CDCLQ_DTYPE_F16 or _BF16). codes t x n,
 // scales t x ceil(n / 128)
 hipError_t ckpt_save(hipStream_t st, int dtype, const uint16_t* x, long ldx, long t, long n, int8_t* codes,

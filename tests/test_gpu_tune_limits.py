@@ -78,3 +78,28 @@ def test_views_of_one_row_are_contiguous(ctx, tune):
     two = torch.zeros(2, n + 8, dtype=torch.int8, device="cuda")[:, :n]
     with pytest.raises(ValueError, match="contiguous"):
         tune.checkpoint_restore(ctx, tune.Checkpoint(two, torch.zeros(2, 2, device="cuda"), torch.bfloat16))
+
+
+def test_gradient_of_more_adapters_than_work_items_along_x(ctx, tune):
+    """32768 adapters of rank 128 on 769 columns: 2^24 and some workgroups of 256 write dA and dB. Three of the
+    adapters have a token each; they have to get what a call with those three alone gives, the others zeros."""
+    r, rank, m, n, b = 32768, 128, 4, 769, torch.bfloat16
+    packed, _, _ = make_layer(ctx, tune, 3, m, n, 4, 128)
+    few = make_adapters(tune, 2, 3, rank, m, n, b)
+    at = torch.tensor([5, 20000, r - 1], device="cuda")
+    a, bb = torch.zeros(r, rank, n, dtype=b, device="cuda"), torch.zeros(r, m, rank, dtype=b, device="cuda")
+    a[at], bb[at] = few.a, few.b
+    scaling = torch.ones(r, device="cuda")
+    scaling[at] = few.scaling
+    x, dy = normal(1, 3, n, dtype=b), normal(2, 3, m, dtype=b)
+    results = []
+    for ad, q in ((tune.Adapters(a, bb, scaling), at.int()), (few, torch.arange(3, dtype=torch.int32, device="cuda"))):
+        y, low = tune.adapter_linear(packed, x, ad, q, return_low=True)
+        results.append((y,) + tune.adapter_linear_backward(packed, dy, tune.checkpoint_save(ctx, x), low, ad, q))
+    (y, dx, da, db), (y3, dx3, da3, db3) = results
+    assert torch.equal(y, y3) and torch.equal(dx, dx3)
+    assert torch.equal(da[at], da3) and torch.equal(db[at], db3)
+    da[at], db[at] = 0, 0
+    assert not da.any() and not db.any()
+    del a, bb, ad, results, y, dx, da, db
+    torch.cuda.empty_cache()

@@ -187,7 +187,9 @@ __global__ __launch_bounds__(64 * WP * WQ, 2) void k_loss_tiles(const uint16_t* 
                                                                 float* __restrict__ hit, int d) {
   typedef MmaTile<T, false, false, FP, FQ, WP, WQ, U> M;
   __shared__ __align__(1024) uint8_t lds[M::LDS];
-  const MmaTileAt at = mma_tile_at(blockIdx.x, np, nq);
+  const int id = blockIdx.x + blockIdx.y * gridDim.x;
+  if (id >= np * nq) return;
+  const MmaTileAt at = mma_tile_at(id, np, nq);
   const int p0 = at.p * M::BP, q0 = at.q * M::BQ, count = (int)info[0];
   if (q0 >= count) return;
   mma_f4 acc[FP][FQ];
@@ -535,7 +537,7 @@ hipError_t forward(hipStream_t st, const LossArgs& a, const LossPlan& p) {
   e = with_loss_shape(p.tiles, p.direct, [&](auto s, auto u) {
     typedef decltype(s) S;
     const int np = (int)((a.v + S::bp - 1) / S::bp), nq = (int)((a.t + S::bq - 1) / S::bq);
-    k_loss_tiles<T, S::fp, S::fq, S::wp, S::wq, decltype(u)::value><<<np * nq, S::threads, 0, st>>>(
+    k_loss_tiles<T, S::fp, S::fq, S::wp, S::wq, decltype(u)::value><<<launch_grid((long)np * nq), S::threads, 0, st>>>(
         w, ldw, (int)a.v, reinterpret_cast<uint16_t*>(ws + p.xc), p.dp, reinterpret_cast<uint32_t*>(ws + p.info), np, nq,
         reinterpret_cast<LossTok*>(ws + p.tok), reinterpret_cast<float2*>(ws + p.part), (int)a.t,
         reinterpret_cast<float*>(ws + p.hit), (int)a.d);

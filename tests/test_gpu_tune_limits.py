@@ -103,3 +103,23 @@ def test_gradient_of_more_adapters_than_work_items_along_x(ctx, tune):
     assert not da.any() and not db.any()
     del a, bb, ad, results, y, dx, da, db
     torch.cuda.empty_cache()
+
+
+def test_loss_of_more_tiles_than_work_items_along_x(ctx, tune):
+    """2^22 tokens over 2^17 entries: 2^23 tiles of 512 threads. The losses of tokens from all over are compared
+    with 64 bits (8 products of values up to 8 in f32, and a few ulp of values below 2^5)."""
+    t, d, v, b = 1 << 22, 8, 1 << 17, torch.bfloat16
+    x, w = normal(1, t, d, dtype=b), normal(2, v, d, dtype=b)
+    y = torch.randint(0, v, (t,), generator=torch.Generator(device="cuda").manual_seed(3), device="cuda")
+    y[::5] = -100
+    loss, lse = tune.vocab_loss(ctx, x, w, y)
+    on = y != -100
+    assert not loss[~on].any() and not lse[~on].any() and torch.isfinite(loss).all() and (loss[on] > 0).all()
+    for rows in torch.arange(1, t, 1999, device="cuda").split(512):
+        rows = rows[on[rows]]
+        l = x[rows].double() @ w.double().T
+        want = torch.logsumexp(l, 1)
+        assert (lse[rows].double() - want).abs().max() <= 1e-4
+        assert (loss[rows].double() - (want - l.gather(1, y[rows][:, None])[:, 0])).abs().max() <= 1e-4
+    del x, w, y, loss, lse, on
+    torch.cuda.empty_cache()

@@ -10,7 +10,7 @@
 // (A^T u) to its own registers. Tokens keep their order: a fragment of 16 tokens goes through the distinct
 // adapters among them, one in all but the fragments where requests meet, and a token takes only its own
 // adapter's result, so that what another adapter holds cannot reach it. low and u enter the matrix cores as
-// the sum of two 16-bit values of a vector scaled to [0.5, 1): about 16 bits of it are kept.
+// the sum of two 16-bit values of a vector scaled below 1 (by least_exp): about 16 bits of it are kept.
 //
 // 4096 tokens, 4096 -> 14336, 4 bits, rank 64, bf16: forward product 425-450 us (1.1 PF, 3.5 rounds of tiles), that
 // of the gradient 340-356 (1.4 PF, one round), both bound by power where all CUs work; 2000 tokens, 2048 -> 5632:
@@ -232,9 +232,15 @@ __device__ __forceinline__ int next_adapter(int q, uint64_t& left) {
 }
 
 // Ranks jt, jt + 32, ... of token ot, by 32 threads: out (t x rank) = low, or scaling low with `scaled`;
-// hl[t][2 rp]: scaling low / 2^e as two 16-bit values, hscale[t] = 2^e; e is not below kLeastExp, where
-// f16's smallest values times its largest weights lie under half of its smallest result.
-constexpr int kLeastExp = -24, kMostExp = 120;  // 2^120 and a value of up to 2^8 stay finite
+// hl[t][2 rp]: scaling low / 2^e as two 16-bit values, hscale[t] = 2^e. e has a floor, since k_wide divides its
+// sums by 2^e. f16: -24, where its smallest values times its largest weights lie under half of its smallest
+// result; a sum of f16 products is below 2^54 and stays finite. bf16: 0. Its sums reach f32's largest numbers, and
+// its range is f32's: smaller vectors need no scale.
+template <class T>
+constexpr int least_exp() {
+  return T::kind == Bf16::kind ? 0 : -24;
+}
+constexpr int kMostExp = 120;  // 2^120 and a value of up to 2^8 stay finite
 constexpr float kMostScale = 0x1p40f;  // up to here sums divided by 2^e keep what counts of them
 template <class T, int N>
 __device__ __forceinline__ void low_out(const float (&v)[N], int ot, int t, int rank, int rp, int adapters,
@@ -248,7 +254,7 @@ __device__ __forceinline__ void low_out(const float (&v)[N], int ot, int t, int 
 #pragma unroll
   for (int s = 16; s; s >>= 1) m = fmaxf(m, __shfl_xor(m, s));
   if (ot >= t) return;
-  const int e = m > 0.0f && m < __builtin_inff() ? min(max(kLeastExp, __builtin_amdgcn_frexp_expf(m)), kMostExp) : 0;
+  const int e = m > 0.0f && m < __builtin_inff() ? min(max(least_exp<T>(), __builtin_amdgcn_frexp_expf(m)), kMostExp) : 0;
   if (jt == 0 && hscale) hscale[ot] = ldexpf(1.0f, e);
 #pragma unroll
   for (int i = 0; i < N; ++i) {

@@ -11,8 +11,10 @@
 // vocabulary; the piece's logits are made again and turned into d (16 bits) in memory, then two
 // products give dx (f32 sums over the pieces) and the piece's rows of dw.
 //
-// d is held in the operands' 16-bit type because the matrix cores need both operands alike; it is scaled by
-// g_t / max |g| (and 2^15 in f16, whose range would lose small probabilities), both undone in f32.
+// d is held in the operands' 16-bit type because the matrix cores need both operands alike. bf16: scaled by
+// g_t / max |g|, undone in f32. f16, whose range is short: by g_t over its own power of two, times 2^15, so that a
+// token's small probabilities are kept however little it weighs beside the others. dx takes the power of two back
+// in f32; for dw it goes into x (k_loss_weigh), exactly but for what passes f16's smallest number there.
 //
 // The products bound it, and those by the card's power where they are large (matrix cores busy 65-70% at
 // 1.6-1.9 GHz; the library's product: 1.34-1.40 PF). d = 4096, vocabulary 128256, bf16: forward of 2048 tokens
@@ -32,17 +34,17 @@ namespace {
 constexpr float LOG2E = 1.4426950408889634f;
 
 // Compact list of the tokens that count, in order; zero loss and lse of the others. One workgroup.
-// info: [0] their number, [1] bits of max |g| over the finite g (backward only).
+// info: [0] their number, [1] bits of max |g| over the finite g, [2] of the least but zero (backward only).
 __global__ __launch_bounds__(1024) void k_loss_tokens(const int64_t* __restrict__ y, long ignore, int t,
                                                       const float* __restrict__ g, int* __restrict__ idx,
                                                       int* __restrict__ pos, uint32_t* __restrict__ info,
                                                       float* __restrict__ loss, float* __restrict__ lse) {
   __shared__ int base;
   __shared__ int wsum[16];
-  __shared__ float wmax[16];
+  __shared__ float wmax[16], wmin[16];
   const int lane = threadIdx.x & 63, wv = threadIdx.x >> 6;
   if (threadIdx.x == 0) base = 0;
-  float m = 0.0f;
+  float m = 0.0f, least = __builtin_inff();
   __syncthreads();
   for (int t0 = 0; t0 < t; t0 += 1024) {
     const int i = t0 + threadIdx.x;
@@ -61,6 +63,7 @@ __global__ __launch_bounds__(1024) void k_loss_tokens(const int64_t* __restrict_
       if (on && g) {
         const float a = __builtin_fabsf(g[i]);
         if (a < __builtin_inff()) m = fmaxf(m, a);
+        if (a > 0.0f) least = fminf(least, a);
       }
     }
     __syncthreads();
@@ -68,13 +71,14 @@ __global__ __launch_bounds__(1024) void k_loss_tokens(const int64_t* __restrict_
       for (int w = 0; w < 16; ++w) base += wsum[w];
     __syncthreads();
   }
-  for (int s = 32; s; s >>= 1) m = fmaxf(m, __shfl_xor(m, s));
-  if (lane == 0) wmax[wv] = m;
+  for (int s = 32; s; s >>= 1) m = fmaxf(m, __shfl_xor(m, s)), least = fminf(least, __shfl_xor(least, s));
+  if (lane == 0) wmax[wv] = m, wmin[wv] = least;
   __syncthreads();
   if (threadIdx.x == 0) {
-    for (int w = 0; w < 16; ++w) m = fmaxf(m, wmax[w]);
+    for (int w = 0; w < 16; ++w) m = fmaxf(m, wmax[w]), least = fminf(least, wmin[w]);
     info[0] = base;
     info[1] = __float_as_uint(m);
+    info[2] = __float_as_uint(least);
   }
 }
 
@@ -82,8 +86,15 @@ __global__ __launch_bounds__(1024) void k_loss_tokens(const int64_t* __restrict_
 struct LossTok {
   int target;  // -1: outside the vocabulary
   float lse, weight;
-  int pad;
+  int16_t shift;  // f16: exponent of its weight less that of the largest
+  uint16_t xmax;  // f16, where the shifts differ: pattern of its largest finite |x|
 };
+// Exponent of a weight (that of 2^(e - 1) <= |g| < 2^e), 0 of zero.
+__device__ __forceinline__ int weight_exp(float g) { return g > 0.0f ? __builtin_amdgcn_frexp_expf(g) : 0; }
+// f16: do the weights' powers of two differ (info as k_loss_tokens leaves it)
+__device__ __forceinline__ bool weights_differ(float top, float least) {
+  return least < top && weight_exp(least) != weight_exp(top);
+}
 struct GatherArgs {
   const uint16_t* x;
   long ldx;
@@ -91,15 +102,17 @@ struct GatherArgs {
   const int64_t* y;
   int v;
   const float *lse, *g;  // gradient
-  float gscale;
+  int half, weigh;       // gradient: in f16; and dw is asked for
   uint16_t* xc;
   LossTok* tok;
   float* hit;  // forward
 };
 // Token t as the i-th packed one: its row of x in dp elements, zeros past d, and its LossTok.
-__device__ __forceinline__ void gather_token(const GatherArgs& k, int t, int i, float top) {
+__device__ __forceinline__ void gather_token(const GatherArgs& k, int t, int i, float top, float least) {
   const uint16_t* src = k.x + (long)t * k.ldx;
   uint16_t* dst = k.xc + (long)i * k.dp;
+  uint32_t xmax = 0;
+  const bool find = k.weigh && weights_differ(top, least);
   for (int c = 8 * threadIdx.x; c < k.dp; c += 2048) {
     uint16_t v[8];
     if (c + 8 <= k.d) {
@@ -109,6 +122,20 @@ __device__ __forceinline__ void gather_token(const GatherArgs& k, int t, int i, 
       for (int j = 0; j < 8; ++j) v[j] = c + j < k.d ? src[c + j] : (uint16_t)0;
     }
     __builtin_memcpy(__builtin_assume_aligned(dst + c, 16), v, 16);
+    if (find)
+#pragma unroll
+      for (int j = 0; j < 8; ++j) {
+        const uint32_t a = v[j] & 0x7fffu;
+        if (a < 0x7c00u) xmax = max(xmax, a);
+      }
+  }
+  if (find) {
+    __shared__ uint32_t wx[4];
+#pragma unroll
+    for (int s = 32; s; s >>= 1) xmax = max(xmax, (uint32_t)__shfl_xor((int)xmax, s));
+    if ((threadIdx.x & 63) == 0) wx[threadIdx.x >> 6] = xmax;
+    __syncthreads();
+    xmax = max(max(wx[0], wx[1]), max(wx[2], wx[3]));
   }
   if (threadIdx.x == 0) {
     const int64_t y = k.y[t];
@@ -116,11 +143,18 @@ __device__ __forceinline__ void gather_token(const GatherArgs& k, int t, int i, 
     o.target = y >= 0 && y < k.v ? (int)y : -1;
     o.lse = k.lse ? k.lse[t] : 0.0f;
     o.weight = 0.0f;
+    o.shift = 0;
     if (k.g) {
-      o.weight = top > 0.0f ? k.g[t] / top * k.gscale : k.g[t];
+      const float g = k.g[t], a = __builtin_fabsf(g);
+      if (k.half) {
+        if (a > 0.0f && a < __builtin_inff()) o.shift = (int16_t)(weight_exp(a) - weight_exp(top));
+        o.weight = ldexpf(g, 15 - weight_exp(top) - o.shift);
+      } else {
+        o.weight = top > 0.0f ? g / top : g;
+      }
       if (o.target < 0) o.weight = __builtin_nanf("");
     }
-    o.pad = 0;
+    o.xmax = (uint16_t)xmax;
     k.tok[i] = o;
     if (k.hit) k.hit[i] = __builtin_nanf("");  // replaced by the tile that holds the target
   }
@@ -128,7 +162,7 @@ __device__ __forceinline__ void gather_token(const GatherArgs& k, int t, int i, 
 __global__ __launch_bounds__(256) void k_loss_gather(GatherArgs k, const int* __restrict__ idx,
                                                      const uint32_t* __restrict__ info) {
   const int i = blockIdx.x;
-  if (i < (int)info[0]) gather_token(k, idx[i], i, __uint_as_float(info[1]));
+  if (i < (int)info[0]) gather_token(k, idx[i], i, __uint_as_float(info[1]), __uint_as_float(info[2]));
 }
 // Both of the above in one launch for few tokens: every workgroup (one a token) counts for itself, t / 256
 // tokens a thread, which costs less than a launch up to kCountTokens (a forward call over 8000 x 1024: 256 tokens
@@ -138,10 +172,10 @@ __global__ __launch_bounds__(256) void k_loss_pack(GatherArgs k, long ignore, in
                                                    int* __restrict__ pos, uint32_t* __restrict__ info,
                                                    float* __restrict__ loss, float* __restrict__ lse) {
   __shared__ int wbefore[4], wall[4];
-  __shared__ float wtop[4];
+  __shared__ float wtop[4], wleast[4];
   const int i = blockIdx.x, lane = threadIdx.x & 63, wv = threadIdx.x >> 6;
   int before = 0, all = 0;
-  float top = 0.0f;
+  float top = 0.0f, least = __builtin_inff();
   for (int j = threadIdx.x; j < t; j += 256) {
     if (k.y[j] == ignore) continue;
     ++all;
@@ -149,6 +183,7 @@ __global__ __launch_bounds__(256) void k_loss_pack(GatherArgs k, long ignore, in
     if (k.g) {
       const float a = __builtin_fabsf(k.g[j]);
       if (a < __builtin_inff()) top = fmaxf(top, a);
+      if (a > 0.0f) least = fminf(least, a);
     }
   }
 #pragma unroll
@@ -156,15 +191,18 @@ __global__ __launch_bounds__(256) void k_loss_pack(GatherArgs k, long ignore, in
     before += __shfl_xor(before, s);
     all += __shfl_xor(all, s);
     top = fmaxf(top, __shfl_xor(top, s));
+    least = fminf(least, __shfl_xor(least, s));
   }
-  if (lane == 0) wbefore[wv] = before, wall[wv] = all, wtop[wv] = top;
+  if (lane == 0) wbefore[wv] = before, wall[wv] = all, wtop[wv] = top, wleast[wv] = least;
   __syncthreads();
   before = wbefore[0] + wbefore[1] + wbefore[2] + wbefore[3];
   all = wall[0] + wall[1] + wall[2] + wall[3];
   top = fmaxf(fmaxf(wtop[0], wtop[1]), fmaxf(wtop[2], wtop[3]));
+  least = fminf(fminf(wleast[0], wleast[1]), fminf(wleast[2], wleast[3]));
   if (i == 0 && threadIdx.x == 0) {
     info[0] = all;
     info[1] = __float_as_uint(top);
+    info[2] = __float_as_uint(least);
   }
   const bool on = k.y[i] != ignore;
   if (threadIdx.x == 0) {
@@ -173,7 +211,35 @@ __global__ __launch_bounds__(256) void k_loss_pack(GatherArgs k, long ignore, in
     if (!on && loss) loss[i] = 0.0f;
     if (!on && lse) lse[i] = 0.0f;
   }
-  if (on) gather_token(k, i, before, top);
+  if (on) gather_token(k, i, before, top, least);
+}
+
+// f16, weights of several powers of two: xg = x 2^(up + shift) for dw, 2^up what brings the largest |x| to f16's
+// upper end, so that a token's x keeps its bits until its weight is about 2^-20 of the largest. info[3] = up.
+__global__ __launch_bounds__(256) void k_loss_weigh(const uint16_t* __restrict__ xc, int dp,
+                                                    const LossTok* __restrict__ tok, uint32_t* __restrict__ info,
+                                                    uint16_t* __restrict__ xg) {
+  __shared__ uint32_t wx[4];
+  const int count = (int)info[0];
+  if (!weights_differ(__uint_as_float(info[1]), __uint_as_float(info[2]))) return;
+  uint32_t xmax = 0;
+  for (int i = threadIdx.x; i < count; i += 256) xmax = max(xmax, (uint32_t)tok[i].xmax);
+#pragma unroll
+  for (int s = 32; s; s >>= 1) xmax = max(xmax, (uint32_t)__shfl_xor((int)xmax, s));
+  if ((threadIdx.x & 63) == 0) wx[threadIdx.x >> 6] = xmax;
+  __syncthreads();
+  xmax = max(max(wx[0], wx[1]), max(wx[2], wx[3]));
+  const int raise = xmax ? 16 - __builtin_amdgcn_frexp_expf(F16::widen((uint16_t)xmax)) : 0;
+  if (blockIdx.x == 0 && threadIdx.x == 0) info[3] = (uint32_t)raise;
+  const long total = (long)count * (dp / 8);
+  for (long e = blockIdx.x * 256l + threadIdx.x; e < total; e += gridDim.x * 256l) {
+    const int by = raise + tok[e / (dp / 8)].shift;
+    uint16_t v[8];
+    *reinterpret_cast<uint4*>(v) = *reinterpret_cast<const uint4*>(xc + 8 * e);
+#pragma unroll
+    for (int j = 0; j < 8; ++j) v[j] = F16::narrow(ldexpf(F16::widen(v[j]), by));
+    *reinterpret_cast<uint4*>(xg + 8 * e) = *reinterpret_cast<const uint4*>(v);
+  }
 }
 
 __global__ __launch_bounds__(256) void k_pad16(PadJob j) { pad_rows16(j, blockIdx.x, gridDim.x); }
@@ -355,21 +421,29 @@ __global__ __launch_bounds__(64 * WP * WQ, 2) void k_loss_dx(const uint16_t* __r
   }
 }
 
-// dw[v0 + v][c] = top 2^-S sum_t d[t][v] xc[t][c]
+// dw[v0 + v][c] = sum_t d[t][v] xc[t][c], times what d was divided by; in f16 with weights of several powers of two
+// of xg (k_loss_weigh)
 template <class T, int FP, int FQ, int WP, int WQ>
 __global__ __launch_bounds__(64 * WP * WQ, 2) void k_loss_dw(const uint16_t* __restrict__ xc, int dp, int dcols,
                                                              const uint16_t* __restrict__ d, long ldd, int rows,
                                                              const uint32_t* __restrict__ info, int np, int nq,
-                                                             float gscale, uint16_t* __restrict__ dw, long lddw) {
+                                                             const uint16_t* __restrict__ xg,
+                                                             uint16_t* __restrict__ dw, long lddw) {
   typedef MmaTile<T, true, true, FP, FQ, WP, WQ> M;
   __shared__ __align__(1024) uint8_t lds[M::LDS];
   const MmaTileAt at = mma_tile_at(blockIdx.x, np, nq);
   const int p0 = at.p * M::BP, q0 = at.q * M::BQ, count = (int)info[0];
+  const float top = __uint_as_float(info[1]);
+  float k = top > 0.0f ? top : 1.0f;
+  if constexpr (T::kind == F16::kind) {
+    int e = weight_exp(top) - 15;
+    if (weights_differ(top, __uint_as_float(info[2]))) xc = xg, e -= (int)info[3];
+    k = ldexpf(1.0f, e);
+  }
   mma_f4 acc[FP][FQ];
   M::clear(acc);
   if (count > 0)
     M::run(lds_offset(lds), MmaOp{xc, dp, dp}, MmaOp{d, ldd, (int)ldd}, p0, q0, 0, count, acc);
-  const float top = __uint_as_float(info[1]), k = (top > 0.0f ? top : 1.0f) / gscale;
 #pragma unroll
   for (int f = 0; f < FP; ++f)
 #pragma unroll
@@ -377,19 +451,23 @@ __global__ __launch_bounds__(64 * WP * WQ, 2) void k_loss_dw(const uint16_t* __r
   M::store(lds_offset(lds), acc, p0, q0, dcols, rows, dw, lddw);
 }
 
-// dx[t] = top 2^-S sum over the splits of dxacc at the token's packed place; 0 where it does not count
+// dx[t] = sum over the splits of dxacc at the token's packed place, times what its d was divided by; 0 where it does
+// not count
 template <class T>
 __global__ __launch_bounds__(256) void k_loss_dx_out(const float* __restrict__ dxacc, int np, int bq, int piece, int round,
                                                      int t, int d, int dp,
                                                      const int* __restrict__ pos, const uint32_t* __restrict__ info,
-                                                     float gscale, uint16_t* __restrict__ dx, long lddx, int vec) {
-  const float top = __uint_as_float(info[1]), k = (top > 0.0f ? top : 1.0f) / gscale;
+                                                     const LossTok* __restrict__ tok, uint16_t* __restrict__ dx,
+                                                     long lddx, int vec) {
+  const float top = __uint_as_float(info[1]), all = top > 0.0f ? top : 1.0f;
   const DxSplit sp = dx_split((int)info[0], np, bq, piece, round);
   const long total = (long)t * dp / 4, apart = (long)sp.nq * bq * dp;
   for (long e = blockIdx.x * 256l + threadIdx.x; e < total; e += gridDim.x * 256l) {
     const int i = (int)(4 * e / dp), c = (int)(4 * e - (long)i * dp), at = pos[i];
     mma_f4 s = {};
+    float k = all;
     if (at >= 0) {
+      if constexpr (T::kind == F16::kind) k = ldexpf(1.0f, weight_exp(top) + tok[at].shift - 15);
       const float* a = dxacc + (long)at * dp + c;
 #pragma unroll 8
       for (int j = 0; j < sp.splits; ++j) s += *reinterpret_cast<const mma_f4*>(a + j * apart);
@@ -490,6 +568,7 @@ LossPlan loss_plan(long t, long d, long v, bool pad_w, bool grad) {
     // few tokens: dw's stores are what costs, and two small tiles on a CU overlap theirs with each other's loads
     // (62 tokens, 50001 x 1000: 36 us, large tiles 42; 64, 128256 x 4096: 363 and 370; 300: 664 and 580)
     p.dw_tiles = t <= 192 || mma_cost(p.dp, p.piece, t, 4, 1, false) < mma_cost(p.dp, p.piece, t, 0, 1, false) ? 4 : 0;
+    p.xg = take(2 * (size_t)t * p.dp);  // f16 alone writes it
     p.d = take(2 * (size_t)t * p.piece);
     p.dxacc = take(p.dx_bytes);
   }
@@ -500,14 +579,14 @@ LossPlan loss_plan(long t, long d, long v, bool pad_w, bool grad) {
 namespace {
 
 // The packed tokens, and W where the tiles cannot read it as it is
-hipError_t prepare(hipStream_t st, const LossArgs& a, const LossPlan& p, float gscale, const uint16_t** w, long* ldw) {
+hipError_t prepare(hipStream_t st, const LossArgs& a, const LossPlan& p, bool half, const uint16_t** w, long* ldw) {
   char* ws = static_cast<char*>(a.work);
   const bool grad = a.dx || a.dw;
   int *idx = reinterpret_cast<int*>(ws + p.idx), *pos = grad ? reinterpret_cast<int*>(ws + p.pos) : nullptr;
   uint32_t* info = reinterpret_cast<uint32_t*>(ws + p.info);
   float *loss = grad ? nullptr : a.loss, *lse = grad ? nullptr : a.lse_out;
-  const GatherArgs k = {a.x, a.ldx, (int)a.d, p.dp, a.targets, (int)a.v, a.lse_in, a.dloss, gscale,
-                        reinterpret_cast<uint16_t*>(ws + p.xc), reinterpret_cast<LossTok*>(ws + p.tok),
+  const GatherArgs k = {a.x, a.ldx, (int)a.d, p.dp, a.targets, (int)a.v, a.lse_in, a.dloss,
+                        grad && half, grad && half && a.dw, reinterpret_cast<uint16_t*>(ws + p.xc), reinterpret_cast<LossTok*>(ws + p.tok),
                         grad ? nullptr : reinterpret_cast<float*>(ws + p.hit)};
   if (a.t > 0 && a.t <= kCountTokens) {
     k_loss_pack<<<(int)a.t, 256, 0, st>>>(k, a.ignore, (int)a.t, idx, pos, info, loss, lse);
@@ -532,7 +611,7 @@ hipError_t forward(hipStream_t st, const LossArgs& a, const LossPlan& p) {
   char* ws = static_cast<char*>(a.work);
   const uint16_t* w;
   long ldw;
-  hipError_t e = prepare(st, a, p, 1.0f, &w, &ldw);
+  hipError_t e = prepare(st, a, p, false, &w, &ldw);
   if (e != hipSuccess) return e;
   e = with_loss_shape(p.tiles, p.direct, [&](auto s, auto u) {
     typedef decltype(s) S;
@@ -553,17 +632,23 @@ hipError_t forward(hipStream_t st, const LossArgs& a, const LossPlan& p) {
 template <class T>
 hipError_t backward(hipStream_t st, const LossArgs& a, const LossPlan& p) {
   char* ws = static_cast<char*>(a.work);
-  const float gscale = T::kind == F16::kind ? 32768.0f : 1.0f;
+  constexpr bool half = T::kind == F16::kind;
   const uint16_t* w;
   long ldw;
-  hipError_t e = prepare(st, a, p, gscale, &w, &ldw);
+  hipError_t e = prepare(st, a, p, half, &w, &ldw);
   if (e != hipSuccess) return e;
   uint32_t* info = reinterpret_cast<uint32_t*>(ws + p.info);
   uint16_t* xc = reinterpret_cast<uint16_t*>(ws + p.xc);
   uint16_t* d = reinterpret_cast<uint16_t*>(ws + p.d);
   float* dxacc = reinterpret_cast<float*>(ws + p.dxacc);
   LossTok* tok = reinterpret_cast<LossTok*>(ws + p.tok);
+  uint16_t* xg = reinterpret_cast<uint16_t*>(ws + p.xg);
   const int t = (int)a.t, v = (int)a.v;
+  if (half && a.dw && t) {
+    k_loss_weigh<<<blocks_for((long)t * (p.dp / 8), 256 * 4, 512), 256, 0, st>>>(xc, p.dp, tok, info, xg);
+    e = hipGetLastError();
+    if (e != hipSuccess) return e;
+  }
   for (int i = 0; i < p.pieces; ++i) {
     const int v0 = i * p.piece;
     if (v0 >= v) break;
@@ -591,7 +676,7 @@ hipError_t backward(hipStream_t st, const LossArgs& a, const LossPlan& p) {
         typedef decltype(s) S;
         const int np = (p.dp + S::bp - 1) / S::bp, nq = (rows + S::bq - 1) / S::bq;
         k_loss_dw<T, S::fp, S::fq, S::wp, S::wq><<<np * nq, S::threads, 0, st>>>(
-            xc, p.dp, (int)a.d, d, p.piece, rows, info, np, nq, gscale, a.dw + (long)v0 * a.lddw, a.lddw);
+            xc, p.dp, (int)a.d, d, p.piece, rows, info, np, nq, xg, a.dw + (long)v0 * a.lddw, a.lddw);
         return hipGetLastError();
       };
       e = p.dw_tiles == 4 ? go(MmaShape<4, 4, 2, 2>{}) : go(MmaShape<8, 4, 2, 4>{});
@@ -603,7 +688,7 @@ hipError_t backward(hipStream_t st, const LossArgs& a, const LossPlan& p) {
     const MmaShapeTime s = kMmaTimes[p.dx_tiles];
     k_loss_dx_out<T><<<blocks_for((long)t * p.dp, 4 * 256), 256, 0, st>>>(
         dxacc, (p.dp + s.bp - 1) / s.bp, s.bq, p.piece, p.dx_round, t, (int)a.d, p.dp, reinterpret_cast<int*>(ws + p.pos),
-        info, gscale, a.dx, a.lddx, vec);
+        info, tok, a.dx, a.lddx, vec);
   }
   return hipGetLastError();
 }

@@ -294,7 +294,7 @@ struct LossArgs {
   void* work;
 };
 struct LossPlan {
-  size_t bytes, info, idx, pos, tok, xc, wpad, hit, part, d, dxacc;  // offsets into the workspace
+  size_t bytes, info, idx, pos, tok, xc, xg, wpad, hit, part, d, dxacc;  // offsets into the workspace
   size_t dx_bytes;
   int dp, slab, nslabs, pieces, piece, dx_round;
   int tiles, dx_tiles, dw_tiles;  // tile shapes (mma16.h)

@@ -12,9 +12,10 @@
 // products give dx (f32 sums over the pieces) and the piece's rows of dw.
 //
 // d is held in the operands' 16-bit type because the matrix cores need both operands alike. bf16: scaled by
-// g_t / max |g|, undone in f32. f16, whose range is short: by g_t over its own power of two, times 2^15, so that a
-// token's small probabilities are kept however little it weighs beside the others. dx takes the power of two back
-// in f32; for dw it goes into x (k_loss_weigh), exactly but for what passes f16's smallest number there.
+// g_t / max |g|, the largest undone in f32. f16, whose range is short: times 2^15, and where all tokens weigh the same
+// without g, which dx and dw take in f32. Where they differ by g_t over its own power of two, so that a token's small
+// probabilities are kept however little it weighs beside the others; dx takes the power of two in f32, and dw reads
+// x with it (k_loss_weigh), exactly but for what passes f16's smallest number there.
 //
 // The products bound it, and those by the card's power where they are large (matrix cores busy 65-70% at
 // 1.6-1.9 GHz; the library's product: 1.34-1.40 PF). d = 4096, vocabulary 128256, bf16: forward of 2048 tokens
@@ -34,17 +35,20 @@ namespace {
 constexpr float LOG2E = 1.4426950408889634f;
 
 // Compact list of the tokens that count, in order; zero loss and lse of the others. One workgroup.
-// info: [0] their number, [1] bits of max |g| over the finite g, [2] of the least but zero (backward only).
+// info: [0] their number; backward only: [1] bits of max |g| over the finite g, [2] whether the g differ, [3] the
+// bits of one of them.
 __global__ __launch_bounds__(1024) void k_loss_tokens(const int64_t* __restrict__ y, long ignore, int t,
                                                       const float* __restrict__ g, int* __restrict__ idx,
                                                       int* __restrict__ pos, uint32_t* __restrict__ info,
                                                       float* __restrict__ loss, float* __restrict__ lse) {
   __shared__ int base;
   __shared__ int wsum[16];
-  __shared__ float wmax[16], wmin[16];
+  __shared__ float wmax[16];
+  __shared__ uint32_t wlow[16], whigh[16];
   const int lane = threadIdx.x & 63, wv = threadIdx.x >> 6;
   if (threadIdx.x == 0) base = 0;
-  float m = 0.0f, least = __builtin_inff();
+  float m = 0.0f;
+  uint32_t low = ~0u, high = 0;
   __syncthreads();
   for (int t0 = 0; t0 < t; t0 += 1024) {
     const int i = t0 + threadIdx.x;
@@ -63,7 +67,7 @@ __global__ __launch_bounds__(1024) void k_loss_tokens(const int64_t* __restrict_
       if (on && g) {
         const float a = __builtin_fabsf(g[i]);
         if (a < __builtin_inff()) m = fmaxf(m, a);
-        if (a > 0.0f) least = fminf(least, a);
+        low = min(low, __float_as_uint(g[i])), high = max(high, __float_as_uint(g[i]));
       }
     }
     __syncthreads();
@@ -71,14 +75,19 @@ __global__ __launch_bounds__(1024) void k_loss_tokens(const int64_t* __restrict_
       for (int w = 0; w < 16; ++w) base += wsum[w];
     __syncthreads();
   }
-  for (int s = 32; s; s >>= 1) m = fmaxf(m, __shfl_xor(m, s)), least = fminf(least, __shfl_xor(least, s));
-  if (lane == 0) wmax[wv] = m, wmin[wv] = least;
+  for (int s = 32; s; s >>= 1) {
+    m = fmaxf(m, __shfl_xor(m, s));
+    low = min(low, (uint32_t)__shfl_xor((int)low, s));
+    high = max(high, (uint32_t)__shfl_xor((int)high, s));
+  }
+  if (lane == 0) wmax[wv] = m, wlow[wv] = low, whigh[wv] = high;
   __syncthreads();
   if (threadIdx.x == 0) {
-    for (int w = 0; w < 16; ++w) m = fmaxf(m, wmax[w]), least = fminf(least, wmin[w]);
+    for (int w = 0; w < 16; ++w) m = fmaxf(m, wmax[w]), low = min(low, wlow[w]), high = max(high, whigh[w]);
     info[0] = base;
     info[1] = __float_as_uint(m);
-    info[2] = __float_as_uint(least);
+    info[2] = low < high;
+    info[3] = high;
   }
 }
 
@@ -86,14 +95,13 @@ __global__ __launch_bounds__(1024) void k_loss_tokens(const int64_t* __restrict_
 struct LossTok {
   int target;  // -1: outside the vocabulary
   float lse, weight;
-  int16_t shift;  // f16: exponent of its weight less that of the largest
-  uint16_t xmax;  // f16, where the shifts differ: pattern of its largest finite |x|
+  uint32_t xmax;  // f16, where the weights differ: pattern of its largest finite |x|
 };
-// Exponent of a weight (that of 2^(e - 1) <= |g| < 2^e), 0 of zero.
-__device__ __forceinline__ int weight_exp(float g) { return g > 0.0f ? __builtin_amdgcn_frexp_expf(g) : 0; }
-// f16: do the weights' powers of two differ (info as k_loss_tokens leaves it)
-__device__ __forceinline__ bool weights_differ(float top, float least) {
-  return least < top && weight_exp(least) != weight_exp(top);
+// f16, weights that differ: the power of two that d leaves out of g, 2^(e - 1) <= |g| < 2^e; that of the largest for
+// 0, infinities and NaN
+__device__ __forceinline__ int weight_exp(float g, float top) {
+  const float a = __builtin_fabsf(g), b = a > 0.0f && a < __builtin_inff() ? a : top;
+  return b > 0.0f ? __builtin_amdgcn_frexp_expf(b) : 0;
 }
 struct GatherArgs {
   const uint16_t* x;
@@ -108,11 +116,11 @@ struct GatherArgs {
   float* hit;  // forward
 };
 // Token t as the i-th packed one: its row of x in dp elements, zeros past d, and its LossTok.
-__device__ __forceinline__ void gather_token(const GatherArgs& k, int t, int i, float top, float least) {
+__device__ __forceinline__ void gather_token(const GatherArgs& k, int t, int i, float top, bool differ) {
   const uint16_t* src = k.x + (long)t * k.ldx;
   uint16_t* dst = k.xc + (long)i * k.dp;
   uint32_t xmax = 0;
-  const bool find = k.weigh && weights_differ(top, least);
+  const bool find = k.weigh && differ;
   for (int c = 8 * threadIdx.x; c < k.dp; c += 2048) {
     uint16_t v[8];
     if (c + 8 <= k.d) {
@@ -143,18 +151,13 @@ __device__ __forceinline__ void gather_token(const GatherArgs& k, int t, int i, 
     o.target = y >= 0 && y < k.v ? (int)y : -1;
     o.lse = k.lse ? k.lse[t] : 0.0f;
     o.weight = 0.0f;
-    o.shift = 0;
     if (k.g) {
-      const float g = k.g[t], a = __builtin_fabsf(g);
-      if (k.half) {
-        if (a > 0.0f && a < __builtin_inff()) o.shift = (int16_t)(weight_exp(a) - weight_exp(top));
-        o.weight = ldexpf(g, 15 - weight_exp(top) - o.shift);
-      } else {
-        o.weight = top > 0.0f ? g / top : g;
-      }
+      const float g = k.g[t];
+      if (k.half) o.weight = differ ? ldexpf(g, 15 - weight_exp(g, top)) : 0x1p15f;
+      else o.weight = top > 0.0f ? g / top : g;
       if (o.target < 0) o.weight = __builtin_nanf("");
     }
-    o.xmax = (uint16_t)xmax;
+    o.xmax = xmax;
     k.tok[i] = o;
     if (k.hit) k.hit[i] = __builtin_nanf("");  // replaced by the tile that holds the target
   }
@@ -162,7 +165,7 @@ __device__ __forceinline__ void gather_token(const GatherArgs& k, int t, int i, 
 __global__ __launch_bounds__(256) void k_loss_gather(GatherArgs k, const int* __restrict__ idx,
                                                      const uint32_t* __restrict__ info) {
   const int i = blockIdx.x;
-  if (i < (int)info[0]) gather_token(k, idx[i], i, __uint_as_float(info[1]), __uint_as_float(info[2]));
+  if (i < (int)info[0]) gather_token(k, idx[i], i, __uint_as_float(info[1]), info[2] != 0);
 }
 // Both of the above in one launch for few tokens: every workgroup (one a token) counts for itself, t / 256
 // tokens a thread, which costs less than a launch up to kCountTokens (a forward call over 8000 x 1024: 256 tokens
@@ -172,10 +175,12 @@ __global__ __launch_bounds__(256) void k_loss_pack(GatherArgs k, long ignore, in
                                                    int* __restrict__ pos, uint32_t* __restrict__ info,
                                                    float* __restrict__ loss, float* __restrict__ lse) {
   __shared__ int wbefore[4], wall[4];
-  __shared__ float wtop[4], wleast[4];
+  __shared__ float wtop[4];
+  __shared__ uint32_t wlow[4], whigh[4];
   const int i = blockIdx.x, lane = threadIdx.x & 63, wv = threadIdx.x >> 6;
   int before = 0, all = 0;
-  float top = 0.0f, least = __builtin_inff();
+  float top = 0.0f;
+  uint32_t low = ~0u, high = 0;
   for (int j = threadIdx.x; j < t; j += 256) {
     if (k.y[j] == ignore) continue;
     ++all;
@@ -183,7 +188,7 @@ __global__ __launch_bounds__(256) void k_loss_pack(GatherArgs k, long ignore, in
     if (k.g) {
       const float a = __builtin_fabsf(k.g[j]);
       if (a < __builtin_inff()) top = fmaxf(top, a);
-      if (a > 0.0f) least = fminf(least, a);
+      low = min(low, __float_as_uint(k.g[j])), high = max(high, __float_as_uint(k.g[j]));
     }
   }
 #pragma unroll
@@ -191,18 +196,21 @@ __global__ __launch_bounds__(256) void k_loss_pack(GatherArgs k, long ignore, in
     before += __shfl_xor(before, s);
     all += __shfl_xor(all, s);
     top = fmaxf(top, __shfl_xor(top, s));
-    least = fminf(least, __shfl_xor(least, s));
+    low = min(low, (uint32_t)__shfl_xor((int)low, s));
+    high = max(high, (uint32_t)__shfl_xor((int)high, s));
   }
-  if (lane == 0) wbefore[wv] = before, wall[wv] = all, wtop[wv] = top, wleast[wv] = least;
+  if (lane == 0) wbefore[wv] = before, wall[wv] = all, wtop[wv] = top, wlow[wv] = low, whigh[wv] = high;
   __syncthreads();
   before = wbefore[0] + wbefore[1] + wbefore[2] + wbefore[3];
   all = wall[0] + wall[1] + wall[2] + wall[3];
   top = fmaxf(fmaxf(wtop[0], wtop[1]), fmaxf(wtop[2], wtop[3]));
-  least = fminf(fminf(wleast[0], wleast[1]), fminf(wleast[2], wleast[3]));
+  low = min(min(wlow[0], wlow[1]), min(wlow[2], wlow[3]));
+  high = max(max(whigh[0], whigh[1]), max(whigh[2], whigh[3]));
   if (i == 0 && threadIdx.x == 0) {
     info[0] = all;
     info[1] = __float_as_uint(top);
-    info[2] = __float_as_uint(least);
+    info[2] = low < high;
+    info[3] = high;
   }
   const bool on = k.y[i] != ignore;
   if (threadIdx.x == 0) {
@@ -211,19 +219,21 @@ __global__ __launch_bounds__(256) void k_loss_pack(GatherArgs k, long ignore, in
     if (!on && loss) loss[i] = 0.0f;
     if (!on && lse) lse[i] = 0.0f;
   }
-  if (on) gather_token(k, i, before, top, least);
+  if (on) gather_token(k, i, before, top, low < high);
 }
 
-// f16, weights of several powers of two: xg = x 2^(up + shift) for dw, 2^up what brings the largest |x| to f16's
-// upper end, so that a token's x keeps its bits until its weight is about 2^-20 of the largest. info[3] = up.
+// f16, weights that differ: xg = x 2^(up + e - E) for dw, e and E the exponents of the token's and the largest weight
+// and 2^up what brings the largest |x| to f16's upper end: x keeps its bits down to weights of about 2^-20 of the
+// largest. info[3] = up.
 __global__ __launch_bounds__(256) void k_loss_weigh(const uint16_t* __restrict__ xc, int dp,
-                                                    const LossTok* __restrict__ tok, uint32_t* __restrict__ info,
+                                                    const LossTok* __restrict__ tok, const int* __restrict__ idx,
+                                                    const float* __restrict__ g, uint32_t* __restrict__ info,
                                                     uint16_t* __restrict__ xg) {
   __shared__ uint32_t wx[4];
   const int count = (int)info[0];
-  if (!weights_differ(__uint_as_float(info[1]), __uint_as_float(info[2]))) return;
+  if (!info[2]) return;
   uint32_t xmax = 0;
-  for (int i = threadIdx.x; i < count; i += 256) xmax = max(xmax, (uint32_t)tok[i].xmax);
+  for (int i = threadIdx.x; i < count; i += 256) xmax = max(xmax, tok[i].xmax);
 #pragma unroll
   for (int s = 32; s; s >>= 1) xmax = max(xmax, (uint32_t)__shfl_xor((int)xmax, s));
   if ((threadIdx.x & 63) == 0) wx[threadIdx.x >> 6] = xmax;
@@ -231,9 +241,10 @@ __global__ __launch_bounds__(256) void k_loss_weigh(const uint16_t* __restrict__
   xmax = max(max(wx[0], wx[1]), max(wx[2], wx[3]));
   const int raise = xmax ? 16 - __builtin_amdgcn_frexp_expf(F16::widen((uint16_t)xmax)) : 0;
   if (blockIdx.x == 0 && threadIdx.x == 0) info[3] = (uint32_t)raise;
+  const float top = __uint_as_float(info[1]);
   const long total = (long)count * (dp / 8);
   for (long e = blockIdx.x * 256l + threadIdx.x; e < total; e += gridDim.x * 256l) {
-    const int by = raise + tok[e / (dp / 8)].shift;
+    const int by = raise + weight_exp(g[idx[e / (dp / 8)]], top) - weight_exp(top, top);
     uint16_t v[8];
     *reinterpret_cast<uint4*>(v) = *reinterpret_cast<const uint4*>(xc + 8 * e);
 #pragma unroll
@@ -421,8 +432,8 @@ __global__ __launch_bounds__(64 * WP * WQ, 2) void k_loss_dx(const uint16_t* __r
   }
 }
 
-// dw[v0 + v][c] = sum_t d[t][v] xc[t][c], times what d was divided by; in f16 with weights of several powers of two
-// of xg (k_loss_weigh)
+// dw[v0 + v][c] = sum_t d[t][v] xc[t][c], times what d and x were divided by; in f16 with weights that differ of xg
+// (k_loss_weigh)
 template <class T, int FP, int FQ, int WP, int WQ>
 __global__ __launch_bounds__(64 * WP * WQ, 2) void k_loss_dw(const uint16_t* __restrict__ xc, int dp, int dcols,
                                                              const uint16_t* __restrict__ d, long ldd, int rows,
@@ -436,9 +447,8 @@ __global__ __launch_bounds__(64 * WP * WQ, 2) void k_loss_dw(const uint16_t* __r
   const float top = __uint_as_float(info[1]);
   float k = top > 0.0f ? top : 1.0f;
   if constexpr (T::kind == F16::kind) {
-    int e = weight_exp(top) - 15;
-    if (weights_differ(top, __uint_as_float(info[2]))) xc = xg, e -= (int)info[3];
-    k = ldexpf(1.0f, e);
+    if (info[2]) xc = xg, k = ldexpf(1.0f, weight_exp(top, top) - 15 - (int)info[3]);
+    else k = __uint_as_float(info[3]) * 0x1p-15f;
   }
   mma_f4 acc[FP][FQ];
   M::clear(acc);
@@ -457,7 +467,7 @@ template <class T>
 __global__ __launch_bounds__(256) void k_loss_dx_out(const float* __restrict__ dxacc, int np, int bq, int piece, int round,
                                                      int t, int d, int dp,
                                                      const int* __restrict__ pos, const uint32_t* __restrict__ info,
-                                                     const LossTok* __restrict__ tok, uint16_t* __restrict__ dx,
+                                                     const float* __restrict__ g, uint16_t* __restrict__ dx,
                                                      long lddx, int vec) {
   const float top = __uint_as_float(info[1]), all = top > 0.0f ? top : 1.0f;
   const DxSplit sp = dx_split((int)info[0], np, bq, piece, round);
@@ -467,7 +477,7 @@ __global__ __launch_bounds__(256) void k_loss_dx_out(const float* __restrict__ d
     mma_f4 s = {};
     float k = all;
     if (at >= 0) {
-      if constexpr (T::kind == F16::kind) k = ldexpf(1.0f, weight_exp(top) + tok[at].shift - 15);
+      if constexpr (T::kind == F16::kind) k = info[2] ? ldexpf(1.0f, weight_exp(g[i], top) - 15) : g[i] * 0x1p-15f;
       const float* a = dxacc + (long)at * dp + c;
 #pragma unroll 8
       for (int j = 0; j < sp.splits; ++j) s += *reinterpret_cast<const mma_f4*>(a + j * apart);
@@ -645,7 +655,7 @@ hipError_t backward(hipStream_t st, const LossArgs& a, const LossPlan& p) {
   uint16_t* xg = reinterpret_cast<uint16_t*>(ws + p.xg);
   const int t = (int)a.t, v = (int)a.v;
   if (half && a.dw && t) {
-    k_loss_weigh<<<blocks_for((long)t * (p.dp / 8), 256 * 4, 512), 256, 0, st>>>(xc, p.dp, tok, info, xg);
+    k_loss_weigh<<<blocks_for((long)t * (p.dp / 8), 256 * 4, 512), 256, 0, st>>>(xc, p.dp, tok, reinterpret_cast<int*>(ws + p.idx), a.dloss, info, xg);
     e = hipGetLastError();
     if (e != hipSuccess) return e;
   }
@@ -688,7 +698,7 @@ hipError_t backward(hipStream_t st, const LossArgs& a, const LossPlan& p) {
     const MmaShapeTime s = kMmaTimes[p.dx_tiles];
     k_loss_dx_out<T><<<blocks_for((long)t * p.dp, 4 * 256), 256, 0, st>>>(
         dxacc, (p.dp + s.bp - 1) / s.bp, s.bq, p.piece, p.dx_round, t, (int)a.d, p.dp, reinterpret_cast<int*>(ws + p.pos),
-        info, tok, a.dx, a.lddx, vec);
+        info, a.dloss, a.dx, a.lddx, vec);
   }
   return hipGetLastError();
 }

@@ -219,7 +219,11 @@ def adapter_linear(packed: PackedLinear, x: torch.Tensor, adapters: Adapters | N
     """y (T x d_out) = x W^T with each token's adapter beside it: y_t = W x_t + scaling[q] B_q (A_q x_t),
     q = request[t] (int32, -1: none). With return_low also low = A_q x_t (T x rank, float32), which the
     backward pass takes. The requests may come in any order; calls of more than 192 tokens and the backward
-    pass are faster when the tokens of an adapter stand together."""
+    pass are faster when the tokens of an adapter stand together.
+
+    Up to 192 tokens the weights are exact; in larger calls, and in every backward pass, each weight is rounded
+    to x's type (so a token's bits differ between the two; split a call where that matters). The time and the
+    workspace of such calls go by all adapters of the set, with or without tokens."""
     ctx = packed.ctx
     code, ld = _code(x, "x"), _matrix(ctx, x, "x", None, None, packed.d_in)
     t = x.shape[0]

@@ -471,7 +471,7 @@ struct WideArgs {
   const int* request;
   uint16_t* out;  // t x rows
   long ldo;
-  int splits, share;  // of k; the low-rank term goes with the first
+  int share;  // of k, a split's; the low-rank term goes with the first
   float* parts;       // [split][t][rows rounded up to 4] instead of out, or null
 };
 
@@ -617,7 +617,8 @@ __global__ __launch_bounds__(64 * WP * WQ, 2) void k_wide(WideArgs a) {
 // A lane reads 8 neighbouring columns of 8 tokens, the next ones while these are multiplied: row i of the
 // f-th MFMA operand is column 8 i + f. The item's l lies in LDS, its token list beside it; it enters the
 // matrix cores as the sum of two 16-bit values, in f16 divided by 2^e to keep it in range (e grows with the
-// largest l so far, the sums go along).
+// largest l so far, the sums go along): 2^-15 of an element is lost at most down to 2^-10 of the item's largest,
+// below that 2^-25 of the largest.
 struct OuterJob {
   const void* x;
   const float* xscale;
@@ -1111,7 +1112,6 @@ WidePlan wide_plan(long rows, long t, long k, bool strided, bool parts_anyway) {
 
 template <class T, bool PS>
 hipError_t wide_product(hipStream_t st, const WidePlan& p, WideArgs w) {
-  w.splits = p.splits;
   w.share = p.share;
   return with_mma_shape(p.pick, [&](auto s) {
     typedef decltype(s) S;

@@ -8,8 +8,9 @@
 //
 // Both directions are one pass over memory, which bounds them: 16 lanes take a block, 16 bytes of x and 8 of
 // codes each, so that a wavefront's loads are whole lines and the maximum takes four lane exchanges.
-// 16384 x 14336 bf16: saved in 145 us (4.9 TB/s; with a division for each code 184), restored in 109 (6.5 TB/s, the
-// codes partly from the last cache), one after the other in 260 (5.5 TB/s); 512 x 4096: 4.3 and 3.3 us.
+// 16384 x 14336 bf16: saved in 185 us on average, 147 at least (4.8 TB/s; with a division for each code 230 and 184),
+// restored in 117 and 109 (6.5 TB/s, the codes partly from the last cache), one after the other in 262 (5.4 TB/s);
+// 512 x 4096: 4.1 and 3.2 us.
 #include <hip/hip_runtime.h>
 
 #include <algorithm>

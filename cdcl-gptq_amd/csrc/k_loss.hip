@@ -19,8 +19,8 @@
 //
 // The products bound it, and those by the card's power where they are large (matrix cores busy 65-70% at
 // 1.6-1.9 GHz; the library's product: 1.34-1.40 PF). d = 4096, vocabulary 128256, bf16: forward of 2048 tokens
-// 1.66 ms (1.30 PF); gradient of 4096 tokens, a tenth ignored, in four pieces: d 829 us, dx 722, dw 748 each (1.17,
-// 1.36, 1.31 PF of the tiles' work), joining dx 30 us.
+// 1.69 ms (1.27 PF); gradient of 4096 tokens, a tenth ignored, in four pieces: d 842 us, dx 747, dw 759 each (1.15,
+// 1.31, 1.29 PF of the tiles' work), joining dx 28 us.
 #include <hip/hip_runtime.h>
 
 #include <algorithm>
@@ -554,7 +554,8 @@ LossPlan loss_plan(long t, long d, long v, bool pad_w, bool grad) {
     p.part = take(sizeof(float2) * (size_t)t * p.nslabs);
   } else {
     // pieces of the vocabulary: d of a piece takes at most 256 MB (about what the last-level cache
-    // keeps) and the whole vocabulary where that is less
+    // keeps) and the whole vocabulary where that is less; beyond 2^19 tokens a piece of the least size, 256
+    // entries, takes more (2 GB at 2^22)
     const size_t rows = up(v, 256), most = std::max<size_t>(256, ((size_t)128 << 20) / t / 256 * 256);
     p.pieces = (int)((rows + most - 1) / most);
     p.piece = (int)up((rows + p.pieces - 1) / p.pieces, 256);

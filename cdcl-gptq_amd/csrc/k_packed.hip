@@ -8,9 +8,10 @@
 // 16x16x32 MFMAs). Per group run: sum of (2^b + q) x on the matrix cores, exact operands, f32 sums; then
 // scale (that - (2^b + zero) sum x) in f32, so that no weight is ever rounded. The wavefronts' sums
 // meet in LDS, where the low-rank term is added in f32. What bounds it is the read of the codes, for few rows
-// the latency of the first of them: 32 tokens of 32 adapters of rank 16, 4096 -> 14336 in 4 bits: 16.3 us
-// (46 MB, 2.8 TB/s); one token, 4096 -> 4096: 5.2 us; 128 tokens, 4096 -> 14336: 55 us, by then the matrix cores
-// and the decoding. k_few_inputs before it takes 4-6 us, of which the launch and the loads' latency are most.
+// the latency of the first of them: 32 tokens of 32 adapters of rank 16, 4096 -> 14336 in 4 bits: 15.8 us
+// (46 MB, 2.9 TB/s); one token, 4096 -> 4096: 5.2 us. Every 64 tokens decode the codes again, and the matrix cores
+// and the decoding bound it then: 64 tokens, 4096 -> 14336: 33 us a call, 128: 58, 192: 84. k_few_inputs before it
+// takes 4-6 us, of which the launch and the loads' latency are most.
 #include <hip/hip_runtime.h>
 
 #include <algorithm>
@@ -369,7 +370,8 @@ __global__ __launch_bounds__(64 * W) void k_packed_few(PackedView v, FewArgs k) 
 template <class T, int B, int NT>
 hipError_t few_tiles(hipStream_t st, const PackedView& v, const FewArgs& k) {
   // Two row tiles share the activations' operands where that leaves two workgroups a CU (14336 rows of
-  // 4096, 32 tokens: 25 us with two, 30 with one, 26 with four); few rows take 16 wavefronts each.
+  // 4096, 32 tokens: 16 us with two, 21 with one); few rows take 16 wavefronts each (4096 rows of 4096, a
+  // token: 5.3 us, 6.0 with eight; 1001 of 1350: 4.6 and 5.0).
   const int groups = (k.t + 16 * NT - 1) / (16 * NT);
   if (v.tiles >= 512) k_packed_few<T, B, 2, NT, 8><<<dim3((v.tiles + 1) / 2, groups), 512, 0, st>>>(v, k);
   else if (v.tiles <= 256) k_packed_few<T, B, 1, NT, 16><<<dim3(v.tiles, groups), 1024, 0, st>>>(v, k);

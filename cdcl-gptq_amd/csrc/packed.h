@@ -124,7 +124,9 @@ __device__ __forceinline__ float packed_scale(uint32_t sz) {
 __device__ __forceinline__ float packed_zero(uint32_t sz) { return (float)(sz >> 16); }
 
 // W in 16 bits, [tiles * 16][slots]: scale (code - zero), exact in f32, rounded once (the matrix cores
-// take both operands in the activations' type). By workgroups of 256 threads, b of nb.
+// take both operands in the activations' type; two 16-bit values for each weight would be exact and take twice the
+// products). The error of a product over it grows from the output's own rounding to about 1.3 times that (2000
+// tokens, 2048 -> 5632, bf16: 0.0022 of its size against 0.0017). By workgroups of 256 threads, b of nb.
 template <class T, int U>
 __device__ __forceinline__ void packed_expand_by(const PackedView& v, uint16_t* w16, long b, long nb) {
   const int lane = threadIdx.x & 63, q = lane >> 4, ns = packed_slots(v);

@@ -368,7 +368,8 @@ size_t cdclq_packed_bytes(const cdclq_packed* packed);
  * smaller rank are padded with zeros. low (t x rank f32, may be NULL) receives A_q x_t for the gradient.
  * What a token or an adapter holds reaches no other token's or adapter's results, NaN and infinities
  * included; a token with an infinity may get NaN where the sum is one. The workspace of more than 192
- * tokens holds the layer in 16 bits. */
+ * tokens holds the layer in 16 bits: there, and in every gradient, each weight is rounded to dtype, while up to
+ * 192 tokens the weights are exact. */
 size_t cdclq_adapter_work_bytes(const cdclq_packed* packed, const void* x, size_t ldx, size_t t, const void* a,
                                 const void* b, size_t adapters, size_t rank, int grad);
 int cdclq_adapter_linear_device(cdclq_ctx* ctx, const cdclq_packed* packed, const void* x, size_t ldx, size_t t,
@@ -393,8 +394,8 @@ int cdclq_vocab_loss_device(cdclq_ctx* ctx, const void* x, size_t ldx, const voi
                             size_t v, int dtype, const int64_t* targets, int64_t ignore_index, float* loss, float* lse,
                             void* work, size_t work_bytes, void* stream);
 /* The gradient for dloss[t] = d(objective) / d(loss[t]): dx (t x d, 0 at ignored tokens) and, unless
- * dw is NULL, dw (v x d); lse is the forward call's. With a target outside 0..v the token's dx and all
- * of dw are NaN. grad = 1 in cdclq_vocab_work_bytes. */
+ * dw is NULL, dw (v x d); lse is the forward call's. A token's dx keeps its precision whatever the other
+ * tokens' dloss. With a target outside 0..v the token's dx and all of dw are NaN. grad = 1 in cdclq_vocab_work_bytes. */
 int cdclq_vocab_loss_backward_device(cdclq_ctx* ctx, const void* x, size_t ldx, const void* w, size_t ldw, size_t t,
                                      size_t d, size_t v, int dtype, const int64_t* targets, int64_t ignore_index,
                                      const float* lse, const float* dloss, void* dx, size_t lddx, void* dw, size_t lddw,

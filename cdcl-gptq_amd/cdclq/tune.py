@@ -7,10 +7,13 @@ The operators that a quantized model needs once its weights are frozen:
   checkpoint_save / checkpoint_restore   a layer's input kept in 8 bits until the backward pass
   vocab_loss / vocab_loss_backward       softmax cross entropy over a large vocabulary and its
                                          gradient, without the logits in memory
-  linear, cross_entropy                  the same as differentiable functions of torch's autograd
+  embed / embed_backward                 the tokens' rows of the embedding table, and its gradient
+  Gradients, grad_norm / clip_grads      the norm of a step's gradients, and the gradients clipped to it
+  constrain_logits                       penalties for repeated tokens, biases and grammar masks
+  linear, cross_entropy, embedding       the same as differentiable functions of torch's autograd
 
-Tensors are torch tensors on the context's GPU, bfloat16 or float16, with contiguous rows (any row
-stride). Every call is enqueued on torch's current stream and returns without waiting; scratch
+Tensors are torch tensors on the context's GPU, bfloat16 or float16 (gradients and logits float32 as well), with
+contiguous rows (any row stride). Every call is enqueued on torch's current stream and returns without waiting; scratch
 memory comes from torch's allocator, so that calls may be made on several streams and captured into
 a graph. A refused argument raises CdclqError (or TypeError / ValueError for a tensor of the wrong
 kind) before anything is enqueued.
@@ -23,10 +26,11 @@ from dataclasses import dataclass
 import numpy as np
 import torch
 
-from . import DTYPE_BF16, DTYPE_F16, Context, check_row_width, lib as _L
+from . import DTYPE_BF16, DTYPE_F16, DTYPE_F32, Context, check_row_width, lib as _L
 
 BLOCK = 128  # features per scale of an 8-bit checkpoint
 _CODES = {torch.bfloat16: DTYPE_BF16, torch.float16: DTYPE_F16}
+_CODES32 = {torch.float32: DTYPE_F32, **_CODES}
 
 
 _empty = torch.empty
@@ -311,6 +315,204 @@ def vocab_loss_backward(ctx: Context, x: torch.Tensor, w: torch.Tensor, targets:
     return dx, dw
 
 
+# ---------------------------------------------------------------- token embedding
+def embed(ctx: Context, table: torch.Tensor, tokens: torch.Tensor, scale: float = 1.0,
+          ignore_index: int = -100) -> torch.Tensor:
+    """scale * table[tokens] (table V x d, tokens int64), T x d, rounded once. A token that is ignore_index gives a
+    row of zeros, any other outside 0..V a row of NaN."""
+    code, ldt = _code(table, "table"), _matrix(ctx, table, "table")
+    v, d = table.shape
+    t = tokens.numel()
+    _vector(ctx, tokens, "tokens", torch.int64, t)
+    out = _empty(t, d, dtype=table.dtype, device=table.device)
+    ctx.check(_L().cdclq_embed_device(ctx.ptr, table.data_ptr(), ldt, v, d, code, tokens.data_ptr(), t, scale,
+                                      ignore_index, out.data_ptr(), d, _stream(ctx)))
+    return out
+
+
+def embed_backward(ctx: Context, dy: torch.Tensor, tokens: torch.Tensor, vocab: int, scale: float = 1.0,
+                   ignore_index: int = -100, into: torch.Tensor | None = None) -> torch.Tensor:
+    """The gradient of embed's table (vocab x d) for dy (T x d), in dy's type: scale times the float32 sum of the dy
+    of each token, zeros elsewhere. into (dy's type or float32) is a gradient to which it is added, as that of a tied
+    head; only rows with tokens are touched then, and into is returned. With a token outside 0..vocab that is not
+    ignore_index all of it is NaN."""
+    code, ld = _code(dy, "dy"), _matrix(ctx, dy, "dy")
+    t, d = dy.shape
+    _vector(ctx, tokens, "tokens", torch.int64, t)
+    if into is None:
+        de = _empty(vocab, d, dtype=dy.dtype, device=dy.device)
+        kind, lde = code, d
+    else:
+        de = into
+        if de.dtype != dy.dtype and de.dtype != torch.float32:
+            raise TypeError(f"into is {de.dtype}, need {dy.dtype} or torch.float32")
+        kind, lde = _CODES32[de.dtype], _matrix(ctx, de, "into", None, vocab, d)
+    L = _L()
+    work = _work(L.cdclq_embed_work_bytes(t, d, vocab), dy.device)
+    ctx.check(L.cdclq_embed_backward_device(ctx.ptr, dy.data_ptr(), ld, t, d, vocab, code, tokens.data_ptr(), scale,
+                                            ignore_index, into is not None, de.data_ptr(), lde, kind, work.data_ptr(),
+                                            work.numel(), _stream(ctx)))
+    return de
+
+
+# ---------------------------------------------------------------- gradient norms and clipping
+_GRAD = np.dtype([("x", np.uintp), ("out", np.uintp), ("count", np.uintp), ("dtype", np.int32), ("out_dtype", np.int32)])
+
+
+class Gradients:
+    """The gradients of a step as one set: tensors (float32, bfloat16 or float16, contiguous, of any shapes), to be
+    clipped in place, or into out: tensors of the same shapes, each of its gradient's type or float32 (the gradients
+    of 32-bit master weights). With adapters = R every tensor's first dimension is R, the adapters of users that train
+    together, and each adapter has a norm of its own. The set may be kept over steps that keep their tensors."""
+
+    def __init__(self, ctx: Context, tensors, out=None, adapters: int | None = None):
+        self.ctx, self.tensors, self.out = ctx, list(tensors), None if out is None else list(out)
+        self.parts = 1 if adapters is None else int(adapters)
+        self.shape = () if adapters is None else (self.parts,)
+        outs = self.tensors if self.out is None else self.out
+        if len(outs) != len(self.tensors):
+            raise ValueError(f"{len(self.tensors)} gradients and {len(outs)} outputs")
+        if adapters is not None and self.parts < 1:
+            raise ValueError(f"adapters is {adapters}, need at least 1")
+        self.table = np.zeros(len(outs), _GRAD)
+        codes = []
+        for x, o in zip(self.tensors, outs):
+            for g, name in ((x, "a gradient"), (o, "an output")):
+                if g.get_device() != ctx.device:
+                    raise ValueError(f"{name} is on {g.device}, the context on cuda:{ctx.device}")
+                if g.dtype not in _CODES32:
+                    raise TypeError(f"{name} is {g.dtype}, need float32, bfloat16 or float16")
+                if not g.is_contiguous():
+                    raise ValueError(f"{name} of shape {tuple(g.shape)} has strides {g.stride()}, it must be contiguous")
+            if o.shape != x.shape:
+                raise ValueError(f"an output has shape {tuple(o.shape)}, its gradient {tuple(x.shape)}")
+            if o.dtype != x.dtype and o.dtype != torch.float32:
+                raise TypeError(f"an output is {o.dtype}, need {x.dtype} or torch.float32")
+            if adapters is not None and (x.dim() == 0 or x.shape[0] != self.parts):
+                raise ValueError(f"a gradient has shape {tuple(x.shape)}, need {self.parts} adapters first")
+            codes.append((x.numel(), _CODES32[x.dtype], _CODES32[o.dtype]))
+        if codes:
+            self.table["count"], self.table["dtype"], self.table["out_dtype"] = zip(*codes)
+        self.at = None
+        self._addresses()
+        self.work_bytes = _L().cdclq_grad_work_bytes(self.table.ctypes.data, len(codes), self.parts)
+
+    def _addresses(self) -> int:
+        """The table's address, with the tensors' present addresses in it."""
+        at = [x.data_ptr() for x in self.tensors]
+        if self.out is not None:
+            at += [x.data_ptr() for x in self.out]
+        if at != self.at:
+            n = len(self.tensors)
+            self.table["x"], self.table["out"] = at[:n], at[-n:] if n else []
+            self.at, self.ptr = at, self.table.ctypes.data
+        return self.ptr
+
+
+def _grad_call(grads: Gradients):
+    if not isinstance(grads, Gradients):
+        raise TypeError(f"need Gradients, got {type(grads).__name__}")
+    ctx = grads.ctx
+    dev = torch.device("cuda", ctx.device)
+    norm = _empty(grads.shape, dtype=torch.float32, device=dev)
+    return ctx, grads._addresses(), len(grads.tensors), norm, _work(grads.work_bytes, dev)
+
+
+def grad_norm(grads: Gradients) -> torch.Tensor:
+    """The 2-norm of all gradients together, float32: of one element, or with adapters of one for each. Squares are
+    summed in 64 bits."""
+    ctx, table, n, norm, work = _grad_call(grads)
+    ctx.check(_L().cdclq_grad_norm_device(ctx.ptr, table, n, grads.parts, norm.data_ptr(), work.data_ptr(),
+                                          work.numel(), _stream(ctx)))
+    return norm
+
+
+def clip_grads(grads: Gradients, max_norm: float) -> torch.Tensor:
+    """grad_norm, and the gradients times min(1, max_norm / (norm + 1e-6)), in place or, where the set has them, into
+    its outputs (which are always written). Gradients (an adapter's) whose norm is NaN or infinite are not scaled."""
+    ctx, table, n, norm, work = _grad_call(grads)
+    ctx.check(_L().cdclq_clip_grads_device(ctx.ptr, table, n, grads.parts, max_norm, norm.data_ptr(), work.data_ptr(),
+                                           work.numel(), _stream(ctx)))
+    return norm
+
+
+# ---------------------------------------------------------------- constraints on logits
+def _tight(ctx: Context, x: torch.Tensor, name: str, dtype, rows: int, cols=None):
+    _matrix(ctx, x, name, dtype, rows, cols)
+    if not x.is_contiguous():
+        raise ValueError(f"{name} must be contiguous")
+
+
+def constrain_logits(ctx: Context, logits: torch.Tensor, history: torch.Tensor | None = None,
+                     lengths: torch.Tensor | None = None, prompts: torch.Tensor | None = None,
+                     repetition: torch.Tensor | None = None, frequency: torch.Tensor | None = None,
+                     presence: torch.Tensor | None = None, bias_tokens: torch.Tensor | None = None,
+                     biases: torch.Tensor | None = None, mask: torch.Tensor | None = None,
+                     mask_rows: torch.Tensor | None = None, out: torch.Tensor | None = None) -> torch.Tensor:
+    """The logits (R x V, float32, bfloat16 or float16) of a decode step with each request's constraints, in this
+    order, in float32, rounded once; out may be logits itself (only what changes is touched then).
+
+    history (int64, R x width): the tokens of each request, of which the first lengths (int32, R; default all) count,
+    the first prompts (int32, R; default none) of those are the prompt's and the others generated; tokens outside 0..V
+    stand for none. A token of the history has its logit divided by repetition (float32, R) if that is above 0, else
+    multiplied; one generated c > 0 times loses frequency * c + presence (float32, R).
+    bias_tokens (int64, R x B), biases (float32, R x B): what is added to a token's logit; tokens outside 0..V stand
+    for none, of a token that is there several times all are added.
+    mask (int32, M x ceil(V / 32)): a grammar's tokens, token i is allowed if bit i % 32 of word i // 32 is set, the
+    others get -infinity. mask_rows (int32, R): the row of mask for each request, -1 for none, any other outside 0..M
+    gives a row of NaN; without mask_rows M is R."""
+    code = _CODES32.get(logits.dtype)
+    if code is None:
+        raise TypeError(f"logits is {logits.dtype}, need float32, bfloat16 or float16")
+    ld = _matrix(ctx, logits, "logits")
+    r, v = logits.shape
+    hp = lp = pp = bt = bv = mp = mr = None
+    ldh = width = nb = ldm = masks = 0
+    if history is not None:
+        ldh = _matrix(ctx, history, "history", torch.int64, r)
+        width, hp = history.shape[1], history.data_ptr()
+        if lengths is not None:
+            _vector(ctx, lengths, "lengths", torch.int32, r)
+            lp = lengths.data_ptr()
+        if prompts is not None:
+            _vector(ctx, prompts, "prompts", torch.int32, r)
+            pp = prompts.data_ptr()
+    elif lengths is not None or prompts is not None:
+        raise ValueError("lengths or prompts without a history")
+    by = []
+    for x, name in ((repetition, "repetition"), (frequency, "frequency"), (presence, "presence")):
+        if x is None:
+            by.append(None)
+            continue
+        if history is None:
+            raise ValueError(f"{name} without a history")
+        _vector(ctx, x, name, torch.float32, r)
+        by.append(x.data_ptr())
+    if (bias_tokens is None) != (biases is None):
+        raise ValueError("bias_tokens and biases belong together")
+    if biases is not None:
+        _tight(ctx, bias_tokens, "bias_tokens", torch.int64, r)
+        nb = bias_tokens.shape[1]
+        _tight(ctx, biases, "biases", torch.float32, r, nb)
+        bt, bv = bias_tokens.data_ptr(), biases.data_ptr()
+    if mask is not None:
+        ldm = _matrix(ctx, mask, "mask", torch.int32, r if mask_rows is None else None, -(-v // 32))
+        masks, mp = mask.shape[0], mask.data_ptr()
+        if mask_rows is not None:
+            _vector(ctx, mask_rows, "mask_rows", torch.int32, r)
+            mr = mask_rows.data_ptr()
+    elif mask_rows is not None:
+        raise ValueError("mask_rows without a mask")
+    if out is None:
+        out = _empty(r, v, dtype=logits.dtype, device=logits.device)
+        ldo = v
+    else:
+        ldo = _matrix(ctx, out, "out", logits.dtype, r, v)
+    ctx.check(_L().cdclq_constrain_logits_device(ctx.ptr, logits.data_ptr(), ld, r, v, code, hp, ldh, width, lp, pp, *by,
+                                                 bt, bv, nb, mp, ldm, masks, mr, out.data_ptr(), ldo, _stream(ctx)))
+    return out
+
+
 # ---------------------------------------------------------------- as differentiable functions
 def _first_order(backward):
     """A backward pass that has no gradient of its own and refuses to take part in a graph (create_graph). Its
@@ -318,7 +520,7 @@ def _first_order(backward):
     once_differentiable makes, is reached only where the graph happens to lead through it."""
     def run(fn, *grads):
         if torch.is_grad_enabled():
-            raise RuntimeError("cdclq.tune: linear and cross_entropy have gradients of first order only "
+            raise RuntimeError("cdclq.tune: linear, cross_entropy and embedding have gradients of first order only "
                                "(create_graph is not supported)")
         return backward(fn, *grads)
     return run
@@ -387,3 +589,25 @@ def cross_entropy(ctx: Context, x: torch.Tensor, w: torch.Tensor, targets: torch
     """The mean of vocab_loss over the tokens that take part (0 if none does), for autograd: gradients (of
     first order only) of x and, where w asks for it, of w."""
     return _CrossEntropy.apply(x, w, ctx, targets, ignore_index)
+
+
+class _Embedding(torch.autograd.Function):
+    @staticmethod
+    def forward(fn, table, ctx, tokens, scale, ignore_index):
+        fn.save_for_backward(tokens)
+        fn.ctx, fn.vocab, fn.scale, fn.ignore_index = ctx, table.shape[0], scale, ignore_index
+        return embed(ctx, table, tokens, scale, ignore_index)
+
+    @staticmethod
+    @_first_order
+    def backward(fn, dy):
+        (tokens,) = fn.saved_tensors
+        return embed_backward(fn.ctx, dy.contiguous(), tokens, fn.vocab, fn.scale, fn.ignore_index), None, None, None, None
+
+
+def embedding(ctx: Context, table: torch.Tensor, tokens: torch.Tensor, scale: float = 1.0,
+              ignore_index: int = -100) -> torch.Tensor:
+    """embed for autograd: the gradient (dense, of first order only) of table."""
+    if not (torch.is_grad_enabled() and table.requires_grad):
+        return embed(ctx, table, tokens, scale, ignore_index)
+    return _Embedding.apply(table, ctx, tokens, scale, ignore_index)

@@ -343,4 +343,45 @@ hipError_t adapter_wide(hipStream_t st, int dtype, const PackedView& v, const Ad
 size_t grad_work_bytes(const PackedView& v, const AdapterArgs& a);
 hipError_t adapter_grad(hipStream_t st, int dtype, const PackedView& v, const AdapterArgs& a, void* work);
 
+// ---- k_embed.hip: token embedding (table v x d, 16-bit) and the gradient of its table (de: dtype or f32; add: onto
+// what it holds)
+hipError_t embed_rows(hipStream_t st, int dtype, const uint16_t* table, long ldt, long v, long d, const int64_t* ids,
+                      long t, float scale, int64_t ignore, uint16_t* out, long ldo);
+size_t embed_work_bytes(long t, long d, long v);
+hipError_t embed_grad(hipStream_t st, int dtype, const uint16_t* dy, long lddy, long t, long d, long v,
+                      const int64_t* ids, float scale, int64_t ignore, bool add, void* de, long lde, int de_dtype,
+                      void* work);
+
+// ---- k_clip.hip: gradient norms and clipping; every tensor in `parts` equal parts
+struct GradTensor {
+  const void* x;
+  void* out;  // may be x
+  long n;     // elements
+  int dtype, out_dtype;
+};
+size_t clip_work_bytes(const GradTensor* g, size_t n, int parts);
+hipError_t grad_norm(hipStream_t st, const GradTensor* g, size_t n, int parts, float* norm, void* work);
+hipError_t clip_grads(hipStream_t st, const GradTensor* g, size_t n, int parts, double most, float* norm, void* work);
+
+// ---- k_constrain.hip: penalties, biases and grammar masks on logits
+struct ConstrainArgs {
+  const void* logits;  // r x v
+  long ld, r, v;
+  const int64_t* history;  // r x width, or null
+  long ldh;
+  int width;
+  const int *lengths, *prompts;                      // r, or null: width, 0
+  const float *repetition, *frequency, *presence;    // r, or null: 1, 0, 0
+  const int64_t* bias_tokens;                        // r x biases
+  const float* bias;
+  int biases;
+  const uint32_t* mask;  // masks x words, or null
+  long ldm;
+  int masks;
+  const int* mask_rows;  // r, or null: row by row
+  void* out;
+  long ldo;
+};
+hipError_t constrain_logits(hipStream_t st, int dtype, const ConstrainArgs& a);
+
 }  // namespace cdclq

@@ -1,6 +1,6 @@
 // C-ABI entry points of the operators that train and serve adapters on a packed model
 // (include/cdclq.h): validation, workspace plans and the k_ckpt.hip / k_loss.hip / k_packed.hip /
-// k_adapt.hip launches. They enqueue on the caller's stream and return; only the opening and closing of
+// k_adapt.hip / k_embed.hip / k_clip.hip / k_constrain.hip launches. They enqueue on the caller's stream and return; only the opening and closing of
 // a packed layer allocates device memory and waits.
 #include <hip/hip_runtime.h>
 
@@ -235,6 +235,74 @@ size_t linear_bytes(const PackedView& v, const AdapterArgs& r) {
   return (size_t)r.t <= kFewTokens ? few_work_bytes(v, r.t, r.rank) : wide_work_bytes(v, r);
 }
 
+int check_embed(cdclq_ctx* ctx, size_t t, size_t d, size_t v, int dtype) {
+  CK(check_half(ctx, dtype));
+  if (d == 0 || v == 0) return fail(ctx, CDCLQ_INVALID_ARG, "hidden width and vocabulary must be > 0");
+  CK(check_size(ctx, "token count", t, kMaxTokens));
+  CK(check_size(ctx, "hidden width", d, kMaxWidth));
+  return check_size(ctx, "vocabulary", v, kMaxVocab);
+}
+
+int check_type(cdclq_ctx* ctx, int dtype) {
+  if (dtype != CDCLQ_DTYPE_F32 && dtype != CDCLQ_DTYPE_F16 && dtype != CDCLQ_DTYPE_BF16)
+    return fail(ctx, CDCLQ_INVALID_ARG, "unsupported dtype " + std::to_string(dtype) + " (need F32, F16 or BF16)");
+  return CDCLQ_OK;
+}
+constexpr size_t type_bytes(int dtype) { return dtype == CDCLQ_DTYPE_F32 ? 4 : 2; }
+
+// Whether two matrices (rows, row stride, columns, bytes an element) share memory.
+bool overlap(const void* a, size_t ra, size_t lda, size_t ca, size_t ea, const void* b, size_t rb, size_t ldb,
+             size_t cb, size_t eb) {
+  if (!ra || !rb) return false;
+  const uintptr_t x = (uintptr_t)a, y = (uintptr_t)b;
+  return x < y + ((rb - 1) * ldb + cb) * eb && y < x + ((ra - 1) * lda + ca) * ea;
+}
+
+constexpr size_t kMaxParts = 32768, kMaxPart = (size_t)1 << 30, kMaxGrad = (size_t)1 << 40;
+
+// The host array's tensors after checks; clip: their outputs as well, which nothing else may overlap.
+int grad_tensors(cdclq_ctx* ctx, const cdclq_grad* grads, size_t n, size_t parts, bool clip, std::vector<GradTensor>* out) {
+  if (n && !grads) return fail(ctx, CDCLQ_INVALID_ARG, "null buffer argument");
+  CK(check_size(ctx, "tensor count", n, (size_t)1 << 20));
+  if (parts == 0) return fail(ctx, CDCLQ_INVALID_ARG, "gradients need at least one part");
+  CK(check_size(ctx, "adapter count", parts, kMaxParts));
+  out->resize(n);
+  struct Range {
+    uintptr_t from, to;
+  };
+  std::vector<Range> used;
+  if (clip) used.reserve(2 * n);
+  for (size_t i = 0; i < n; ++i) {
+    const cdclq_grad& g = grads[i];
+    CK(check_type(ctx, g.dtype));
+    CK(check_size(ctx, "gradient of", g.count, kMaxGrad));
+    if (g.count % parts)
+      return fail(ctx, CDCLQ_INVALID_ARG, "gradient " + std::to_string(i) + " of " + std::to_string(g.count) +
+                                              " elements is not " + std::to_string(parts) + " equal parts");
+    if (parts > 1) CK(check_size(ctx, "part of", g.count / parts, kMaxPart));
+    if (g.count && !g.x) return fail(ctx, CDCLQ_INVALID_ARG, "null buffer argument");
+    (*out)[i] = {g.x, g.out, (long)g.count, g.dtype, g.dtype};
+    if (!clip) continue;
+    CK(check_type(ctx, g.out_dtype));
+    if (g.out_dtype != g.dtype && g.out_dtype != CDCLQ_DTYPE_F32)
+      return fail(ctx, CDCLQ_INVALID_ARG, "a clipped gradient keeps its dtype or becomes F32");
+    if (g.count && !g.out) return fail(ctx, CDCLQ_INVALID_ARG, "null buffer argument");
+    (*out)[i].out_dtype = g.out_dtype;
+    if (!g.count) continue;
+    if (g.x == g.out && g.out_dtype != g.dtype)
+      return fail(ctx, CDCLQ_INVALID_ARG, "a gradient that is clipped in place keeps its dtype");
+    const uintptr_t x = (uintptr_t)g.x, o = (uintptr_t)g.out;
+    used.push_back({x, x + g.count * type_bytes(g.dtype)});
+    if (o != x) used.push_back({o, o + g.count * type_bytes(g.out_dtype)});
+  }
+  auto before = [](const Range& a, const Range& b) { return a.from < b.from; };
+  if (!std::is_sorted(used.begin(), used.end(), before)) std::sort(used.begin(), used.end(), before);
+  for (size_t i = 1; i < used.size(); ++i)
+    if (used[i].from < used[i - 1].to)
+      return fail(ctx, CDCLQ_INVALID_ARG, "gradients or their outputs overlap (the same tensor twice?)");
+  return CDCLQ_OK;
+}
+
 }  // namespace
 
 extern "C" {
@@ -429,6 +497,150 @@ int cdclq_adapter_backward_device(cdclq_ctx* ctx, const cdclq_packed* packed, co
   OnDevice on(ctx->device);
   HIPCK(on.err);
   HIPCK(adapter_grad((hipStream_t)stream, dtype, v, r, work));
+  return CDCLQ_OK;
+}
+
+int cdclq_embed_device(cdclq_ctx* ctx, const void* table, size_t ldt, size_t v, size_t d, int dtype,
+                       const int64_t* tokens, size_t t, float scale, int64_t ignore_index, void* out, size_t ldo,
+                       void* stream) {
+  if (!ctx) return CDCLQ_INVALID_ARG;
+  ctx->err.clear();
+  CK(check_embed(ctx, t, d, v, dtype));
+  CK(check_rows(ctx, "table", ldt, d));
+  CK(check_rows(ctx, "out", ldo, d));
+  if (t == 0) return CDCLQ_OK;
+  if (!table || !tokens || !out) return fail(ctx, CDCLQ_INVALID_ARG, "null buffer argument");
+  if (overlap(table, v, ldt, d, 2, out, t, ldo, d, 2)) return fail(ctx, CDCLQ_INVALID_ARG, "out overlaps the table");
+  OnDevice on(ctx->device);
+  HIPCK(on.err);
+  HIPCK(embed_rows((hipStream_t)stream, dtype, static_cast<const uint16_t*>(table), (long)ldt, (long)v, (long)d, tokens,
+                   (long)t, scale, ignore_index, static_cast<uint16_t*>(out), (long)ldo));
+  return CDCLQ_OK;
+}
+
+size_t cdclq_embed_work_bytes(size_t t, size_t d, size_t v) {
+  if (d == 0 || v == 0 || t > kMaxTokens || d > kMaxWidth || v > kMaxVocab) return 0;
+  return embed_work_bytes((long)t, (long)d, (long)v);
+}
+
+int cdclq_embed_backward_device(cdclq_ctx* ctx, const void* dy, size_t lddy, size_t t, size_t d, size_t v, int dtype,
+                                const int64_t* tokens, float scale, int64_t ignore_index, int add, void* de,
+                                size_t lde, int de_dtype, void* work, size_t work_bytes, void* stream) {
+  if (!ctx) return CDCLQ_INVALID_ARG;
+  ctx->err.clear();
+  CK(check_embed(ctx, t, d, v, dtype));
+  if (de_dtype != dtype && de_dtype != CDCLQ_DTYPE_F32)
+    return fail(ctx, CDCLQ_INVALID_ARG, "the table's gradient is of dy's dtype or F32");
+  CK(check_rows(ctx, "dy", lddy, d));
+  CK(check_rows(ctx, "de", lde, d));
+  if (!de || (t && (!dy || !tokens))) return fail(ctx, CDCLQ_INVALID_ARG, "null buffer argument");
+  if (t == 0 && add) return CDCLQ_OK;
+  if (overlap(dy, t, lddy, d, 2, de, v, lde, d, type_bytes(de_dtype)))
+    return fail(ctx, CDCLQ_INVALID_ARG, "the table's gradient overlaps dy");
+  CK(check_work(ctx, work, work_bytes, embed_work_bytes((long)t, (long)d, (long)v)));
+  OnDevice on(ctx->device);
+  HIPCK(on.err);
+  HIPCK(embed_grad((hipStream_t)stream, dtype, static_cast<const uint16_t*>(dy), (long)lddy, (long)t, (long)d, (long)v,
+                   tokens, scale, ignore_index, add != 0, de, (long)lde, de_dtype, work));
+  return CDCLQ_OK;
+}
+
+size_t cdclq_grad_work_bytes(const cdclq_grad* grads, size_t n, size_t parts) {
+  if ((n && !grads) || n > (size_t)1 << 20 || parts == 0 || parts > kMaxParts) return 0;
+  try {
+    std::vector<GradTensor> g(n);
+    for (size_t i = 0; i < n; ++i) {
+      if (grads[i].count > kMaxGrad) return 0;
+      g[i].n = (long)grads[i].count;
+    }
+    return clip_work_bytes(g.data(), n, (int)parts);
+  } catch (const std::bad_alloc&) {
+    return 0;
+  }
+}
+
+int cdclq_grad_norm_device(cdclq_ctx* ctx, const cdclq_grad* grads, size_t n, size_t parts, float* norm, void* work,
+                           size_t work_bytes, void* stream) {
+  if (!ctx) return CDCLQ_INVALID_ARG;
+  ctx->err.clear();
+  try {
+    std::vector<GradTensor> g;
+    CK(grad_tensors(ctx, grads, n, parts, false, &g));
+    if (!norm) return fail(ctx, CDCLQ_INVALID_ARG, "null buffer argument");
+    CK(check_work(ctx, work, work_bytes, clip_work_bytes(g.data(), n, (int)parts)));
+    OnDevice on(ctx->device);
+    HIPCK(on.err);
+    HIPCK(grad_norm((hipStream_t)stream, g.data(), n, (int)parts, norm, work));
+  } catch (const std::bad_alloc&) {
+    return fail(ctx, CDCLQ_OOM, "host allocation failed");
+  }
+  return CDCLQ_OK;
+}
+
+int cdclq_clip_grads_device(cdclq_ctx* ctx, const cdclq_grad* grads, size_t n, size_t parts, double max_norm,
+                            float* norm, void* work, size_t work_bytes, void* stream) {
+  if (!ctx) return CDCLQ_INVALID_ARG;
+  ctx->err.clear();
+  if (!(max_norm >= 0.0)) return fail(ctx, CDCLQ_INVALID_ARG, "max_norm must be >= 0");
+  try {
+    std::vector<GradTensor> g;
+    CK(grad_tensors(ctx, grads, n, parts, true, &g));
+    if (!norm) return fail(ctx, CDCLQ_INVALID_ARG, "null buffer argument");
+    CK(check_work(ctx, work, work_bytes, clip_work_bytes(g.data(), n, (int)parts)));
+    OnDevice on(ctx->device);
+    HIPCK(on.err);
+    HIPCK(clip_grads((hipStream_t)stream, g.data(), n, (int)parts, max_norm, norm, work));
+  } catch (const std::bad_alloc&) {
+    return fail(ctx, CDCLQ_OOM, "host allocation failed");
+  }
+  return CDCLQ_OK;
+}
+
+int cdclq_constrain_logits_device(cdclq_ctx* ctx, const void* logits, size_t ld, size_t r, size_t v, int dtype,
+                                  const int64_t* history, size_t ld_history, size_t width, const int32_t* lengths,
+                                  const int32_t* prompts, const float* repetition, const float* frequency,
+                                  const float* presence, const int64_t* bias_tokens, const float* biases, size_t nbias,
+                                  const uint32_t* mask, size_t ld_mask, size_t nmasks, const int32_t* mask_rows,
+                                  void* out, size_t ldo, void* stream) {
+  if (!ctx) return CDCLQ_INVALID_ARG;
+  ctx->err.clear();
+  CK(check_type(ctx, dtype));
+  if (v == 0) return fail(ctx, CDCLQ_INVALID_ARG, "vocabulary must be > 0");
+  CK(check_size(ctx, "request count", r, kMaxTokens));
+  CK(check_size(ctx, "vocabulary", v, kMaxVocab));
+  CK(check_rows(ctx, "logits", ld, v));
+  CK(check_rows(ctx, "out", ldo, v));
+  CK(check_size(ctx, "history", width, ((size_t)1 << 20) - 1));
+  CK(check_size(ctx, "bias count", nbias, 1024));
+  CK(check_size(ctx, "mask count", nmasks, kMaxTokens));
+  CK(check_rows(ctx, "history", ld_history, width));
+  if (nmasks) CK(check_rows(ctx, "mask", ld_mask, (v + 31) / 32));
+  if (mask && !mask_rows && nmasks != r)
+    return fail(ctx, CDCLQ_INVALID_ARG, std::to_string(nmasks) + " masks for " + std::to_string(r) + " requests need mask_rows");
+  if (r == 0) return CDCLQ_OK;
+  if (!logits || !out || (width && !history) || (nmasks && !mask) || (nbias && (!bias_tokens || !biases)))
+    return fail(ctx, CDCLQ_INVALID_ARG, "null buffer argument");
+  if ((logits != out || ld != ldo) && overlap(logits, r, ld, v, type_bytes(dtype), out, r, ldo, v, type_bytes(dtype)))
+    return fail(ctx, CDCLQ_INVALID_ARG, "out overlaps the logits (in place it has their address and row stride)");
+  ConstrainArgs a = {};
+  a.logits = logits;
+  a.ld = (long)ld, a.r = (long)r, a.v = (long)v;
+  a.history = width ? history : nullptr;
+  a.ldh = (long)ld_history;
+  a.width = (int)width;
+  a.lengths = lengths, a.prompts = prompts;
+  a.repetition = repetition, a.frequency = frequency, a.presence = presence;
+  a.bias_tokens = bias_tokens, a.bias = biases;
+  a.biases = (int)nbias;
+  a.mask = mask;
+  a.ldm = (long)ld_mask;
+  a.masks = (int)nmasks;
+  a.mask_rows = mask_rows;
+  a.out = out;
+  a.ldo = (long)ldo;
+  OnDevice on(ctx->device);
+  HIPCK(on.err);
+  HIPCK(constrain_logits((hipStream_t)stream, dtype, a));
   return CDCLQ_OK;
 }
 

@@ -401,6 +401,59 @@ int cdclq_vocab_loss_backward_device(cdclq_ctx* ctx, const void* x, size_t ldx, 
                                      const float* lse, const float* dloss, void* dx, size_t lddx, void* dw, size_t lddw,
                                      void* work, size_t work_bytes, void* stream);
 
+/* Token embedding: out (t x d) = scale * table[tokens[i]], table v x d, rounded once. A token equal to ignore_index
+ * gives a row of zeros, any other outside 0..v a row of NaN. */
+int cdclq_embed_device(cdclq_ctx* ctx, const void* table, size_t ldt, size_t v, size_t d, int dtype,
+                       const int64_t* tokens, size_t t, float scale, int64_t ignore_index, void* out, size_t ldo,
+                       void* stream);
+/* The gradient of its table for dy (t x d): de (v x d, de_dtype: dtype or CDCLQ_DTYPE_F32) = scale times the sum of the
+ * rows of each token, 0 in rows without tokens; with add != 0 the sums are added to what de holds (the gradient of a tied
+ * head) and rows without tokens are left alone. Sums are f32, in the tokens' order. Ignored tokens do not take part; with
+ * any other token outside 0..v all of de is NaN. */
+size_t cdclq_embed_work_bytes(size_t t, size_t d, size_t v);
+int cdclq_embed_backward_device(cdclq_ctx* ctx, const void* dy, size_t lddy, size_t t, size_t d, size_t v, int dtype,
+                                const int64_t* tokens, float scale, int64_t ignore_index, int add, void* de,
+                                size_t lde, int de_dtype, void* work, size_t work_bytes, void* stream);
+
+/* One tensor of a step's gradients: count elements at x (dtype F32, F16 or BF16), tightly packed. */
+typedef struct cdclq_grad {
+  const void* x;
+  void* out; /* cdclq_clip_grads_device: where the clipped gradient goes; x for in place */
+  size_t count;
+  int32_t dtype;
+  int32_t out_dtype; /* dtype or CDCLQ_DTYPE_F32; dtype in place */
+} cdclq_grad;
+/* norm[g] (f32) = sqrt of the sum of squares over part g of all n tensors, summed in f64; every tensor is `parts` equal
+ * parts one behind the other (the adapters of several users, the first dimension; 1: the norm of all). `grads` is a
+ * host array, read before the call returns. parts <= 32768, a part of parts > 1 up to 2^30 elements. */
+size_t cdclq_grad_work_bytes(const cdclq_grad* grads, size_t n, size_t parts);
+int cdclq_grad_norm_device(cdclq_ctx* ctx, const cdclq_grad* grads, size_t n, size_t parts, float* norm, void* work,
+                           size_t work_bytes, void* stream);
+/* The norms as above, and out = x * min(1, max_norm / (norm + 1e-6)) of each part. Where a norm is NaN or infinite the
+ * part is not scaled. Outputs and gradients must not overlap, but for an out that is its x. max_norm >= 0. */
+int cdclq_clip_grads_device(cdclq_ctx* ctx, const cdclq_grad* grads, size_t n, size_t parts, double max_norm,
+                            float* norm, void* work, size_t work_bytes, void* stream);
+
+/* Constraints on the logits (r x v; dtype F32, F16 or BF16) of a decode step, for each request (row), in this order
+ * and in f32, rounded once; each is left out by NULL (0 biases, no mask):
+ *   a token of the history:              l = l > 0 ? l / repetition : l * repetition
+ *   a token generated c > 0 times:       l = l - (frequency * c + presence)
+ *   a token with biases:                 l = l + their sum
+ *   a token whose bit of the mask is 0:  l = -infinity
+ * history: r x width tokens (row stride ld_history), of which the first lengths[i] count (NULL: all; held to 0..width)
+ * and the first prompts[i] of those are the prompt's (NULL: 0), the others generated; tokens outside 0..v stand for
+ * none. repetition, frequency, presence: r values each. bias_tokens / biases: r x nbias, tokens outside 0..v stand for
+ * none, a token that is there several times gets the sum in their order. mask: nmasks x ceil(v / 32) words (row stride
+ * ld_mask), token i at bit i % 32 of word i / 32; mask_rows[i]: the request's row of it, -1 for none, any other value
+ * outside 0..nmasks gives a row of NaN; NULL: row i (nmasks = r). out may be logits (with the same stride); it must not
+ * overlap it otherwise. Logits that nothing applies to keep their bits. width < 2^20, nbias <= 1024. */
+int cdclq_constrain_logits_device(cdclq_ctx* ctx, const void* logits, size_t ld, size_t r, size_t v, int dtype,
+                                  const int64_t* history, size_t ld_history, size_t width, const int32_t* lengths,
+                                  const int32_t* prompts, const float* repetition, const float* frequency,
+                                  const float* presence, const int64_t* bias_tokens, const float* biases, size_t nbias,
+                                  const uint32_t* mask, size_t ld_mask, size_t nmasks, const int32_t* mask_rows,
+                                  void* out, size_t ldo, void* stream);
+
 /* ---- Device memory staging for callers without their own GPU runtime binding. ---- */
 int cdclq_device_alloc(cdclq_ctx* ctx, size_t bytes, void** ptr);
 int cdclq_device_free(cdclq_ctx* ctx, void* ptr);

@@ -79,20 +79,23 @@ template <class T>
 __device__ __forceinline__ double squares(const void* base, long part, long n, long i0, long i1) {
   const auto* x = static_cast<const typename Row8<T>::stored*>(base) + part * n;
   double s = 0.0;
-  for (long i = i0 + 8 * threadIdx.x; i < i1; i += 8192) {  // four steps' loads in flight
+  auto add = [&](float f) {
+    const double v = (double)f;
+    s = __builtin_fma(v, v, s);
+  };
+  for (long i = i0 + 8 * threadIdx.x; i + 8 <= i1; i += 8192) {  // four steps' loads in flight
     Row8<T> r[4];
 #pragma unroll
     for (int u = 0; u < 4; ++u)
-      if (i + 2048 * u < i1) r[u] = row8_load<T>(x + i + 2048 * u, i1 - i - 2048 * u);
+      if (i + 2048 * u + 8 <= i1) r[u] = row8_load<T>(x + i + 2048 * u);
 #pragma unroll
     for (int u = 0; u < 4; ++u)
-      if (i + 2048 * u < i1)
+      if (i + 2048 * u + 8 <= i1)
 #pragma unroll
-        for (int k = 0; k < 8; ++k) {
-          const double v = (double)r[u].get(k);
-          s = __builtin_fma(v, v, s);
-        }
+        for (int k = 0; k < 8; ++k) add(r[u].get(k));
   }
+  const long i = i1 - ((i1 - i0) & 7) + threadIdx.x;  // the elements past the last eight
+  if (i < i1) add(Row8<T>::widen(x[i]));
   return s;
 }
 
@@ -136,7 +139,7 @@ __device__ __forceinline__ void scaled(const void* from, void* to, const ClipAt&
   auto load = [&](long i) {
 #pragma unroll
     for (int u = 0; u < 4; ++u)
-      if (i + 2048 * u < a.i1) r[u] = row8_load<T>(x + i + 2048 * u, a.i1 - i - 2048 * u);
+      if (i + 2048 * u + 8 <= a.i1) r[u] = row8_load<T>(x + i + 2048 * u);
   };
   long i = a.i0 + 8 * threadIdx.x;
   if (!place) load(i);
@@ -148,18 +151,20 @@ __device__ __forceinline__ void scaled(const void* from, void* to, const ClipAt&
     if (by == 1.0f) return;
     load(i);
   }
-  while (i < a.i1) {
+  while (i + 8 <= a.i1) {
 #pragma unroll
     for (int u = 0; u < 4; ++u) {
-      if (i + 2048 * u >= a.i1) continue;
+      if (i + 2048 * u + 8 > a.i1) continue;
       Row8<O> o;
 #pragma unroll
       for (int k = 0; k < 8; ++k) o.set(k, by * r[u].get(k));
-      row8_store<O>(y + i + 2048 * u, a.i1 - i - 2048 * u, o);
+      row8_store<O>(y + i + 2048 * u, o);
     }
     i += 8192;
     load(i);
   }
+  i = a.i1 - ((a.i1 - a.i0) & 7) + threadIdx.x;  // the elements past the last eight
+  if (i < a.i1) y[i] = Row8<O>::narrow(by * Row8<T>::widen(x[i]));
 }
 
 __global__ __launch_bounds__(256) void k_clip(const OutTensors s, uint32_t blocks, int parts, int log_chunk, long first,

@@ -45,7 +45,7 @@ __global__ __launch_bounds__(TH) void k_constrain(ConstrainArgs a, long rows8, i
 #pragma unroll
     for (int k = 0; k < K; ++k) {
       const int i = 8 * (k * TH + (int)threadIdx.x);
-      if (i < n) x[k] = row8_load<T>(in + i, n - i);
+      if (i + 8 <= n) x[k] = row8_load<T>(in + i);
     }
   }
   const long mrow = a.mask_rows ? a.mask_rows[row] : a.mask ? row : -1;
@@ -101,14 +101,17 @@ __global__ __launch_bounds__(TH) void k_constrain(ConstrainArgs a, long rows8, i
   }
   const float rep = a.repetition ? a.repetition[row] : 1.0f, freq = a.frequency ? a.frequency[row] : 0.0f,
               pres = a.presence ? a.presence[row] : 0.0f;
+  auto apply = [&](float l, uint32_t m) {
+    const uint32_t c = m & kCount;
+    if (m & ~kBias) l = l > 0.0f ? l / rep : l * rep;
+    if (c) l -= freq * (float)c + pres;
+    if (m & kBias) l += bias[((m & kBias) >> 20) - 1];
+    return l;
+  };
 #pragma unroll
   for (int k = 0; k < K; ++k) {
     const int i = 8 * (k * TH + (int)threadIdx.x);
-    if (i >= n) continue;
-    if (wrong) {
-      row8_store<T>(out + i, n - i, row8_fill<T>(__builtin_nanf("")));
-      continue;
-    }
+    if (i + 8 > n) continue;
     uint32_t m[8] = {};
     uint32_t any = 0;
     if (marks) {
@@ -118,25 +121,30 @@ __global__ __launch_bounds__(TH) void k_constrain(ConstrainArgs a, long rows8, i
       for (int j = 0; j < 8; ++j) any |= m[j];
     }
     if constexpr (PLACE) {
-      if (!any && open[k] == 0xff) continue;
-      if (open[k]) x[k] = row8_load<T>(in + i, n - i);
+      if (!any && open[k] == 0xff && !wrong) continue;
+      if (open[k]) x[k] = row8_load<T>(in + i);
     }
-    if (any) {
+    if (any)
 #pragma unroll
-      for (int j = 0; j < 8; ++j) {
-        if (!m[j]) continue;
-        float l = x[k].get(j);
-        const uint32_t c = m[j] & kCount;
-        if (m[j] & ~kBias) l = l > 0.0f ? l / rep : l * rep;
-        if (c) l -= freq * (float)c + pres;
-        if (m[j] & kBias) l += bias[((m[j] & kBias) >> 20) - 1];
-        x[k].set(j, l);
-      }
-    }
+      for (int j = 0; j < 8; ++j)
+        if (m[j]) x[k].set(j, apply(x[k].get(j), m[j]));
+    if (open[k] != 0xff)
 #pragma unroll
-    for (int j = 0; j < 8; ++j)
-      if (!(open[k] >> j & 1)) x[k].set(j, -__builtin_inff());
-    row8_store<T>(out + i, n - i, x[k]);
+      for (int j = 0; j < 8; ++j)
+        if (!(open[k] >> j & 1)) x[k].set(j, -__builtin_inff());
+    if (wrong)
+#pragma unroll
+      for (int j = 0; j < 8; ++j) x[k].set(j, __builtin_nanf(""));
+    row8_store<T>(out + i, x[k]);
+  }
+  const int i = (n & ~7) + (int)threadIdx.x;  // the tokens past the last eight
+  if (i < n) {
+    auto l = in[i];
+    const uint32_t m = marks ? word[i] : 0;
+    if (m) l = Row8<T>::narrow(apply(Row8<T>::widen(l), m));
+    if (mask && !(mask[i / 8] >> (i & 7) & 1)) l = Row8<T>::narrow(-__builtin_inff());
+    if (wrong) l = Row8<T>::narrow(__builtin_nanf(""));
+    out[i] = l;
   }
 }
 

@@ -7,15 +7,16 @@
 //
 // The gradient sums a row's tokens in their order, in f32, with one rounding at the end and no float atomics:
 // equal inputs give equal bits. Three forms by the number of tokens:
-//   few     one launch. A workgroup takes a token, finds the others of its id by comparing all ids, and leaves
-//           unless it is the first of them. Further workgroups clear the rows without tokens.
+//   few     a launch that clears dE, one in which a workgroup takes a token, finds the others of its id by comparing all
+//           ids, and leaves unless it is the first of them.
 //   ranked  a token's place among the sorted ones is the number of smaller (id, position) pairs, counted by
-//           comparing all pairs of tokens in one launch, which clears the table at the same time. Then chunks
-//           of the sorted tokens are summed; runs of equal ids that pass a chunk's end are joined by a third.
-//   sorted  the places from a radix sort, 8 or 9 bits a pass, a launch more than the passes.
+//           comparing all pairs of tokens in one launch, which clears dE beside it. Then chunks of the sorted tokens
+//           are summed; runs of equal ids that pass a chunk's end are joined by a third launch.
+//   sorted  the places from a radix sort of 5 to 9 bits a pass, whose launches clear dE beside them.
 #include <hip/hip_runtime.h>
 
 #include <algorithm>
+#include <type_traits>
 
 #include "cdclq.h"
 #include "kernels.h"
@@ -28,7 +29,7 @@ typedef unsigned long long u64;
 
 // Tokens up to which each form is taken.
 constexpr long kFewIds = 512, kRankedIds = 8192;
-constexpr int kTile = 4096;  // ids of a workgroup of the radix sort
+constexpr int kTile = 2048;  // ids of a workgroup of the radix sort
 
 __device__ __forceinline__ long block_id() { return blockIdx.x + (long)blockIdx.y * gridDim.x; }
 
@@ -64,127 +65,152 @@ __global__ __launch_bounds__(256) void k_embed_rows(const uint16_t* __restrict__
                                                     long parts) {
   const long unit = block_id() * (256 / lanes) + threadIdx.x / lanes;
   if (unit >= t * parts) return;
-  const long row = unit / parts, c0 = (unit - row * parts) * lanes * 64 + 8 * (threadIdx.x & (lanes - 1));
+  const int lane = threadIdx.x & (lanes - 1);
+  const long row = unit / parts, part = unit - row * parts, c0 = part * lanes * 64 + 8 * lane;
   const uint32_t key = id_key(ids[row], ignore, (uint32_t)v);
+  const bool is = key < (uint32_t)v;
+  const float other = key == (uint32_t)v ? 0.0f : __builtin_nanf("");
+  const uint16_t* from = table + (is ? key : 0) * ldt;
   uint16_t* to = out + row * ldo;
-  if (key >= (uint32_t)v) {
-    const Row8<T> f = row8_fill<T>(key == (uint32_t)v ? 0.0f : __builtin_nanf(""));
-    for (int k = 0; k < 8; ++k)
-      if (c0 + 8l * lanes * k < d) row8_store<T>(to + c0 + 8l * lanes * k, d - c0 - 8l * lanes * k, f);
-    return;
-  }
-  const uint16_t* from = table + key * ldt;
   Row8<T> x[8];
 #pragma unroll
   for (int k = 0; k < 8; ++k) {
     const long c = c0 + 8l * lanes * k;
-    if (c < d) x[k] = row8_load<T>(from + c, d - c);
+    if (c + 8 <= d) x[k] = row8_load<T>(from + c);
   }
 #pragma unroll
   for (int k = 0; k < 8; ++k) {
     const long c = c0 + 8l * lanes * k;
-    if (c >= d) continue;
-    if (scale != 1.0f)
+    if (c + 8 > d) continue;
+    if (scale != 1.0f || !is)
 #pragma unroll
-      for (int i = 0; i < 8; ++i) x[k].set(i, scale * x[k].get(i));
-    row8_store<T>(to + c, d - c, x[k]);
+      for (int i = 0; i < 8; ++i) x[k].set(i, is ? scale * x[k].get(i) : other);
+    row8_store<T>(to + c, x[k]);
   }
+  if (part == parts - 1)  // the elements past the last eight
+    for (long c = (d & ~7l) + lane; c < d; c += lanes)
+      to[c] = !is ? T::narrow(other) : scale != 1.0f ? T::narrow(scale * T::widen(from[c])) : from[c];
 }
 
-// x in every element of rows [r0, r1) of dE that `skip` (one flag a row, or null) does not name.
+// x in every element of share b of nb of dE's elements [e0, e1) in rows of d, counted row by row.
 template <class O>
-__device__ __forceinline__ void fill_rows(const EmbedView& a, long r0, long r1, const uint8_t* skip, float x) {
-  auto* de = static_cast<typename Row8<O>::stored*>(a.de);
-  const Row8<O> f = row8_fill<O>(x);
-  const int per = blockDim.x / a.lanes, l = threadIdx.x & (a.lanes - 1);
-  for (long r = r0 + threadIdx.x / a.lanes; r < r1; r += per) {
-    if (skip && skip[r - r0]) continue;
-    for (long c = 8 * l; c < a.d; c += 8 * a.lanes) row8_store<O>(de + r * a.lde + c, a.d - c, f);
+__device__ __forceinline__ void fill(const EmbedView& a, long e0, long e1, long b, long nb, float x) {
+  typedef typename Row8<O>::stored E;
+  E* const de = static_cast<E*>(a.de);
+  const E one = Row8<O>::narrow(x);
+  Row8<O> eight;
+#pragma unroll
+  for (int i = 0; i < 8; ++i) eight.v[i] = one;
+  if (a.lde == a.d) {  // one piece of memory
+    const long n = e1 - e0, per = ((n + nb - 1) / nb + 7) & ~7l;
+    const long from = e0 + min(n, b * per), to = e0 + min(n, (b + 1) * per);
+    long i = from + 8 * (long)threadIdx.x;
+    for (; i + 8 <= to; i += 8 * blockDim.x) row8_store<O>(de + i, eight);
+    for (; i < to; ++i) de[i] = one;
+    return;
+  }
+  const long r1 = e1 / a.d;
+  for (long r = e0 / a.d + b; r < r1; r += nb) {
+    long c = 8 * (long)threadIdx.x;
+    for (; c + 8 <= a.d; c += 8 * blockDim.x) row8_store<O>(de + r * a.lde + c, eight);
+    for (; c < a.d; ++c) de[r * a.lde + c] = one;
   }
 }
-
+// Zeros in part `i` of `n` of dE's rows.
+template <class O>
+__device__ __forceinline__ void clear(const EmbedView& a, int i, int n, long b, long nb) {
+  if (b < nb) fill<O>(a, a.v * i / n * a.d, a.v * (i + 1) / n * a.d, b, nb, 0.0f);
+}
 // dE = NaN throughout, by all workgroups of a launch (an id outside 0..v).
 template <class O>
 __device__ void poison(const EmbedView& a, long b, long nb) {
-  const long per = (a.v + nb - 1) / nb;
-  fill_rows<O>(a, min(a.v, b * per), min(a.v, (b + 1) * per), nullptr, __builtin_nanf(""));
+  fill<O>(a, 0, a.v * a.d, b, nb, __builtin_nanf(""));
 }
 
-// A finished sum of eight columns into dE: the only rounding.
-template <class O>
+// A finished sum of eight columns into dE: the only rounding. ALL: all eight are there.
+template <class O, bool ALL>
 __device__ __forceinline__ void finish8(const EmbedView& a, uint32_t row, long c, const float* sum) {
   auto* p = static_cast<typename Row8<O>::stored*>(a.de) + row * a.lde + c;
+  const int n = ALL ? 8 : (int)(a.d - c);
   Row8<O> r;
   if (a.add) {
-    r = row8_load<O>(p, a.d - c);
+    if constexpr (ALL) r = row8_load<O>(p);
+    else r = row8_load<O>(p, n);
 #pragma unroll
     for (int i = 0; i < 8; ++i) r.set(i, __builtin_fmaf(a.scale, sum[i], r.get(i)));
   } else {
 #pragma unroll
     for (int i = 0; i < 8; ++i) r.set(i, a.scale * sum[i]);
   }
-  row8_store<O>(p, a.d - c, r);
+  if constexpr (ALL) row8_store<O>(p, r);
+  else row8_store<O>(p, r, n);
+}
+template <class T, bool ALL>
+__device__ __forceinline__ Row8<T> load8(const EmbedView& a, long row, long c) {
+  const uint16_t* p = a.dy + row * a.lddy + c;
+  if constexpr (ALL) return row8_load<T>(p);
+  else return row8_load<T>(p, (int)(a.d - c));
+}
+
+template <class O>
+__global__ __launch_bounds__(512) void k_embed_clear(EmbedView a) {
+  clear<O>(a, 0, 1, block_id(), (long)gridDim.x * gridDim.y);
 }
 
 // ---------------------------------------------------------------- few tokens
-// Workgroups below t slabs: token b / slabs, 8 x 256 columns. The others clear `rows` rows each.
+// Workgroup b: token b / slabs, 8 x 256 columns.
 template <class T, class O>
-__global__ __launch_bounds__(256) void k_embed_few(EmbedView a, int slabs, long sums, int rows) {
+__global__ __launch_bounds__(256) void k_embed_few(EmbedView a, int slabs) {
   __shared__ u64 same[kFewIds / 64], bad[kFewIds / 64];
-  __shared__ uint8_t has[1024];
   const long b = block_id();
   const int wv = threadIdx.x >> 6, lane = threadIdx.x & 63;
-  const long blocks = sums + (a.add ? 0 : (a.v + rows - 1) / rows);
-  if (b >= blocks) return;
-  const bool sum = b < sums;
-  const int tok = sum ? (int)(b / slabs) : 0;
-  const long r0 = sum ? 0 : (b - sums) * rows;
-  if (!sum)
-    for (int i = threadIdx.x; i < rows; i += 256) has[i] = 0;
-  __syncthreads();
-  const uint32_t v = (uint32_t)a.v;
-  const uint32_t own = sum ? id_key(a.ids[tok], a.ignore, v) : 0;
+  if (b >= a.t * slabs) return;
+  const int tok = (int)(b / slabs);
+  const uint32_t v = (uint32_t)a.v, own = id_key(a.ids[tok], a.ignore, v);
   for (int w = wv; 64 * w < a.t; w += 4) {
     const int i = 64 * w + lane;
     const uint32_t k = i < a.t ? id_key(a.ids[i], a.ignore, v) : v;
     const u64 s = __ballot(i < a.t && k == own), n = __ballot(k > v);
     if (lane == 0) same[w] = s, bad[w] = n;
-    if (!sum && k >= r0 && k < min((long)v, r0 + rows)) has[k - r0] = 1;
   }
   __syncthreads();
   const int words = (int)((a.t + 63) / 64);
   u64 any = 0;
   for (int w = 0; w < words; ++w) any |= bad[w];
-  if (any) return poison<O>(a, b, blocks);
-  if (!sum) return fill_rows<O>(a, r0, min(a.v, r0 + rows), has, 0.0f);
+  if (any) return poison<O>(a, b, a.t * slabs);
   if (own >= v) return;
   for (int w = 0; w <= tok / 64; ++w)
     if (same[w] & (w < tok / 64 ? ~0ull : (1ull << (tok & 63)) - 1)) return;  // an earlier token sums them
   const long c = ((b - (long)tok * slabs) * 256 + threadIdx.x) * 8;
   if (c >= a.d) return;
-  float acc[8] = {};
-  int w = tok / 64;
-  u64 left = same[w];
-  while (true) {  // eight rows' loads together
-    int at[8];
+  auto sum = [&](auto all) {
+    constexpr bool ALL = decltype(all)::value;
+    float acc[8] = {};
+    int w = tok / 64;
+    u64 left = same[w];
+    while (true) {  // eight rows' loads together
+      int at[8];
 #pragma unroll
-    for (int k = 0; k < 8; ++k) {
-      while (!left && w + 1 < words) left = same[++w];
-      at[k] = left ? 64 * w + __builtin_ctzll(left) : -1;
-      left &= left - 1;
+      for (int k = 0; k < 8; ++k) {
+        while (!left && w + 1 < words) left = same[++w];
+        at[k] = left ? 64 * w + __builtin_ctzll(left) : -1;
+        left &= left - 1;
+      }
+      Row8<T> x[8];
+#pragma unroll
+      for (int k = 0; k < 8; ++k)
+        if (at[k] >= 0) x[k] = load8<T, ALL>(a, at[k], c);
+#pragma unroll
+      for (int k = 0; k < 8; ++k)
+        if (at[k] >= 0)
+#pragma unroll
+          for (int i = 0; i < 8; ++i) acc[i] += x[k].get(i);
+      if (at[7] < 0) break;
     }
-    Row8<T> x[8];
-#pragma unroll
-    for (int k = 0; k < 8; ++k)
-      if (at[k] >= 0) x[k] = row8_load<T>(a.dy + at[k] * a.lddy + c, a.d - c);
-#pragma unroll
-    for (int k = 0; k < 8; ++k)
-      if (at[k] >= 0)
-#pragma unroll
-        for (int i = 0; i < 8; ++i) acc[i] += x[k].get(i);
-    if (at[7] < 0) break;
-  }
-  finish8<O>(a, own, c, acc);
+    finish8<O, ALL>(a, own, c, acc);
+  };
+  if (c + 8 <= a.d) sum(std::true_type{});
+  else sum(std::false_type{});
 }
 
 // ---------------------------------------------------------------- places of the sorted tokens
@@ -192,15 +218,12 @@ __global__ __launch_bounds__(256) void k_embed_few(EmbedView a, int slabs, long 
 // workgroup's own tokens an equal id counts, behind them it does not. Workgroups from `ranks` on clear dE.
 template <class O>
 __global__ __launch_bounds__(1024) void k_embed_rank(EmbedView a, long ranks, long fills, uint32_t* __restrict__ keys,
-                                                     int* __restrict__ order) {
+                                                     int* __restrict__ order, uint32_t* __restrict__ runs) {
   __shared__ uint32_t key[kRankedIds];
   __shared__ int part[16][64];
   const long b = block_id();
-  if (b >= ranks) {
-    const long f = b - ranks, per = (a.v + fills - 1) / fills;
-    if (f < fills) fill_rows<O>(a, min(a.v, f * per), min(a.v, (f + 1) * per), nullptr, 0.0f);
-    return;
-  }
+  if (b >= ranks) return clear<O>(a, 0, 1, b - ranks, fills);
+  if (b == 0 && threadIdx.x == 0) *runs = 0;
   const int t = (int)a.t, t0 = (int)b * 64, lane = threadIdx.x & 63, wv = threadIdx.x >> 6;
   const int seg = (t + 63) / 64 * 4;  // a multiple of 4; 16 of them hold all
   for (int i = threadIdx.x; i < 16 * seg; i += 1024)
@@ -232,67 +255,83 @@ __global__ __launch_bounds__(1024) void k_embed_rank(EmbedView a, long ranks, lo
   }
 }
 
-// Digits of the first pass counted by tile, hist[tile][digit]; the next pass's counts cleared. Workgroups from
-// `tiles` on clear dE.
+// One pass of the radix sort is two launches. Each clears a share of dE beside it, by the workgroups from `tiles` on.
+struct SortPass {
+  int tiles, bits, shift;
+  int launch, launches;  // for the clearing
+  long fills;
+  uint32_t* hist;  // [tile][digit]
+  const uint32_t* keys;  // null: the ids themselves
+  const int* order;
+  uint32_t* keys_to;
+  int* order_to;
+  uint32_t* runs;
+};
+
+// The ids of each digit by tile.
 template <class O>
-__global__ __launch_bounds__(512) void k_embed_count(EmbedView a, long tiles, long fills, int bits,
-                                                     uint32_t* __restrict__ hist, uint32_t* __restrict__ next) {
+__global__ __launch_bounds__(512) void k_embed_count(EmbedView a, SortPass p) {
   __shared__ uint32_t n[512];
   const long b = block_id();
-  if (b >= tiles) {
-    const long f = b - tiles, per = (a.v + fills - 1) / fills;
-    if (f < fills) fill_rows<O>(a, min(a.v, f * per), min(a.v, (f + 1) * per), nullptr, 0.0f);
-    return;
-  }
+  if (b >= p.tiles) return clear<O>(a, p.launch, p.launches, b - p.tiles, p.fills);
+  if (b == 0 && threadIdx.x == 0) *p.runs = 0;
   n[threadIdx.x] = 0;
   __syncthreads();
-  const int digits = 1 << bits;
+  const int digits = 1 << p.bits;
+#pragma unroll
   for (int k = 0; k < kTile / 512; ++k) {
     const long i = b * kTile + k * 512 + threadIdx.x;
-    if (i < a.t) atomicAdd(&n[id_key(a.ids[i], a.ignore, (uint32_t)a.v) & (digits - 1)], 1u);
+    if (i < a.t) {
+      const uint32_t key = p.keys ? p.keys[i] : id_key(a.ids[i], a.ignore, (uint32_t)a.v);
+      atomicAdd(&n[(key >> p.shift) & (digits - 1)], 1u);
+    }
   }
   __syncthreads();
-  if ((int)threadIdx.x < digits) {
-    hist[b * digits + threadIdx.x] = n[threadIdx.x];
-    next[b * digits + threadIdx.x] = 0;
-  }
+  if ((int)threadIdx.x < digits) p.hist[b * digits + threadIdx.x] = n[threadIdx.x];
 }
 
-// One pass of the radix sort, stable: a workgroup of 8 wavefronts moves a tile, each wavefront 512 neighbouring
-// ids in 8 rounds of 64. A round's lanes of one digit find each other by a ballot for each bit. The digits' places
-// are summed from all tiles' counts by every workgroup (a scan of its own would be a launch more). `next`:
-// the next pass's counts, by the places' tiles (whole numbers: any order gives the same), `clear` the ones after.
-template <bool FIRST>
-__global__ __launch_bounds__(512) void k_embed_sort(EmbedView a, int tiles, int bits, int shift,
-                                                    const uint32_t* __restrict__ hist, const uint32_t* __restrict__ keys,
-                                                    const int* __restrict__ order, uint32_t* __restrict__ keys_to,
-                                                    int* __restrict__ order_to, uint32_t* __restrict__ next,
-                                                    uint32_t* __restrict__ clear) {
+// Stable: a workgroup of 8 wavefronts moves a tile, each wavefront 256 neighbouring ids in 4 rounds of 64. A round's
+// lanes of one digit find each other by a ballot for each bit. The digits' places are summed from all tiles' counts by
+// every workgroup (a scan of its own would be a launch more).
+template <class O>
+__global__ __launch_bounds__(512) void k_embed_sort(EmbedView a, SortPass p) {
   __shared__ uint32_t place[8][512];
   __shared__ uint32_t scan[8];
-  const int wv = threadIdx.x >> 6, lane = threadIdx.x & 63, digits = 1 << bits;
-  const long base = (long)blockIdx.x * kTile + wv * 512;
-  uint32_t key[8];
-  int tok[8], rank[8];
+  if (block_id() >= p.tiles) return clear<O>(a, p.launch, p.launches, block_id() - p.tiles, p.fills);
+  constexpr int R = kTile / 512;
+  const int wv = threadIdx.x >> 6, lane = threadIdx.x & 63, digits = 1 << p.bits;
+  const long tile = block_id(), base = tile * kTile + wv * (64 * R);
+  uint32_t key[R];
+  int tok[R], rank[R];
 #pragma unroll
-  for (int k = 0; k < 8; ++k) {
+  for (int k = 0; k < R; ++k) {
     const long i = base + 64 * k + lane;
     key[k] = ~0u, tok[k] = 0;
     if (i < a.t) {
-      key[k] = FIRST ? id_key(a.ids[i], a.ignore, (uint32_t)a.v) : keys[i];
-      tok[k] = FIRST ? (int)i : order[i];
+      key[k] = p.keys ? p.keys[i] : id_key(a.ids[i], a.ignore, (uint32_t)a.v);
+      tok[k] = p.keys ? p.order[i] : (int)i;
     }
   }
 #pragma unroll
   for (int w = 0; w < 8; ++w) place[w][threadIdx.x] = 0;
+  // the digit's tokens in all tiles, and in the tiles before this one
+  uint32_t all = 0, before = 0;
+  if ((int)threadIdx.x < digits) {
+#pragma unroll 16
+    for (int i = 0; i < p.tiles; ++i) {
+      const uint32_t c = p.hist[(long)i * digits + threadIdx.x];
+      all += c;
+      before += i < tile ? c : 0;
+    }
+  }
   __syncthreads();
   volatile uint32_t* mine = place[wv];
 #pragma unroll
-  for (int k = 0; k < 8; ++k) {
+  for (int k = 0; k < R; ++k) {
     const bool on = base + 64 * k + lane < a.t;
-    const uint32_t digit = (key[k] >> shift) & (digits - 1);
+    const uint32_t digit = (key[k] >> p.shift) & (digits - 1);
     u64 peers = __ballot(on);
-    for (int j = 0; j < bits; ++j) {
+    for (int j = 0; j < p.bits; ++j) {
       const u64 ones = __ballot((digit >> j) & 1);
       peers &= (digit >> j) & 1 ? ones : ~ones;
     }
@@ -303,17 +342,6 @@ __global__ __launch_bounds__(512) void k_embed_sort(EmbedView a, int tiles, int 
     if (on && r == 0) mine[digit] = old + (uint32_t)__popcll(peers);
     __builtin_amdgcn_wave_barrier();
     rank[k] = (int)old + r;
-  }
-  // the digit's tokens in all tiles, and in the tiles before this one
-  uint32_t all = 0, before = 0;
-  if ((int)threadIdx.x < digits) {
-#pragma unroll 8
-    for (int i = 0; i < tiles; ++i) {
-      const uint32_t c = hist[(long)i * digits + threadIdx.x];
-      all += c;
-      before += i < (int)blockIdx.x ? c : 0;
-    }
-    if (clear) clear[(long)blockIdx.x * digits + threadIdx.x] = 0;
   }
   uint32_t sum = all;  // of the digits up to this one
 #pragma unroll
@@ -333,122 +361,137 @@ __global__ __launch_bounds__(512) void k_embed_sort(EmbedView a, int tiles, int 
   }
   __syncthreads();
 #pragma unroll
-  for (int k = 0; k < 8; ++k) {
+  for (int k = 0; k < R; ++k) {
     if (base + 64 * k + lane >= a.t) continue;
-    const uint32_t to = place[wv][(key[k] >> shift) & (digits - 1)] + rank[k];
-    keys_to[to] = key[k];
-    order_to[to] = tok[k];
-    if (next) atomicAdd(&next[(long)(to / kTile) * digits + ((key[k] >> (shift + bits)) & (digits - 1))], 1u);
+    const uint32_t to = place[wv][(key[k] >> p.shift) & (digits - 1)] + rank[k];
+    p.keys_to[to] = key[k];
+    p.order_to[to] = tok[k];
   }
 }
 
 // ---------------------------------------------------------------- sums of the sorted tokens
+// The sorted tokens, and where the sums of runs that pass a chunk's end are kept: rows of dp columns.
+struct Sorted {
+  const uint32_t* keys;
+  const int* order;
+  int chunk;
+  long chunks, dp;
+  float *head, *tail;
+  uint32_t *runs, *starts;  // how many such runs, and the chunks where they begin, in any order
+};
+
 // `lanes` lanes take a chunk of the sorted tokens and 8 columns each. A run of equal ids that begins and ends in the
 // chunk is finished here; one that came from the chunk before leaves its sum in head[chunk], one that goes on into
 // the next in tail[chunk] (head if it came, too).
 template <class T, class O>
-__global__ __launch_bounds__(256) void k_embed_sums(EmbedView a, const uint32_t* __restrict__ keys,
-                                                    const int* __restrict__ order, int chunk, long chunks, long parts,
-                                                    float* __restrict__ head, float* __restrict__ tail) {
+__global__ __launch_bounds__(256) void k_embed_sums(EmbedView a, Sorted s, long parts) {
   const long unit = block_id() * (256 / a.lanes) + threadIdx.x / a.lanes;
-  if (unit >= chunks * parts) return;
+  if (unit >= s.chunks * parts) return;
   const long ch = unit / parts, c = ((unit - ch * parts) * a.lanes + (threadIdx.x & (a.lanes - 1))) * 8;
   if (c >= a.d) return;
-  const long p0 = ch * chunk, p1 = min(a.t, p0 + chunk);
+  const long p0 = ch * s.chunk, p1 = min(a.t, p0 + s.chunk);
   const uint32_t v = (uint32_t)a.v;
-  bool came = p0 > 0 && keys[p0 - 1] == keys[p0];
-  uint32_t cur = keys[p0];
-  float acc[8] = {};
-  auto part = [&](float* to) {
-    float* p = to + ch * a.d + c;
+  auto sum = [&](auto all) {
+    constexpr bool ALL = decltype(all)::value;
+    bool came = p0 > 0 && s.keys[p0 - 1] == s.keys[p0];
+    uint32_t cur = s.keys[p0];
+    float acc[8] = {};
+    auto part = [&](float* to) {
+      float* p = to + ch * s.dp + c;
+      *reinterpret_cast<float4*>(p) = make_float4(acc[0], acc[1], acc[2], acc[3]);
+      *reinterpret_cast<float4*>(p + 4) = make_float4(acc[4], acc[5], acc[6], acc[7]);
+    };
+    for (long p = p0; p < p1 && cur < v; p += 8) {
+      uint32_t k[8];
+      Row8<T> x[8];
 #pragma unroll
-    for (int i = 0; i < 8; ++i)
-      if (c + i < a.d) p[i] = acc[i];
-  };
-  for (long p = p0; p < p1 && cur < v; p += 8) {
-    uint32_t k[8];
-    Row8<T> x[8];
-#pragma unroll
-    for (int j = 0; j < 8; ++j) {
-      k[j] = p + j < p1 ? keys[p + j] : v;
-      if (k[j] < v) x[j] = row8_load<T>(a.dy + (long)order[p + j] * a.lddy + c, a.d - c);
-    }
-#pragma unroll
-    for (int j = 0; j < 8; ++j) {
-      if (p + j >= p1 || cur >= v) continue;
-      if (k[j] != cur) {
-        if (came) part(head);
-        else finish8<O>(a, cur, c, acc);
-        came = false;
-        cur = k[j];
-#pragma unroll
-        for (int i = 0; i < 8; ++i) acc[i] = 0.0f;
+      for (int j = 0; j < 8; ++j) {
+        const long i = min(p + j, p1 - 1);
+        k[j] = s.keys[i];
+        x[j] = load8<T, ALL>(a, s.order[i], c);
       }
-      if (cur < v)
+#pragma unroll
+      for (int j = 0; j < 8; ++j) {
+        if (p + j >= p1 || cur >= v) continue;
+        if (k[j] != cur) {
+          if (came) part(s.head);
+          else finish8<O, ALL>(a, cur, c, acc);
+          came = false;
+          cur = k[j];
+#pragma unroll
+          for (int i = 0; i < 8; ++i) acc[i] = 0.0f;
+        }
 #pragma unroll
         for (int i = 0; i < 8; ++i) acc[i] += x[j].get(i);
+      }
     }
-  }
-  if (cur >= v) return;
-  if (came) part(head);
-  else if (p1 < a.t && keys[p1] == cur) part(tail);
-  else finish8<O>(a, cur, c, acc);
+    if (cur >= v) return;
+    if (came) {
+      part(s.head);
+    } else if (p1 < a.t && s.keys[p1] == cur) {
+      part(s.tail);
+      if (c == 0) s.starts[atomicAdd(s.runs, 1u)] = (uint32_t)ch;
+    } else {
+      finish8<O, ALL>(a, cur, c, acc);
+    }
+  };
+  if (c + 8 <= a.d) sum(std::true_type{});
+  else sum(std::false_type{});
 }
 
-// A run that passes the end of the chunk where it began: its parts summed in order, a quarter of them each
-// wavefront, 256 columns a workgroup.
+// The runs that pass the end of the chunk where they began, each by 256 columns a workgroup: their parts summed in
+// order, a quarter of them each wavefront.
 template <class O>
-__global__ __launch_bounds__(256) void k_embed_join(EmbedView a, const uint32_t* __restrict__ keys, int chunk,
-                                                    long chunks, long slabs, const float* __restrict__ head,
-                                                    const float* __restrict__ tail) {
+__global__ __launch_bounds__(256) void k_embed_join(EmbedView a, Sorted s, uint32_t slabs) {
   __shared__ float red[4][256];
-  const long b = block_id(), v = a.v;
-  if (keys[a.t - 1] > v) return poison<O>(a, b, (long)gridDim.x * gridDim.y);
-  if (b >= chunks * slabs) return;
-  const long ch = b / slabs, end = (ch + 1) * chunk;
-  if (end >= a.t) return;
-  const uint32_t k = keys[end - 1];
-  if (k >= v || keys[end] != k) return;
-  if (ch > 0 && keys[ch * chunk - 1] == k) return;  // it began before
+  const long b = block_id(), nb = (long)gridDim.x * gridDim.y;
+  if (s.keys[a.t - 1] > a.v) return poison<O>(a, b, nb);
   const int wv = threadIdx.x >> 6, lane = threadIdx.x & 63;
-  long last = ch + 1;  // the chunk where it ends
-  while (true) {
-    const long at = (last + lane + 1) * chunk;
-    const u64 on = __ballot(at < a.t && keys[at] == k && keys[at - 1] == k);
-    if (~on) {
-      last += __builtin_ctzll(~on);
-      break;
+  const long items = (long)*s.runs * slabs;
+  for (long it = b; it < items; it += nb) {
+    const long run = it / slabs, slab = it - run * slabs, ch = s.starts[run];
+    const uint32_t k = s.keys[(ch + 1) * s.chunk];
+    long last = ch + 1;  // the chunk where it ends
+    while (true) {
+      const long at = (last + lane + 1) * s.chunk;
+      const u64 on = __ballot(at < a.t && s.keys[at] == k);
+      if (~on) {
+        last += __builtin_ctzll(~on);
+        break;
+      }
+      last += 64;
     }
-    last += 64;
-  }
-  const long n = last - ch, c = (b - ch * slabs) * 256 + 4 * lane;
-  const long from = ch + 1 + n * wv / 4, to = ch + 1 + n * (wv + 1) / 4;
-  float s[4] = {};
+    const long n = last - ch, c = slab * 256 + 4 * lane;
+    const long from = ch + 1 + n * wv / 4, to = ch + 1 + n * (wv + 1) / 4;
+    float4 f = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
+    if (c < s.dp)
 #pragma unroll 8
-  for (long i = from; i < to; ++i)
+      for (long i = from; i < to; ++i) {
+        const float4 h = *reinterpret_cast<const float4*>(s.head + i * s.dp + c);
+        f.x += h.x, f.y += h.y, f.z += h.z, f.w += h.w;
+      }
+    *reinterpret_cast<float4*>(&red[wv][4 * lane]) = f;
+    __syncthreads();
+    const long c8 = slab * 256 + 8 * threadIdx.x;
+    if (threadIdx.x < 32 && c8 < a.d) {
+      float sum[8];
 #pragma unroll
-    for (int j = 0; j < 4; ++j)
-      if (c + j < a.d) s[j] += head[i * a.d + c + j];
+      for (int i = 0; i < 8; ++i) {
+        sum[i] = s.tail[ch * s.dp + c8 + i];
 #pragma unroll
-  for (int j = 0; j < 4; ++j) red[wv][4 * lane + j] = s[j];
-  __syncthreads();
-  if (threadIdx.x >= 32) return;
-  const long c8 = (b - ch * slabs) * 256 + 8 * threadIdx.x;
-  if (c8 >= a.d) return;
-  float sum[8];
-#pragma unroll
-  for (int i = 0; i < 8; ++i) {
-    sum[i] = c8 + i < a.d ? tail[ch * a.d + c8 + i] : 0.0f;
-#pragma unroll
-    for (int w = 0; w < 4; ++w) sum[i] += red[w][8 * threadIdx.x + i];
+        for (int w = 0; w < 4; ++w) sum[i] += red[w][8 * threadIdx.x + i];
+      }
+      if (c8 + 8 <= a.d) finish8<O, true>(a, k, c8, sum);
+      else finish8<O, false>(a, k, c8, sum);
+    }
+    __syncthreads();
   }
-  finish8<O>(a, k, c8, sum);
 }
 
 struct EmbedPlan {
-  int chunk, bits, passes;
-  long chunks, tiles;
-  size_t keys[2], order[2], hist[3], head, tail, bytes;
+  int chunk, bits, passes, tiles;
+  long chunks, dp;
+  size_t keys[2], order[2], hist, head, tail, runs, starts, bytes;
 };
 EmbedPlan embed_plan(long t, long d, long v) {
   EmbedPlan p = {};
@@ -465,8 +508,8 @@ EmbedPlan embed_plan(long t, long d, long v) {
     while ((v + 1) >> total) ++total;
     p.passes = (total + 8) / 9;
     p.bits = (total + p.passes - 1) / p.passes;
-    p.tiles = (t + kTile - 1) / kTile;
-    for (int i = 0; i < 3; ++i) p.hist[i] = take(4 * p.tiles << p.bits);
+    p.tiles = (int)((t + kTile - 1) / kTile);
+    p.hist = take((size_t)4 * p.tiles << p.bits);
   }
   // Chunks as long as leaves 4096 wavefronts (a wavefront reads 8 rows' 16 bytes a lane at once).
   const long waves = (d + 511) / 512 * t;
@@ -474,53 +517,57 @@ EmbedPlan embed_plan(long t, long d, long v) {
   while (p.chunk < 64 && waves / p.chunk > 8192) p.chunk *= 2;
   while ((t + p.chunk - 1) / p.chunk > 16384) p.chunk *= 2;
   p.chunks = (t + p.chunk - 1) / p.chunk;
-  p.head = take(4 * p.chunks * d);
-  p.tail = take(4 * p.chunks * d);
+  p.dp = (d + 7) / 8 * 8;
+  p.head = take(4 * p.chunks * p.dp);
+  p.tail = take(4 * p.chunks * p.dp);
+  p.runs = take(4);
+  p.starts = take(4 * p.chunks);
   return p;
 }
 
+// Workgroups that clear n elements of dE: 64 KB each, or as many as fill the card several times.
+long clearing(const EmbedView& a, long n) { return a.add ? 0 : std::max(1l, std::min(n / 32768, 4096l)); }
+
 template <class T, class O>
 hipError_t backward(hipStream_t st, EmbedView a, void* work) {
-  const bool clear = !a.add;
   if (a.t <= kFewIds) {
+    if (!a.add) k_embed_clear<O><<<launch_grid(clearing(a, a.v * a.d)), 512, 0, st>>>(a);
     const int slabs = (int)((a.d + 2047) / 2048);
-    // rows of 128 KB to a clearing workgroup, which looks at all ids once
-    const int rows = (int)std::max(1l, std::min(1024l, 65536 / a.d));
-    const long sums = a.t * slabs, fills = clear ? (a.v + rows - 1) / rows : 0;
-    k_embed_few<T, O><<<launch_grid(std::max(1l, sums + fills)), 256, 0, st>>>(a, slabs, sums, rows);
+    if (a.t) k_embed_few<T, O><<<launch_grid(a.t * slabs), 256, 0, st>>>(a, slabs);
     return hipGetLastError();
   }
   const EmbedPlan p = embed_plan(a.t, a.d, a.v);
   char* w = static_cast<char*>(work);
-  uint32_t *keys[2], *hist[3];
+  uint32_t* keys[2];
   int* order[2];
   for (int i = 0; i < 2; ++i) {
     keys[i] = reinterpret_cast<uint32_t*>(w + p.keys[i]);
     order[i] = reinterpret_cast<int*>(w + p.order[i]);
   }
-  for (int i = 0; i < 3; ++i) hist[i] = reinterpret_cast<uint32_t*>(w + p.hist[i]);
-  float *head = reinterpret_cast<float*>(w + p.head), *tail = reinterpret_cast<float*>(w + p.tail);
+  uint32_t* const runs = reinterpret_cast<uint32_t*>(w + p.runs);
   int at = 0;
   if (a.t <= kRankedIds) {
-    const long ranks = (a.t + 63) / 64, fills = clear ? std::min(a.v, 4096l) : 0;
-    k_embed_rank<O><<<launch_grid(ranks + fills), 1024, 0, st>>>(a, ranks, fills, keys[0], order[0]);
+    const long ranks = (a.t + 63) / 64, fills = clearing(a, a.v * a.d);
+    k_embed_rank<O><<<launch_grid(ranks + fills), 1024, 0, st>>>(a, ranks, fills, keys[0], order[0], runs);
   } else {
-    const long fills = clear ? std::min(a.v, 4096l) : 0;
-    k_embed_count<O><<<launch_grid(p.tiles + fills), 512, 0, st>>>(a, p.tiles, fills, p.bits, hist[0], hist[1]);
-    const int tiles = (int)p.tiles;
-    uint32_t* next = p.passes > 1 ? hist[1] : nullptr;
-    k_embed_sort<true><<<tiles, 512, 0, st>>>(a, tiles, p.bits, 0, hist[0], nullptr, nullptr, keys[0], order[0], next, hist[2]);
-    for (int i = 1; i < p.passes; ++i) {
-      next = i + 1 < p.passes ? hist[i + 1] : nullptr;
-      k_embed_sort<false><<<tiles, 512, 0, st>>>(a, tiles, p.bits, i * p.bits, hist[i], keys[at], order[at], keys[at ^ 1],
-                                                 order[at ^ 1], next, nullptr);
+    const int n = 2 * p.passes;
+    const long fills = clearing(a, a.v * a.d / n);
+    at = 1;
+    for (int i = 0; i < p.passes; ++i) {
+      SortPass s = {p.tiles, p.bits, i * p.bits, 2 * i, n, fills, reinterpret_cast<uint32_t*>(w + p.hist), i ? keys[at] : nullptr,
+                    order[at], keys[at ^ 1], order[at ^ 1], runs};
+      k_embed_count<O><<<launch_grid(p.tiles + fills), 512, 0, st>>>(a, s);
+      ++s.launch;
+      k_embed_sort<O><<<launch_grid(p.tiles + fills), 512, 0, st>>>(a, s);
       at ^= 1;
     }
   }
+  const Sorted s = {keys[at], order[at], p.chunk, p.chunks, p.dp, reinterpret_cast<float*>(w + p.head),
+                    reinterpret_cast<float*>(w + p.tail), runs, reinterpret_cast<uint32_t*>(w + p.starts)};
   const long parts = (a.d + 8l * a.lanes - 1) / (8l * a.lanes), units = p.chunks * parts, per = 256 / a.lanes;
-  k_embed_sums<T, O><<<launch_grid((units + per - 1) / per), 256, 0, st>>>(a, keys[at], order[at], p.chunk, p.chunks, parts, head, tail);
+  k_embed_sums<T, O><<<launch_grid((units + per - 1) / per), 256, 0, st>>>(a, s, parts);
   const long slabs = (a.d + 255) / 256;
-  k_embed_join<O><<<launch_grid(p.chunks * slabs), 256, 0, st>>>(a, keys[at], p.chunk, p.chunks, slabs, head, tail);
+  k_embed_join<O><<<(int)std::min(p.chunks * slabs, 2048l), 256, 0, st>>>(a, s, (uint32_t)slabs);
   return hipGetLastError();
 }
 

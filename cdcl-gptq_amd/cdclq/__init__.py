@@ -163,7 +163,8 @@ def lib() -> C.CDLL:
         "cdclq_grad_norm_device": ([vp, vp, sz, sz, vp, vp, sz, vp], i32),
         "cdclq_clip_grads_device": ([vp, vp, sz, sz, C.c_double, vp, vp, sz, vp], i32),
         "cdclq_constrain_logits_device": ([vp, vp, sz, sz, sz, i32, vp, sz, sz, vp, vp, vp, vp, vp, vp, vp, sz, vp, sz,
-                                           sz, vp, vp, sz, vp], i32),
+                                           sz, vp, vp, sz, vp, sz, vp], i32),
+        "cdclq_constrain_work_bytes": ([sz, sz, sz], sz),
         "cdclq_device_alloc": ([vp, sz, C.POINTER(vp)], i32),
         "cdclq_device_free": ([vp, vp], i32),
         "cdclq_memcpy_h2d": ([vp, vp, vp, sz], i32),
@@ -214,7 +215,8 @@ def exported_symbols() -> list[str]:
         "cdclq_adapter_linear_device", "cdclq_adapter_backward_device",
         "cdclq_vocab_loss_device", "cdclq_vocab_loss_backward_device",
         "cdclq_embed_device", "cdclq_embed_work_bytes", "cdclq_embed_backward_device", "cdclq_grad_work_bytes",
-        "cdclq_grad_norm_device", "cdclq_clip_grads_device", "cdclq_constrain_logits_device",
+        "cdclq_grad_norm_device", "cdclq_clip_grads_device", "cdclq_constrain_work_bytes",
+        "cdclq_constrain_logits_device",
     ]
 
 

@@ -7,11 +7,13 @@
 // its product with x rounded to f32 and to the output's type. 1e-6 keeps c finite, as trainers do it. A norm that
 // is NaN or infinite in f32 clips nothing (c = 1): the gradients stay as they are, for the caller to look at.
 //
-// Both passes are bound by memory. A workgroup takes a chunk of one tensor's part; the tensors' addresses come as the
-// launch's arguments, so that a captured call keeps them and none has to be copied to the GPU first. The first pass
-// leaves one f64 sum a chunk. Each workgroup of the second sums its part's chunks itself, all in the same order, while
-// its first loads are on their way: a launch between the two would cost more. In place nothing is read again where
-// c = 1.
+// Both passes are bound by memory. A part's elements, over all tensors, are chunks of 8192; a workgroup takes every
+// J-th of a part's, so that a part has J sums whatever its size, and each workgroup of the second pass adds them up
+// itself, all in the same order: a launch between the two would cost more. The second pass goes backwards, through what
+// the first one left in the last cache. In place nothing is read again where c = 1.
+// The tensors' addresses come as a launch's arguments, so that a captured call keeps them and the host has nothing to copy
+// or to wait for; sets of more than one launch takes are written to a table in the workspace by small launches first
+// (448 tensors of 84 MB: 113 us as three launches a pass, with the table 66).
 #include <hip/hip_runtime.h>
 
 #include <algorithm>
@@ -23,44 +25,55 @@
 namespace cdclq {
 namespace {
 
-// Tensors of one launch: their arguments keep below 4 KB.
-template <int N, bool OUT>
-struct ClipTensors {
-  const void* x[N];
-  void* out[OUT ? N : 1];
-  uint32_t n[N];      // elements of a part
-  uint32_t start[N];  // first workgroup
-  uint8_t kind[N];    // dtype of x, | 4: out is f32 whatever x is
+constexpr int kTensors = 150;           // of one launch: its arguments keep below 4 KB
+constexpr int kChunk = 8192;            // elements
+constexpr long kMostPart = 1l << 30;    // elements of a part that one entry of the tables takes
+constexpr long kMostSums = 2048;        // of all parts together, where parts have several: as many workgroups as run at once
+
+// One tensor, or a piece of it.
+struct ClipEntry {
+  const void* x;
+  void* out;
+  uint32_t n;      // elements of a part
+  uint32_t start;  // its first chunk among a part's
+  uint32_t kind;   // dtype of x, | 4: out is f32 whatever x is
+};
+
+// The tensors as a launch's arguments.
+struct ClipArgs {
+  const void* x[kTensors];
+  void* out[kTensors];
+  uint32_t n[kTensors], start[kTensors];
+  uint8_t kind[kTensors];
   int count;
 };
-typedef ClipTensors<200, false> NormTensors;
-typedef ClipTensors<144, true> OutTensors;
-static_assert(sizeof(NormTensors) < 3900 && sizeof(OutTensors) < 3900, "a launch's arguments");
-
-// Where a workgroup stands.
-struct ClipAt {
-  int tensor, part;
-  long slot;  // of its part's sums
-  long i0, i1;  // elements of the part
+static_assert(sizeof(ClipArgs) < 3900, "a launch's arguments");
+// The tensors in device memory, and the tensor of each chunk.
+struct ClipTable {
+  const ClipEntry* entries;
+  const uint32_t* who;
 };
-template <class S>
-__device__ __forceinline__ ClipAt clip_at(const S& s, uint32_t b, int parts, int log_chunk, long first) {
+
+__device__ __forceinline__ ClipEntry entry_of(const ClipArgs& s, uint32_t chunk) {
   const int lane = threadIdx.x & 63;
   int e = -1;
 #pragma unroll
-  for (int i = 0; i < (int)(sizeof(s.n) / 4 + 63) / 64; ++i) {
+  for (int i = 0; i < (kTensors + 63) / 64; ++i) {
     const int j = 64 * i + lane;
-    e += __popcll(__ballot(j < s.count && s.start[min(j, s.count - 1)] <= b));
+    e += __popcll(__ballot(j < s.count && s.start[min(j, s.count - 1)] <= chunk));
   }
   e = __builtin_amdgcn_readfirstlane(e);
-  const uint32_t n = s.n[e], per = (uint32_t)(((uint64_t)n + (1u << log_chunk) - 1) >> log_chunk);
-  const uint32_t in = b - s.start[e], part = in / per, ch = in - part * per;
-  ClipAt a;
-  a.tensor = e, a.part = (int)part;
-  a.slot = first + s.start[e] / (uint32_t)parts + ch;
-  a.i0 = (long)ch << log_chunk;
-  a.i1 = min((long)n, a.i0 + (1l << log_chunk));
-  return a;
+  return {s.x[e], s.out[e], s.n[e], s.start[e], s.kind[e]};
+}
+__device__ __forceinline__ ClipEntry entry_of(const ClipTable& s, uint32_t chunk) { return s.entries[s.who[chunk]]; }
+
+__global__ __launch_bounds__(256) void k_clip_table(const ClipArgs s, uint32_t base, ClipEntry* __restrict__ entries,
+                                                    uint32_t* __restrict__ who) {
+  for (int e = blockIdx.x; e < s.count; e += gridDim.x) {
+    const uint32_t chunks = (s.n[e] + kChunk - 1) / kChunk;
+    for (uint32_t i = threadIdx.x; i < chunks; i += 256) who[s.start[e] + i] = base + e;
+    if (threadIdx.x == 0) entries[base + e] = {s.x[e], s.out[e], s.n[e], s.start[e], s.kind[e]};
+  }
 }
 
 // Sum of v over 256 threads in a fixed order; all get it.
@@ -75,206 +88,193 @@ __device__ __forceinline__ double sum256(double v) {
   return v;
 }
 
+// The sum of the squares of elements [i0, i1), on to s.
 template <class T>
-__device__ __forceinline__ double squares(const void* base, long part, long n, long i0, long i1) {
-  const auto* x = static_cast<const typename Row8<T>::stored*>(base) + part * n;
-  double s = 0.0;
+__device__ __forceinline__ double squares(const void* base, long i0, long i1, double s) {
+  const auto* x = static_cast<const typename Row8<T>::stored*>(base);
   auto add = [&](float f) {
     const double v = (double)f;
     s = __builtin_fma(v, v, s);
   };
-  for (long i = i0 + 8 * threadIdx.x; i + 8 <= i1; i += 8192) {  // four steps' loads in flight
-    Row8<T> r[4];
+  Row8<T> r[kChunk / 2048];
+  const long i = i0 + 8 * threadIdx.x;
 #pragma unroll
-    for (int u = 0; u < 4; ++u)
-      if (i + 2048 * u + 8 <= i1) r[u] = row8_load<T>(x + i + 2048 * u);
+  for (int u = 0; u < kChunk / 2048; ++u)
+    if (i + 2048 * u + 8 <= i1) r[u] = row8_load<T>(x + i + 2048 * u);
 #pragma unroll
-    for (int u = 0; u < 4; ++u)
-      if (i + 2048 * u + 8 <= i1)
+  for (int u = 0; u < kChunk / 2048; ++u)
+    if (i + 2048 * u + 8 <= i1)
 #pragma unroll
-        for (int k = 0; k < 8; ++k) add(r[u].get(k));
-  }
-  const long i = i1 - ((i1 - i0) & 7) + threadIdx.x;  // the elements past the last eight
-  if (i < i1) add(Row8<T>::widen(x[i]));
+      for (int k = 0; k < 8; ++k) add(r[u].get(k));
+  const long last = i1 - ((i1 - i0) & 7) + threadIdx.x;  // the elements past the last eight
+  if (last < i1) add(Row8<T>::widen(x[last]));
   return s;
 }
 
-__global__ __launch_bounds__(256) void k_norm_parts(const NormTensors s, uint32_t blocks, int parts, int log_chunk,
-                                                    long first, long slots, double* __restrict__ sums) {
-  const uint32_t b = blockIdx.x;
-  if (b >= blocks) return;
-  const ClipAt a = clip_at(s, b, parts, log_chunk, first);
-  const void* x = s.x[a.tensor];
-  const long n = s.n[a.tensor];
-  double v;
-  switch (s.kind[a.tensor] & 3) {
-    case F32::kind: v = squares<F32>(x, a.part, n, a.i0, a.i1); break;
-    case F16::kind: v = squares<F16>(x, a.part, n, a.i0, a.i1); break;
-    default: v = squares<Bf16>(x, a.part, n, a.i0, a.i1); break;
+// Workgroup part * each + j: chunks j, j + each, ... of a part.
+template <class S>
+__global__ __launch_bounds__(256) void k_norm_parts(const S s, uint32_t chunks, uint32_t each, uint32_t sums_all,
+                                                    double* __restrict__ sums) {
+  const uint32_t b = blockIdx.x + blockIdx.y * gridDim.x;
+  if (b >= sums_all) return;
+  const uint32_t part = b / each;
+  double v = 0.0;
+  for (uint32_t c = b - part * each; c < chunks; c += each) {
+    const ClipEntry e = entry_of(s, c);
+    const long i0 = part * (long)e.n + (long)(c - e.start) * kChunk, i1 = min(i0 + kChunk, (part + 1) * (long)e.n);
+    switch (e.kind & 3) {
+      case F32::kind: v = squares<F32>(e.x, i0, i1, v); break;
+      case F16::kind: v = squares<F16>(e.x, i0, i1, v); break;
+      default: v = squares<Bf16>(e.x, i0, i1, v); break;
+    }
   }
   v = sum256(v);
-  if (threadIdx.x == 0) sums[a.part * slots + a.slot] = v;
+  if (threadIdx.x == 0) sums[b] = v;
 }
 
-// The norm of a part from its chunks' sums, by 256 threads.
-__device__ __forceinline__ double norm_of(const double* sums, long slots) {
+// The norm of a part from its sums, by 256 threads.
+__device__ __forceinline__ double norm_of(const double* sums, uint32_t n) {
   double v = 0.0;
 #pragma unroll 8
-  for (long i = threadIdx.x; i < slots; i += 256) v += sums[i];
+  for (uint32_t i = threadIdx.x; i < n; i += 256) v += sums[i];
   return __builtin_sqrt(sum256(v));
 }
 
-__global__ __launch_bounds__(256) void k_norm(const double* __restrict__ sums, long slots, float* __restrict__ norm) {
-  const double n = norm_of(sums + blockIdx.x * slots, slots);
+__global__ __launch_bounds__(256) void k_norm(const double* __restrict__ sums, uint32_t each, float* __restrict__ norm) {
+  const double n = norm_of(sums + blockIdx.x * (long)each, each);
   if (threadIdx.x == 0) norm[blockIdx.x] = (float)n;
 }
 
+// y = by x over elements [i0, i1).
 template <class T, class O>
-__device__ __forceinline__ void scaled(const void* from, void* to, const ClipAt& a, long n, const double* sums,
-                                       long slots, double most, float* norm) {
-  const auto* x = static_cast<const typename Row8<T>::stored*>(from) + a.part * n;
-  auto* y = static_cast<typename Row8<O>::stored*>(to) + a.part * n;
-  const bool place = from == to;
-  Row8<T> r[4];
-  auto load = [&](long i) {
+__device__ __forceinline__ void scaled(const void* from, void* to, long i0, long i1, float by) {
+  const auto* x = static_cast<const typename Row8<T>::stored*>(from);
+  auto* y = static_cast<typename Row8<O>::stored*>(to);
+  Row8<T> r[kChunk / 2048];
+  const long i = i0 + 8 * threadIdx.x;
 #pragma unroll
-    for (int u = 0; u < 4; ++u)
-      if (i + 2048 * u + 8 <= a.i1) r[u] = row8_load<T>(x + i + 2048 * u);
-  };
-  long i = a.i0 + 8 * threadIdx.x;
-  if (!place) load(i);
-  const double got = norm_of(sums, slots);
-  if (norm && threadIdx.x == 0) norm[a.part] = (float)got;
+  for (int u = 0; u < kChunk / 2048; ++u)
+    if (i + 2048 * u + 8 <= i1) r[u] = row8_load<T>(x + i + 2048 * u);
+#pragma unroll
+  for (int u = 0; u < kChunk / 2048; ++u) {
+    if (i + 2048 * u + 8 > i1) continue;
+    Row8<O> o;
+#pragma unroll
+    for (int k = 0; k < 8; ++k) o.set(k, by * r[u].get(k));
+    row8_store<O>(y + i + 2048 * u, o);
+  }
+  const long last = i1 - ((i1 - i0) & 7) + threadIdx.x;  // the elements past the last eight
+  if (last < i1) y[last] = Row8<O>::narrow(by * Row8<T>::widen(x[last]));
+}
+
+template <class S>
+__global__ __launch_bounds__(256) void k_clip(const S s, uint32_t chunks, uint32_t each, uint32_t sums_all,
+                                              const double* __restrict__ sums, double most, float* __restrict__ norm) {
+  const uint32_t b = blockIdx.x + blockIdx.y * gridDim.x;
+  if (b >= sums_all) return;
+  const uint32_t part = b / each, j = b - part * each;
+  const double got = norm_of(sums + part * (long)each, each);
+  if (j == 0 && threadIdx.x == 0) norm[part] = (float)got;
   float by = 1.0f;
   if (__builtin_isfinite((float)got)) by = (float)__builtin_fmin(1.0, most / (got + 1e-6));
-  if (place) {
-    if (by == 1.0f) return;
-    load(i);
-  }
-  while (i + 8 <= a.i1) {
-#pragma unroll
-    for (int u = 0; u < 4; ++u) {
-      if (i + 2048 * u + 8 > a.i1) continue;
-      Row8<O> o;
-#pragma unroll
-      for (int k = 0; k < 8; ++k) o.set(k, by * r[u].get(k));
-      row8_store<O>(y + i + 2048 * u, o);
+  if (j >= chunks) return;
+  for (uint32_t c = j + (chunks - 1 - j) / each * each;; c -= each) {
+    const ClipEntry e = entry_of(s, c);
+    const long i0 = part * (long)e.n + (long)(c - e.start) * kChunk, i1 = min(i0 + kChunk, (part + 1) * (long)e.n);
+    if (e.x != e.out || by != 1.0f) {
+      switch (e.kind) {
+        case F32::kind:
+        case F32::kind | 4: scaled<F32, F32>(e.x, e.out, i0, i1, by); break;
+        case F16::kind: scaled<F16, F16>(e.x, e.out, i0, i1, by); break;
+        case F16::kind | 4: scaled<F16, F32>(e.x, e.out, i0, i1, by); break;
+        case Bf16::kind: scaled<Bf16, Bf16>(e.x, e.out, i0, i1, by); break;
+        default: scaled<Bf16, F32>(e.x, e.out, i0, i1, by); break;
+      }
     }
-    i += 8192;
-    load(i);
-  }
-  i = a.i1 - ((a.i1 - a.i0) & 7) + threadIdx.x;  // the elements past the last eight
-  if (i < a.i1) y[i] = Row8<O>::narrow(by * Row8<T>::widen(x[i]));
-}
-
-__global__ __launch_bounds__(256) void k_clip(const OutTensors s, uint32_t blocks, int parts, int log_chunk, long first,
-                                              long slots, const double* __restrict__ sums, double most, float* norm) {
-  const uint32_t b = blockIdx.x;
-  if (b >= blocks) return;
-  const ClipAt a = clip_at(s, b, parts, log_chunk, first);
-  const void* x = s.x[a.tensor];
-  void* y = s.out[a.tensor];
-  const long n = s.n[a.tensor];
-  sums += a.part * slots;
-  if (a.slot) norm = nullptr;  // a part's first chunk says its norm
-  switch (s.kind[a.tensor]) {
-    case F32::kind:
-    case F32::kind | 4: return scaled<F32, F32>(x, y, a, n, sums, slots, most, norm);
-    case F16::kind: return scaled<F16, F16>(x, y, a, n, sums, slots, most, norm);
-    case F16::kind | 4: return scaled<F16, F32>(x, y, a, n, sums, slots, most, norm);
-    case Bf16::kind: return scaled<Bf16, Bf16>(x, y, a, n, sums, slots, most, norm);
-    default: return scaled<Bf16, F32>(x, y, a, n, sums, slots, most, norm);
+    if (c < each) return;
   }
 }
 
-constexpr long kMostPart = 1l << 30;    // elements of a part that one entry of the tables takes
-constexpr long kMostBlocks = 1l << 23;  // workgroups of a launch: its work-items keep below 2^32
-
+// What a call needs, from the tensors' sizes alone.
 struct ClipPlan {
-  int log_chunk;
-  long slots;  // chunks of a part, over all tensors
+  uint32_t entries, chunks;  // chunks of a part
+  uint32_t each, sums;       // sums of a part, and of all
+  size_t table, who, bytes;  // in the workspace, behind the sums; none where the arguments take all tensors
 };
-// Chunks of 4096 elements, or as long as leaves about 2048 of them: every workgroup of the second pass reads its part's
-// sums.
 ClipPlan clip_plan(const GradTensor* g, size_t n, int parts) {
-  long total = 0;
-  for (size_t i = 0; i < n; ++i) total += g[i].n;
-  ClipPlan p = {12, 0};
-  while (((total / parts >> p.log_chunk) > 2048 || total >> p.log_chunk > kMostBlocks / 2) && p.log_chunk < 30) ++p.log_chunk;
-  const long chunk = 1l << p.log_chunk;
-  for (size_t i = 0; i < n; ++i) {
-    const long e = g[i].n / parts, whole = e / kMostPart;  // a whole entry's chunks end with it
-    p.slots += whole * (kMostPart >> p.log_chunk) + (e - whole * kMostPart + chunk - 1) / chunk;
+  ClipPlan p = {};
+  for (size_t i = 0; i < n; ++i)
+    for (long e = g[i].n / parts; e > 0; e -= kMostPart) {
+      ++p.entries;
+      p.chunks += (uint32_t)((std::min(e, kMostPart) + kChunk - 1) / kChunk);
+    }
+  p.each = (uint32_t)std::max(1l, std::min((long)p.chunks, kMostSums / parts));
+  p.sums = p.each * (uint32_t)parts;
+  p.bytes = (8 * (size_t)p.sums + 255) / 256 * 256;
+  if (p.entries > kTensors) {
+    p.table = p.bytes;
+    p.who = p.table + ((size_t)p.entries * sizeof(ClipEntry) + 255) / 256 * 256;
+    p.bytes = p.who + ((size_t)p.chunks * 4 + 255) / 256 * 256;
   }
   return p;
 }
 
-// Fills tables of S with the tensors (those of one part only in pieces of kMostPart elements) and hands each to `go`.
-template <class S, bool OUT, class F>
-hipError_t each_table(const GradTensor* g, size_t n, int parts, const ClipPlan& p, F go) {
-  constexpr int N = sizeof(S::n) / 4;
-  S s;
+// Hands the tensors to `go`, as arguments or as a table.
+template <class F>
+hipError_t with_tensors(hipStream_t st, const GradTensor* g, size_t n, int parts, const ClipPlan& p, char* work, F go) {
+  ClipArgs s;
   s.count = 0;
-  long slot = 0, first = 0;
-  uint64_t blocks = 0;
-  auto flush = [&]() -> hipError_t {
-    if (!s.count) return hipSuccess;
-    go(s, (uint32_t)blocks, first);
-    first = slot;
-    blocks = 0;
+  uint32_t chunk = 0, base = 0;
+  ClipEntry* const entries = reinterpret_cast<ClipEntry*>(work + p.table);
+  uint32_t* const who = reinterpret_cast<uint32_t*>(work + p.who);
+  auto table = [&] {
+    k_clip_table<<<std::min(s.count, 128), 256, 0, st>>>(s, base, entries, who);
+    base += (uint32_t)s.count;
     s.count = 0;
-    return hipGetLastError();
   };
   for (size_t i = 0; i < n; ++i) {
     const long e = g[i].n / parts;
     const size_t size = g[i].dtype == CDCLQ_DTYPE_F32 ? 4 : 2, out_size = g[i].out_dtype == CDCLQ_DTYPE_F32 ? 4 : 2;
     for (long at = 0; at < e; at += kMostPart) {
-      const long len = std::min(kMostPart, e - at), per = (len + (1l << p.log_chunk) - 1) >> p.log_chunk;
-      if (s.count == N || blocks + (uint64_t)per * parts > (uint64_t)kMostBlocks) {
-        const hipError_t err = flush();
-        if (err != hipSuccess) return err;
-      }
+      if (s.count == kTensors) table();
+      const long len = std::min(kMostPart, e - at);
       const int k = s.count++;
       s.x[k] = static_cast<const char*>(g[i].x) + at * size;
-      if constexpr (OUT) s.out[k] = static_cast<char*>(g[i].out) + at * out_size;
+      s.out[k] = static_cast<char*>(g[i].out) + at * out_size;
       s.n[k] = (uint32_t)len;
-      s.start[k] = (uint32_t)blocks;
+      s.start[k] = chunk;
       s.kind[k] = (uint8_t)(g[i].dtype | (g[i].out_dtype == CDCLQ_DTYPE_F32 ? 4 : 0));
-      blocks += (uint64_t)per * parts;
-      slot += per;
+      chunk += (uint32_t)((len + kChunk - 1) / kChunk);
     }
   }
-  return flush();
-}
-
-hipError_t parts_of(hipStream_t st, const GradTensor* g, size_t n, int parts, const ClipPlan& p, double* sums) {
-  return each_table<NormTensors, false>(g, n, parts, p, [&](const NormTensors& s, uint32_t blocks, long first) {
-    k_norm_parts<<<blocks, 256, 0, st>>>(s, blocks, parts, p.log_chunk, first, p.slots, sums);
-  });
+  if (p.entries > kTensors) {
+    table();
+    go(ClipTable{entries, who});
+  } else {
+    go(s);
+  }
+  return hipGetLastError();
 }
 
 }  // namespace
 
-size_t clip_work_bytes(const GradTensor* g, size_t n, int parts) {
-  return (8 * (size_t)clip_plan(g, n, parts).slots * parts + 255) / 256 * 256;
-}
+size_t clip_work_bytes(const GradTensor* g, size_t n, int parts) { return clip_plan(g, n, parts).bytes; }
 
 hipError_t grad_norm(hipStream_t st, const GradTensor* g, size_t n, int parts, float* norm, void* work) {
   const ClipPlan p = clip_plan(g, n, parts);
-  const hipError_t e = parts_of(st, g, n, parts, p, static_cast<double*>(work));
-  if (e != hipSuccess) return e;
-  k_norm<<<parts, 256, 0, st>>>(static_cast<const double*>(work), p.slots, norm);
-  return hipGetLastError();
+  double* sums = static_cast<double*>(work);
+  return with_tensors(st, g, n, parts, p, static_cast<char*>(work), [&](const auto& s) {
+    k_norm_parts<<<launch_grid(p.sums), 256, 0, st>>>(s, p.chunks, p.each, p.sums, sums);
+    k_norm<<<parts, 256, 0, st>>>(sums, p.each, norm);
+  });
 }
 
 hipError_t clip_grads(hipStream_t st, const GradTensor* g, size_t n, int parts, double most, float* norm, void* work) {
   const ClipPlan p = clip_plan(g, n, parts);
-  if (p.slots == 0) return grad_norm(st, g, n, parts, norm, work);  // nothing but norms of 0
   double* sums = static_cast<double*>(work);
-  const hipError_t e = parts_of(st, g, n, parts, p, sums);
-  if (e != hipSuccess) return e;
-  return each_table<OutTensors, true>(g, n, parts, p, [&](const OutTensors& s, uint32_t blocks, long first) {
-    k_clip<<<blocks, 256, 0, st>>>(s, blocks, parts, p.log_chunk, first, p.slots, sums, most, norm);
+  return with_tensors(st, g, n, parts, p, static_cast<char*>(work), [&](const auto& s) {
+    k_norm_parts<<<launch_grid(p.sums), 256, 0, st>>>(s, p.chunks, p.each, p.sums, sums);
+    k_clip<<<launch_grid(p.sums), 256, 0, st>>>(s, p.chunks, p.each, p.sums, sums, most, norm);
   });
 }
 

@@ -24,22 +24,130 @@ namespace {
 
 constexpr uint32_t kPrompt = 1u << 31, kCount = (1u << 20) - 1, kBias = 2047u << 20;
 
+// Tokens of histories, counted once a slab, from which on they are sorted by slab first.
+constexpr long kMostScans = 1l << 22;
+
+// The histories' tokens by slab: those of request r and slab s at place[start[r][s]] up to start[r][s + 1], each its
+// place in the slab, | kPrompt.
+struct Binned {
+  const uint32_t *start, *place;
+};
+
+// A workgroup takes a request: counts, their running sum, and the tokens' places, in any order within a slab.
+__global__ __launch_bounds__(1024) void k_constrain_bin(ConstrainArgs a, int log_slab, int slabs, uint32_t* __restrict__ start,
+                                                        uint32_t* __restrict__ place) {
+  extern __shared__ __align__(16) uint32_t word[];  // a slab's count, then where its next token goes
+  __shared__ uint32_t sums[16];
+  const long row = blockIdx.x + (long)blockIdx.y * gridDim.x;
+  if (row >= a.r) return;
+  const int tid = threadIdx.x, lane = tid & 63, wv = tid >> 6;
+  for (int i = tid; i < slabs; i += 1024) word[i] = 0;
+  __syncthreads();
+  const int len = a.lengths ? max(0, min(a.lengths[row], a.width)) : a.width, prompt = a.prompts ? a.prompts[row] : 0;
+  const int64_t* h = a.history + row * a.ldh;
+  int64_t tok[8];
+  auto load = [&](int i0) {
+#pragma unroll
+    for (int u = 0; u < 8; ++u) tok[u] = i0 + 1024 * u < len ? h[i0 + 1024 * u] : -1;
+  };
+  auto is = [&](int u) { return (uint64_t)tok[u] < (uint64_t)a.v; };
+  // A history of one round's tokens stays in registers with what the counters held.
+  uint32_t rank[8];
+  for (int i0 = tid; i0 < len; i0 += 8192) {
+    load(i0);
+#pragma unroll
+    for (int u = 0; u < 8; ++u)
+      if (is(u)) rank[u] = atomicAdd(&word[(uint32_t)tok[u] >> log_slab], 1u);
+  }
+  __syncthreads();
+  uint32_t before = (uint32_t)(row * a.width);
+  for (int s0 = 0; s0 < slabs; s0 += 1024) {
+    const uint32_t n = s0 + tid < slabs ? word[s0 + tid] : 0;
+    uint32_t sum = n;
+#pragma unroll
+    for (int k = 1; k < 64; k <<= 1) {
+      const uint32_t up = (uint32_t)__shfl_up((int)sum, k);
+      if (lane >= k) sum += up;
+    }
+    if (lane == 63) sums[wv] = sum;
+    __syncthreads();
+    uint32_t all = 0;
+#pragma unroll
+    for (int w = 0; w < 16; ++w) {
+      if (w < wv) sum += sums[w];
+      all += sums[w];
+    }
+    if (s0 + tid < slabs) {
+      word[s0 + tid] = before + sum - n;
+      start[row * (slabs + 1) + s0 + tid] = before + sum - n;
+    }
+    before += all;
+    __syncthreads();
+  }
+  if (tid == 0) start[row * (slabs + 1) + slabs] = before;
+  const bool once = len <= 8192;
+  for (int i0 = tid; i0 < len; i0 += 8192) {
+    if (!once) load(i0);
+#pragma unroll
+    for (int u = 0; u < 8; ++u) {
+      if (!is(u)) continue;
+      uint32_t* const w = &word[(uint32_t)tok[u] >> log_slab];
+      place[once ? *w + rank[u] : atomicAdd(w, 1u)] = ((uint32_t)tok[u] & ((1u << log_slab) - 1)) | (i0 + 1024 * u < prompt ? kPrompt : 0);
+    }
+  }
+}
 
 // LDS: TH * 8 * K words if there is a history or a bias, then the biases' values and places.
 template <class T, int TH, int K, bool PLACE>
-__global__ __launch_bounds__(TH) void k_constrain(ConstrainArgs a, long rows8, int slabs) {
+__global__ __launch_bounds__(TH) void k_constrain(ConstrainArgs a, Binned bins, long rows8, int slabs) {
   extern __shared__ __align__(16) uint32_t word[];
   constexpr int SLAB = TH * 8 * K;
   // workgroup b: XCD b % 8 takes the requests of that remainder, slab by slab
   const long b = blockIdx.x + (long)blockIdx.y * gridDim.x, at = b >> 3;
   const long row = (at / slabs) * 8 + (b & 7);
   if (at >= rows8 * slabs || row >= a.r) return;
-  const int slab0 = (int)(at % slabs) * SLAB;  // 8 workgroups later the next slab
+  const int slab = (int)(at % slabs), slab0 = slab * SLAB;
   const auto* in = static_cast<const typename Row8<T>::stored*>(a.logits) + row * a.ld + slab0;
   auto* out = static_cast<typename Row8<T>::stored*>(a.out) + row * a.ldo + slab0;
   const int n = (int)min((long)SLAB, a.v - slab0);
   const bool marks = a.history || a.biases;
 
+  // Loads come back in the order in which they are asked for: the few that the counting waits for, then the logits.
+  uint32_t next = ~0u, end = 0;  // the slab's tokens, binned
+  int64_t tok[8];                // or the history's
+  int len = 0, prompt = 0;
+  const int64_t* h = a.history + row * a.ldh;
+  auto tokens = [&](int i0) {
+#pragma unroll
+    for (int u = 0; u < 8; ++u) tok[u] = i0 + u * TH < len ? (int64_t)((uint64_t)h[i0 + u * TH] - slab0) : -1;
+  };
+  if (bins.start) {
+    const uint32_t* s = bins.start + row * (slabs + 1) + slab;
+    end = s[1];
+    next = s[0] + threadIdx.x;
+  } else if (a.history) {
+    len = a.lengths ? max(0, min(a.lengths[row], a.width)) : a.width;
+    prompt = a.prompts ? a.prompts[row] : 0;
+    tokens(threadIdx.x);
+  }
+  uint32_t place = next < end ? bins.place[next] : 0;
+  const long mrow = a.mask_rows ? a.mask_rows[row] : a.mask ? row : -1;
+  const bool wrong = mrow < -1 || (mrow >= 0 && mrow >= a.masks);  // no such mask
+  const uint8_t* mask = mrow < 0 || wrong ? nullptr
+                                          : reinterpret_cast<const uint8_t*>(a.mask + mrow * a.ldm) + slab0 / 8;
+  int64_t btok = -1;  // a bias each lane of the first wavefront
+  float bval = 0.0f;
+  auto biases = [&](int i) {
+    btok = i < a.biases ? (int64_t)((uint64_t)a.bias_tokens[row * a.biases + i] - slab0) : -1;
+    bval = i < a.biases ? a.bias[row * a.biases + i] : 0.0f;
+  };
+  if (threadIdx.x < 64) biases(threadIdx.x);
+  uint8_t open[K];
+#pragma unroll
+  for (int k = 0; k < K; ++k) {
+    const int i = k * TH + (int)threadIdx.x;
+    open[k] = mask && 8 * i < n ? mask[i] : 0xff;
+  }
   Row8<T> x[K];
   if constexpr (!PLACE) {
 #pragma unroll
@@ -48,54 +156,59 @@ __global__ __launch_bounds__(TH) void k_constrain(ConstrainArgs a, long rows8, i
       if (i + 8 <= n) x[k] = row8_load<T>(in + i);
     }
   }
-  const long mrow = a.mask_rows ? a.mask_rows[row] : a.mask ? row : -1;
-  const bool wrong = mrow < -1 || (mrow >= 0 && mrow >= a.masks);  // no such mask
-  const uint8_t* mask = mrow < 0 || wrong ? nullptr
-                                          : reinterpret_cast<const uint8_t*>(a.mask + mrow * a.ldm) + slab0 / 8;
-  uint8_t open[K];
-#pragma unroll
-  for (int k = 0; k < K; ++k) {
-    const int i = k * TH + (int)threadIdx.x;
-    open[k] = mask && 8 * i < n ? mask[i] : 0xff;
-  }
   float* const bias = reinterpret_cast<float*>(word + SLAB);
   if (marks) {
-    int* const place = reinterpret_cast<int*>(bias + a.biases);
 #pragma unroll
     for (int k = 0; k < 2 * K; ++k) reinterpret_cast<uint4*>(word)[k * TH + threadIdx.x] = make_uint4(0, 0, 0, 0);
-    for (int i = threadIdx.x; i < a.biases; i += TH) {
-      const int64_t tok = a.bias_tokens[row * a.biases + i] - slab0;
-      place[i] = (uint64_t)tok < (uint64_t)n ? (int)tok : -1;
-    }
     __syncthreads();
-    if (a.history) {
-      const int len = a.lengths ? max(0, min(a.lengths[row], a.width)) : a.width;
-      const int prompt = a.prompts ? a.prompts[row] : 0;
-      const int64_t* h = a.history + row * a.ldh;
-      for (int i0 = threadIdx.x; i0 < len; i0 += 8 * TH) {
-        int64_t tok[8];
+    while (next < end) {
+      if (place & kPrompt) atomicOr(&word[place & ~kPrompt], kPrompt);
+      else atomicAdd(&word[place], 1u);
+      next += TH;
+      if (next < end) place = bins.place[next];
+    }
+    for (int i0 = threadIdx.x; i0 < len;) {
 #pragma unroll
-        for (int u = 0; u < 8; ++u) tok[u] = i0 + u * TH < len ? h[i0 + u * TH] - slab0 : -1;
-#pragma unroll
-        for (int u = 0; u < 8; ++u) {
-          if ((uint64_t)tok[u] >= (uint64_t)n) continue;
-          if (i0 + u * TH < prompt) atomicOr(&word[tok[u]], kPrompt);
-          else atomicAdd(&word[tok[u]], 1u);
+      for (int u = 0; u < 8; ++u) {
+        if ((uint64_t)tok[u] >= (uint64_t)n) continue;
+        if (i0 + u * TH < prompt) atomicOr(&word[tok[u]], kPrompt);
+        else atomicAdd(&word[tok[u]], 1u);
+      }
+      i0 += 8 * TH;
+      if (i0 < len) tokens(i0);
+    }
+    // The slab's biases: a wavefront lists them in their order; the first of a token's carries them all, summed.
+    if (a.biases && threadIdx.x < 64) {
+      const int lane = threadIdx.x;
+      int* const at = reinterpret_cast<int*>(bias + a.biases);
+      int m = 0;
+      for (int i0 = 0; i0 < a.biases; i0 += 64) {
+        if (i0) biases(i0 + lane);
+        const bool here = (uint64_t)btok < (uint64_t)n;
+        const unsigned long long on = __ballot(here);
+        if (here) {
+          const int j = m + __popcll(on & ((1ull << lane) - 1));
+          at[j] = (int)btok;
+          bias[j] = bval;
+        }
+        m += __popcll(on);
+      }
+      __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
+      for (int i0 = 0; i0 < m; i0 += 64) {
+        const int i = i0 + lane, p = i < m ? at[i] : -1;
+        bool first = i < m;
+        float s = 0.0f;
+        for (int j = 0; j < m; ++j) {
+          const bool same = at[j] == p;
+          first = first && !(same && j < i);
+          if (same) s += bias[j];
+        }
+        __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
+        if (first) {
+          bias[i] = s;
+          atomicOr(&word[p], (uint32_t)(i + 1) << 20);
         }
       }
-    }
-    // the first of a token's biases carries them all, summed in their order
-    for (int i = threadIdx.x; i < a.biases; i += TH) {
-      const int p = place[i];
-      if (p < 0) continue;
-      bool first = true;
-      for (int j = 0; j < i; ++j) first = first && place[j] != p;
-      if (!first) continue;
-      float s = a.bias[row * a.biases + i];
-      for (int j = i + 1; j < a.biases; ++j)
-        if (place[j] == p) s += a.bias[row * a.biases + j];
-      bias[i] = s;
-      atomicOr(&word[p], (uint32_t)(i + 1) << 20);
     }
     __syncthreads();
   }
@@ -131,10 +244,10 @@ __global__ __launch_bounds__(TH) void k_constrain(ConstrainArgs a, long rows8, i
     if (open[k] != 0xff)
 #pragma unroll
       for (int j = 0; j < 8; ++j)
-        if (!(open[k] >> j & 1)) x[k].set(j, -__builtin_inff());
+        if (!(open[k] >> j & 1)) x[k].v[j] = Row8<T>::narrow(-__builtin_inff());
     if (wrong)
 #pragma unroll
-      for (int j = 0; j < 8; ++j) x[k].set(j, __builtin_nanf(""));
+      for (int j = 0; j < 8; ++j) x[k].v[j] = Row8<T>::narrow(__builtin_nanf(""));
     row8_store<T>(out + i, x[k]);
   }
   const int i = (n & ~7) + (int)threadIdx.x;  // the tokens past the last eight
@@ -148,33 +261,62 @@ __global__ __launch_bounds__(TH) void k_constrain(ConstrainArgs a, long rows8, i
   }
 }
 
+// Tokens of a slab and threads of its workgroup: the largest that leaves 512 workgroups.
+struct SlabShape {
+  int threads, per;  // 8 per tokens a thread
+  int slab() const { return 8 * threads * per; }
+  int count(long v) const { return (int)((v + slab() - 1) / slab()); }
+};
+SlabShape slab_shape(long r, long v) {
+  const long tokens = r * v;
+  return tokens >= 512l * 8192 ? SlabShape{512, 2} : tokens >= 512l * 4096 ? SlabShape{256, 2} : SlabShape{128, 1};
+}
+
+// Whether the histories are sorted by slab in a launch before.
+bool binned(long r, long v, long width) {
+  return r * slab_shape(r, v).count(v) * width > kMostScans && r * width < (1l << 32);
+}
+
 template <class T, int TH, int K>
-hipError_t launch(hipStream_t st, const ConstrainArgs& a) {
+hipError_t launch(hipStream_t st, const ConstrainArgs& a, void* work) {
   constexpr int SLAB = TH * 8 * K;
   const int slabs = (int)((a.v + SLAB - 1) / SLAB);
   const long rows8 = (a.r + 7) / 8;
+  Binned bins = {};
+  if (a.history && binned(a.r, a.v, a.width)) {
+    uint32_t* start = static_cast<uint32_t*>(work);
+    uint32_t* place = start + a.r * (slabs + 1);
+    k_constrain_bin<<<launch_grid(a.r), 1024, 4 * slabs, st>>>(a, __builtin_ctz(SLAB), slabs, start, place);
+    bins = {start, place};
+  }
   const size_t lds = a.history || a.biases ? 4 * SLAB + 8 * (size_t)a.biases : 0;
   const dim3 grid = launch_grid(rows8 * slabs * 8);
-  if (a.logits == a.out) k_constrain<T, TH, K, true><<<grid, TH, lds, st>>>(a, rows8, slabs);
-  else k_constrain<T, TH, K, false><<<grid, TH, lds, st>>>(a, rows8, slabs);
+  if (a.logits == a.out) k_constrain<T, TH, K, true><<<grid, TH, lds, st>>>(a, bins, rows8, slabs);
+  else k_constrain<T, TH, K, false><<<grid, TH, lds, st>>>(a, bins, rows8, slabs);
   return hipGetLastError();
 }
 
 template <class T>
-hipError_t constrain(hipStream_t st, const ConstrainArgs& a) {
-  const long tokens = a.r * a.v;
-  if (tokens >= 512l * 8192) return launch<T, 512, 2>(st, a);
-  if (tokens >= 512l * 4096) return launch<T, 256, 2>(st, a);
-  return launch<T, 128, 1>(st, a);
+hipError_t constrain(hipStream_t st, const ConstrainArgs& a, void* work) {
+  switch (slab_shape(a.r, a.v).threads) {
+    case 512: return launch<T, 512, 2>(st, a, work);
+    case 256: return launch<T, 256, 2>(st, a, work);
+    default: return launch<T, 128, 1>(st, a, work);
+  }
 }
 
 }  // namespace
 
-hipError_t constrain_logits(hipStream_t st, int dtype, const ConstrainArgs& a) {
+size_t constrain_work_bytes(long r, long v, long width) {
+  if (!width || !binned(r, v, width)) return 0;
+  return (4 * (size_t)(r * (slab_shape(r, v).count(v) + 1) + r * width) + 255) / 256 * 256;
+}
+
+hipError_t constrain_logits(hipStream_t st, int dtype, const ConstrainArgs& a, void* work) {
   switch (dtype) {
-    case CDCLQ_DTYPE_BF16: return constrain<Bf16>(st, a);
-    case CDCLQ_DTYPE_F16: return constrain<F16>(st, a);
-    default: return constrain<F32>(st, a);
+    case CDCLQ_DTYPE_BF16: return constrain<Bf16>(st, a, work);
+    case CDCLQ_DTYPE_F16: return constrain<F16>(st, a, work);
+    default: return constrain<F32>(st, a, work);
   }
 }
 

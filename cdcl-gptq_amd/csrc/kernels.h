@@ -382,6 +382,7 @@ struct ConstrainArgs {
   void* out;
   long ldo;
 };
-hipError_t constrain_logits(hipStream_t st, int dtype, const ConstrainArgs& a);
+size_t constrain_work_bytes(long r, long v, long width);
+hipError_t constrain_logits(hipStream_t st, int dtype, const ConstrainArgs& a, void* work);
 
 }  // namespace cdclq

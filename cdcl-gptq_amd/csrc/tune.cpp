@@ -596,12 +596,17 @@ int cdclq_clip_grads_device(cdclq_ctx* ctx, const cdclq_grad* grads, size_t n, s
   return CDCLQ_OK;
 }
 
+size_t cdclq_constrain_work_bytes(size_t r, size_t v, size_t width) {
+  if (v == 0 || r > kMaxTokens || v > kMaxVocab || width >= (size_t)1 << 20) return 0;
+  return constrain_work_bytes((long)r, (long)v, (long)width);
+}
+
 int cdclq_constrain_logits_device(cdclq_ctx* ctx, const void* logits, size_t ld, size_t r, size_t v, int dtype,
                                   const int64_t* history, size_t ld_history, size_t width, const int32_t* lengths,
                                   const int32_t* prompts, const float* repetition, const float* frequency,
                                   const float* presence, const int64_t* bias_tokens, const float* biases, size_t nbias,
                                   const uint32_t* mask, size_t ld_mask, size_t nmasks, const int32_t* mask_rows,
-                                  void* out, size_t ldo, void* stream) {
+                                  void* out, size_t ldo, void* work, size_t work_bytes, void* stream) {
   if (!ctx) return CDCLQ_INVALID_ARG;
   ctx->err.clear();
   CK(check_type(ctx, dtype));
@@ -625,6 +630,7 @@ int cdclq_constrain_logits_device(cdclq_ctx* ctx, const void* logits, size_t ld,
   ConstrainArgs a = {};
   a.logits = logits;
   a.ld = (long)ld, a.r = (long)r, a.v = (long)v;
+  CK(check_work(ctx, work, work_bytes, constrain_work_bytes(a.r, a.v, (long)width)));
   a.history = width ? history : nullptr;
   a.ldh = (long)ld_history;
   a.width = (int)width;
@@ -640,7 +646,7 @@ int cdclq_constrain_logits_device(cdclq_ctx* ctx, const void* logits, size_t ld,
   a.ldo = (long)ldo;
   OnDevice on(ctx->device);
   HIPCK(on.err);
-  HIPCK(constrain_logits((hipStream_t)stream, dtype, a));
+  HIPCK(constrain_logits((hipStream_t)stream, dtype, a, work));
   return CDCLQ_OK;
 }
 

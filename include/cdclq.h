@@ -447,12 +447,13 @@ int cdclq_clip_grads_device(cdclq_ctx* ctx, const cdclq_grad* grads, size_t n, s
  * ld_mask), token i at bit i % 32 of word i / 32; mask_rows[i]: the request's row of it, -1 for none, any other value
  * outside 0..nmasks gives a row of NaN; NULL: row i (nmasks = r). out may be logits (with the same stride); it must not
  * overlap it otherwise. Logits that nothing applies to keep their bits. width < 2^20, nbias <= 1024. */
+size_t cdclq_constrain_work_bytes(size_t r, size_t v, size_t width);
 int cdclq_constrain_logits_device(cdclq_ctx* ctx, const void* logits, size_t ld, size_t r, size_t v, int dtype,
                                   const int64_t* history, size_t ld_history, size_t width, const int32_t* lengths,
                                   const int32_t* prompts, const float* repetition, const float* frequency,
                                   const float* presence, const int64_t* bias_tokens, const float* biases, size_t nbias,
                                   const uint32_t* mask, size_t ld_mask, size_t nmasks, const int32_t* mask_rows,
-                                  void* out, size_t ldo, void* stream);
+                                  void* out, size_t ldo, void* work, size_t work_bytes, void* stream);
 
 /* ---- Device memory staging for callers without their own GPU runtime binding. ---- */
 int cdclq_device_alloc(cdclq_ctx* ctx, size_t bytes, void** ptr);

@@ -89,7 +89,7 @@ def test_norm_and_clipping(ctx, tune, dtype, shapes, share):
         assert all(torch.equal(x, b) for x, b in zip(place, tensors))
 
 
-@pytest.mark.parametrize("count", [143, 144, 145, 200, 201, 448])
+@pytest.mark.parametrize("count", [149, 150, 151, 300, 301, 448])
 def test_many_tensors(ctx, tune, count):
     """More than one launch's tables hold; the three types side by side."""
     tensors = [normal(i, 3 + 37 * i % 901, 5, std=1 + i % 5, dtype=TYPES[i % 3]) for i in range(count)]

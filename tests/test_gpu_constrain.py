@@ -138,7 +138,7 @@ def check(got, want, bound, dtype):
 
 SIZES = [(1, 1, 1, 1, 1), (1, 31, 5, 2, 1), (3, 33, 40, 3, 2), (2, 1000, 0, 0, 2), (2, 1000, 100, 0, 0), (5, 1025, 0, 30, 0),
          (9, 5001, 300, 20, 3), (17, 8193, 2000, 300, 4), (1, 128256, 5000, 1024, 1), (70, 32000, 70, 5, 10),
-         (300, 16390, 33, 4, 7)]
+         (300, 16390, 33, 4, 7), (64, 40001, 9000, 100, 9), (3, 300_000, 20_000, 70, 2)]
 
 
 @pytest.mark.parametrize("dtype", TYPES)

@@ -17,8 +17,9 @@ def test_embed_workspace_sizes(d, v):
         n = L.cdclq_embed_work_bytes(t, d, v)
         assert n % 256 == 0
         assert n == 0 if t <= 512 else n >= 8 * t  # ids and places of the sorted tokens
-        # the runs that pass a chunk's end: at most two rows of float32 for eight tokens, and the tables
-        assert n <= 18 * t + 1024 * 12 * (t // 4096 + 1) + d * (t // 4 + 512) * 4 + 4096
+        # two sets of those, the runs that pass a chunk's end (two rows of float32 for eight tokens, padded to eight
+        # columns), the counts of 512 digits for 2048 tokens
+        assert n <= 17 * t + (d + 7) // 8 * 8 * (t // 8 + 1) * 8 + 2048 * (t // 2048 + 1) + 4096
 
 
 def test_sizes_outside_the_limits_ask_for_nothing():
@@ -34,14 +35,15 @@ def test_sizes_outside_the_limits_ask_for_nothing():
 
 @pytest.mark.parametrize("parts", [1, 8, 32768])
 def test_grad_workspace_holds_few_sums(parts):
-    """One 64-bit sum a chunk: about 2048 chunks of each part and one more a tensor at the most, over any sizes."""
-    for counts in ([0], [1] * 300, [1 << 20, 17, 0, 4096], [1 << 30] * 3, [(1 << 33) + 5, 1]):
+    """64-bit sums, 2048 or one for each part, and of more than 150 tensors a table and 4 bytes for 8192 elements of a
+    part, over any sizes."""
+    for counts in ([0], [1] * 150, [1] * 300, [1 << 20, 17, 0, 4096], [1 << 30] * 3, [(1 << 33) + 5, 1]):
         g = np.zeros(len(counts), GRAD)
         g["count"] = np.array(counts, np.uint64) // (1 if parts == 1 else 512) * parts
         n = L.cdclq_grad_work_bytes(g.ctypes.data, len(counts), parts)
-        held = sum(c > 0 for c in g["count"])
-        assert n % 256 == 0 and n >= 8 * parts * held
-        assert n <= 8 * parts * (2049 + 16 + len(counts)) + 256
+        chunks = sum(-(-int(c) // parts // 8192) + 1 for c in g["count"])
+        assert n % 256 == 0 and 8 * parts <= n <= 8 * max(2048, parts) + 256 + (len(counts) > 150) * (
+            32 * len(counts) + 4 * chunks + 512)
 
 
 def test_null_handles_are_refused():
@@ -52,7 +54,7 @@ def test_null_handles_are_refused():
     assert L.cdclq_grad_norm_device(None, 0, 0, 1, 0, 0, 0, 0) == bad
     assert L.cdclq_clip_grads_device(None, 0, 0, 1, 1.0, 0, 0, 0, 0) == bad
     assert L.cdclq_constrain_logits_device(None, 0, 8, 1, 8, cdclq.DTYPE_F32, 0, 0, 0, 0, 0, 0, 0, 0, 0, 0, 0, 0, 0, 0, 0, 0,
-                                           8, 0) == bad
+                                           8, 0, 0, 0) == bad
 
 
 # ---------------------------------------------------------------- the differentiable embedding

@@ -34,6 +34,7 @@ _CODES32 = {torch.float32: DTYPE_F32, **_CODES}
 
 
 _empty = torch.empty
+_data_ptr = torch.Tensor.data_ptr
 _current_stream = torch._C._cuda_getCurrentRawStream  # the handle alone: a Stream object costs a microsecond
 
 
@@ -393,15 +394,14 @@ class Gradients:
             codes.append((x.numel(), _CODES32[x.dtype], _CODES32[o.dtype]))
         if codes:
             self.table["count"], self.table["dtype"], self.table["out_dtype"] = zip(*codes)
-        self.at = None
+        self.all = self.tensors + (self.out or [])
+        self.at, self.device = None, torch.device("cuda", ctx.device)
         self._addresses()
         self.work_bytes = _L().cdclq_grad_work_bytes(self.table.ctypes.data, len(codes), self.parts)
 
     def _addresses(self) -> int:
         """The table's address, with the tensors' present addresses in it."""
-        at = [x.data_ptr() for x in self.tensors]
-        if self.out is not None:
-            at += [x.data_ptr() for x in self.out]
+        at = list(map(_data_ptr, self.all))
         if at != self.at:
             n = len(self.tensors)
             self.table["x"], self.table["out"] = at[:n], at[-n:] if n else []
@@ -412,10 +412,8 @@ class Gradients:
 def _grad_call(grads: Gradients):
     if not isinstance(grads, Gradients):
         raise TypeError(f"need Gradients, got {type(grads).__name__}")
-    ctx = grads.ctx
-    dev = torch.device("cuda", ctx.device)
-    norm = _empty(grads.shape, dtype=torch.float32, device=dev)
-    return ctx, grads._addresses(), len(grads.tensors), norm, _work(grads.work_bytes, dev)
+    norm = _empty(grads.shape, dtype=torch.float32, device=grads.device)
+    return grads.ctx, grads._addresses(), len(grads.tensors), norm, _work(grads.work_bytes, grads.device)
 
 
 def grad_norm(grads: Gradients) -> torch.Tensor:
@@ -423,7 +421,7 @@ def grad_norm(grads: Gradients) -> torch.Tensor:
     summed in 64 bits."""
     ctx, table, n, norm, work = _grad_call(grads)
     ctx.check(_L().cdclq_grad_norm_device(ctx.ptr, table, n, grads.parts, norm.data_ptr(), work.data_ptr(),
-                                          work.numel(), _stream(ctx)))
+                                          grads.work_bytes, _stream(ctx)))
     return norm
 
 
@@ -432,7 +430,7 @@ def clip_grads(grads: Gradients, max_norm: float) -> torch.Tensor:
     its outputs (which are always written). Gradients (an adapter's) whose norm is NaN or infinite are not scaled."""
     ctx, table, n, norm, work = _grad_call(grads)
     ctx.check(_L().cdclq_clip_grads_device(ctx.ptr, table, n, grads.parts, max_norm, norm.data_ptr(), work.data_ptr(),
-                                           work.numel(), _stream(ctx)))
+                                           grads.work_bytes, _stream(ctx)))
     return norm
 
 

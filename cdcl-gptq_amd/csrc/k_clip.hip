@@ -7,7 +7,7 @@
 // its product with x rounded to f32 and to the output's type. 1e-6 keeps c finite, as trainers do it. A norm that
 // is NaN or infinite in f32 clips nothing (c = 1): the gradients stay as they are, for the caller to look at.
 //
-// Both passes are bound by memory. A part's elements, over all tensors, are chunks of 8192; a workgroup takes every
+// Both passes are bound by memory. A part's elements, over all tensors, are chunks of 4096; a workgroup takes every
 // J-th of a part's, so that a part has J sums whatever its size, and each workgroup of the second pass adds them up
 // itself, all in the same order: a launch between the two would cost more. The second pass goes backwards, through what
 // the first one left in the last cache. In place nothing is read again where c = 1.
@@ -26,9 +26,9 @@ namespace cdclq {
 namespace {
 
 constexpr int kTensors = 150;           // of one launch: its arguments keep below 4 KB
-constexpr int kChunk = 8192;            // elements
+constexpr int kChunk = 4096;            // elements
 constexpr long kMostPart = 1l << 30;    // elements of a part that one entry of the tables takes
-constexpr long kMostSums = 2048;        // of all parts together, where parts have several: as many workgroups as run at once
+constexpr long kMostSums = 4096;        // of all parts together, where parts have several
 
 // One tensor, or a piece of it.
 struct ClipEntry {
@@ -119,8 +119,12 @@ __global__ __launch_bounds__(256) void k_norm_parts(const S s, uint32_t chunks, 
   if (b >= sums_all) return;
   const uint32_t part = b / each;
   double v = 0.0;
-  for (uint32_t c = b - part * each; c < chunks; c += each) {
-    const ClipEntry e = entry_of(s, c);
+  uint32_t c = b - part * each;
+  ClipEntry next;
+  if (c < chunks) next = entry_of(s, c);
+  for (; c < chunks; c += each) {
+    const ClipEntry e = next;
+    if (c + each < chunks) next = entry_of(s, c + each);
     const long i0 = part * (long)e.n + (long)(c - e.start) * kChunk, i1 = min(i0 + kChunk, (part + 1) * (long)e.n);
     switch (e.kind & 3) {
       case F32::kind: v = squares<F32>(e.x, i0, i1, v); break;
@@ -154,7 +158,7 @@ __device__ __forceinline__ void scaled(const void* from, void* to, long i0, long
   const long i = i0 + 8 * threadIdx.x;
 #pragma unroll
   for (int u = 0; u < kChunk / 2048; ++u)
-    if (i + 2048 * u + 8 <= i1) r[u] = row8_load<T>(x + i + 2048 * u);
+    if (i + 2048 * u + 8 <= i1) r[u] = row8_load<T, true>(x + i + 2048 * u);
 #pragma unroll
   for (int u = 0; u < kChunk / 2048; ++u) {
     if (i + 2048 * u + 8 > i1) continue;
@@ -173,13 +177,17 @@ __global__ __launch_bounds__(256) void k_clip(const S s, uint32_t chunks, uint32
   const uint32_t b = blockIdx.x + blockIdx.y * gridDim.x;
   if (b >= sums_all) return;
   const uint32_t part = b / each, j = b - part * each;
+  uint32_t c = j + (chunks - 1 - j) / each * each;  // of those below chunks
+  ClipEntry next;
+  if (j < chunks) next = entry_of(s, c);
   const double got = norm_of(sums + part * (long)each, each);
   if (j == 0 && threadIdx.x == 0) norm[part] = (float)got;
   float by = 1.0f;
   if (__builtin_isfinite((float)got)) by = (float)__builtin_fmin(1.0, most / (got + 1e-6));
   if (j >= chunks) return;
-  for (uint32_t c = j + (chunks - 1 - j) / each * each;; c -= each) {
-    const ClipEntry e = entry_of(s, c);
+  for (;; c -= each) {
+    const ClipEntry e = next;
+    if (c >= each) next = entry_of(s, c - each);
     const long i0 = part * (long)e.n + (long)(c - e.start) * kChunk, i1 = min(i0 + kChunk, (part + 1) * (long)e.n);
     if (e.x != e.out || by != 1.0f) {
       switch (e.kind) {

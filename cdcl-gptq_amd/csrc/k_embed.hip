@@ -29,6 +29,7 @@ typedef unsigned long long u64;
 
 // Tokens up to which each form is taken.
 constexpr long kFewIds = 512, kRankedIds = 8192;
+constexpr long kMostWaves = 2048;  // that sum chunks, as long as those have fewer than 64 tokens
 constexpr int kTile = 2048;  // ids of a workgroup of the radix sort
 
 __device__ __forceinline__ long block_id() { return blockIdx.x + (long)blockIdx.y * gridDim.x; }
@@ -92,8 +93,8 @@ __global__ __launch_bounds__(256) void k_embed_rows(const uint16_t* __restrict__
       to[c] = !is ? T::narrow(other) : scale != 1.0f ? T::narrow(scale * T::widen(from[c])) : from[c];
 }
 
-// x in every element of share b of nb of dE's elements [e0, e1) in rows of d, counted row by row.
-template <class O>
+// x in every element of share b of nb of dE's elements [e0, e1) in rows of d, counted row by row. KEEP: through the L2.
+template <class O, bool KEEP>
 __device__ __forceinline__ void fill(const EmbedView& a, long e0, long e1, long b, long nb, float x) {
   typedef typename Row8<O>::stored E;
   E* const de = static_cast<E*>(a.de);
@@ -105,26 +106,26 @@ __device__ __forceinline__ void fill(const EmbedView& a, long e0, long e1, long 
     const long n = e1 - e0, per = ((n + nb - 1) / nb + 7) & ~7l;
     const long from = e0 + min(n, b * per), to = e0 + min(n, (b + 1) * per);
     long i = from + 8 * (long)threadIdx.x;
-    for (; i + 8 <= to; i += 8 * blockDim.x) row8_store<O>(de + i, eight);
+    for (; i + 8 <= to; i += 8 * blockDim.x) row8_store<O, KEEP>(de + i, eight);
     for (; i < to; ++i) de[i] = one;
     return;
   }
   const long r1 = e1 / a.d;
   for (long r = e0 / a.d + b; r < r1; r += nb) {
     long c = 8 * (long)threadIdx.x;
-    for (; c + 8 <= a.d; c += 8 * blockDim.x) row8_store<O>(de + r * a.lde + c, eight);
+    for (; c + 8 <= a.d; c += 8 * blockDim.x) row8_store<O, KEEP>(de + r * a.lde + c, eight);
     for (; c < a.d; ++c) de[r * a.lde + c] = one;
   }
 }
 // Zeros in part `i` of `n` of dE's rows.
-template <class O>
+template <class O, bool KEEP>
 __device__ __forceinline__ void clear(const EmbedView& a, int i, int n, long b, long nb) {
-  if (b < nb) fill<O>(a, a.v * i / n * a.d, a.v * (i + 1) / n * a.d, b, nb, 0.0f);
+  if (b < nb) fill<O, KEEP>(a, a.v * i / n * a.d, a.v * (i + 1) / n * a.d, b, nb, 0.0f);
 }
 // dE = NaN throughout, by all workgroups of a launch (an id outside 0..v).
 template <class O>
 __device__ void poison(const EmbedView& a, long b, long nb) {
-  fill<O>(a, 0, a.v * a.d, b, nb, __builtin_nanf(""));
+  fill<O, true>(a, 0, a.v * a.d, b, nb, __builtin_nanf(""));
 }
 
 // A finished sum of eight columns into dE: the only rounding. ALL: all eight are there.
@@ -148,13 +149,13 @@ __device__ __forceinline__ void finish8(const EmbedView& a, uint32_t row, long c
 template <class T, bool ALL>
 __device__ __forceinline__ Row8<T> load8(const EmbedView& a, long row, long c) {
   const uint16_t* p = a.dy + row * a.lddy + c;
-  if constexpr (ALL) return row8_load<T>(p);
+  if constexpr (ALL) return row8_load<T, true>(p);
   else return row8_load<T>(p, (int)(a.d - c));
 }
 
 template <class O>
 __global__ __launch_bounds__(512) void k_embed_clear(EmbedView a) {
-  clear<O>(a, 0, 1, block_id(), (long)gridDim.x * gridDim.y);
+  clear<O, true>(a, 0, 1, block_id(), (long)gridDim.x * gridDim.y);
 }
 
 // ---------------------------------------------------------------- few tokens
@@ -222,7 +223,7 @@ __global__ __launch_bounds__(1024) void k_embed_rank(EmbedView a, long ranks, lo
   __shared__ uint32_t key[kRankedIds];
   __shared__ int part[16][64];
   const long b = block_id();
-  if (b >= ranks) return clear<O>(a, 0, 1, b - ranks, fills);
+  if (b >= ranks) return clear<O, true>(a, 0, 1, b - ranks, fills);
   if (b == 0 && threadIdx.x == 0) *runs = 0;
   const int t = (int)a.t, t0 = (int)b * 64, lane = threadIdx.x & 63, wv = threadIdx.x >> 6;
   const int seg = (t + 63) / 64 * 4;  // a multiple of 4; 16 of them hold all
@@ -273,7 +274,7 @@ template <class O>
 __global__ __launch_bounds__(512) void k_embed_count(EmbedView a, SortPass p) {
   __shared__ uint32_t n[512];
   const long b = block_id();
-  if (b >= p.tiles) return clear<O>(a, p.launch, p.launches, b - p.tiles, p.fills);
+  if (b >= p.tiles) return clear<O, false>(a, p.launch, p.launches, b - p.tiles, p.fills);
   if (b == 0 && threadIdx.x == 0) *p.runs = 0;
   n[threadIdx.x] = 0;
   __syncthreads();
@@ -297,7 +298,7 @@ template <class O>
 __global__ __launch_bounds__(512) void k_embed_sort(EmbedView a, SortPass p) {
   __shared__ uint32_t place[8][512];
   __shared__ uint32_t scan[8];
-  if (block_id() >= p.tiles) return clear<O>(a, p.launch, p.launches, block_id() - p.tiles, p.fills);
+  if (block_id() >= p.tiles) return clear<O, false>(a, p.launch, p.launches, block_id() - p.tiles, p.fills);
   constexpr int R = kTile / 512;
   const int wv = threadIdx.x >> 6, lane = threadIdx.x & 63, digits = 1 << p.bits;
   const long tile = block_id(), base = tile * kTile + wv * (64 * R);
@@ -383,52 +384,82 @@ struct Sorted {
 // `lanes` lanes take a chunk of the sorted tokens and 8 columns each. A run of equal ids that begins and ends in the
 // chunk is finished here; one that came from the chunk before leaves its sum in head[chunk], one that goes on into
 // the next in tail[chunk] (head if it came, too).
-template <class T, class O>
+// Rows of more than 256 columns (WAVE): the 64 lanes of a wavefront have a chunk in common, so that its ids and places
+// are scalars (loaded as constants: this kernel does not write them) and the runs are told apart by scalar branches; 16
+// rows' loads are on their way.
+template <class T, class O, bool WAVE>
 __global__ __launch_bounds__(256) void k_embed_sums(EmbedView a, Sorted s, long parts) {
-  const long unit = block_id() * (256 / a.lanes) + threadIdx.x / a.lanes;
+  const int lanes = WAVE ? 64 : a.lanes;
+  const long unit = WAVE ? block_id() * 4 + __builtin_amdgcn_readfirstlane(threadIdx.x >> 6)
+                         : block_id() * (256 / lanes) + threadIdx.x / lanes;
   if (unit >= s.chunks * parts) return;
-  const long ch = unit / parts, c = ((unit - ch * parts) * a.lanes + (threadIdx.x & (a.lanes - 1))) * 8;
-  if (c >= a.d) return;
+  const long ch = unit / parts, c = ((unit - ch * parts) * lanes + (threadIdx.x & (lanes - 1))) * 8;
   const long p0 = ch * s.chunk, p1 = min(a.t, p0 + s.chunk);
   const uint32_t v = (uint32_t)a.v;
+  typedef const __attribute__((address_space(4))) uint32_t* Keys;
+  typedef const __attribute__((address_space(4))) int* Order;
+  const std::conditional_t<WAVE, Keys, const uint32_t*> keys = (decltype(keys))(uintptr_t)s.keys;
+  const std::conditional_t<WAVE, Order, const int*> order = (decltype(order))(uintptr_t)s.order;
   auto sum = [&](auto all) {
     constexpr bool ALL = decltype(all)::value;
-    bool came = p0 > 0 && s.keys[p0 - 1] == s.keys[p0];
-    uint32_t cur = s.keys[p0];
+    constexpr int U = 8;
+    bool came = p0 > 0 && keys[p0 - 1] == keys[p0];
+    uint32_t cur = keys[p0];
     float acc[8] = {};
     auto part = [&](float* to) {
       float* p = to + ch * s.dp + c;
       *reinterpret_cast<float4*>(p) = make_float4(acc[0], acc[1], acc[2], acc[3]);
       *reinterpret_cast<float4*>(p + 4) = make_float4(acc[4], acc[5], acc[6], acc[7]);
     };
-    for (long p = p0; p < p1 && cur < v; p += 8) {
-      uint32_t k[8];
-      Row8<T> x[8];
+    auto add = [&](uint32_t k, const Row8<T>& x) {
+      if (k != cur) {
+        if (came) part(s.head);
+        else finish8<O, ALL>(a, cur, c, acc);
+        came = false;
+        cur = k;
 #pragma unroll
-      for (int j = 0; j < 8; ++j) {
-        const long i = min(p + j, p1 - 1);
-        k[j] = s.keys[i];
-        x[j] = load8<T, ALL>(a, s.order[i], c);
+        for (int i = 0; i < 8; ++i) acc[i] = 0.0f;
       }
 #pragma unroll
-      for (int j = 0; j < 8; ++j) {
-        if (p + j >= p1 || cur >= v) continue;
-        if (k[j] != cur) {
-          if (came) part(s.head);
-          else finish8<O, ALL>(a, cur, c, acc);
-          came = false;
-          cur = k[j];
+      for (int i = 0; i < 8; ++i) acc[i] += x.get(i);
+    };
+    if constexpr (WAVE) {
+      Row8<T> x[2][U];
+      auto load = [&](long p, Row8<T>* to) {
 #pragma unroll
-          for (int i = 0; i < 8; ++i) acc[i] = 0.0f;
+        for (int j = 0; j < U; ++j) to[j] = load8<T, ALL>(a, order[min(p + j, p1 - 1)], c);
+      };
+      auto use = [&](long p, const Row8<T>* from) {
+#pragma unroll
+        for (int j = 0; j < U; ++j)
+          if (p + j < p1 && cur < v) add(keys[p + j], from[j]);
+      };
+      load(p0, x[0]);
+      for (long p = p0; p < p1 && cur < v; p += 2 * U) {
+        if (p + U < p1) load(p + U, x[1]);
+        use(p, x[0]);
+        if (p + 2 * U < p1) load(p + 2 * U, x[0]);
+        if (p + U < p1) use(p + U, x[1]);
+      }
+    } else {
+      for (long p = p0; p < p1 && cur < v; p += U) {
+        uint32_t k[U];
+        Row8<T> x[U];
+#pragma unroll
+        for (int j = 0; j < U; ++j) {
+          const long i = min(p + j, p1 - 1);
+          k[j] = keys[i];
+          x[j] = load8<T, ALL>(a, order[i], c);
         }
 #pragma unroll
-        for (int i = 0; i < 8; ++i) acc[i] += x[j].get(i);
+        for (int j = 0; j < U; ++j)
+          if (p + j < p1 && cur < v) add(k[j], x[j]);
       }
     }
     if (cur >= v) return;
     if (came) {
       part(s.head);
-    } else if (p1 < a.t && s.keys[p1] == cur) {
+    } else if (p1 < a.t && keys[p1] == cur) {
       part(s.tail);
       if (c == 0) s.starts[atomicAdd(s.runs, 1u)] = (uint32_t)ch;
     } else {
@@ -436,7 +467,7 @@ __global__ __launch_bounds__(256) void k_embed_sums(EmbedView a, Sorted s, long 
     }
   };
   if (c + 8 <= a.d) sum(std::true_type{});
-  else sum(std::false_type{});
+  else if (c < a.d) sum(std::false_type{});
 }
 
 // The runs that pass the end of the chunk where they began, each by 256 columns a workgroup: their parts summed in
@@ -511,10 +542,9 @@ EmbedPlan embed_plan(long t, long d, long v) {
     p.tiles = (int)((t + kTile - 1) / kTile);
     p.hist = take((size_t)4 * p.tiles << p.bits);
   }
-  // Chunks as long as leaves 4096 wavefronts (a wavefront reads 8 rows' 16 bytes a lane at once).
   const long waves = (d + 511) / 512 * t;
   p.chunk = 8;
-  while (p.chunk < 64 && waves / p.chunk > 8192) p.chunk *= 2;
+  while (p.chunk < 64 && waves / p.chunk > kMostWaves) p.chunk *= 2;
   while ((t + p.chunk - 1) / p.chunk > 16384) p.chunk *= 2;
   p.chunks = (t + p.chunk - 1) / p.chunk;
   p.dp = (d + 7) / 8 * 8;
@@ -525,8 +555,9 @@ EmbedPlan embed_plan(long t, long d, long v) {
   return p;
 }
 
-// Workgroups that clear n elements of dE: 64 KB each, or as many as fill the card several times.
-long clearing(const EmbedView& a, long n) { return a.add ? 0 : std::max(1l, std::min(n / 32768, 4096l)); }
+// Workgroups that clear n elements of dE, a store a thread or a few: 4096 tokens, 128256 x 4096: 198 us a step, with 64 KB
+// each 218, with 1 MB 213.
+long clearing(const EmbedView& a, long n) { return a.add ? 0 : std::max(1l, std::min(n / 8192, 1l << 20)); }
 
 template <class T, class O>
 hipError_t backward(hipStream_t st, EmbedView a, void* work) {
@@ -565,7 +596,9 @@ hipError_t backward(hipStream_t st, EmbedView a, void* work) {
   const Sorted s = {keys[at], order[at], p.chunk, p.chunks, p.dp, reinterpret_cast<float*>(w + p.head),
                     reinterpret_cast<float*>(w + p.tail), runs, reinterpret_cast<uint32_t*>(w + p.starts)};
   const long parts = (a.d + 8l * a.lanes - 1) / (8l * a.lanes), units = p.chunks * parts, per = 256 / a.lanes;
-  k_embed_sums<T, O><<<launch_grid((units + per - 1) / per), 256, 0, st>>>(a, s, parts);
+  const dim3 grid = launch_grid((units + per - 1) / per);
+  if (a.lanes == 64) k_embed_sums<T, O, true><<<grid, 256, 0, st>>>(a, s, parts);
+  else k_embed_sums<T, O, false><<<grid, 256, 0, st>>>(a, s, parts);
   const long slabs = (a.d + 255) / 256;
   k_embed_join<O><<<(int)std::min(p.chunks * slabs, 2048l), 256, 0, st>>>(a, s, (uint32_t)slabs);
   return hipGetLastError();

@@ -33,15 +33,34 @@ struct Row8<F32> {
   __device__ __forceinline__ void set(int i, float x) { v[i] = x; }
 };
 
-template <class T>
+// LAST: what nobody reads again soon, past the L2 (non-temporal). The rows of an embedding's gradient (32768 x 2048:
+// 124 us a step, so 115) and gradients on their second, last reading (2.8 GB: 736 us, so 713); logits rather not (41, 44).
+template <class T, bool LAST = false>
 __device__ __forceinline__ Row8<T> row8_load(const typename Row8<T>::stored* p) {
+  typedef uint32_t u4 __attribute__((ext_vector_type(4), aligned(2)));
   Row8<T> r;
-  __builtin_memcpy(r.v, p, sizeof(r.v));
+  u4 t[sizeof(r.v) / 16];
+#pragma unroll
+  for (int i = 0; i < (int)(sizeof(r.v) / 16); ++i) {
+    if constexpr (LAST) t[i] = __builtin_nontemporal_load(reinterpret_cast<const u4*>(p) + i);
+    else t[i] = reinterpret_cast<const u4*>(p)[i];
+  }
+  __builtin_memcpy(r.v, t, sizeof(r.v));
   return r;
 }
-template <class T>
+// Past the L2 (non-temporal): results that no later workgroup of the launch reads. Written lines that the L2 holds when
+// a kernel ends have to leave it then: 16384 rows of 4096 from an embedding 40 us, so 36; gradients clipped into f32
+// 82 and 78; logits 48 and 41. FILL: clearing, which is faster through it (50001 x 1000 rows: 23 us, past it 31).
+template <class T, bool FILL = false>
 __device__ __forceinline__ void row8_store(typename Row8<T>::stored* p, const Row8<T>& r) {
-  __builtin_memcpy(p, r.v, sizeof(r.v));
+  typedef uint32_t u4 __attribute__((ext_vector_type(4), aligned(2)));
+  u4 t[sizeof(r.v) / 16];
+  __builtin_memcpy(t, r.v, sizeof(r.v));
+#pragma unroll
+  for (int i = 0; i < (int)(sizeof(r.v) / 16); ++i) {
+    if constexpr (FILL) reinterpret_cast<u4*>(p)[i] = t[i];
+    else __builtin_nontemporal_store(t[i], reinterpret_cast<u4*>(p) + i);
+  }
 }
 // The first n < 8 of them, the others 0.
 template <class T>

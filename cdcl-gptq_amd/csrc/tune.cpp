@@ -270,8 +270,8 @@ int grad_tensors(cdclq_ctx* ctx, const cdclq_grad* grads, size_t n, size_t parts
   struct Range {
     uintptr_t from, to;
   };
-  std::vector<Range> used;
-  if (clip) used.reserve(2 * n);
+  std::vector<Range> read, written;  // apart: buckets' views are in order by themselves
+  if (clip) read.reserve(n), written.reserve(n);
   for (size_t i = 0; i < n; ++i) {
     const cdclq_grad& g = grads[i];
     CK(check_type(ctx, g.dtype));
@@ -292,14 +292,19 @@ int grad_tensors(cdclq_ctx* ctx, const cdclq_grad* grads, size_t n, size_t parts
     if (g.x == g.out && g.out_dtype != g.dtype)
       return fail(ctx, CDCLQ_INVALID_ARG, "a gradient that is clipped in place keeps its dtype");
     const uintptr_t x = (uintptr_t)g.x, o = (uintptr_t)g.out;
-    used.push_back({x, x + g.count * type_bytes(g.dtype)});
-    if (o != x) used.push_back({o, o + g.count * type_bytes(g.out_dtype)});
+    read.push_back({x, x + g.count * type_bytes(g.dtype)});
+    if (o != x) written.push_back({o, o + g.count * type_bytes(g.out_dtype)});
   }
   auto before = [](const Range& a, const Range& b) { return a.from < b.from; };
-  if (!std::is_sorted(used.begin(), used.end(), before)) std::sort(used.begin(), used.end(), before);
-  for (size_t i = 1; i < used.size(); ++i)
-    if (used[i].from < used[i - 1].to)
-      return fail(ctx, CDCLQ_INVALID_ARG, "gradients or their outputs overlap (the same tensor twice?)");
+  for (auto* r : {&read, &written})
+    if (!std::is_sorted(r->begin(), r->end(), before)) std::sort(r->begin(), r->end(), before);
+  uintptr_t end = 0;  // of the ranges so far, both lists by address
+  for (size_t i = 0, j = 0; i < read.size() || j < written.size();) {
+    const bool first = j == written.size() || (i < read.size() && read[i].from < written[j].from);
+    const Range& r = first ? read[i++] : written[j++];
+    if (r.from < end) return fail(ctx, CDCLQ_INVALID_ARG, "gradients or their outputs overlap (the same tensor twice?)");
+    end = r.to;
+  }
   return CDCLQ_OK;
 }
 

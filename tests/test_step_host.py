@@ -35,14 +35,14 @@ def test_sizes_outside_the_limits_ask_for_nothing():
 
 @pytest.mark.parametrize("parts", [1, 8, 32768])
 def test_grad_workspace_holds_few_sums(parts):
-    """64-bit sums, 2048 or one for each part, and of more than 150 tensors a table and 4 bytes for 8192 elements of a
+    """64-bit sums, 4096 or one for each part, and of more than 150 tensors a table and 4 bytes for 4096 elements of a
     part, over any sizes."""
     for counts in ([0], [1] * 150, [1] * 300, [1 << 20, 17, 0, 4096], [1 << 30] * 3, [(1 << 33) + 5, 1]):
         g = np.zeros(len(counts), GRAD)
         g["count"] = np.array(counts, np.uint64) // (1 if parts == 1 else 512) * parts
         n = L.cdclq_grad_work_bytes(g.ctypes.data, len(counts), parts)
-        chunks = sum(-(-int(c) // parts // 8192) + 1 for c in g["count"])
-        assert n % 256 == 0 and 8 * parts <= n <= 8 * max(2048, parts) + 256 + (len(counts) > 150) * (
+        chunks = sum(-(-int(c) // parts // 4096) + 1 for c in g["count"])
+        assert n % 256 == 0 and 8 * parts <= n <= 8 * max(4096, parts) + 256 + (len(counts) > 150) * (
             32 * len(counts) + 4 * chunks + 512)
 
 

@@ -37,7 +37,8 @@ struct Binned {
 __global__ __launch_bounds__(1024) void k_constrain_bin(ConstrainArgs a, int log_slab, int slabs, uint32_t* __restrict__ start,
                                                         uint32_t* __restrict__ place) {
   extern __shared__ __align__(16) uint32_t word[];  // a slab's count, then where its next token goes
-  __shared__ uint32_t sums[16];
+  constexpr int kOnce = 8192;  // tokens that a round takes, 8 a thread
+  __shared__ uint32_t sums[16], sorted[kOnce];
   const long row = blockIdx.x + (long)blockIdx.y * gridDim.x;
   if (row >= a.r) return;
   const int tid = threadIdx.x, lane = tid & 63, wv = tid >> 6;
@@ -53,14 +54,14 @@ __global__ __launch_bounds__(1024) void k_constrain_bin(ConstrainArgs a, int log
   auto is = [&](int u) { return (uint64_t)tok[u] < (uint64_t)a.v; };
   // A history of one round's tokens stays in registers with what the counters held.
   uint32_t rank[8];
-  for (int i0 = tid; i0 < len; i0 += 8192) {
+  for (int i0 = tid; i0 < len; i0 += kOnce) {
     load(i0);
 #pragma unroll
     for (int u = 0; u < 8; ++u)
       if (is(u)) rank[u] = atomicAdd(&word[(uint32_t)tok[u] >> log_slab], 1u);
   }
   __syncthreads();
-  uint32_t before = (uint32_t)(row * a.width);
+  uint32_t all = 0;
   for (int s0 = 0; s0 < slabs; s0 += 1024) {
     const uint32_t n = s0 + tid < slabs ? word[s0 + tid] : 0;
     uint32_t sum = n;
@@ -71,29 +72,35 @@ __global__ __launch_bounds__(1024) void k_constrain_bin(ConstrainArgs a, int log
     }
     if (lane == 63) sums[wv] = sum;
     __syncthreads();
-    uint32_t all = 0;
+    sum += all;
 #pragma unroll
     for (int w = 0; w < 16; ++w) {
       if (w < wv) sum += sums[w];
       all += sums[w];
     }
     if (s0 + tid < slabs) {
-      word[s0 + tid] = before + sum - n;
-      start[row * (slabs + 1) + s0 + tid] = before + sum - n;
+      word[s0 + tid] = sum - n;
+      start[row * (slabs + 1) + s0 + tid] = (uint32_t)(row * a.width) + sum - n;
     }
-    before += all;
     __syncthreads();
   }
-  if (tid == 0) start[row * (slabs + 1) + slabs] = before;
-  const bool once = len <= 8192;
-  for (int i0 = tid; i0 < len; i0 += 8192) {
-    if (!once) load(i0);
+  if (tid == 0) start[row * (slabs + 1) + slabs] = (uint32_t)(row * a.width) + all;
+  uint32_t* const to = place + row * a.width;
+  const uint32_t low = (1u << log_slab) - 1;
+  auto value = [&](int u, int i) { return ((uint32_t)tok[u] & low) | (i < prompt ? kPrompt : 0); };
+  if (len <= kOnce) {  // sorted in LDS, so that whole lines are written
 #pragma unroll
-    for (int u = 0; u < 8; ++u) {
-      if (!is(u)) continue;
-      uint32_t* const w = &word[(uint32_t)tok[u] >> log_slab];
-      place[once ? *w + rank[u] : atomicAdd(w, 1u)] = ((uint32_t)tok[u] & ((1u << log_slab) - 1)) | (i0 + 1024 * u < prompt ? kPrompt : 0);
-    }
+    for (int u = 0; u < 8; ++u)
+      if (tid < len && is(u)) sorted[word[(uint32_t)tok[u] >> log_slab] + rank[u]] = value(u, tid + 1024 * u);
+    __syncthreads();
+    for (uint32_t i = tid; i < all; i += 1024) to[i] = sorted[i];
+    return;
+  }
+  for (int i0 = tid; i0 < len; i0 += kOnce) {
+    load(i0);
+#pragma unroll
+    for (int u = 0; u < 8; ++u)
+      if (is(u)) to[atomicAdd(&word[(uint32_t)tok[u] >> log_slab], 1u)] = value(u, i0 + 1024 * u);
   }
 }
 
@@ -156,6 +163,8 @@ __global__ __launch_bounds__(TH) void k_constrain(ConstrainArgs a, Binned bins, 
       if (i + 8 <= n) x[k] = row8_load<T>(in + i);
     }
   }
+  const float rep = a.repetition ? a.repetition[row] : 1.0f, freq = a.frequency ? a.frequency[row] : 0.0f,
+              pres = a.presence ? a.presence[row] : 0.0f;
   float* const bias = reinterpret_cast<float*>(word + SLAB);
   if (marks) {
 #pragma unroll
@@ -212,8 +221,6 @@ __global__ __launch_bounds__(TH) void k_constrain(ConstrainArgs a, Binned bins, 
     }
     __syncthreads();
   }
-  const float rep = a.repetition ? a.repetition[row] : 1.0f, freq = a.frequency ? a.frequency[row] : 0.0f,
-              pres = a.presence ? a.presence[row] : 0.0f;
   auto apply = [&](float l, uint32_t m) {
     const uint32_t c = m & kCount;
     if (m & ~kBias) l = l > 0.0f ? l / rep : l * rep;

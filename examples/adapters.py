@@ -3,11 +3,14 @@
 A toy language model (embedding, one MLP block, head) gets its two projections quantized and packed by
 the engine. Each user then has a next-token rule of their own, and their low-rank adapters are trained
 together, every batch holding tokens of all of them: the packed projections with adapters forward and
-backward, the inputs kept as 8-bit checkpoints, the loss over the vocabulary without its logits.
-After that the perplexity of every user's text is measured and single tokens of all users, and of one
-without adapters, are decoded in one batch.
+backward, the inputs kept as 8-bit checkpoints, the loss over the vocabulary without its logits, each
+user's gradients clipped to a norm of their own on the way to the 32-bit weights.
+After that the perplexity of every user's text is measured, single tokens of all users, and of one
+without adapters, are decoded in one batch, and short texts are written in which words of the users'
+texts only may stand and repeated ones are penalized.
 
-    python examples/adapters.py [--steps 60] [--width 512] [--vocab 4096] [--train-head] [--dtype bf16]
+    python examples/adapters.py [--steps 60] [--width 512] [--vocab 4096] [--train-head] [--train-embed]
+                                [--clip 1.0] [--dtype bf16]
 """
 import argparse
 import math
@@ -66,17 +69,39 @@ class Model:
 
     def states(self, tokens, user):
         """Hidden states for autograd."""
-        e = self.embed[tokens]
+        e = tune.embedding(self.ctx, self.embed, tokens)
         u = torch.nn.functional.silu(tune.linear(self.up, e, self.up_ad, user))
         return e + tune.linear(self.down, u, self.down_ad, user)
 
-    def decode(self, tokens, user):
-        """The likeliest next token of each request."""
+    def decode(self, tokens, user, **constraints):
+        """The likeliest next token of each request, under constraints as tune.constrain_logits takes them."""
         with torch.no_grad():
-            e = self.embed[tokens]
+            e = tune.embed(self.ctx, self.embed, tokens)
             u = torch.nn.functional.silu(tune.adapter_linear(self.up, e, self.up_ad, user))
             h = e + tune.adapter_linear(self.down, u, self.down_ad, user)
-            return (h @ self.head.T).argmax(1)
+            logits = h @ self.head.T
+            if constraints:
+                tune.constrain_logits(self.ctx, logits, out=logits, **constraints)
+            return logits.argmax(1)
+
+    def write(self, tokens, user, steps, words):
+        """Texts of `steps` tokens after the first ones: a token's second use costs more than its first, and only
+        `words` may stand in them."""
+        r, v = len(tokens), self.head.shape[0]
+        allowed = torch.zeros(-(-v // 32) * 32, dtype=torch.int64, device="cuda")
+        allowed[words] = 1
+        bits = (allowed.view(1, -1, 32) << torch.arange(32, device="cuda")).sum(2)
+        mask = torch.where(bits >= 1 << 31, bits - (1 << 32), bits).int()
+        history = torch.zeros(r, steps + 1, dtype=torch.int64, device="cuda")
+        history[:, 0] = tokens
+        lengths = torch.ones(r, dtype=torch.int32, device="cuda")
+        limits = dict(history=history, lengths=lengths, prompts=torch.ones_like(lengths),
+                      repetition=torch.full((r,), 1.1, device="cuda"), frequency=torch.full((r,), 0.5, device="cuda"),
+                      mask=mask, mask_rows=torch.zeros_like(lengths))
+        for i in range(steps):
+            history[:, i + 1] = tokens = self.decode(tokens, user, **limits)
+            lengths += 1
+        return history
 
     def perplexity(self, tokens, user, targets):
         with torch.no_grad():
@@ -97,6 +122,8 @@ def main(argv=None):
     p.add_argument("--lr", type=float, default=5e-3)
     p.add_argument("--dtype", choices=["bf16", "f16"], default="bf16")
     p.add_argument("--train-head", action="store_true", help="train the head's weights as well")
+    p.add_argument("--train-embed", action="store_true", help="train the embedding as well")
+    p.add_argument("--clip", type=float, default=math.inf, help="largest norm of a user's gradients")
     p.add_argument("--seed", type=int, default=0)
     o = p.parse_args(argv)
     ctx = cdclq.Context(0)
@@ -121,15 +148,22 @@ def main(argv=None):
     held = text(1000)
     before = m.perplexity(*held)
     # 32-bit copies of what is trained: small steps would vanish in 16 bits
-    live = m.weights() + ([m.head.requires_grad_()] if o.train_head else [])
+    rest = ([m.head.requires_grad_()] if o.train_head else []) + ([m.embed.requires_grad_()] if o.train_embed else [])
+    live = m.weights() + rest
     master = [w.detach().float().requires_grad_() for w in live]
+    for w32 in master:
+        w32.grad = torch.empty_like(w32)
+    users = len(live) - len(rest)
     opt = torch.optim.Adam(master, lr=o.lr)
     for step in range(o.steps):
         tokens, user, target = batch(o.tokens)
         loss = tune.cross_entropy(ctx, m.states(tokens, user), m.head, target)
         loss.backward()
-        for w, w32 in zip(live, master):
-            w32.grad = w.grad.float()
+        # every user by the norm of their own gradients, what they share by its own
+        for grads, out, adapters in (([w.grad for w in live[:users]], master[:users], o.users),
+                                     ([w.grad for w in rest], master[users:], None)):
+            tune.clip_grads(tune.Gradients(ctx, grads, out=[w32.grad for w32 in out], adapters=adapters), o.clip)
+        for w in live:
             w.grad = None
         opt.step()
         with torch.no_grad():
@@ -148,8 +182,11 @@ def main(argv=None):
         right += (got[: o.users] == rules[:, w]).sum().item()
     accuracy = right / (o.users * o.words)
     print(f"decoded {o.users * o.words} tokens, {100 * accuracy:.1f}% by their user's rule")
+    texts = m.write(words[torch.arange(o.users + 1, device="cuda") % o.words], user, 8, words)
+    for u, text in enumerate(texts.tolist()):
+        print(f"user {u if u < o.users else None}: {' '.join(map(str, text))}")
     ctx.clear_cache()
-    return {"before": before, "after": after, "accuracy": accuracy}
+    return {"before": before, "after": after, "accuracy": accuracy, "texts": texts.tolist(), "words": words.tolist()}
 
 
 if __name__ == "__main__":

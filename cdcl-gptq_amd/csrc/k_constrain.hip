@@ -109,10 +109,10 @@ template <class T, int TH, int K, bool PLACE>
 __global__ __launch_bounds__(TH) void k_constrain(ConstrainArgs a, Binned bins, long rows8, int slabs) {
   extern __shared__ __align__(16) uint32_t word[];
   constexpr int SLAB = TH * 8 * K;
-  // workgroup b: XCD b % 8 takes the requests of that remainder, slab by slab
-  const long b = blockIdx.x + (long)blockIdx.y * gridDim.x, at = b >> 3;
-  const long row = (at / slabs) * 8 + (b & 7);
-  if (at >= rows8 * slabs || row >= a.r) return;
+  // Workgroup b of many requests: XCD b % 8 takes those of that remainder, slab by slab. Of few: slabs over all XCDs.
+  const long b = blockIdx.x + (long)blockIdx.y * gridDim.x, at = rows8 ? b >> 3 : b;
+  const long row = rows8 ? (at / slabs) * 8 + (b & 7) : at / slabs;
+  if (row >= a.r) return;
   const int slab = (int)(at % slabs), slab0 = slab * SLAB;
   const auto* in = static_cast<const typename Row8<T>::stored*>(a.logits) + row * a.ld + slab0;
   auto* out = static_cast<typename Row8<T>::stored*>(a.out) + row * a.ldo + slab0;
@@ -207,6 +207,7 @@ __global__ __launch_bounds__(TH) void k_constrain(ConstrainArgs a, Binned bins, 
         const int i = i0 + lane, p = i < m ? at[i] : -1;
         bool first = i < m;
         float s = 0.0f;
+#pragma unroll 8
         for (int j = 0; j < m; ++j) {
           const bool same = at[j] == p;
           first = first && !(same && j < i);
@@ -288,7 +289,7 @@ template <class T, int TH, int K>
 hipError_t launch(hipStream_t st, const ConstrainArgs& a, void* work) {
   constexpr int SLAB = TH * 8 * K;
   const int slabs = (int)((a.v + SLAB - 1) / SLAB);
-  const long rows8 = (a.r + 7) / 8;
+  const long rows8 = a.r >= 64 ? (a.r + 7) / 8 : 0;
   Binned bins = {};
   if (a.history && binned(a.r, a.v, a.width)) {
     uint32_t* start = static_cast<uint32_t*>(work);
@@ -297,7 +298,7 @@ hipError_t launch(hipStream_t st, const ConstrainArgs& a, void* work) {
     bins = {start, place};
   }
   const size_t lds = a.history || a.biases ? 4 * SLAB + 8 * (size_t)a.biases : 0;
-  const dim3 grid = launch_grid(rows8 * slabs * 8);
+  const dim3 grid = launch_grid((rows8 ? 8 * rows8 : a.r) * slabs);
   if (a.logits == a.out) k_constrain<T, TH, K, true><<<grid, TH, lds, st>>>(a, bins, rows8, slabs);
   else k_constrain<T, TH, K, false><<<grid, TH, lds, st>>>(a, bins, rows8, slabs);
   return hipGetLastError();

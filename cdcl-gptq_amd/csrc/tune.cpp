@@ -267,6 +267,7 @@ int grad_tensors(cdclq_ctx* ctx, const cdclq_grad* grads, size_t n, size_t parts
   if (parts == 0) return fail(ctx, CDCLQ_INVALID_ARG, "gradients need at least one part");
   CK(check_size(ctx, "adapter count", parts, kMaxParts));
   out->resize(n);
+  size_t total = 0;
   struct Range {
     uintptr_t from, to;
   };
@@ -275,7 +276,9 @@ int grad_tensors(cdclq_ctx* ctx, const cdclq_grad* grads, size_t n, size_t parts
   for (size_t i = 0; i < n; ++i) {
     const cdclq_grad& g = grads[i];
     CK(check_type(ctx, g.dtype));
-    CK(check_size(ctx, "gradient of", g.count, kMaxGrad));
+    CK(check_size(ctx, "gradients of", g.count, kMaxGrad));
+    total += g.count;
+    CK(check_size(ctx, "gradients of", total, kMaxGrad));
     if (g.count % parts)
       return fail(ctx, CDCLQ_INVALID_ARG, "gradient " + std::to_string(i) + " of " + std::to_string(g.count) +
                                               " elements is not " + std::to_string(parts) + " equal parts");
@@ -554,8 +557,9 @@ size_t cdclq_grad_work_bytes(const cdclq_grad* grads, size_t n, size_t parts) {
   if ((n && !grads) || n > (size_t)1 << 20 || parts == 0 || parts > kMaxParts) return 0;
   try {
     std::vector<GradTensor> g(n);
+    size_t total = 0;
     for (size_t i = 0; i < n; ++i) {
-      if (grads[i].count > kMaxGrad) return 0;
+      if (grads[i].count > kMaxGrad || (total += grads[i].count) > kMaxGrad) return 0;
       g[i].n = (long)grads[i].count;
     }
     return clip_work_bytes(g.data(), n, (int)parts);

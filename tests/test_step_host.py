@@ -13,10 +13,10 @@ GRAD = tune._GRAD
 
 @pytest.mark.parametrize("d,v", [(1, 1), (8, 510), (64, 511), (1000, 50001), (4096, 128256), (1 << 20, 64), (64, 1 << 24)])
 def test_embed_workspace_sizes(d, v):
-    for t in (0, 1, 512, 513, 8192, 8193, 100_000, 1 << 22):
+    for t in (0, 1, 128, 129, 512, 8192, 8193, 100_000, 1 << 22):
         n = L.cdclq_embed_work_bytes(t, d, v)
         assert n % 256 == 0
-        assert n == 0 if t <= 512 else n >= 8 * t  # ids and places of the sorted tokens
+        assert n == 0 if t <= 128 else n >= 8 * t  # ids and places of the sorted tokens
         # two sets of those, the runs that pass a chunk's end (two rows of float32 for eight tokens, padded to eight
         # columns), the counts of 512 digits for 2048 tokens
         assert n <= 17 * t + (d + 7) // 8 * 8 * (t // 8 + 1) * 8 + 2048 * (t // 2048 + 1) + 4096
@@ -31,6 +31,9 @@ def test_sizes_outside_the_limits_ask_for_nothing():
     assert L.cdclq_grad_work_bytes(None, 1, 1) == 0
     g["count"] = 1 << 41
     assert L.cdclq_grad_work_bytes(g.ctypes.data, 1, 1) == 0
+    g = np.zeros(5, GRAD)  # together
+    g["count"] = 1 << 38
+    assert L.cdclq_grad_work_bytes(g.ctypes.data, 4, 1) and L.cdclq_grad_work_bytes(g.ctypes.data, 5, 1) == 0
 
 
 @pytest.mark.parametrize("parts", [1, 8, 32768])

@@ -50,7 +50,8 @@ __device__ __forceinline__ Row8<T> row8_load(const typename Row8<T>::stored* p) 
 }
 // Past the L2 (non-temporal): results that no later workgroup of the launch reads. Written lines that the L2 holds when
 // a kernel ends have to leave it then: 16384 rows of 4096 from an embedding 40 us, so 36; gradients clipped into f32
-// 82 and 78; logits 48 and 41. FILL: clearing, which is faster through it (50001 x 1000 rows: 23 us, past it 31).
+// 82 and 78; logits 48 and 41. FILL: clearing, which is faster through it (50001 x 1000 rows: 23 us, past it 31). f32
+// goes through it, too: a lane's 32 bytes are two stores, of half lines each.
 template <class T, bool FILL = false>
 __device__ __forceinline__ void row8_store(typename Row8<T>::stored* p, const Row8<T>& r) {
   typedef uint32_t u4 __attribute__((ext_vector_type(4), aligned(2)));
@@ -58,7 +59,7 @@ __device__ __forceinline__ void row8_store(typename Row8<T>::stored* p, const Ro
   __builtin_memcpy(t, r.v, sizeof(r.v));
 #pragma unroll
   for (int i = 0; i < (int)(sizeof(r.v) / 16); ++i) {
-    if constexpr (FILL) reinterpret_cast<u4*>(p)[i] = t[i];
+    if constexpr (FILL || sizeof(r.v) > 16) reinterpret_cast<u4*>(p)[i] = t[i];
     else __builtin_nontemporal_store(t[i], reinterpret_cast<u4*>(p) + i);
   }
 }

@@ -9,8 +9,14 @@
 // come it counts the history's tokens of its slab in LDS, a word a token:
 //   bit 31 in the prompt      bits 30..20 the token's bias + 1      bits 19..0 times generated
 // (whole numbers: the order of the additions does not matter). Every slab of a request reads the whole history, so
-// slabs are as large as leaves enough workgroups, and a request's slabs lie on one XCD, whose L2 then holds its
-// history. In place, only what changes is read or written, and tokens that the mask shuts out are not read.
+// slabs are as large as leaves enough workgroups, and where there are many requests a request's slabs lie on one XCD, whose
+// L2 then holds its history; long histories of many requests are sorted by slab in a launch before. In place, only what
+// changes is read or written, and tokens that the mask shuts out are not read.
+// 256 requests, 128256 bf16 tokens, histories of 6100 on average, 32 biases, half with a mask: 39.6 us, 8 of them the
+// sorting; without history, biases and masks 20 (131 MB, part of them in the last cache). What bounds it between the two
+// are the instructions for tokens that have been: a wavefront takes them for all its lanes wherever one has such a
+// token (the vector units issue 70% of the time). One token's logit made by one thread, in a pass before the copying, took
+// 2 us more: its barriers and the gathered logits cost what it saves; slabs of one wavefront, without barriers, 14 more.
 #include <hip/hip_runtime.h>
 
 #include <algorithm>
@@ -23,9 +29,6 @@ namespace cdclq {
 namespace {
 
 constexpr uint32_t kPrompt = 1u << 31, kCount = (1u << 20) - 1, kBias = 2047u << 20;
-
-// Tokens of histories, counted once a slab, from which on they are sorted by slab first.
-constexpr long kMostScans = 1l << 22;
 
 // The histories' tokens by slab: those of request r and slab s at place[start[r][s]] up to start[r][s + 1], each its
 // place in the slab, | kPrompt.
@@ -269,26 +272,25 @@ __global__ __launch_bounds__(TH) void k_constrain(ConstrainArgs a, Binned bins, 
   }
 }
 
-// Tokens of a slab and threads of its workgroup: the largest that leaves 512 workgroups.
-struct SlabShape {
-  int threads, per;  // 8 per tokens a thread
-  int slab() const { return 8 * threads * per; }
-  int count(long v) const { return (int)((v + slab() - 1) / slab()); }
-};
-SlabShape slab_shape(long r, long v) {
-  const long tokens = r * v;
-  return tokens >= 512l * 8192 ? SlabShape{512, 2} : tokens >= 512l * 4096 ? SlabShape{256, 2} : SlabShape{128, 1};
-}
+// Slabs of 1024 tokens by 128 threads or of 8192 by 512, these from 2^20 logits on: 128256 tokens, histories of 500, half
+// of the requests with a mask: one request 4.5 us and 5.3, 16 requests 8.4 and 5.8, 128 requests 21 and 14.5. (4096 by
+// 256: 5.2, 6.2 and 14.8.)
+bool large_slabs(long r, long v) { return r * v >= 1l << 20; }
+long slabs_of(long r, long v) { return large_slabs(r, v) ? (v + 8191) / 8192 : (v + 1023) / 1024; }
 
-// Whether the histories are sorted by slab in a launch before.
+// Whether the histories are sorted by slab in a launch before: where a workgroup would take many rounds to look at one,
+// or all of them much work. 128256 tokens, histories of 1000 and 8192 at most, sorted and not: one request 7.4 and 4.9
+// us, 9.2 and 12.5; 8 requests 8.3 and 5.6, 10.6 and 15.1; 64 requests of 4000 14.1 and 10.8; 256 of 1000 27.8 and
+// 26.2, of 2000 28.9 and 28.7.
 bool binned(long r, long v, long width) {
-  return r * slab_shape(r, v).count(v) * width > kMostScans && r * width < (1l << 32);
+  return (width > 32l * (large_slabs(r, v) ? 512 : 128) || r * slabs_of(r, v) * width > 1l << 23) && r * width < 1l << 32;
 }
 
 template <class T, int TH, int K>
 hipError_t launch(hipStream_t st, const ConstrainArgs& a, void* work) {
   constexpr int SLAB = TH * 8 * K;
   const int slabs = (int)((a.v + SLAB - 1) / SLAB);
+  // (of 256 requests 27.6 us by XCD and 28.7 without, of 16 9.1 and 6.6)
   const long rows8 = a.r >= 64 ? (a.r + 7) / 8 : 0;
   Binned bins = {};
   if (a.history && binned(a.r, a.v, a.width)) {
@@ -306,18 +308,14 @@ hipError_t launch(hipStream_t st, const ConstrainArgs& a, void* work) {
 
 template <class T>
 hipError_t constrain(hipStream_t st, const ConstrainArgs& a, void* work) {
-  switch (slab_shape(a.r, a.v).threads) {
-    case 512: return launch<T, 512, 2>(st, a, work);
-    case 256: return launch<T, 256, 2>(st, a, work);
-    default: return launch<T, 128, 1>(st, a, work);
-  }
+  return large_slabs(a.r, a.v) ? launch<T, 512, 2>(st, a, work) : launch<T, 128, 1>(st, a, work);
 }
 
 }  // namespace
 
 size_t constrain_work_bytes(long r, long v, long width) {
   if (!width || !binned(r, v, width)) return 0;
-  return (4 * (size_t)(r * (slab_shape(r, v).count(v) + 1) + r * width) + 255) / 256 * 256;
+  return (4 * (size_t)(r * (slabs_of(r, v) + 1) + r * width) + 255) / 256 * 256;
 }
 
 hipError_t constrain_logits(hipStream_t st, int dtype, const ConstrainArgs& a, void* work) {

@@ -28,8 +28,8 @@ namespace {
 typedef unsigned long long u64;
 
 // Tokens up to which each form is taken. Rows of 2048, added to a gradient that exists: 128 tokens 8.4 us in the first and
-// 13.8 in the second, all of one id 25 and 13 (256: 8.3 and 13.7, 47 and 14; into a new gradient 18.6 and 18.1); 8192
-// tokens 35 in the second and 40 in the third, 12000 49 and 49.
+// 13.8 in the second, all of one id 25 and 13 (256: 8.3 and 13.7, 47 and 14; into a new gradient 18.6 and 18.1); 4096
+// tokens 20 in the second and 32 in the third, 8192 33 and 40, 12000 50 and 50.
 constexpr long kFewIds = 128, kRankedIds = 8192;
 constexpr long kMostWaves = 2048;  // that sum chunks, as long as those have fewer than 64 tokens
 constexpr int kTile = 2048;  // ids of a workgroup of the radix sort
@@ -217,25 +217,29 @@ __global__ __launch_bounds__(256) void k_embed_few(EmbedView a, int slabs) {
 }
 
 // ---------------------------------------------------------------- places of the sorted tokens
-// By workgroups of 1024 threads: 64 tokens, a 16th of all ids each wavefront, from LDS. In front of the
-// workgroup's own tokens an equal id counts, behind them it does not. Workgroups from `ranks` on clear dE.
-template <class O>
+// Ids of one of n shares of t, a multiple of 4.
+inline __host__ __device__ int rank_segment(int t, int n) { return (t + 4 * n - 1) / (4 * n) * 4; }
+// By workgroups of 1024 threads: 64 / G tokens, each with G lanes of every wavefront, which share all ids between them,
+// from LDS (4096 tokens: 20.4 us the gradient with 4 lanes a token, 24.6 with one). In front of the workgroup's own tokens an equal id counts, behind them it does not. Workgroups from `ranks`
+// on clear dE.
+template <class O, int G>
 __global__ __launch_bounds__(1024) void k_embed_rank(EmbedView a, long ranks, long fills, uint32_t* __restrict__ keys,
                                                      int* __restrict__ order, uint32_t* __restrict__ runs) {
-  __shared__ uint32_t key[kRankedIds];
-  __shared__ int part[16][64];
+  constexpr int NT = 64 / G, SEGS = 16 * G;
+  extern __shared__ __align__(16) uint32_t key[];
+  __shared__ int part[SEGS][NT];
   const long b = block_id();
   if (b >= ranks) return clear<O, true>(a, 0, 1, b - ranks, fills);
   if (b == 0 && threadIdx.x == 0) *runs = 0;
-  const int t = (int)a.t, t0 = (int)b * 64, lane = threadIdx.x & 63, wv = threadIdx.x >> 6;
-  const int seg = (t + 63) / 64 * 4;  // a multiple of 4; 16 of them hold all
-  for (int i = threadIdx.x; i < 16 * seg; i += 1024)
+  const int t = (int)a.t, lane = threadIdx.x & (NT - 1), sg = threadIdx.x / NT;
+  const int t0 = (int)b * NT, seg = rank_segment(t, SEGS);
+  for (int i = threadIdx.x; i < SEGS * seg; i += 1024)
     key[i] = i < t ? id_key(a.ids[i], a.ignore, (uint32_t)a.v) : ~0u;
   __syncthreads();
   const uint32_t own = t0 + lane < t ? key[t0 + lane] : ~0u;
   int n = 0;
-  const int s0 = wv * seg, s1 = s0 + seg;
-  const int before = min(s1, max(s0, t0)), after = min(s1, max(s0, t0 + 64));
+  const int s0 = sg * seg, s1 = s0 + seg;
+  const int before = min(s1, max(s0, t0)), after = min(s1, max(s0, t0 + NT));
 #pragma unroll 4
   for (int s = s0; s < before; s += 4) {
     const uint4 k = *reinterpret_cast<const uint4*>(key + s);
@@ -247,15 +251,21 @@ __global__ __launch_bounds__(1024) void k_embed_rank(EmbedView a, long ranks, lo
     const uint4 k = *reinterpret_cast<const uint4*>(key + s);
     n += k.x < own, n += k.y < own, n += k.z < own, n += k.w < own;
   }
-  part[wv][lane] = n;
+  part[sg][lane] = n;
   __syncthreads();
-  if (wv == 0 && t0 + lane < t) {
+  if (threadIdx.x < NT && t0 + lane < t) {
     int at = 0;
 #pragma unroll
-    for (int w = 0; w < 16; ++w) at += part[w][lane];
+    for (int w = 0; w < SEGS; ++w) at += part[w][lane];
     keys[at] = own;
     order[at] = t0 + lane;
   }
+}
+template <class O, int G>
+void rank(hipStream_t st, const EmbedView& a, long fills, uint32_t* keys, int* order, uint32_t* runs) {
+  const long ranks = (a.t * G + 63) / 64;
+  const size_t lds = 4 * (size_t)(16 * G) * rank_segment((int)a.t, 16 * G);
+  k_embed_rank<O, G><<<launch_grid(ranks + fills), 1024, lds, st>>>(a, ranks, fills, keys, order, runs);
 }
 
 // One pass of the radix sort is two launches. Each clears a share of dE beside it, by the workgroups from `tiles` on.
@@ -580,8 +590,9 @@ hipError_t backward(hipStream_t st, EmbedView a, void* work) {
   uint32_t* const runs = reinterpret_cast<uint32_t*>(w + p.runs);
   int at = 0;
   if (a.t <= kRankedIds) {
-    const long ranks = (a.t + 63) / 64, fills = clearing(a, a.v * a.d);
-    k_embed_rank<O><<<launch_grid(ranks + fills), 1024, 0, st>>>(a, ranks, fills, keys[0], order[0], runs);
+    const long fills = clearing(a, a.v * a.d);  // as many lanes a token as give every CU a workgroup
+    if (a.t > 4096) rank<O, 2>(st, a, fills, keys[0], order[0], runs);
+    else rank<O, 4>(st, a, fills, keys[0], order[0], runs);
   } else {
     const int n = 2 * p.passes;
     const long fills = clearing(a, a.v * a.d / n);

@@ -2,7 +2,7 @@
 // their data: 16 bytes a lane of the 16-bit types, 32 of f32. Rows may start at any element: the 16-byte accesses
 // of gfx950 need no more alignment than an element's. The loops over whole units have no other path for a row's last,
 // shorter one: with it beside each access the compiler waits for every load by itself (16384 embedding rows of
-// 4096: 68 us, without 41).
+// 4096: 68 us, without 40).
 #pragma once
 
 #include "mma16.h"

@@ -509,9 +509,9 @@ def constrain_logits(ctx: Context, logits: torch.Tensor, history: torch.Tensor |
     L = _L()
     need = L.cdclq_constrain_work_bytes(r, v, width) if width else 0
     work = _work(need, logits.device) if need else None
-    ctx.check(L.cdclq_constrain_logits_device(ctx.ptr, logits.data_ptr(), ld, r, v, code, hp, ldh, width, lp, pp, *by, bt, bv,
-                                              nb, mp, ldm, masks, mr, out.data_ptr(), ldo, work.data_ptr() if need else None,
-                                              need, _stream(ctx)))
+    ctx.check(L.cdclq_constrain_logits_device(ctx.ptr, logits.data_ptr(), ld, r, v, code, hp, ldh, width, lp, pp, *by,
+                                              bt, bv, nb, mp, ldm, masks, mr, out.data_ptr(), ldo,
+                                              work.data_ptr() if need else None, need, _stream(ctx)))
     return out
 
 

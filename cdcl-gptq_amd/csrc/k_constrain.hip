@@ -37,8 +37,8 @@ struct Binned {
 };
 
 // A workgroup takes a request: counts, their running sum, and the tokens' places, in any order within a slab.
-__global__ __launch_bounds__(1024) void k_constrain_bin(ConstrainArgs a, int log_slab, int slabs, uint32_t* __restrict__ start,
-                                                        uint32_t* __restrict__ place) {
+__global__ __launch_bounds__(1024) void k_constrain_bin(ConstrainArgs a, int log_slab, int slabs,
+                                                        uint32_t* __restrict__ start, uint32_t* __restrict__ place) {
   extern __shared__ __align__(16) uint32_t word[];  // a slab's count, then where its next token goes
   constexpr int kOnce = 8192;  // tokens that a round takes, 8 a thread
   __shared__ uint32_t sums[16], sorted[kOnce];

@@ -33,7 +33,9 @@ typedef unsigned long long u64;
 // 13.8 in the second, all of one id 25 and 13 (256: 8.3 and 13.7, 47 and 14; into a new gradient 18.6 and 18.1); 4096
 // tokens 20 in the second and 32 in the third, 8192 33 and 40, 12000 50 and 50.
 constexpr long kFewIds = 128, kRankedIds = 8192;
-constexpr long kMostWaves = 2048;  // that sum chunks, as long as those have fewer than 64 tokens
+// Wavefronts that sum chunks, as long as those have fewer than 64 tokens: 32768 x 2048: 104 us a step, with four times as
+// many (chunks of 16, more runs to join) 113.
+constexpr long kMostWaves = 2048;
 constexpr int kTile = 2048;  // ids of a workgroup of the radix sort
 
 __device__ __forceinline__ long block_id() { return blockIdx.x + (long)blockIdx.y * gridDim.x; }
@@ -222,8 +224,8 @@ __global__ __launch_bounds__(256) void k_embed_few(EmbedView a, int slabs) {
 // Ids of one of n shares of t, a multiple of 4.
 inline __host__ __device__ int rank_segment(int t, int n) { return (t + 4 * n - 1) / (4 * n) * 4; }
 // By workgroups of 1024 threads: 64 / G tokens, each with G lanes of every wavefront, which share all ids between them,
-// from LDS (4096 tokens: 20.4 us the gradient with 4 lanes a token, 24.6 with one). In front of the workgroup's own tokens an equal id counts, behind them it does not. Workgroups from `ranks`
-// on clear dE.
+// from LDS (4096 tokens: 20.4 us the gradient with 4 lanes a token, 24.6 with one). In front of the workgroup's own tokens
+// an equal id counts, behind them it does not. Workgroups from `ranks` on clear dE.
 template <class O, int G>
 __global__ __launch_bounds__(1024) void k_embed_rank(EmbedView a, long ranks, long fills, uint32_t* __restrict__ keys,
                                                      int* __restrict__ order, uint32_t* __restrict__ runs) {
@@ -307,7 +309,7 @@ __global__ __launch_bounds__(512) void k_embed_count(EmbedView a, SortPass p) {
 
 // Stable: a workgroup of 8 wavefronts moves a tile, each wavefront 256 neighbouring ids in 4 rounds of 64. A round's
 // lanes of one digit find each other by a ballot for each bit. The digits' places are summed from all tiles' counts by
-// every workgroup (a scan of its own would be a launch more).
+// every workgroup (running sums in a launch of their own: 16384 ids 37.3 us and 37.5, 131072 66 and 72, 2^21 254 and 273).
 template <class O>
 __global__ __launch_bounds__(512) void k_embed_sort(EmbedView a, SortPass p) {
   __shared__ uint32_t place[8][512];
@@ -600,8 +602,8 @@ hipError_t backward(hipStream_t st, EmbedView a, void* work) {
     const long fills = clearing(a, a.v * a.d / n);
     at = 1;
     for (int i = 0; i < p.passes; ++i) {
-      SortPass s = {p.tiles, p.bits, i * p.bits, 2 * i, n, fills, reinterpret_cast<uint32_t*>(w + p.hist), i ? keys[at] : nullptr,
-                    order[at], keys[at ^ 1], order[at ^ 1], runs};
+      SortPass s = {p.tiles, p.bits, i * p.bits, 2 * i, n, fills, reinterpret_cast<uint32_t*>(w + p.hist),
+                    i ? keys[at] : nullptr, order[at], keys[at ^ 1], order[at ^ 1], runs};
       k_embed_count<O><<<launch_grid(p.tiles + fills), 512, 0, st>>>(a, s);
       ++s.launch;
       k_embed_sort<O><<<launch_grid(p.tiles + fills), 512, 0, st>>>(a, s);
@@ -626,8 +628,8 @@ hipError_t embed_rows(hipStream_t st, int dtype, const uint16_t* table, long ldt
   const int lanes = row_lanes(d);
   const long parts = (d + 64l * lanes - 1) / (64l * lanes), per = 256 / lanes;
   const dim3 grid = launch_grid((t * parts + per - 1) / per);
-  if (dtype == CDCLQ_DTYPE_BF16) k_embed_rows<Bf16><<<grid, 256, 0, st>>>(table, ldt, v, d, ids, t, scale, ignore, out, ldo, lanes, parts);
-  else k_embed_rows<F16><<<grid, 256, 0, st>>>(table, ldt, v, d, ids, t, scale, ignore, out, ldo, lanes, parts);
+  const auto rows = dtype == CDCLQ_DTYPE_BF16 ? k_embed_rows<Bf16> : k_embed_rows<F16>;
+  rows<<<grid, 256, 0, st>>>(table, ldt, v, d, ids, t, scale, ignore, out, ldo, lanes, parts);
   return hipGetLastError();
 }
 

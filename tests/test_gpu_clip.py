@@ -279,5 +279,11 @@ def test_refusals(ctx, tune):
                  (cdclq.CdclqError, lambda: tune.clip_grads(tune.Gradients(ctx, [x[:2]], out=[x[1:3]]), 1.0))]:
         with pytest.raises(e):
             f()
+    g, n = tune.Gradients(ctx, [x]), torch.empty((), device="cuda")
+    for work, size in ((0, 0), (torch.empty(1024, dtype=torch.uint8, device="cuda").data_ptr(), g.work_bytes - 1)):
+        for call in (lambda: cdclq.lib().cdclq_grad_norm_device(ctx.ptr, g.ptr, 1, 1, n.data_ptr(), work, size, 0),
+                     lambda: cdclq.lib().cdclq_clip_grads_device(ctx.ptr, g.ptr, 1, 1, 1.0, n.data_ptr(), work, size, 0)):
+            assert call() == cdclq.INVALID_ARG and b"workspace" in cdclq.lib().cdclq_last_error(ctx.ptr)
+    assert cdclq.lib().cdclq_grad_norm_device(ctx.ptr, g.ptr, 1, 7, n.data_ptr(), 0, 0, 0) == cdclq.INVALID_ARG  # parts
     assert torch.equal(x, normal(1, 4, 6)) and torch.equal(y, normal(2, 4, 6))
     close_norm(tune.grad_norm(tune.Gradients(ctx, [x, x])), norms([x, x])[0])  # nothing is written: twice is twice

@@ -316,6 +316,13 @@ def test_refusals(ctx, tune):
         tune.constrain_logits(ctx, x, history=torch.zeros(r, 1 << 20, dtype=torch.int64, device="cuda"))
     with pytest.raises(cdclq.CdclqError, match="vocabulary"):
         tune.constrain_logits(ctx, x[:, :0])
+    h, big = torch.zeros(64, 16_000, dtype=torch.int64, device="cuda"), normal(3, 64, 20_000)
+    assert cdclq.lib().cdclq_constrain_work_bytes(64, 20_000, 16_000) == 0  # looked at by every slab
+    assert cdclq.lib().cdclq_constrain_work_bytes(64, 20_000, 60_000) > 4 * 64 * 60_000
+    rc = cdclq.lib().cdclq_constrain_logits_device(ctx.ptr, big.data_ptr(), 20_000, 64, 20_000, cdclq.DTYPE_F32, h.data_ptr(),
+                                                   16_000, 15_999 + 50_000, 0, 0, 0, 0, 0, 0, 0, 0, 0, 0, 0, 0, big.data_ptr(),
+                                                   20_000, 0, 0, 0)
+    assert rc == cdclq.INVALID_ARG  # rows of the history shorter than its width, and no workspace
     with pytest.raises(ValueError, match="without a history"):
         tune.constrain_logits(ctx, x, repetition=k["repetition"])
     assert torch.equal(x, normal(1, r, v))

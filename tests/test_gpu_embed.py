@@ -124,7 +124,7 @@ def test_rows_of_strided_tables(ctx, tune, dtype, offset, ld):
 # ---------------------------------------------------------------- gradient
 SIZES = [(1, 1, 1), (1, 8, 3), (7, 33, 20), (64, 100, 50), (65, 4096, 70), (128, 72, 50), (129, 72, 50), (511, 72, 1000), (512, 130, 20),
          (513, 130, 20), (600, 2056, 300), (1025, 65, 5000), (4096, 64, 257), (8192, 40, 999), (8193, 40, 999),
-         (12289, 24, 100), (20000, 520, 70000), (70001, 8, 300)]
+         (12289, 24, 100), (20000, 520, 70000), (70001, 8, 300), (530_001, 8, 70_000), (1_100_000, 16, 500)]
 
 
 @pytest.mark.parametrize("dtype", TYPES)

@@ -9,8 +9,8 @@
 //
 // The gradient sums a row's tokens in their order, in f32, with one rounding at the end and no float atomics:
 // equal inputs give equal bits. Three forms by the number of tokens:
-//   few     a launch that clears dE, one in which a workgroup takes a token, finds the others of its id by comparing all
-//           ids, and leaves unless it is the first of them.
+//   few     one launch: a workgroup takes a token, finds the others of its id by comparing all ids, and leaves unless it
+//           is the first of them; other workgroups clear the rows without tokens.
 //   ranked  a token's place among the sorted ones is the number of smaller (id, position) pairs, counted by
 //           comparing all pairs of tokens in one launch, which clears dE beside it. Then chunks of the sorted tokens
 //           are summed; runs of equal ids that pass a chunk's end are joined by a third launch.
@@ -33,6 +33,7 @@ typedef unsigned long long u64;
 // 13.8 in the second, all of one id 25 and 13 (256: 8.3 and 13.7, 47 and 14; into a new gradient 18.6 and 18.1); 4096
 // tokens 20 in the second and 32 in the third, 8192 33 and 40, 12000 50 and 50.
 constexpr long kFewIds = 128, kRankedIds = 8192;
+static_assert(kFewIds <= 256, "64 ids a wavefront of k_embed_few");
 // Wavefronts that sum chunks, as long as those have fewer than 64 tokens: 32768 x 2048: 104 us a step, with four times as
 // many (chunks of 16, more runs to join) 113.
 constexpr long kMostWaves = 2048;
@@ -159,32 +160,44 @@ __device__ __forceinline__ Row8<T> load8(const EmbedView& a, long row, long c) {
   else return row8_load<T>(p, (int)(a.d - c));
 }
 
-template <class O>
-__global__ __launch_bounds__(512) void k_embed_clear(EmbedView a) {
-  clear<O, true>(a, 0, 1, block_id(), (long)gridDim.x * gridDim.y);
-}
-
 // ---------------------------------------------------------------- few tokens
-// Workgroup b: token b / slabs, 8 x 256 columns.
+// Rows that a workgroup clears: 16 KB of them.
+inline long few_rows(long d) { return std::max(1l, std::min(8192 / d, 1024l)); }
+
+// Workgroups below t slabs: token b / slabs, 8 x 256 columns. The others clear `rows` rows each, but those of tokens
+// (77 tokens, 1000 of 50001: 16.8 us, 6.0 TB/s; with the clearing as a launch before 15.2 + 4.6).
 template <class T, class O>
-__global__ __launch_bounds__(256) void k_embed_few(EmbedView a, int slabs) {
+__global__ __launch_bounds__(256) void k_embed_few(EmbedView a, int slabs, int rows) {
   __shared__ u64 same[kFewIds / 64], bad[kFewIds / 64];
-  const long b = block_id();
+  __shared__ uint8_t has[1024];
+  const long b = block_id(), sums = a.t * slabs, blocks = sums + (a.add ? 0 : (a.v + rows - 1) / rows);
   const int wv = threadIdx.x >> 6, lane = threadIdx.x & 63;
-  if (b >= a.t * slabs) return;
-  const int tok = (int)(b / slabs);
-  const uint32_t v = (uint32_t)a.v, own = id_key(a.ids[tok], a.ignore, v);
-  for (int w = wv; 64 * w < a.t; w += 4) {
-    const int i = 64 * w + lane;
+  if (b >= blocks) return;
+  const bool clears = b >= sums;
+  const int tok = clears ? 0 : (int)(b / slabs), words = (int)((a.t + 63) / 64);
+  const long r0 = clears ? (b - sums) * rows : 0, r1 = min(a.v, r0 + rows);
+  const uint32_t v = (uint32_t)a.v, own = clears ? 0 : id_key(a.ids[tok], a.ignore, v);
+  if (clears)
+    for (int i = threadIdx.x; i < rows; i += 256) has[i] = 0;
+  __syncthreads();
+  if (wv < words) {  // `same`: the tokens of this one's id, or those of the rows to clear
+    const int i = 64 * wv + lane;
     const uint32_t k = i < a.t ? id_key(a.ids[i], a.ignore, v) : v;
-    const u64 s = __ballot(i < a.t && k == own), n = __ballot(k > v);
-    if (lane == 0) same[w] = s, bad[w] = n;
+    const bool mine = clears ? k < v && k >= r0 && k < r1 : i < a.t && k == own;
+    const u64 s = __ballot(mine), n = __ballot(k > v);
+    if (lane == 0) same[wv] = s, bad[wv] = n;
+    if (clears && mine) has[k - r0] = 1;
   }
   __syncthreads();
-  const int words = (int)((a.t + 63) / 64);
-  u64 any = 0;
-  for (int w = 0; w < words; ++w) any |= bad[w];
-  if (any) return poison<O>(a, b, a.t * slabs);
+  u64 any = 0, hit = 0;
+  for (int w = 0; w < words; ++w) any |= bad[w], hit |= same[w];
+  if (any) return poison<O>(a, b, blocks);
+  if (clears) {
+    if (!hit) return fill<O, true>(a, r0 * a.d, r1 * a.d, 0, 1, 0.0f);
+    for (long r = r0; r < r1; ++r)
+      if (!has[r - r0]) fill<O, true>(a, r * a.d, (r + 1) * a.d, 0, 1, 0.0f);
+    return;
+  }
   if (own >= v) return;
   for (int w = 0; w <= tok / 64; ++w)
     if (same[w] & (w < tok / 64 ? ~0ull : (1ull << (tok & 63)) - 1)) return;  // an earlier token sums them
@@ -578,9 +591,9 @@ long clearing(const EmbedView& a, long n) { return a.add ? 0 : std::max(1l, std:
 template <class T, class O>
 hipError_t backward(hipStream_t st, EmbedView a, void* work) {
   if (a.t <= kFewIds) {
-    if (!a.add) k_embed_clear<O><<<launch_grid(clearing(a, a.v * a.d)), 512, 0, st>>>(a);
-    const int slabs = (int)((a.d + 2047) / 2048);
-    if (a.t) k_embed_few<T, O><<<launch_grid(a.t * slabs), 256, 0, st>>>(a, slabs);
+    const int slabs = (int)((a.d + 2047) / 2048), rows = (int)few_rows(a.d);
+    const long blocks = a.t * slabs + (a.add ? 0 : (a.v + rows - 1) / rows);
+    k_embed_few<T, O><<<launch_grid(blocks), 256, 0, st>>>(a, slabs, rows);
     return hipGetLastError();
   }
   const EmbedPlan p = embed_plan(a.t, a.d, a.v);

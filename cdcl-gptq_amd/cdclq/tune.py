@@ -349,10 +349,11 @@ def embed_backward(ctx: Context, dy: torch.Tensor, tokens: torch.Tensor, vocab: 
             raise TypeError(f"into is {de.dtype}, need {dy.dtype} or torch.float32")
         kind, lde = _CODES32[de.dtype], _matrix(ctx, de, "into", None, vocab, d)
     L = _L()
-    work = _work(L.cdclq_embed_work_bytes(t, d, vocab), dy.device)
+    need = L.cdclq_embed_work_bytes(t, d, vocab)
+    work = _work(need, dy.device) if need else None
     ctx.check(L.cdclq_embed_backward_device(ctx.ptr, dy.data_ptr(), ld, t, d, vocab, code, tokens.data_ptr(), scale,
-                                            ignore_index, into is not None, de.data_ptr(), lde, kind, work.data_ptr(),
-                                            work.numel(), _stream(ctx)))
+                                            ignore_index, into is not None, de.data_ptr(), lde, kind,
+                                            work.data_ptr() if need else None, need, _stream(ctx)))
     return de
 
 
@@ -370,50 +371,53 @@ class Gradients:
         self.ctx, self.tensors, self.out = ctx, list(tensors), None if out is None else list(out)
         self.parts = 1 if adapters is None else int(adapters)
         self.shape = () if adapters is None else (self.parts,)
-        outs = self.tensors if self.out is None else self.out
-        if len(outs) != len(self.tensors):
-            raise ValueError(f"{len(self.tensors)} gradients and {len(outs)} outputs")
+        if self.out is not None and len(self.out) != len(self.tensors):
+            raise ValueError(f"{len(self.tensors)} gradients and {len(self.out)} outputs")
         if adapters is not None and self.parts < 1:
             raise ValueError(f"adapters is {adapters}, need at least 1")
-        self.table = np.zeros(len(outs), _GRAD)
-        codes = []
-        for x, o in zip(self.tensors, outs):
-            for g, name in ((x, "a gradient"), (o, "an output")):
-                if g.get_device() != ctx.device:
-                    raise ValueError(f"{name} is on {g.device}, the context on cuda:{ctx.device}")
-                if g.dtype not in _CODES32:
-                    raise TypeError(f"{name} is {g.dtype}, need float32, bfloat16 or float16")
-                if not g.is_contiguous():
-                    raise ValueError(f"{name} of shape {tuple(g.shape)} has strides {g.stride()}, it must be contiguous")
-            if o.shape != x.shape:
-                raise ValueError(f"an output has shape {tuple(o.shape)}, its gradient {tuple(x.shape)}")
-            if o.dtype != x.dtype and o.dtype != torch.float32:
+        self.all, self.device = self.tensors + (self.out or []), torch.device("cuda", ctx.device)
+        self._read()
+
+    def _read(self):
+        """Checks the tensors and writes the table of what they are and where."""
+        kinds, device, n = _CODES32, self.ctx.device, len(self.tensors)
+        for g in self.all:
+            if g.dtype not in kinds:
+                raise TypeError(f"a gradient or output is {g.dtype}, need float32, bfloat16 or float16")
+            if g.get_device() != device:
+                raise ValueError(f"a gradient or output is on {g.device}, the context on cuda:{device}")
+            if not g.is_contiguous():
+                raise ValueError(f"a gradient or output of shape {tuple(g.shape)} has strides {g.stride()}, it must be "
+                                 "contiguous")
+        rows = []
+        for x, o in zip(self.tensors, self.all[-n:]):
+            shape, kind = x.shape, kinds[x.dtype]
+            if o is not x and o.shape != shape:
+                raise ValueError(f"an output has shape {tuple(o.shape)}, its gradient {tuple(shape)}")
+            to = kinds[o.dtype]
+            if to != kind and to != DTYPE_F32:
                 raise TypeError(f"an output is {o.dtype}, need {x.dtype} or torch.float32")
-            if adapters is not None and (x.dim() == 0 or x.shape[0] != self.parts):
-                raise ValueError(f"a gradient has shape {tuple(x.shape)}, need {self.parts} adapters first")
-            codes.append((x.numel(), _CODES32[x.dtype], _CODES32[o.dtype]))
-        if codes:
-            self.table["count"], self.table["dtype"], self.table["out_dtype"] = zip(*codes)
-        self.all = self.tensors + (self.out or [])
-        self.at, self.device = None, torch.device("cuda", ctx.device)
-        self._addresses()
-        self.work_bytes = _L().cdclq_grad_work_bytes(self.table.ctypes.data, len(codes), self.parts)
+            if self.shape and (not shape or shape[0] != self.parts):
+                raise ValueError(f"a gradient has shape {tuple(shape)}, need {self.parts} adapters first")
+            rows.append((x.data_ptr(), o.data_ptr(), x.numel(), kind, to))
+        self.table = np.array(rows, _GRAD)
+        self.ptr = self.table.ctypes.data
+        self.work_bytes = _L().cdclq_grad_work_bytes(self.ptr, n, self.parts)
+        self.at = list(map(_data_ptr, self.all))
 
     def _addresses(self) -> int:
-        """The table's address, with the tensors' present addresses in it."""
-        at = list(map(_data_ptr, self.all))
-        if at != self.at:
-            n = len(self.tensors)
-            self.table["x"], self.table["out"] = at[:n], at[-n:] if n else []
-            self.at, self.ptr = at, self.table.ctypes.data
+        """The table's address; tensors that have other memory by now (their .data set) are read again."""
+        if list(map(_data_ptr, self.all)) != self.at:
+            self._read()
         return self.ptr
 
 
 def _grad_call(grads: Gradients):
     if not isinstance(grads, Gradients):
         raise TypeError(f"need Gradients, got {type(grads).__name__}")
+    table = grads._addresses()
     norm = _empty(grads.shape, dtype=torch.float32, device=grads.device)
-    return grads.ctx, grads._addresses(), len(grads.tensors), norm, _work(grads.work_bytes, grads.device)
+    return grads.ctx, table, len(grads.tensors), norm, _work(grads.work_bytes, grads.device)
 
 
 def grad_norm(grads: Gradients) -> torch.Tensor:

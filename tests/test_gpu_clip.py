@@ -212,6 +212,20 @@ def test_a_set_follows_its_tensors(ctx, tune):
     b = tune.grad_norm(g)
     close_norm(b, norms([x])[0])
     assert a != b
+    for n, dtype in ((10, torch.float32), (50_000, torch.float32), (0, torch.float32)):  # of other sizes, too
+        x.data = normal(3, n, dtype=dtype)
+        close_norm(tune.grad_norm(g), norms([x])[0])
+        before = x.clone()
+        tune.clip_grads(g, 1.0)
+        check_clipped([x], [before], norms([before])[0], 1.0)
+    x.data = normal(4, 20, 30).t()
+    with pytest.raises(ValueError, match="contiguous"):
+        tune.grad_norm(g)
+    out = normal(5, 100)
+    h = tune.Gradients(ctx, [normal(6, 100)], out=[out])
+    out.data = normal(5, 99)
+    with pytest.raises(ValueError, match="shape"):
+        tune.clip_grads(h, 1.0)
 
 
 def test_captured_and_replayed(ctx, tune):

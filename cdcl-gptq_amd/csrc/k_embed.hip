@@ -4,8 +4,8 @@
 //
 // An id equal to the ignored one stands for no token: y_t = 0, and it adds nothing. Any other id outside 0..v
 // gives a row of NaN and a gradient that is NaN throughout. Both directions only move memory: 16384 rows of 4096 of a
-// table of 128256 36 us (188 MB, 5.2 TB/s); rows and gradient of 4096 tokens there 195 us, 174 of them the clearing of
-// 1.05 GB (6.0 TB/s); of 32768 tokens, 2048 of 32000, 101 us: rows 31, sorting and clearing 28, sums 39, runs of chunks 6.
+// table of 128256 36 us (188 MB, 5.2 TB/s); rows and gradient of 4096 tokens there 180 us, 159 of them the clearing of
+// 1.05 GB (6.6 TB/s); of 32768 tokens, 2048 of 32000, 101 us: rows 31, sorting and clearing 28, sums 39, runs of chunks 6.
 //
 // The gradient sums a row's tokens in their order, in f32, with one rounding at the end and no float atomics:
 // equal inputs give equal bits. Three forms by the number of tokens:
@@ -100,7 +100,8 @@ __global__ __launch_bounds__(256) void k_embed_rows(const uint16_t* __restrict__
       to[c] = !is ? T::narrow(other) : scale != 1.0f ? T::narrow(scale * T::widen(from[c])) : from[c];
 }
 
-// x in every element of share b of nb of dE's elements [e0, e1) in rows of d, counted row by row. KEEP: through the L2.
+// x in every element of share b of nb of dE's elements [e0, e1) in rows of d, counted row by row. KEEP: through the L2,
+// which is better for a few rows beside sums (77 tokens, 50001 x 1000: 19.5 us a step, past it 21.3).
 template <class O, bool KEEP>
 __device__ __forceinline__ void fill(const EmbedView& a, long e0, long e1, long b, long nb, float x) {
   typedef typename Row8<O>::stored E;
@@ -124,10 +125,10 @@ __device__ __forceinline__ void fill(const EmbedView& a, long e0, long e1, long 
     for (; c < a.d; ++c) de[r * a.lde + c] = one;
   }
 }
-// Zeros in part `i` of `n` of dE's rows.
-template <class O, bool KEEP>
+// Zeros in part `i` of `n` of dE's rows, past the L2 (4096 tokens, 128256 x 4096: 180 us a step, through it 196).
+template <class O>
 __device__ __forceinline__ void clear(const EmbedView& a, int i, int n, long b, long nb) {
-  if (b < nb) fill<O, KEEP>(a, a.v * i / n * a.d, a.v * (i + 1) / n * a.d, b, nb, 0.0f);
+  if (b < nb) fill<O, false>(a, a.v * i / n * a.d, a.v * (i + 1) / n * a.d, b, nb, 0.0f);
 }
 // dE = NaN throughout, by all workgroups of a launch (an id outside 0..v).
 template <class O>
@@ -165,11 +166,11 @@ __device__ __forceinline__ Row8<T> load8(const EmbedView& a, long row, long c) {
 inline long few_rows(long d) { return std::max(1l, std::min(8192 / d, 1024l)); }
 
 // Workgroups below t slabs: token b / slabs, 8 x 256 columns. The others clear `rows` rows each, but those of tokens
-// (77 tokens, 1000 of 50001: 16.8 us, 6.0 TB/s; with the clearing as a launch before 15.2 + 4.6).
+// (77 tokens, 1000 of 50001: 16.5 us, 6.1 TB/s; with the clearing as a launch before 15.2 + 4.6).
 template <class T, class O>
 __global__ __launch_bounds__(256) void k_embed_few(EmbedView a, int slabs, int rows) {
   __shared__ u64 same[kFewIds / 64], bad[kFewIds / 64];
-  __shared__ uint8_t has[1024];
+  __shared__ uint32_t hits[32];  // a bit for each row to clear that has tokens
   const long b = block_id(), sums = a.t * slabs, blocks = sums + (a.add ? 0 : (a.v + rows - 1) / rows);
   const int wv = threadIdx.x >> 6, lane = threadIdx.x & 63;
   if (b >= blocks) return;
@@ -177,8 +178,7 @@ __global__ __launch_bounds__(256) void k_embed_few(EmbedView a, int slabs, int r
   const int tok = clears ? 0 : (int)(b / slabs), words = (int)((a.t + 63) / 64);
   const long r0 = clears ? (b - sums) * rows : 0, r1 = min(a.v, r0 + rows);
   const uint32_t v = (uint32_t)a.v, own = clears ? 0 : id_key(a.ids[tok], a.ignore, v);
-  if (clears)
-    for (int i = threadIdx.x; i < rows; i += 256) has[i] = 0;
+  if (threadIdx.x < 32) hits[threadIdx.x] = 0;
   __syncthreads();
   if (wv < words) {  // `same`: the tokens of this one's id, or those of the rows to clear
     const int i = 64 * wv + lane;
@@ -186,16 +186,28 @@ __global__ __launch_bounds__(256) void k_embed_few(EmbedView a, int slabs, int r
     const bool mine = clears ? k < v && k >= r0 && k < r1 : i < a.t && k == own;
     const u64 s = __ballot(mine), n = __ballot(k > v);
     if (lane == 0) same[wv] = s, bad[wv] = n;
-    if (clears && mine) has[k - r0] = 1;
+    if (clears && mine) atomicOr(&hits[(k - r0) >> 5], 1u << ((k - r0) & 31));
   }
   __syncthreads();
-  u64 any = 0, hit = 0;
-  for (int w = 0; w < words; ++w) any |= bad[w], hit |= same[w];
+  u64 any = 0;
+  for (int w = 0; w < words; ++w) any |= bad[w];
   if (any) return poison<O>(a, b, blocks);
-  if (clears) {
-    if (!hit) return fill<O, true>(a, r0 * a.d, r1 * a.d, 0, 1, 0.0f);
-    for (long r = r0; r < r1; ++r)
-      if (!has[r - r0]) fill<O, true>(a, r * a.d, (r + 1) * a.d, 0, 1, 0.0f);
+  if (clears) {  // the rows between those of tokens
+    const int n = (int)(r1 - r0);
+    for (int i = 0; i < n;) {
+      int e = i;
+      while (e < n) {
+        const uint32_t m = hits[e >> 5] >> (e & 31);
+        if (m) {
+          e += __builtin_ctz(m);
+          break;
+        }
+        e = (e | 31) + 1;
+      }
+      e = min(e, n);
+      if (e > i) fill<O, true>(a, (r0 + i) * a.d, (r0 + e) * a.d, 0, 1, 0.0f);
+      i = e + 1;
+    }
     return;
   }
   if (own >= v) return;
@@ -246,7 +258,7 @@ __global__ __launch_bounds__(1024) void k_embed_rank(EmbedView a, long ranks, lo
   extern __shared__ __align__(16) uint32_t key[];
   __shared__ int part[SEGS][NT];
   const long b = block_id();
-  if (b >= ranks) return clear<O, true>(a, 0, 1, b - ranks, fills);
+  if (b >= ranks) return clear<O>(a, 0, 1, b - ranks, fills);
   if (b == 0 && threadIdx.x == 0) *runs = 0;
   const int t = (int)a.t, lane = threadIdx.x & (NT - 1), sg = threadIdx.x / NT;
   const int t0 = (int)b * NT, seg = rank_segment(t, SEGS);
@@ -303,7 +315,7 @@ template <class O>
 __global__ __launch_bounds__(512) void k_embed_count(EmbedView a, SortPass p) {
   __shared__ uint32_t n[512];
   const long b = block_id();
-  if (b >= p.tiles) return clear<O, false>(a, p.launch, p.launches, b - p.tiles, p.fills);
+  if (b >= p.tiles) return clear<O>(a, p.launch, p.launches, b - p.tiles, p.fills);
   if (b == 0 && threadIdx.x == 0) *p.runs = 0;
   n[threadIdx.x] = 0;
   __syncthreads();
@@ -327,7 +339,7 @@ template <class O>
 __global__ __launch_bounds__(512) void k_embed_sort(EmbedView a, SortPass p) {
   __shared__ uint32_t place[8][512];
   __shared__ uint32_t scan[8];
-  if (block_id() >= p.tiles) return clear<O, false>(a, p.launch, p.launches, block_id() - p.tiles, p.fills);
+  if (block_id() >= p.tiles) return clear<O>(a, p.launch, p.launches, block_id() - p.tiles, p.fills);
   constexpr int R = kTile / 512;
   const int wv = threadIdx.x >> 6, lane = threadIdx.x & 63, digits = 1 << p.bits;
   const long tile = block_id(), base = tile * kTile + wv * (64 * R);
@@ -584,8 +596,8 @@ EmbedPlan embed_plan(long t, long d, long v) {
   return p;
 }
 
-// Workgroups that clear n elements of dE, a store a thread or a few: 4096 tokens, 128256 x 4096: 198 us a step, with 64 KB
-// each 218, with 1 MB 213.
+// Workgroups that clear n elements of dE, 16 KB of bf16 each: 4096 tokens, 128256 x 4096: 180 us a step, with 8 KB each
+// 193, with 32 KB 195.
 long clearing(const EmbedView& a, long n) { return a.add ? 0 : std::max(1l, std::min(n / 8192, 1l << 20)); }
 
 template <class T, class O>

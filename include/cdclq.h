@@ -446,7 +446,8 @@ int cdclq_clip_grads_device(cdclq_ctx* ctx, const cdclq_grad* grads, size_t n, s
  * none, a token that is there several times gets the sum in their order. mask: nmasks x ceil(v / 32) words (row stride
  * ld_mask), token i at bit i % 32 of word i / 32; mask_rows[i]: the request's row of it, -1 for none, any other value
  * outside 0..nmasks gives a row of NaN; NULL: row i (nmasks = r). out may be logits (with the same stride); it must not
- * overlap it otherwise. Logits that nothing applies to keep their bits. width < 2^20, nbias <= 1024. */
+ * overlap it otherwise. Logits that nothing applies to keep their bits. width < 2^20, nbias <= 1024. The workspace is
+ * for long histories only (0 bytes: none). */
 size_t cdclq_constrain_work_bytes(size_t r, size_t v, size_t width);
 int cdclq_constrain_logits_device(cdclq_ctx* ctx, const void* logits, size_t ld, size_t r, size_t v, int dtype,
                                   const int64_t* history, size_t ld_history, size_t width, const int32_t* lengths,

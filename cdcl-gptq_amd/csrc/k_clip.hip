@@ -13,9 +13,9 @@
 // the first one left in the last cache. In place nothing is read again where c = 1.
 // The tensors' addresses come as a launch's arguments, so that a captured call keeps them and the host has nothing to copy
 // or to wait for; sets of more than one launch takes are written to a table in the workspace by small launches first
-// (448 tensors, 84 MB into f32: 82 us, as three launches a pass 113). Those today: 63-71 us, of them 10 the table, 18 the
-// norm (4.7 TB/s) and 37 the clipping (6.8 TB/s, its reads from the last cache), the rest the host, which looks at the
-// addresses of 896 tensors; 1.4 GB into a second set: 706 us, 213 (6.5 TB/s) and 464 (6.0).
+// (448 tensors, 84 MB into f32: 82 us, as three launches a pass 113). Those today: 59-66 us, of them 6 the table, 18 the
+// norm (4.7 TB/s) and 37 the clipping (6.8 TB/s, its reads from the last cache), or the host, which looks at the addresses
+// of 896 tensors; 1.4 GB into a second set: 688 us, 214 (6.5 TB/s) and 466 (6.0).
 #include <hip/hip_runtime.h>
 
 #include <algorithm>
@@ -28,6 +28,7 @@ namespace cdclq {
 namespace {
 
 constexpr int kTensors = 150;           // of one launch: its arguments keep below 4 KB
+constexpr int kRows = 230;              // of one launch that writes the table
 constexpr int kChunk = 4096;            // elements
 constexpr long kMostPart = 1l << 30;    // elements of a part that one entry of the tables takes
 constexpr long kMostSums = 4096;        // of all parts together, where parts have several
@@ -50,6 +51,16 @@ struct ClipArgs {
   int count;
 };
 static_assert(sizeof(ClipArgs) < 3900, "a launch's arguments");
+// Some of the tensors as the arguments of a launch that writes the table, 17 bytes each: addresses have 48 bits, and the
+// chunks are counted there (448 tensors in two launches; as three, of ClipArgs, 4 us more).
+struct ClipRows {
+  uint32_t x[kRows], out[kRows], n[kRows];
+  uint16_t x_high[kRows], out_high[kRows];
+  uint8_t kind[kRows];
+  int count;
+  uint32_t base, chunk;  // of the first one: its place in the table, and its first chunk
+};
+static_assert(sizeof(ClipRows) < 3950, "a launch's arguments");
 // The tensors in device memory, and the tensor of each chunk.
 struct ClipTable {
   const ClipEntry* entries;
@@ -69,12 +80,23 @@ __device__ __forceinline__ ClipEntry entry_of(const ClipArgs& s, uint32_t chunk)
 }
 __device__ __forceinline__ ClipEntry entry_of(const ClipTable& s, uint32_t chunk) { return s.entries[s.who[chunk]]; }
 
-__global__ __launch_bounds__(256) void k_clip_table(const ClipArgs s, uint32_t base, ClipEntry* __restrict__ entries,
+// The workgroups blockIdx.y take tensor blockIdx.x: a large one's chunks are many (a head of 525 M elements: 20 us by one
+// workgroup, 5 by 16).
+__global__ __launch_bounds__(256) void k_clip_table(const ClipRows s, ClipEntry* __restrict__ entries,
                                                     uint32_t* __restrict__ who) {
-  for (int e = blockIdx.x; e < s.count; e += gridDim.x) {
-    const uint32_t chunks = (s.n[e] + kChunk - 1) / kChunk;
-    for (uint32_t i = threadIdx.x; i < chunks; i += 256) who[s.start[e] + i] = base + e;
-    if (threadIdx.x == 0) entries[base + e] = {s.x[e], s.out[e], s.n[e], s.start[e], s.kind[e]};
+  __shared__ uint32_t part[4];
+  const int e = blockIdx.x, i = threadIdx.x;
+  auto chunks = [&](int of) { return (s.n[of] + kChunk - 1) / kChunk; };
+  uint32_t start = i < e ? chunks(i) : 0;  // summed: of the tensors before
+#pragma unroll
+  for (int k = 32; k; k >>= 1) start += (uint32_t)__shfl_xor((int)start, k);
+  if ((i & 63) == 0) part[i >> 6] = start;
+  __syncthreads();
+  start = s.chunk + part[0] + part[1] + part[2] + part[3];
+  for (uint32_t c = 256 * blockIdx.y + i; c < chunks(e); c += 256 * gridDim.y) who[start + c] = s.base + e;
+  if (i == 0 && blockIdx.y == 0) {
+    const uint64_t x = (uint64_t)s.x_high[e] << 32 | s.x[e], out = (uint64_t)s.out_high[e] << 32 | s.out[e];
+    entries[s.base + e] = {reinterpret_cast<const void*>(x), reinterpret_cast<void*>(out), s.n[e], start, s.kind[e]};
   }
 }
 
@@ -238,37 +260,55 @@ ClipPlan clip_plan(const GradTensor* g, size_t n, int parts) {
 // Hands the tensors to `go`, as arguments or as a table.
 template <class F>
 hipError_t with_tensors(hipStream_t st, const GradTensor* g, size_t n, int parts, const ClipPlan& p, char* work, F go) {
-  ClipArgs s;
-  s.count = 0;
-  uint32_t chunk = 0, base = 0;
+  auto pieces = [&](auto take) {  // each with its first chunk
+    uint32_t chunk = 0;
+    for (size_t i = 0; i < n; ++i) {
+      const long e = g[i].n / parts;
+      const size_t size = g[i].dtype == CDCLQ_DTYPE_F32 ? 4 : 2, out_size = g[i].out_dtype == CDCLQ_DTYPE_F32 ? 4 : 2;
+      const uint32_t kind = (uint32_t)g[i].dtype | (g[i].out_dtype == CDCLQ_DTYPE_F32 ? 4 : 0);
+      for (long at = 0; at < e; at += kMostPart) {
+        const uint32_t len = (uint32_t)std::min(kMostPart, e - at);
+        take(ClipEntry{static_cast<const char*>(g[i].x) + at * size, static_cast<char*>(g[i].out) + at * out_size, len,
+                       chunk, kind});
+        chunk += (len + kChunk - 1) / kChunk;
+      }
+    }
+  };
+  if (p.entries <= kTensors) {
+    ClipArgs s;
+    s.count = 0;
+    pieces([&](const ClipEntry& e) {
+      const int k = s.count++;
+      s.x[k] = e.x, s.out[k] = e.out, s.n[k] = e.n, s.start[k] = e.start, s.kind[k] = (uint8_t)e.kind;
+    });
+    go(s);
+    return hipGetLastError();
+  }
   ClipEntry* const entries = reinterpret_cast<ClipEntry*>(work + p.table);
   uint32_t* const who = reinterpret_cast<uint32_t*>(work + p.who);
-  auto table = [&] {
-    k_clip_table<<<std::min(s.count, 128), 256, 0, st>>>(s, base, entries, who);
-    base += (uint32_t)s.count;
-    s.count = 0;
+  ClipRows s;
+  s.count = 0, s.base = 0;
+  uint64_t high = 0;
+  long most = 0;  // chunks of a tensor in this launch
+  pieces([&](const ClipEntry& e) { high |= (uint64_t)e.x | (uint64_t)e.out; });
+  if (high >> 48) return hipErrorInvalidDevicePointer;
+  auto write = [&] {
+    k_clip_table<<<dim3(s.count, (unsigned)std::max(1l, std::min(most / 2048, 16l))), 256, 0, st>>>(s, entries, who);
+    s.base += (uint32_t)s.count;
+    s.count = 0, most = 0;
   };
-  for (size_t i = 0; i < n; ++i) {
-    const long e = g[i].n / parts;
-    const size_t size = g[i].dtype == CDCLQ_DTYPE_F32 ? 4 : 2, out_size = g[i].out_dtype == CDCLQ_DTYPE_F32 ? 4 : 2;
-    for (long at = 0; at < e; at += kMostPart) {
-      if (s.count == kTensors) table();
-      const long len = std::min(kMostPart, e - at);
-      const int k = s.count++;
-      s.x[k] = static_cast<const char*>(g[i].x) + at * size;
-      s.out[k] = static_cast<char*>(g[i].out) + at * out_size;
-      s.n[k] = (uint32_t)len;
-      s.start[k] = chunk;
-      s.kind[k] = (uint8_t)(g[i].dtype | (g[i].out_dtype == CDCLQ_DTYPE_F32 ? 4 : 0));
-      chunk += (uint32_t)((len + kChunk - 1) / kChunk);
-    }
-  }
-  if (p.entries > kTensors) {
-    table();
-    go(ClipTable{entries, who});
-  } else {
-    go(s);
-  }
+  pieces([&](const ClipEntry& e) {
+    if (s.count == kRows) write();
+    const uint64_t x = (uint64_t)e.x, out = (uint64_t)e.out;
+    const int k = s.count++;
+    if (k == 0) s.chunk = e.start;
+    s.x[k] = (uint32_t)x, s.x_high[k] = (uint16_t)(x >> 32);
+    s.out[k] = (uint32_t)out, s.out_high[k] = (uint16_t)(out >> 32);
+    s.n[k] = e.n, s.kind[k] = (uint8_t)e.kind;
+    most = std::max(most, (long)e.n / kChunk);
+  });
+  write();
+  go(ClipTable{entries, who});
   return hipGetLastError();
 }
 

@@ -284,7 +284,7 @@ int grad_tensors(cdclq_ctx* ctx, const cdclq_grad* grads, size_t n, size_t parts
                                               " elements is not " + std::to_string(parts) + " equal parts");
     if (parts > 1) CK(check_size(ctx, "part of", g.count / parts, kMaxPart));
     if (g.count && !g.x) return fail(ctx, CDCLQ_INVALID_ARG, "null buffer argument");
-    (*out)[i] = {g.x, g.out, (long)g.count, g.dtype, g.dtype};
+    (*out)[i] = {g.x, clip ? g.out : const_cast<void*>(g.x), (long)g.count, g.dtype, g.dtype};
     if (!clip) continue;
     CK(check_type(ctx, g.out_dtype));
     if (g.out_dtype != g.dtype && g.out_dtype != CDCLQ_DTYPE_F32)

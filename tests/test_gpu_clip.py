@@ -104,6 +104,27 @@ def test_many_tensors(ctx, tune, count):
     assert all(torch.equal(a, b) for a, b in zip(first, out))
 
 
+@pytest.mark.parametrize("count", [229, 230, 231, 460, 461])
+def test_tables_of_several_launches(ctx, tune, count):
+    """Sets at the ends of the launches that write the table; tensors of one and of several chunks, and adapters."""
+    tensors = [normal(i, 2, (7 + 7 * i % 77) * (1 + 613 * (i % 2)), std=1 + i % 5, dtype=TYPES[i % 3])
+               for i in range(count)]
+    for adapters in (None, 2):
+        out = [torch.empty(x.shape, device="cuda") for x in tensors]
+        g = tune.Gradients(ctx, tensors, out=out, adapters=adapters)
+        want = norms(tensors, adapters)
+        close_norm(tune.clip_grads(g, 1.0), want if adapters else want[0])
+        check_clipped(out, tensors, want, 1.0, adapters)
+
+
+@pytest.mark.parametrize("count", [3, 448])
+def test_a_norm_does_not_look_at_outputs(ctx, tune, count):
+    tensors = [normal(i, 40 + i, dtype=TYPES[i % 3]) for i in range(count)]
+    g = tune.Gradients(ctx, tensors)
+    g.table["out"] = 2**64 - 2
+    close_norm(tune.grad_norm(g), norms(tensors)[0])
+
+
 @pytest.mark.parametrize("dtype", TYPES)
 @pytest.mark.parametrize("users", [1, 2, 5, 300])
 def test_each_adapter_by_its_own_norm(ctx, tune, dtype, users):

@@ -277,6 +277,33 @@ def test_captured_and_replayed(ctx, tune, t):
         assert torch.equal(de, tune.embed_backward(ctx, dy, tokens, v))
 
 
+def test_a_captured_differentiable_step(ctx, tune):
+    """Forward and backward by autograd in one graph; nothing made outside it refers to the table when it is captured."""
+    t, d, v = 300, 72, 500
+    start, dy, tokens = normal(1, v, d, dtype=torch.bfloat16), normal(2, t, d, dtype=torch.bfloat16), make_tokens(3, t, v, "any")
+    table = start.clone().requires_grad_()
+
+    def step():
+        y = tune.embedding(ctx, table, tokens, 2.0)
+        return y.detach(), torch.autograd.grad(y, table, dy)[0]
+
+    s = torch.cuda.Stream()
+    s.wait_stream(torch.cuda.current_stream())
+    with torch.cuda.stream(s):
+        step()
+    torch.cuda.current_stream().wait_stream(s)
+    torch.cuda.synchronize()
+    g = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(g):
+        y, de = step()
+    for i in range(4):
+        tokens.copy_(make_tokens(10 + i, t, v, "any"))
+        g.replay()
+        torch.cuda.synchronize()
+        assert torch.equal(y, tune.embed(ctx, start, tokens, 2.0))
+        assert torch.equal(de, tune.embed_backward(ctx, dy, tokens, v, 2.0))
+
+
 def test_two_streams_at_once(ctx, tune):
     v, d, streams = 900, 256, [torch.cuda.Stream() for _ in range(2)]
     jobs = [(make_tokens(i, t, v, "frequent"), normal(i, t, d, dtype=torch.bfloat16)) for i, t in enumerate((9000, 1500))]

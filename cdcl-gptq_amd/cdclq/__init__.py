@@ -215,6 +215,7 @@ def exported_symbols() -> list[str]:
         "cdclq_adapter_linear_device", "cdclq_adapter_backward_device",
         "cdclq_vocab_loss_device", "cdclq_vocab_loss_backward_device",
         "cdclq_embed_device", "cdclq_embed_work_bytes", "cdclq_embed_backward_device", "cdclq_grad_work_bytes",
+        "cdclq_grads_hold",
         "cdclq_grad_norm_device", "cdclq_clip_grads_device", "cdclq_constrain_work_bytes",
         "cdclq_constrain_logits_device",
     ]

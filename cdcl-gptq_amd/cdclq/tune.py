@@ -26,7 +26,7 @@ from dataclasses import dataclass
 import numpy as np
 import torch
 
-from . import DTYPE_BF16, DTYPE_F16, DTYPE_F32, Context, check_row_width, lib as _L
+from . import DTYPE_BF16, DTYPE_F16, DTYPE_F32, LIB_PATH, Context, check_row_width, lib as _L
 
 BLOCK = 128  # features per scale of an 8-bit checkpoint
 _CODES = {torch.bfloat16: DTYPE_BF16, torch.float16: DTYPE_F16}
@@ -34,7 +34,6 @@ _CODES32 = {torch.float32: DTYPE_F32, **_CODES}
 
 
 _empty = torch.empty
-_data_ptr = torch.Tensor.data_ptr
 _current_stream = torch._C._cuda_getCurrentRawStream  # the handle alone: a Stream object costs a microsecond
 
 
@@ -361,6 +360,33 @@ def embed_backward(ctx: Context, dy: torch.Tensor, tokens: torch.Tensor, vocab: 
 _GRAD = np.dtype([("x", np.uintp), ("out", np.uintp), ("count", np.uintp), ("dtype", np.int32), ("out_dtype", np.int32)])
 
 
+class _DLPackExchange(C.Structure):
+    """DLPack's C exchange interface, version 1.3: a fixed interface."""
+
+    _fields_ = [("major", C.c_uint32), ("minor", C.c_uint32), ("before", C.c_void_p), ("allocate", C.c_void_p),
+                ("managed_from_object", C.c_void_p), ("object_from_managed", C.c_void_p), ("look", C.c_void_p),
+                ("stream", C.c_void_p)]
+
+
+_hold = None
+
+
+def _holds(*args) -> bool:
+    """cdclq_grads_hold with torch's function to look at a tensor (asking each from Python for all that counts takes
+    five times as long), called with the interpreter's lock, which that function needs."""
+    global _hold
+    if _hold is None:
+        capsule, name = torch.Tensor.__dlpack_c_exchange_api__, b"dlpack_exchange_api"
+        get = C.PYFUNCTYPE(C.c_void_p, C.py_object, C.c_char_p)(("PyCapsule_GetPointer", C.pythonapi))
+        api = _DLPackExchange.from_address(get(capsule, name))
+        if api.major != 1:
+            raise RuntimeError(f"torch has version {api.major} of DLPack's exchange interface, need 1")
+        call = C.PyDLL(LIB_PATH).cdclq_grads_hold
+        call.argtypes, call.restype = [C.c_void_p, C.c_size_t, C.c_size_t] + [C.c_void_p] * 3, C.c_int
+        _hold = call, api.look
+    return _hold[0](*args, _hold[1])
+
+
 class Gradients:
     """The gradients of a step as one set: tensors (float32, bfloat16 or float16, contiguous, of any shapes), to be
     clipped in place, or into out: tensors of the same shapes, each of its gradient's type or float32 (the gradients
@@ -375,7 +401,10 @@ class Gradients:
             raise ValueError(f"{len(self.tensors)} gradients and {len(self.out)} outputs")
         if adapters is not None and self.parts < 1:
             raise ValueError(f"adapters is {adapters}, need at least 1")
-        self.all, self.device = self.tensors + (self.out or []), torch.device("cuda", ctx.device)
+        self.all, self.device = (*self.tensors, *(self.out or ())), torch.device("cuda", ctx.device)
+        self.objects = np.array(list(map(id, self.all)), np.uintp)  # which self.all keeps alive
+        at, n = self.objects.ctypes.data, len(self.tensors)
+        self.looked = n, self.shape[0] if self.shape else 0, at, None if out is None else at + 8 * n
         self._read()
 
     def _read(self):
@@ -390,7 +419,7 @@ class Gradients:
                 raise ValueError(f"a gradient or output of shape {tuple(g.shape)} has strides {g.stride()}, it must be "
                                  "contiguous")
         rows = []
-        for x, o in zip(self.tensors, self.all[-n:]):
+        for x, o in zip(self.all, self.all[-n:]):
             shape, kind = x.shape, kinds[x.dtype]
             if o is not x and o.shape != shape:
                 raise ValueError(f"an output has shape {tuple(o.shape)}, its gradient {tuple(shape)}")
@@ -403,11 +432,14 @@ class Gradients:
         self.table = np.array(rows, _GRAD)
         self.ptr = self.table.ctypes.data
         self.work_bytes = _L().cdclq_grad_work_bytes(self.ptr, n, self.parts)
-        self.at = list(map(_data_ptr, self.all))
 
     def _addresses(self) -> int:
-        """The table's address; tensors that have other memory by now (their .data set) are read again."""
-        if list(map(_data_ptr, self.all)) != self.at:
+        """The table's address; tensors that have other memory, sizes or types by now (their .data set) are read again."""
+        try:
+            held = _holds(self.ptr, *self.looked)
+        except Exception:  # a tensor that DLPack does not describe
+            held = False
+        if not held:
             self._read()
         return self.ptr
 

@@ -311,6 +311,32 @@ int grad_tensors(cdclq_ctx* ctx, const cdclq_grad* grads, size_t n, size_t parts
   return CDCLQ_OK;
 }
 
+// A tensor as DLPack describes it (its DLTensor, a fixed interface).
+struct DlTensor {
+  void* data;
+  int32_t device_type, device_id;
+  int32_t ndim;
+  uint8_t code, bits;
+  uint16_t lanes;
+  int64_t *shape, *strides;  // in elements; no strides: tightly packed
+  uint64_t byte_offset;
+};
+static_assert(sizeof(DlTensor) == 48, "DLPack's layout");
+
+// Whether a tensor is tightly packed and of this type, number of elements and (if it has any) address.
+bool holds(const DlTensor& t, const void* at, size_t count, int32_t dtype) {
+  constexpr int kFloat = 2, kBfloat = 4;  // DLPack's type codes
+  const int code = dtype == CDCLQ_DTYPE_BF16 ? kBfloat : kFloat;
+  if (t.code != code || (size_t)t.bits != 8 * type_bytes(dtype) || t.lanes != 1) return false;
+  size_t n = 1;
+  bool tight = true;
+  for (int i = t.ndim - 1; i >= 0; --i) {
+    tight = tight && (!t.strides || t.shape[i] == 1 || (size_t)t.strides[i] == n);
+    n *= (size_t)t.shape[i];
+  }
+  return n == count && (n == 0 || (tight && static_cast<const char*>(t.data) + t.byte_offset == at));
+}
+
 }  // namespace
 
 extern "C" {
@@ -566,6 +592,20 @@ size_t cdclq_grad_work_bytes(const cdclq_grad* grads, size_t n, size_t parts) {
   } catch (const std::bad_alloc&) {
     return 0;
   }
+}
+
+int cdclq_grads_hold(const cdclq_grad* grads, size_t n, size_t first, void* const* x, void* const* out, cdclq_look look) {
+  if (n && (!grads || !x || !look)) return 0;
+  for (size_t i = 0; i < n; ++i) {
+    const cdclq_grad& g = grads[i];
+    DlTensor a = {}, b = {};
+    if (look(x[i], &a) || !holds(a, g.x, g.count, g.dtype)) return 0;
+    if (first && (a.ndim < 1 || (size_t)a.shape[0] != first)) return 0;
+    if (!out) continue;
+    if (look(out[i], &b) || !holds(b, g.out, g.count, g.out_dtype)) return 0;
+    if (b.ndim != a.ndim || !std::equal(a.shape, a.shape + a.ndim, b.shape)) return 0;
+  }
+  return 1;
 }
 
 int cdclq_grad_norm_device(cdclq_ctx* ctx, const cdclq_grad* grads, size_t n, size_t parts, float* norm, void* work,

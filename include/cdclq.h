@@ -429,6 +429,12 @@ typedef struct cdclq_grad {
 size_t cdclq_grad_work_bytes(const cdclq_grad* grads, size_t n, size_t parts);
 int cdclq_grad_norm_device(cdclq_ctx* ctx, const cdclq_grad* grads, size_t n, size_t parts, float* norm, void* work,
                            size_t work_bytes, void* stream);
+/* Whether n grads kept from an earlier call still say what their tensors are: 1 if count, types and addresses are those of
+ * the tensor objects x[i] and out[i] (out NULL: not looked at) as they are now, tightly packed, x[i] and out[i] of one
+ * shape, its first dimension `first` (0: any); else 0. look(object, t) describes a tensor by DLPack's DLTensor at t
+ * without keeping a hold on it and returns 0 if it could. Waits for nothing, needs no context. */
+typedef int (*cdclq_look)(void* object, void* dltensor);
+int cdclq_grads_hold(const cdclq_grad* grads, size_t n, size_t first, void* const* x, void* const* out, cdclq_look look);
 /* The norms as above, and out = x * min(1, max_norm / (norm + 1e-6)) of each part. Where a norm is NaN or infinite the
  * part is not scaled. Outputs and gradients must not overlap, but for an out that is its x. max_norm >= 0. */
 int cdclq_clip_grads_device(cdclq_ctx* ctx, const cdclq_grad* grads, size_t n, size_t parts, double max_norm,

@@ -1,0 +1,75 @@
+"""GPU tests of cdclq.tune's embedding, clipping and logit constraints beyond those of the operators' own files: sets of
+gradients whose tensors change at their place, factors and norms at the ends of f32, tensors that autograd has saved,
+gradients of the embedding through the C entry point, rows that lie between each other.
+
+Tolerances are those of the operators' own files: u is the unit roundoff of the output's type, a sum of n rows in f32 is
+off by at most n 2^-24 of the sum of their magnitudes, each other rounding to f32 by 2^-24."""
+import math
+
+import pytest
+import torch
+
+import cdclq
+
+pytestmark = pytest.mark.gpu
+
+U = {torch.bfloat16: 2.0 ** -8, torch.float16: 2.0 ** -11, torch.float32: 2.0 ** -24}
+TINY = {torch.bfloat16: 2.0 ** -133, torch.float16: 2.0 ** -24, torch.float32: 2.0 ** -149}
+U32 = 2.0 ** -24
+TYPES = [torch.bfloat16, torch.float16, torch.float32]
+
+
+@pytest.fixture(scope="module")
+def ctx():
+    c = cdclq.Context(0)
+    yield c
+    c.close()
+
+
+@pytest.fixture(scope="module")
+def tune():
+    from cdclq import tune
+    return tune
+
+
+def rng(seed):
+    return torch.Generator(device="cuda").manual_seed(seed)
+
+
+def normal(seed, *shape, std=1.0, dtype=torch.float32):
+    return (torch.randn(shape, generator=rng(seed), device="cuda") * std).to(dtype)
+
+
+# ---------------------------------------------------------------- a set of gradients that is kept
+@pytest.mark.parametrize("dtype", TYPES)
+@pytest.mark.parametrize("count", [1, 200])
+def test_a_gradient_changed_at_its_place(ctx, tune, dtype, count):
+    """Shorter, longer and of another type in a buffer that others use, too: what lies outside stays."""
+    flat = normal(1, 4000, dtype=dtype)
+    rest = [normal(2 + i, 30) for i in range(count - 1)]
+    x = flat[100:3100]
+    g = tune.Gradients(ctx, [x, *rest])
+    tune.clip_grads(g, math.inf)
+    for dt, n in ((dtype, 10), (dtype, 3500), (torch.float32 if dtype != torch.float32 else torch.bfloat16, 100), (dtype, 0)):
+        before, others = flat.clone(), [r.double().norm() ** 2 for r in rest]
+        x.data = flat[100:].view(dt)[:n] if dt != dtype else flat[100:100 + n]
+        want = (x.double().norm() ** 2 + sum(others)).sqrt()
+        old = x.double()
+        got = tune.clip_grads(g, 0.5)
+        assert abs(got.double() - want) <= 1.01 * U32 * want
+        e = old * min(1.0, 0.5 / (want.item() + 1e-6))
+        assert ((x.double() - e).abs() <= (U[dt] + 2.1 * U32) * e.abs() + TINY[dt]).all()
+        end = 100 + n * x.element_size() // flat.element_size()
+        assert torch.equal(flat[:100], before[:100]) and torch.equal(flat[end:], before[end:])
+
+
+def test_gradients_freed_and_allocated_again(ctx, tune):
+    """set_to_none and a smaller gradient in the block that became free."""
+    x = normal(1, 100_000)
+    g = tune.Gradients(ctx, [x])
+    tune.grad_norm(g)
+    for n in (90_000, 5000, 100_000):
+        x.data = torch.empty(0, device="cuda")
+        x.data = normal(n, n)
+        want = x.double().norm()
+        assert abs(tune.grad_norm(g).double() - want) <= 1.01 * U32 * want

@@ -1,0 +1,128 @@
+"""CPU checks of a set of gradients that is kept over steps: what its table says after its tensors changed. The tensors
+are host memory that says it is on GPU 0; nothing is launched."""
+import types
+
+import numpy as np
+import pytest
+import torch
+
+import cdclq
+from cdclq import tune
+
+CTX = types.SimpleNamespace(device=0)
+CODE = {torch.float32: cdclq.DTYPE_F32, torch.float16: cdclq.DTYPE_F16, torch.bfloat16: cdclq.DTYPE_BF16}
+
+
+class OnGpu(torch.Tensor):
+    def get_device(self):
+        return 0
+
+
+def make(*shape, dtype=torch.float32):
+    return torch.ones(shape, dtype=dtype).as_subclass(OnGpu)
+
+
+def rows(g):
+    """The table as the next call takes it."""
+    assert g._addresses() == g.table.ctypes.data
+    return g.table
+
+
+def same(row, x, out=None):
+    o = x if out is None else out
+    return (row["count"], row["dtype"], row["out_dtype"]) == (x.numel(), CODE[x.dtype], CODE[o.dtype]) and \
+        (x.numel() == 0 or (row["x"], row["out"]) == (x.data_ptr(), o.data_ptr()))
+
+
+CHANGES = {"shorter": lambda x: x.data[:10], "empty": lambda x: x.data[:0], "longer": lambda x: x.base[:1200],
+           "retyped": lambda x: x.data.view(torch.bfloat16), "reshaped": lambda x: x.data.view(20, 50),
+           "moved": lambda x: x.base[7:507], "other": lambda x: make(30, dtype=torch.float16)}
+
+
+@pytest.mark.parametrize("change", CHANGES)
+@pytest.mark.parametrize("count", [1, 3, 200])
+def test_a_tensor_changed_in_place_is_read_again(change, count):
+    """Sizes and types at the address that the tensor had before, too."""
+    tensors = [make(1000 + i) for i in range(count)]
+    x = tensors[count // 2]
+    x.data = (base := make(2000))[:1000]
+    x.base = base
+    g = tune.Gradients(CTX, tensors)
+    assert all(same(r, t) for r, t in zip(rows(g), tensors))
+    x.data = CHANGES[change](x)
+    assert all(same(r, t) for r, t in zip(rows(g), tensors))
+    assert g.work_bytes == cdclq.lib().cdclq_grad_work_bytes(g.ptr, count, 1)
+
+
+def test_resized_and_refilled_tensors():
+    x = make(1000)
+    g = tune.Gradients(CTX, [x])
+    x.resize_(400)
+    assert same(rows(g)[0], x)
+    for n in (300, 20, 900, 1):  # freed first: the allocator may hand out the same place
+        for _ in range(20):
+            x.data = make(0)
+            assert same(rows(g)[0], x)
+            x.data = make(n, dtype=torch.float16 if n == 20 else torch.float32)
+            assert same(rows(g)[0], x)
+
+
+def test_outputs_are_looked_at_as_gradients_are():
+    x, out = make(6, 50, dtype=torch.float16), make(6, 50)
+    g = tune.Gradients(CTX, [x], out=[out])
+    assert same(rows(g)[0], x, out)
+    out.data = out.data.view(torch.float16)[:, ::2].contiguous()
+    assert same(rows(g)[0], x, out)
+    x.data, out.data = x.data[:3], out.data[:3]
+    assert same(rows(g)[0], x, out)
+    out.data = out.data[:2]
+    with pytest.raises(ValueError, match="shape"):
+        g._addresses()
+    out.data = x.data.view(3 * 50)
+    with pytest.raises(ValueError, match="shape"):
+        g._addresses()
+
+
+def test_transposed_in_place_is_refused():
+    x = make(20, 30)
+    g = tune.Gradients(CTX, [x])
+    x.t_()
+    with pytest.raises(ValueError, match="contiguous"):
+        g._addresses()
+    x.t_()
+    assert same(rows(g)[0], x)
+    x.data = make(40, 30)[::2]
+    with pytest.raises(ValueError, match="contiguous"):
+        g._addresses()
+
+
+def test_types_without_kernels_are_refused_later_too():
+    x = make(10)
+    g = tune.Gradients(CTX, [x])
+    x.data = x.data.view(torch.int32)
+    with pytest.raises(TypeError, match="int32"):
+        g._addresses()
+
+
+def test_adapters_stay_the_first_dimension():
+    x = make(4, 6, 5)
+    g = tune.Gradients(CTX, [x], adapters=4)
+    x.data = x.data.view(4, 30)
+    assert same(rows(g)[0], x)
+    x.data = x.data.view(6, 20)
+    with pytest.raises(ValueError, match="adapters first"):
+        g._addresses()
+    x.data = x.data.view(120)[:1].view(())
+    with pytest.raises(ValueError, match="adapters first"):
+        g._addresses()
+
+
+def test_an_unchanged_set_is_not_read_again(monkeypatch):
+    """Gradients of parameters, of size 0 and 1, with strides that say nothing."""
+    param = torch.nn.Parameter(torch.ones(5)).as_subclass(OnGpu)
+    tensors = [make(3, 4), make(0, 7), make(1, 9)[:, :1], make(), make(4, 1).transpose(0, 1), param, make(2)[1:]]
+    out = [make(*t.shape) for t in tensors]
+    for g in (tune.Gradients(CTX, tensors), tune.Gradients(CTX, tensors, out=out), tune.Gradients(CTX, [])):
+        before = g.table.copy()
+        monkeypatch.setattr(g, "_read", lambda: pytest.fail("read again"))
+        assert np.array_equal(rows(g), before)

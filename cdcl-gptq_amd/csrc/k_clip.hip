@@ -3,8 +3,9 @@
 //   n_g = sqrt(sum of x^2 over part g of every tensor)      c_g = min(1, max / (n_g + 1e-6))      out = c_g x
 //
 // g: the adapters of several users that train together, each tensor's first dimension (or one part: all). The
-// squares are summed in f64, so that neither 1e-30 nor 1e30 leaves the range; c is made in f64 and rounded to f32,
-// its product with x rounded to f32 and to the output's type. 1e-6 keeps c finite, as trainers do it. A norm that
+// squares are summed in f64, so that neither 1e-30 nor 1e30 leaves the range; c is made in f64 and rounded to f32 (below
+// f32's normal numbers it stays in f64), its product with x rounded to f32 and to the output's type. 1e-6 keeps c finite,
+// as trainers do it. A norm that
 // is NaN or infinite in f32 clips nothing (c = 1): the gradients stay as they are, for the caller to look at.
 //
 // Both passes are bound by memory. A part's elements, over all tensors, are chunks of 4096; a workgroup takes every
@@ -202,6 +203,23 @@ __device__ __forceinline__ void scaled(const void* from, void* to, long i0, long
   if (last < i1) y[last] = Row8<O>::narrow(by * Row8<T>::widen(x[last]));
 }
 
+// The same for a factor below f32's normal numbers (gradients of 1e30 held to 1e-9), which f32 would hold in few bits or as
+// 0 while the products are ordinary numbers: in f64, element by element.
+__device__ __forceinline__ float element(const void* x, long i, uint32_t kind) {
+  switch (kind & 3) {
+    case F32::kind: return static_cast<const float*>(x)[i];
+    case F16::kind: return F16::widen(static_cast<const uint16_t*>(x)[i]);
+    default: return Bf16::widen(static_cast<const uint16_t*>(x)[i]);
+  }
+}
+__device__ __forceinline__ void scaled_little(const ClipEntry& e, long i0, long i1, double by) {
+  for (long i = i0 + threadIdx.x; i < i1; i += 256) {
+    const float y = (float)(by * (double)element(e.x, i, e.kind));
+    if ((e.kind & 4) || e.kind == F32::kind) static_cast<float*>(e.out)[i] = y;
+    else static_cast<uint16_t*>(e.out)[i] = e.kind == F16::kind ? F16::narrow(y) : Bf16::narrow(y);
+  }
+}
+
 template <class S>
 __global__ __launch_bounds__(256) void k_clip(const S s, uint32_t chunks, uint32_t each, uint32_t sums_all,
                                               const double* __restrict__ sums, double most, float* __restrict__ norm) {
@@ -213,14 +231,18 @@ __global__ __launch_bounds__(256) void k_clip(const S s, uint32_t chunks, uint32
   if (j < chunks) next = entry_of(s, c);
   const double got = norm_of(sums + part * (long)each, each);
   if (j == 0 && threadIdx.x == 0) norm[part] = (float)got;
-  float by = 1.0f;
-  if (__builtin_isfinite((float)got)) by = (float)__builtin_fmin(1.0, most / (got + 1e-6));
+  double exact = 1.0;
+  if (__builtin_isfinite((float)got)) exact = __builtin_fmin(1.0, most / (got + 1e-6));
+  const float by = (float)exact;
+  const bool little = exact < 0x1p-126 && exact > 0.0;
   if (j >= chunks) return;
   for (;; c -= each) {
     const ClipEntry e = next;
     if (c >= each) next = entry_of(s, c - each);
     const long i0 = part * (long)e.n + (long)(c - e.start) * kChunk, i1 = min(i0 + kChunk, (part + 1) * (long)e.n);
-    if (e.x != e.out || by != 1.0f) {
+    if (little) {
+      scaled_little(e, i0, i1, exact);
+    } else if (e.x != e.out || by != 1.0f) {
       switch (e.kind) {
         case F32::kind:
         case F32::kind | 4: scaled<F32, F32>(e.x, e.out, i0, i1, by); break;

@@ -76,3 +76,40 @@ def test_gradients_freed_and_allocated_again(ctx, tune):
         x.data = normal(n, n)
         want = x.double().norm()
         assert abs(tune.grad_norm(g).double() - want) <= 1.01 * U32 * want
+
+
+# ---------------------------------------------------------------- factors and norms at the ends of f32
+def clipped(tensors, want, most, out):
+    """Against min(1, most / (norm + 1e-6)) x in 64 bits: the factor, the product and the result rounded to f32, the
+    result to its type; half a step of the smallest numbers."""
+    by = min(1.0, most / (want + 1e-6))
+    for o, x in zip(out, tensors):
+        e = by * x.double()
+        assert ((o.double() - e).abs() <= (U[o.dtype] + 2.1 * U32) * e.abs() + TINY[o.dtype]).all()
+        assert e.abs().max() < 2.0 ** -140 or o.any()  # something is left of it
+
+
+@pytest.mark.parametrize("dtype", [torch.float32, torch.bfloat16])
+@pytest.mark.parametrize("size,most", [(1e30, 1e-8), (1e30, 1e-16), (1e36, 1e-2), (1e36, 1e-30), (1e28, 1e-9)])
+@pytest.mark.parametrize("n", [5, 70_001])
+def test_factors_below_the_normal_numbers_of_f32(ctx, tune, dtype, size, most, n):
+    """The factor is 1e-40 or 1e-70, its products are ordinary numbers; in place, into the same type and into float32."""
+    tensors = [normal(1, n, dtype=dtype) * size, normal(2, 3, 1001, dtype=dtype) * size]
+    want = sum(x.double().norm() ** 2 for x in tensors).sqrt().item()
+    for kind in (dtype, torch.float32):
+        out = [torch.full(x.shape, math.nan, dtype=kind, device="cuda") for x in tensors]
+        tune.clip_grads(tune.Gradients(ctx, tensors, out=out), most)
+        clipped(tensors, want, most, out)
+    place = [x.clone() for x in tensors]
+    tune.clip_grads(tune.Gradients(ctx, place), most)
+    clipped(tensors, want, most, place)
+
+
+def test_small_factors_of_half_precision(ctx, tune):
+    """Float16 gradients into float32: factors of 1e-40, results of 1e-36."""
+    x = normal(1, 3, 5000, std=1000.0, dtype=torch.float16)
+    out = torch.empty(3, 5000, device="cuda")
+    norm = tune.clip_grads(tune.Gradients(ctx, [x], out=[out], adapters=3), 1e-34)
+    for i in range(3):
+        clipped([x[i]], x[i].double().norm().item(), 1e-34, [out[i]])
+    assert norm.shape == (3,)

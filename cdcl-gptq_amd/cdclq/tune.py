@@ -463,7 +463,8 @@ def grad_norm(grads: Gradients) -> torch.Tensor:
 
 def clip_grads(grads: Gradients, max_norm: float) -> torch.Tensor:
     """grad_norm, and the gradients times min(1, max_norm / (norm + 1e-6)), in place or, where the set has them, into
-    its outputs (which are always written). Gradients (an adapter's) whose norm is NaN or infinite are not scaled."""
+    its outputs (which are always written). Gradients (an adapter's) with a NaN or an infinity among them are not scaled;
+    their norm is NaN or infinite. A norm of finite gradients that float32 does not hold is infinite, too, and scales."""
     ctx, table, n, norm, work = _grad_call(grads)
     ctx.check(_L().cdclq_clip_grads_device(ctx.ptr, table, n, grads.parts, max_norm, norm.data_ptr(), work.data_ptr(),
                                            grads.work_bytes, _stream(ctx)))

@@ -5,8 +5,8 @@
 // g: the adapters of several users that train together, each tensor's first dimension (or one part: all). The
 // squares are summed in f64, so that neither 1e-30 nor 1e30 leaves the range; c is made in f64 and rounded to f32 (below
 // f32's normal numbers it stays in f64), its product with x rounded to f32 and to the output's type. 1e-6 keeps c finite,
-// as trainers do it. A norm that
-// is NaN or infinite in f32 clips nothing (c = 1): the gradients stay as they are, for the caller to look at.
+// as trainers do it. A part with a NaN or an infinity is not clipped (c = 1): its gradients stay as they are, for the
+// caller to look at. A finite norm above f32's numbers is returned as infinite, and clips.
 //
 // Both passes are bound by memory. A part's elements, over all tensors, are chunks of 4096; a workgroup takes every
 // J-th of a part's, so that a part has J sums whatever its size, and each workgroup of the second pass adds them up
@@ -232,7 +232,7 @@ __global__ __launch_bounds__(256) void k_clip(const S s, uint32_t chunks, uint32
   const double got = norm_of(sums + part * (long)each, each);
   if (j == 0 && threadIdx.x == 0) norm[part] = (float)got;
   double exact = 1.0;
-  if (__builtin_isfinite((float)got)) exact = __builtin_fmin(1.0, most / (got + 1e-6));
+  if (__builtin_isfinite(got)) exact = __builtin_fmin(1.0, most / (got + 1e-6));
   const float by = (float)exact;
   const bool little = exact < 0x1p-126 && exact > 0.0;
   if (j >= chunks) return;

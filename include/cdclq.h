@@ -435,8 +435,9 @@ int cdclq_grad_norm_device(cdclq_ctx* ctx, const cdclq_grad* grads, size_t n, si
  * without keeping a hold on it and returns 0 if it could. Waits for nothing, needs no context. */
 typedef int (*cdclq_look)(void* object, void* dltensor);
 int cdclq_grads_hold(const cdclq_grad* grads, size_t n, size_t first, void* const* x, void* const* out, cdclq_look look);
-/* The norms as above, and out = x * min(1, max_norm / (norm + 1e-6)) of each part. Where a norm is NaN or infinite the
- * part is not scaled. Outputs and gradients must not overlap, but for an out that is its x. max_norm >= 0. */
+/* The norms as above, and out = x * min(1, max_norm / (norm + 1e-6)) of each part. A part with a
+ * NaN or an infinity is not scaled (its norm says so; a finite norm that f32 does not hold is infinite, too, and
+ * scales). Outputs and gradients must not overlap, but for an out that is its x. max_norm >= 0. */
 int cdclq_clip_grads_device(cdclq_ctx* ctx, const cdclq_grad* grads, size_t n, size_t parts, double max_norm,
                             float* norm, void* work, size_t work_bytes, void* stream);
 

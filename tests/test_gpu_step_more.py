@@ -86,7 +86,8 @@ def clipped(tensors, want, most, out):
     for o, x in zip(out, tensors):
         e = by * x.double()
         assert ((o.double() - e).abs() <= (U[o.dtype] + 2.1 * U32) * e.abs() + TINY[o.dtype]).all()
-        assert e.abs().max() < 2.0 ** -140 or o.any()  # something is left of it
+        # something is left of it, unless all is below the type's least number (half of it rounds to 0)
+        assert e.abs().max() < TINY[o.dtype] or o.any()
 
 
 @pytest.mark.parametrize("dtype", [torch.float32, torch.bfloat16])
@@ -113,3 +114,24 @@ def test_small_factors_of_half_precision(ctx, tune):
     for i in range(3):
         clipped([x[i]], x[i].double().norm().item(), 1e-34, [out[i]])
     assert norm.shape == (3,)
+
+
+@pytest.mark.parametrize("dtype", [torch.float32, torch.bfloat16])
+@pytest.mark.parametrize("size,most", [(3e37, 1e38), (3e37, 1.0), (3e37, 1e-6), (5e37, 1e-40)])
+def test_norms_above_f32_clip(ctx, tune, dtype, size, most):
+    """Finite gradients whose norm is a number of f64 but not of f32: infinite where it is returned, and the gradients are
+    clipped by what it is; another adapter's norm is as ever."""
+    x = normal(1, 2, 70_001, dtype=dtype)
+    x[0] *= size
+    assert torch.isfinite(x).all()
+    want = x.double().norm(dim=1)
+    assert want[0] > torch.finfo(torch.float32).max
+    out, place = torch.empty(2, 70_001, device="cuda"), x.clone()
+    for n in (tune.clip_grads(tune.Gradients(ctx, [x], out=[out], adapters=2), most),
+              tune.clip_grads(tune.Gradients(ctx, [place], adapters=2), most)):
+        assert n[0] == math.inf and abs(n[1].double() - want[1]) <= 1.01 * U32 * want[1]
+    for i in range(2):
+        clipped([x[i], x[i]], want[i].item(), most, [out[i], place[i]])
+    whole = [torch.empty_like(x)]
+    assert tune.clip_grads(tune.Gradients(ctx, [x], out=whole), most) == math.inf
+    clipped([x], want.norm().item(), most, whole)

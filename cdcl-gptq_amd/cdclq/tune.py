@@ -16,7 +16,8 @@ Tensors are torch tensors on the context's GPU, bfloat16 or float16 (gradients a
 contiguous rows (any row stride). Every call is enqueued on torch's current stream and returns without waiting; scratch
 memory comes from torch's allocator, so that calls may be made on several streams and captured into
 a graph. A refused argument raises CdclqError (or TypeError / ValueError for a tensor of the wrong
-kind) before anything is enqueued.
+kind) before anything is enqueued. A tensor of the caller's that a call writes (gradients clipped in place, into, out)
+counts for autograd as changed in place by an operation that it does not record.
 """
 from __future__ import annotations
 
@@ -35,6 +36,8 @@ _CODES32 = {torch.float32: DTYPE_F32, **_CODES}
 
 _empty = torch.empty
 _current_stream = torch._C._cuda_getCurrentRawStream  # the handle alone: a Stream object costs a microsecond
+# Told of every tensor of the caller's that a call writes: where autograd has saved it, its backward pass is an error.
+_wrote = torch.autograd.graph.increment_version
 
 
 def _code(x: torch.Tensor, name: str) -> int:
@@ -353,6 +356,8 @@ def embed_backward(ctx: Context, dy: torch.Tensor, tokens: torch.Tensor, vocab: 
     ctx.check(L.cdclq_embed_backward_device(ctx.ptr, dy.data_ptr(), ld, t, d, vocab, code, tokens.data_ptr(), scale,
                                             ignore_index, into is not None, de.data_ptr(), lde, kind,
                                             work.data_ptr() if need else None, need, _stream(ctx)))
+    if into is not None:
+        _wrote(into)
     return de
 
 
@@ -402,6 +407,7 @@ class Gradients:
         if adapters is not None and self.parts < 1:
             raise ValueError(f"adapters is {adapters}, need at least 1")
         self.all, self.device = (*self.tensors, *(self.out or ())), torch.device("cuda", ctx.device)
+        self.written = self.all[-len(self.tensors):]
         self.objects = np.array(list(map(id, self.all)), np.uintp)  # which self.all keeps alive
         at, n = self.objects.ctypes.data, len(self.tensors)
         self.looked = n, self.shape[0] if self.shape else 0, at, None if out is None else at + 8 * n
@@ -419,7 +425,7 @@ class Gradients:
                 raise ValueError(f"a gradient or output of shape {tuple(g.shape)} has strides {g.stride()}, it must be "
                                  "contiguous")
         rows = []
-        for x, o in zip(self.all, self.all[-n:]):
+        for x, o in zip(self.all, self.written):
             shape, kind = x.shape, kinds[x.dtype]
             if o is not x and o.shape != shape:
                 raise ValueError(f"an output has shape {tuple(o.shape)}, its gradient {tuple(shape)}")
@@ -468,6 +474,7 @@ def clip_grads(grads: Gradients, max_norm: float) -> torch.Tensor:
     ctx, table, n, norm, work = _grad_call(grads)
     ctx.check(_L().cdclq_clip_grads_device(ctx.ptr, table, n, grads.parts, max_norm, norm.data_ptr(), work.data_ptr(),
                                            grads.work_bytes, _stream(ctx)))
+    _wrote(grads.written)
     return norm
 
 
@@ -538,7 +545,8 @@ def constrain_logits(ctx: Context, logits: torch.Tensor, history: torch.Tensor |
             mr = mask_rows.data_ptr()
     elif mask_rows is not None:
         raise ValueError("mask_rows without a mask")
-    if out is None:
+    fresh = out is None
+    if fresh:
         out = _empty(r, v, dtype=logits.dtype, device=logits.device)
         ldo = v
     else:
@@ -549,6 +557,8 @@ def constrain_logits(ctx: Context, logits: torch.Tensor, history: torch.Tensor |
     ctx.check(L.cdclq_constrain_logits_device(ctx.ptr, logits.data_ptr(), ld, r, v, code, hp, ldh, width, lp, pp, *by,
                                               bt, bv, nb, mp, ldm, masks, mr, out.data_ptr(), ldo,
                                               work.data_ptr() if need else None, need, _stream(ctx)))
+    if not fresh:
+        _wrote(out)
     return out
 
 

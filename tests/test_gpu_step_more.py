@@ -135,3 +135,49 @@ def test_norms_above_f32_clip(ctx, tune, dtype, size, most):
     whole = [torch.empty_like(x)]
     assert tune.clip_grads(tune.Gradients(ctx, [x], out=whole), most) == math.inf
     clipped([x], want.norm().item(), most, whole)
+
+
+# ---------------------------------------------------------------- tensors that autograd has saved
+def writes(ctx, tune, x):
+    """Each call that writes a tensor of its caller's (x: 4 x 40 float32), by name."""
+    other, tokens = normal(1, 4, 40), torch.zeros(4, dtype=torch.int64, device="cuda")
+    dy = normal(2, 4, 40, dtype=torch.bfloat16)
+    return {"clip in place": lambda: tune.clip_grads(tune.Gradients(ctx, [other, x]), 1e-3),
+            "clip into": lambda: tune.clip_grads(tune.Gradients(ctx, [other], out=[x]), 1e-3),
+            "embed into": lambda: tune.embed_backward(ctx, dy, tokens, 4, into=x),
+            "embed nothing into": lambda: tune.embed_backward(ctx, dy[:0], tokens[:0], 4, into=x),
+            "constrain in place": lambda: tune.constrain_logits(ctx, x, out=x, history=tokens[:, None],
+                                                                presence=torch.ones(4, device="cuda")),
+            "constrain into": lambda: tune.constrain_logits(ctx, other, out=x)}
+
+
+@pytest.mark.parametrize("call", ["clip in place", "clip into", "embed into", "embed nothing into", "constrain in place",
+                                  "constrain into"])
+def test_what_autograd_has_saved_and_a_call_writes_is_an_error(ctx, tune, call):
+    x, w = normal(3, 4, 40), normal(4, 4, 40).requires_grad_()
+    y = (x * w).sum()  # keeps x
+    writes(ctx, tune, x)[call]()
+    with pytest.raises(RuntimeError, match="modified by an inplace operation"):
+        y.backward()
+    y = (x * w).sum()
+    tune.grad_norm(tune.Gradients(ctx, [x]))  # reads only
+    tune.constrain_logits(ctx, x)
+    y.backward()
+    assert torch.equal(w.grad, x)
+
+
+@pytest.mark.parametrize("call", ["clip in place", "clip into", "embed into", "constrain in place", "constrain into"])
+def test_refused_calls_and_inference_tensors(ctx, tune, call):
+    """A refused call leaves the counter alone; tensors of inference mode have none."""
+    x = normal(3, 4, 40)
+    before = x._version
+    with pytest.raises((cdclq.CdclqError, ValueError)):
+        tune.constrain_logits(ctx, x[:, :39], out=x[:, 1:])
+    with pytest.raises(cdclq.CdclqError):
+        tune.clip_grads(tune.Gradients(ctx, [x]), -1.0)
+    assert x._version == before
+    with torch.inference_mode():
+        y = x.clone()
+        writes(ctx, tune, y)[call]()
+    writes(ctx, tune, x)[call]()
+    assert torch.equal(x, y)

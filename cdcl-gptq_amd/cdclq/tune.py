@@ -373,23 +373,23 @@ class _DLPackExchange(C.Structure):
                 ("stream", C.c_void_p)]
 
 
-_hold = None
+_exchange = None
 
 
-def _holds(*args) -> bool:
-    """cdclq_grads_hold with torch's function to look at a tensor (asking each from Python for all that counts takes
-    five times as long), called with the interpreter's lock, which that function needs."""
-    global _hold
-    if _hold is None:
-        capsule, name = torch.Tensor.__dlpack_c_exchange_api__, b"dlpack_exchange_api"
-        get = C.PYFUNCTYPE(C.c_void_p, C.py_object, C.c_char_p)(("PyCapsule_GetPointer", C.pythonapi))
-        api = _DLPackExchange.from_address(get(capsule, name))
-        if api.major != 1:
-            raise RuntimeError(f"torch has version {api.major} of DLPack's exchange interface, need 1")
-        call = C.PyDLL(LIB_PATH).cdclq_grads_hold
+def _look():
+    """cdclq_grads_hold, called with the interpreter's lock, and torch's function for it that looks at a tensor (asking
+    each from Python for all that counts takes five times as long). Without one the sets are read in each call."""
+    global _exchange
+    if _exchange is None:
+        call, look = C.PyDLL(LIB_PATH).cdclq_grads_hold, None
         call.argtypes, call.restype = [C.c_void_p, C.c_size_t, C.c_size_t] + [C.c_void_p] * 3, C.c_int
-        _hold = call, api.look
-    return _hold[0](*args, _hold[1])
+        capsule = getattr(torch.Tensor, "__dlpack_c_exchange_api__", None)
+        if capsule is not None:
+            get = C.PYFUNCTYPE(C.c_void_p, C.py_object, C.c_char_p)(("PyCapsule_GetPointer", C.pythonapi))
+            api = _DLPackExchange.from_address(get(capsule, b"dlpack_exchange_api"))
+            look = api.look if api.major == 1 else None
+        _exchange = call, look
+    return _exchange
 
 
 class Gradients:
@@ -407,10 +407,12 @@ class Gradients:
         if adapters is not None and self.parts < 1:
             raise ValueError(f"adapters is {adapters}, need at least 1")
         self.all, self.device = (*self.tensors, *(self.out or ())), torch.device("cuda", ctx.device)
-        self.written = self.all[-len(self.tensors):]
+        self.written = self.counters = self.all[-len(self.tensors):]
+        self.calls = 0
         self.objects = np.array(list(map(id, self.all)), np.uintp)  # which self.all keeps alive
         at, n = self.objects.ctypes.data, len(self.tensors)
-        self.looked = n, self.shape[0] if self.shape else 0, at, None if out is None else at + 8 * n
+        self.holds, look = _look()
+        self.looked = n, self.shape[0] if self.shape else 0, at, None if out is None else at + 8 * n, look
         self._read()
 
     def _read(self):
@@ -442,12 +444,21 @@ class Gradients:
     def _addresses(self) -> int:
         """The table's address; tensors that have other memory, sizes or types by now (their .data set) are read again."""
         try:
-            held = _holds(self.ptr, *self.looked)
+            if self.holds(self.ptr, *self.looked):
+                return self.ptr
         except Exception:  # a tensor that DLPack does not describe
-            held = False
-        if not held:
-            self._read()
+            pass
+        self._read()
         return self.ptr
+
+    def _changed(self):
+        """Tells autograd that the call has written. A kept set does it by bases, whose counters their views have: 448 views
+        of a bucket one by one take 11 us, to find their bases takes 50."""
+        self.calls += 1
+        if self.calls == 2:
+            bases = [o._base for o in self.written]
+            self.counters = tuple({id(c): c for c in (o if b is None else b for o, b in zip(self.written, bases))}.values())
+        _wrote(self.counters)
 
 
 def _grad_call(grads: Gradients):
@@ -474,7 +485,7 @@ def clip_grads(grads: Gradients, max_norm: float) -> torch.Tensor:
     ctx, table, n, norm, work = _grad_call(grads)
     ctx.check(_L().cdclq_clip_grads_device(ctx.ptr, table, n, grads.parts, max_norm, norm.data_ptr(), work.data_ptr(),
                                            grads.work_bytes, _stream(ctx)))
-    _wrote(grads.written)
+    grads._changed()
     return norm
 
 

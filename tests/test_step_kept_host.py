@@ -126,3 +126,52 @@ def test_an_unchanged_set_is_not_read_again(monkeypatch):
         before = g.table.copy()
         monkeypatch.setattr(g, "_read", lambda: pytest.fail("read again"))
         assert np.array_equal(rows(g), before)
+
+
+def test_a_set_without_the_exchange_interface_is_read_in_each_call(monkeypatch):
+    monkeypatch.setattr(tune, "_exchange", None)
+    monkeypatch.delattr(torch.Tensor, "__dlpack_c_exchange_api__")
+    x = make(1000)
+    g = tune.Gradients(CTX, [x])
+    x.data = x.data[:10]
+    assert same(rows(g)[0], x)
+    x.data = x.data.view(2, 5).t()
+    with pytest.raises(ValueError, match="contiguous"):
+        g._addresses()
+    monkeypatch.setattr(tune, "_exchange", None)
+
+
+def test_a_tensor_that_cannot_be_described_is_read_again(monkeypatch):
+    x = make(1000)
+    g = tune.Gradients(CTX, [x])
+    monkeypatch.setattr(g, "holds", lambda *_: (_ for _ in ()).throw(BufferError("no")))
+    x.data = x.data[:10]
+    assert same(rows(g)[0], x)
+
+
+VIEWS = {"alone": lambda: [torch.ones(5), torch.ones(7)], "split": lambda: list(torch.ones(12).split([5, 7])),
+         "of views": lambda: [x.view(-1, 1) for x in torch.ones(3, 12)[1:].flatten().split(12)],
+         "chunks": lambda: list(torch.ones(4, 6).chunk(2)), "unbound": lambda: list(torch.ones(4, 6).unbind()),
+         "detached": lambda: [torch.ones(9).detach()[2:], torch.ones(3).data],
+         "unsafe": lambda: list(torch.ones(12).unsafe_split(4)), "parameters": lambda: [torch.nn.Parameter(torch.ones(4))],
+         "moved": lambda: [moved(x) for x in torch.ones(12).split(6)]}
+
+
+def moved(x):
+    x.data = torch.zeros(3)
+    return x
+
+
+@pytest.mark.parametrize("kind", VIEWS)
+def test_every_written_tensors_counter_is_among_the_sets(kind):
+    """Tensors of buckets have one counter together."""
+    tensors = VIEWS[kind]()
+    for out in (None, [torch.ones_like(x) for x in tensors]):
+        written = tensors if out is None else out
+        g = object.__new__(tune.Gradients)
+        with pytest.raises(ValueError, match="is on cpu"):  # host memory; what it writes is known by then
+            g.__init__(CTX, tensors, out=out)
+        for _ in range(4):
+            before = [x._version for x in written]
+            g._changed()
+            assert all(x._version > b for x, b in zip(written, before))

@@ -26,6 +26,7 @@ from dataclasses import dataclass
 
 import numpy as np
 import torch
+from torch.autograd import forward_ad as _forward
 
 from . import DTYPE_BF16, DTYPE_F16, DTYPE_F32, LIB_PATH, Context, check_row_width, lib as _L
 
@@ -586,6 +587,14 @@ def _first_order(backward):
     return run
 
 
+def _asked(*tensors) -> bool:
+    """Whether autograd asks for a gradient of one of them, or forward-mode differentiation carries a tangent of one, which
+    torch refuses where a function without a formula for it is applied."""
+    if torch.is_grad_enabled() and any(x.requires_grad for x in tensors):
+        return True
+    return _forward._current_level >= 0 and any(_forward.unpack_dual(x).tangent is not None for x in tensors)
+
+
 class _Linear(torch.autograd.Function):
     @staticmethod
     def forward(fn, x, a, b, scaling, packed, adapters, request):
@@ -614,10 +623,10 @@ class _Linear(torch.autograd.Function):
 
 def linear(packed: PackedLinear, x: torch.Tensor, adapters: Adapters | None = None,
            request: torch.Tensor | None = None) -> torch.Tensor:
-    """adapter_linear for autograd: gradients of x and of adapters.a and .b, of first order only; between the
-    passes x is kept as an 8-bit checkpoint. scaling is a constant."""
+    """adapter_linear for autograd: gradients of x and of adapters.a and .b, of first order and reverse mode only;
+    between the passes x is kept as an 8-bit checkpoint. scaling is a constant."""
     wanted = (x,) if adapters is None else (x, adapters.a, adapters.b, adapters.scaling)
-    if not (torch.is_grad_enabled() and any(t.requires_grad for t in wanted)):
+    if not _asked(*wanted):
         return adapter_linear(packed, x, adapters, request)  # no checkpoint, no low
     if adapters is None:
         return _Linear.apply(x, None, None, None, packed, None, request)
@@ -647,7 +656,7 @@ class _CrossEntropy(torch.autograd.Function):
 def cross_entropy(ctx: Context, x: torch.Tensor, w: torch.Tensor, targets: torch.Tensor,
                   ignore_index: int = -100) -> torch.Tensor:
     """The mean of vocab_loss over the tokens that take part (0 if none does), for autograd: gradients (of
-    first order only) of x and, where w asks for it, of w."""
+    first order and reverse mode only) of x and, where w asks for it, of w."""
     return _CrossEntropy.apply(x, w, ctx, targets, ignore_index)
 
 
@@ -667,7 +676,7 @@ class _Embedding(torch.autograd.Function):
 
 def embedding(ctx: Context, table: torch.Tensor, tokens: torch.Tensor, scale: float = 1.0,
               ignore_index: int = -100) -> torch.Tensor:
-    """embed for autograd: the gradient (dense, of first order only) of table."""
-    if not (torch.is_grad_enabled() and table.requires_grad):
+    """embed for autograd: the gradient (dense, of first order and reverse mode only) of table."""
+    if not _asked(table):
         return embed(ctx, table, tokens, scale, ignore_index)
     return _Embedding.apply(table, ctx, tokens, scale, ignore_index)

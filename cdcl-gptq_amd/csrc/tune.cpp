@@ -250,11 +250,16 @@ int check_type(cdclq_ctx* ctx, int dtype) {
 }
 constexpr size_t type_bytes(int dtype) { return dtype == CDCLQ_DTYPE_F32 ? 4 : 2; }
 
-// Whether two matrices (rows, row stride, columns, bytes an element) share memory.
+// Whether two matrices (rows, row stride, columns, bytes an element) share memory. Of strides that differ, whether
+// their ranges do.
 bool overlap(const void* a, size_t ra, size_t lda, size_t ca, size_t ea, const void* b, size_t rb, size_t ldb,
              size_t cb, size_t eb) {
   if (!ra || !rb) return false;
   const uintptr_t x = (uintptr_t)a, y = (uintptr_t)b;
+  if (lda * ea == ldb * eb) {  // b's rows between a's, as the column blocks of one buffer
+    const size_t s = lda * ea, from = y >= x ? (y - x) % s : (s - (x - y) % s) % s;
+    if (from >= ca * ea && from + cb * eb <= s) return false;
+  }
   return x < y + ((rb - 1) * ldb + cb) * eb && y < x + ((ra - 1) * lda + ca) * ea;
 }
 

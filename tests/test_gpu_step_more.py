@@ -181,3 +181,42 @@ def test_refused_calls_and_inference_tensors(ctx, tune, call):
         writes(ctx, tune, y)[call]()
     writes(ctx, tune, x)[call]()
     assert torch.equal(x, y)
+
+
+# ---------------------------------------------------------------- rows between each other
+@pytest.mark.parametrize("dtype", TYPES)
+@pytest.mark.parametrize("r,v,gap", [(1, 40, 0), (5, 33, 0), (5, 1000, 7), (70, 20_000, 1)])
+@pytest.mark.parametrize("first", [True, False])
+def test_logits_and_results_side_by_side(ctx, tune, dtype, r, v, gap, first):
+    """Two halves of one buffer's columns share no memory."""
+    buf = normal(1, r, 2 * v + gap, dtype=dtype)
+    logits, out = (buf[:, :v], buf[:, v + gap:]) if first else (buf[:, v + gap:], buf[:, :v])
+    k = dict(history=torch.randint(0, v, (r, 30), generator=rng(2), device="cuda"), presence=normal(3, r))
+    before, want = buf.clone(), tune.constrain_logits(ctx, logits, **k)
+    assert tune.constrain_logits(ctx, logits, out=out, **k) is out
+    assert torch.equal(out, want)
+    out.copy_(before[:, v + gap:] if first else before[:, :v])
+    assert torch.equal(buf, before)
+    for wrong in (buf[:, 1:v + 1], buf[:, v - 1:2 * v - 1], buf[:, v + gap - 1:2 * v + gap - 1]):
+        if r > 1 and wrong.data_ptr() not in (logits.data_ptr(), out.data_ptr()):
+            with pytest.raises(cdclq.CdclqError, match="overlaps"):
+                tune.constrain_logits(ctx, buf[:, :v] if wrong.data_ptr() < buf.data_ptr() + v * buf.element_size() else
+                                      buf[:, v + gap:], out=wrong)
+    assert torch.equal(buf, before)
+
+
+def test_rows_of_a_table_beside_its_gradient(ctx, tune):
+    """dy and the gradient that it is added to in one buffer."""
+    b, t, v, d = torch.bfloat16, 9, 9, 24
+    buf = normal(1, t, 2 * d, dtype=b)
+    tokens = torch.randint(0, v, (t,), generator=rng(2), device="cuda")
+    want = tune.embed_backward(ctx, buf[:, :d].clone(), tokens, v, into=buf[:, d:].clone())
+    before = buf.clone()
+    tune.embed_backward(ctx, buf[:, :d], tokens, v, into=buf[:, d:])
+    assert torch.equal(buf[:, d:], want) and torch.equal(buf[:, :d], before[:, :d])
+    for wrong in (buf[:, :d], buf[:, 1:d + 1], buf[:, d - 1:2 * d - 1]):
+        with pytest.raises(cdclq.CdclqError, match="overlaps"):
+            tune.embed_backward(ctx, buf[:, :d], tokens, v, into=wrong)
+    with pytest.raises(cdclq.CdclqError, match="overlaps"):  # strides of their own: by their ranges
+        flat = buf.view(-1)
+        tune.embed_backward(ctx, buf[:, :d], tokens, v, into=flat[d: d + v * d].view(v, d))

@@ -220,3 +220,76 @@ def test_rows_of_a_table_beside_its_gradient(ctx, tune):
     with pytest.raises(cdclq.CdclqError, match="overlaps"):  # strides of their own: by their ranges
         flat = buf.view(-1)
         tune.embed_backward(ctx, buf[:, :d], tokens, v, into=flat[d: d + v * d].view(v, d))
+
+
+# ---------------------------------------------------------------- the embedding's gradient
+def ids(seed, t, v):
+    """Tokens, of which the first ones of the vocabulary come more often than the last."""
+    u = torch.rand(t, generator=rng(seed), device="cuda", dtype=torch.float64)
+    return (u * u * v).long().clamp(max=v - 1)
+
+
+def summed(dy, tokens, v, scale):
+    """The gradient in 64 bits, and the bound of its sums' errors: n additions, the scale and its product."""
+    on = (tokens != -100).nonzero().flatten()
+    rows, x = tokens[on], dy[on].double() * scale
+    de, size = (torch.zeros(v, dy.shape[1], dtype=torch.float64, device="cuda").index_put_((rows,), y, accumulate=True)
+                for y in (x, x.abs()))
+    n = torch.zeros(v, dtype=torch.float64, device="cuda").index_put_((rows,), torch.ones_like(rows).double(), accumulate=True)
+    return de, (n + 3)[:, None] * U32 * size, n > 0
+
+
+@pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float16])
+@pytest.mark.parametrize("into", ["same", "f32"])
+@pytest.mark.parametrize("t,d,v", [(1, 9, 5), (2, 9, 5), (7, 1, 3), (64, 130, 77), (65, 2056, 20), (100, 4099, 9), (127, 8, 2),
+                                   (128, 65, 300)])
+@pytest.mark.parametrize("pad", [0, 3])
+def test_few_tokens_added_to_a_gradient(ctx, tune, dtype, into, t, d, v, pad):
+    """Some of them ignored, most ids several times."""
+    kind = dtype if into == "same" else torch.float32
+    tokens, dy = ids(1, t, v), normal(2, t, d, std=0.1, dtype=dtype)
+    tokens[1::7] = -100
+    buf = normal(3, v, d + pad, std=0.5, dtype=kind)
+    before = buf.clone()
+    got = tune.embed_backward(ctx, dy, tokens, v, 0.75, into=buf[:, :d])
+    want, bound, on = summed(dy, tokens, v, 0.75)
+    old = before[:, :d].double()
+    assert on.any() and not torch.equal(got, before[:, :d])
+    e = want + old
+    assert ((got.double() - e).abs() <= bound + U32 * (want.abs() + old.abs()) + U[kind] * (e.abs() + bound) + TINY[kind]).all()
+    assert torch.equal(got[~on], before[:, :d][~on]) and torch.equal(buf[:, d:], before[:, d:])
+
+
+def grad_by_entry_point(ctx, tune, dy, tokens, v, scale, de, add=0):
+    """cdclq_embed_backward_device itself: a new gradient of any type and row stride."""
+    L, (t, d) = cdclq.lib(), dy.shape
+    codes = {torch.float32: cdclq.DTYPE_F32, torch.float16: cdclq.DTYPE_F16, torch.bfloat16: cdclq.DTYPE_BF16}
+    n = L.cdclq_embed_work_bytes(t, d, v)
+    work = torch.empty(max(n, 1), dtype=torch.uint8, device="cuda")
+    ctx.check(L.cdclq_embed_backward_device(ctx.ptr, dy.data_ptr(), d, t, d, v, codes[dy.dtype], tokens.data_ptr(), scale, -100,
+                                            add, de.data_ptr(), de.stride(0), codes[de.dtype], work.data_ptr(), n,
+                                            tune._stream(ctx)))
+
+
+@pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float16])
+@pytest.mark.parametrize("into", ["same", "f32"])
+@pytest.mark.parametrize("pad", [0, 3])
+@pytest.mark.parametrize("d,v", [(33, 50), (65, 1000), (521, 70), (9, 20_000)])
+@pytest.mark.parametrize("t", [0, 1, 77, 600, 9000])
+def test_new_gradients_of_any_type_and_stride(ctx, tune, dtype, into, pad, d, v, t):
+    """Rows without tokens are cleared, what lies between the rows stays."""
+    kind = dtype if into == "same" else torch.float32
+    tokens, dy = ids(1, t, v), normal(2, t, d, std=0.1, dtype=dtype)
+    tokens[1::7] = -100
+    buf = torch.full((v + 1, d + pad), 7.0, dtype=kind, device="cuda")
+    de = buf[:v, :d]
+    grad_by_entry_point(ctx, tune, dy, tokens, v, 1.25, de)
+    want, bound, on = summed(dy, tokens, v, 1.25)
+    assert ((de.double() - want).abs() <= bound + U[kind] * (want.abs() + bound) + TINY[kind]).all()
+    assert not de[~on].any() and (buf[:v, d:] == 7).all() and (buf[v] == 7).all()
+    if t:
+        tokens[t // 2] = v
+        for add in (0, 1):
+            buf[:] = 7.0
+            grad_by_entry_point(ctx, tune, dy, tokens, v, 1.25, de, add)
+            assert de.isnan().all() and (buf[:v, d:] == 7).all() and (buf[v] == 7).all()

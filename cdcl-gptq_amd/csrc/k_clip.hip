@@ -14,9 +14,9 @@
 // the first one left in the last cache. In place nothing is read again where c = 1.
 // The tensors' addresses come as a launch's arguments, so that a captured call keeps them and the host has nothing to copy
 // or to wait for; sets of more than one launch takes are written to a table in the workspace by small launches first
-// (448 tensors, 84 MB into f32: 82 us, as three launches a pass 113). Those today: 59-66 us, of them 6 the table, 18 the
-// norm (4.7 TB/s) and 37 the clipping (6.8 TB/s, its reads from the last cache), or the host, which looks at the addresses
-// of 896 tensors; 1.4 GB into a second set: 688 us, 214 (6.5 TB/s) and 466 (6.0).
+// (448 tensors, 84 MB into f32: 82 us, as three launches a pass 113). Those today: 60 us, of them 6 the table, 18 the
+// norm (4.7 TB/s) and 37 the clipping (6.8 TB/s, its reads from the last cache), in place 50; the host takes 49. 1.4 GB into
+// a second set: 688-700 us, 214 (6.5 TB/s) and 466 (6.0).
 #include <hip/hip_runtime.h>
 
 #include <algorithm>
@@ -32,8 +32,10 @@ constexpr int kTensors = 150;           // of one launch: its arguments keep bel
 constexpr int kRows = 230;              // of one launch that writes the table
 constexpr int kChunk = 4096;            // elements
 constexpr long kMostPart = 1l << 30;    // elements of a part that one entry of the tables takes
-constexpr long kMostSums = 4096;        // of all parts together, where parts have several (84 MB into f32 and 1.4 GB: 59-65 us
-                                        // and 688; with 1536 59 and 714, with 8192 70 and 693)
+// Sums of all parts together, where parts have several: 84 MB into f32, 1.4 GB, and 268 MB into f32 as 1, 16 or 512 parts
+// 61 us, 700 and 170; with 1024 sums 62, 805 and 202, with 2048 60, 700 and 171, with 8192 71, 693 and 173. (3000 parts
+// have one sum each and leave workgroups idle at the end: 393 MB 278, with 8192 258.)
+constexpr long kMostSums = 4096;
 
 // One tensor, or a piece of it.
 struct ClipEntry {

@@ -5,10 +5,12 @@
 // An id equal to the ignored one stands for no token: y_t = 0, and it adds nothing. Any other id outside 0..v
 // gives a row of NaN and a gradient that is NaN throughout. Both directions only move memory: 16384 rows of 4096 of a
 // table of 128256 36 us (188 MB, 5.2 TB/s); rows and gradient of 4096 tokens there 180 us, 159 of them the clearing of
-// 1.05 GB (6.6 TB/s); of 32768 tokens, 2048 of 32000, 101 us: rows 31, sorting and clearing 28, sums 39, runs of chunks 6.
+// 1.05 GB (6.6 TB/s); of 32768 tokens, 2048 of 32000, 101 us. The last one's launches by themselves, in medians: rows 31,
+// sorting and clearing 28, sums 39, runs of chunks 6. Added to a gradient that exists, nothing is cleared beside the ranks
+// and the sort: 4096 tokens, 2048 of 32000, 23 us, of them 7 the ranks, 11 the sums and 5 the runs.
 //
-// The gradient sums a row's tokens in their order, in f32, with one rounding at the end and no float atomics:
-// equal inputs give equal bits. Three forms by the number of tokens:
+// The gradient sums a row's tokens in f32, with one rounding at the end and no float atomics: a chunk's in their order, a
+// run of chunks in four quarters that are added up. Equal inputs give equal bits. Three forms by the number of tokens:
 //   few     one launch: a workgroup takes a token, finds the others of its id by comparing all ids, and leaves unless it
 //           is the first of them; other workgroups clear the rows without tokens.
 //   ranked  a token's place among the sorted ones is the number of smaller (id, position) pairs, counted by
@@ -29,13 +31,13 @@ namespace {
 
 typedef unsigned long long u64;
 
-// Tokens up to which each form is taken. Rows of 2048, added to a gradient that exists: 128 tokens 8.4 us in the first and
-// 13.8 in the second, all of one id 25 and 13 (256: 8.3 and 13.7, 47 and 14; into a new gradient 18.6 and 18.1); 4096
-// tokens 20 in the second and 32 in the third, 8192 33 and 40, 12000 50 and 50.
+// Tokens up to which each form is taken. Rows of 2048 of 32000, added to a gradient that exists: 128 tokens 6.8 us in the
+// first and 14.8 in the second, all of one id 25.5 and 14.8 (256: 6.8 and 14.5, 47 and 14.5; into a new gradient 25 and 30);
+// 4096 tokens 23 in the second and 36 in the third, 8192 36 and 43, 12000 55 and 53.
 constexpr long kFewIds = 128, kRankedIds = 8192;
 static_assert(kFewIds <= 256, "64 ids a wavefront of k_embed_few");
-// Wavefronts that sum chunks, as long as those have fewer than 64 tokens: 32768 x 2048: 104 us a step, with four times as
-// many (chunks of 16, more runs to join) 113.
+// Wavefronts that sum chunks, as long as those have fewer than 64 tokens: 32768 x 2048: 101 us a step, with four times as
+// many (chunks of 16, more runs to join) 105.
 constexpr long kMostWaves = 2048;
 constexpr int kTile = 2048;  // ids of a workgroup of the radix sort
 

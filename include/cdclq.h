@@ -408,8 +408,8 @@ int cdclq_embed_device(cdclq_ctx* ctx, const void* table, size_t ldt, size_t v, 
                        void* stream);
 /* The gradient of its table for dy (t x d): de (v x d, de_dtype: dtype or CDCLQ_DTYPE_F32) = scale times the sum of the
  * rows of each token, 0 in rows without tokens; with add != 0 the sums are added to what de holds (the gradient of a tied
- * head) and rows without tokens are left alone. Sums are f32, in the tokens' order. Ignored tokens do not take part; with
- * any other token outside 0..v all of de is NaN. */
+ * head) and rows without tokens are left alone. Sums are f32, in an order that tokens and sizes alone decide. Ignored
+ * tokens do not take part; with any other token outside 0..v all of de is NaN. */
 size_t cdclq_embed_work_bytes(size_t t, size_t d, size_t v);
 int cdclq_embed_backward_device(cdclq_ctx* ctx, const void* dy, size_t lddy, size_t t, size_t d, size_t v, int dtype,
                                 const int64_t* tokens, float scale, int64_t ignore_index, int add, void* de,

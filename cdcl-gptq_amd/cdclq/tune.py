@@ -408,17 +408,17 @@ class Gradients:
         if adapters is not None and self.parts < 1:
             raise ValueError(f"adapters is {adapters}, need at least 1")
         self.all, self.device = (*self.tensors, *(self.out or ())), torch.device("cuda", ctx.device)
-        self.written = self.counters = self.all[-len(self.tensors):]
-        self.calls = 0
+        self.count, self.calls = len(self.tensors), 0
+        self.written = self.counters = self.all[-self.count:]
         self.objects = np.array(list(map(id, self.all)), np.uintp)  # which self.all keeps alive
-        at, n = self.objects.ctypes.data, len(self.tensors)
+        at, n = self.objects.ctypes.data, self.count
         self.holds, look = _look()
         self.looked = n, self.shape[0] if self.shape else 0, at, None if out is None else at + 8 * n, look
         self._read()
 
     def _read(self):
         """Checks the tensors and writes the table of what they are and where."""
-        kinds, device, n = _CODES32, self.ctx.device, len(self.tensors)
+        kinds, device = _CODES32, self.ctx.device
         for g in self.all:
             if g.dtype not in kinds:
                 raise TypeError(f"a gradient or output is {g.dtype}, need float32, bfloat16 or float16")
@@ -440,7 +440,7 @@ class Gradients:
             rows.append((x.data_ptr(), o.data_ptr(), x.numel(), kind, to))
         self.table = np.array(rows, _GRAD)
         self.ptr = self.table.ctypes.data
-        self.work_bytes = _L().cdclq_grad_work_bytes(self.ptr, n, self.parts)
+        self.work_bytes = _L().cdclq_grad_work_bytes(self.ptr, self.count, self.parts)
 
     def _addresses(self) -> int:
         """The table's address; tensors that have other memory, sizes or types by now (their .data set) are read again."""
@@ -467,7 +467,7 @@ def _grad_call(grads: Gradients):
         raise TypeError(f"need Gradients, got {type(grads).__name__}")
     table = grads._addresses()
     norm = _empty(grads.shape, dtype=torch.float32, device=grads.device)
-    return grads.ctx, table, len(grads.tensors), norm, _work(grads.work_bytes, grads.device)
+    return grads.ctx, table, grads.count, norm, _work(grads.work_bytes, grads.device)
 
 
 def grad_norm(grads: Gradients) -> torch.Tensor:

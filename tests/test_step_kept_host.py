@@ -175,3 +175,27 @@ def test_every_written_tensors_counter_is_among_the_sets(kind):
             before = [x._version for x in written]
             g._changed()
             assert all(x._version > b for x, b in zip(written, before))
+
+
+def test_a_sets_own_count_is_what_a_call_takes(monkeypatch):
+    """Lists that are changed after the set was made are not the set's."""
+    tensors = [make(5), make(6)]
+    g = tune.Gradients(CTX, tensors)
+    tensors.append(make(7))
+    g.tensors.append(make(8))
+    monkeypatch.setattr(tune, "_empty", lambda *_, **__: None)
+    assert tune._grad_call(g)[2] == len(g.table) == 2
+    g.tensors[0].data = make(3)
+    assert same(rows(g)[0], g.tensors[0]) and tune._grad_call(g)[2] == len(g.table) == 2
+
+
+@pytest.mark.parametrize("inside", [True, False])
+def test_views_of_inference_mode_are_written_without_an_error(inside):
+    base = torch.ones(12)
+    with torch.inference_mode():
+        tensors = list((torch.ones(12) if inside else base).split(4))
+    g = object.__new__(tune.Gradients)
+    with pytest.raises(ValueError, match="is on cpu"):
+        g.__init__(CTX, tensors)
+    for _ in range(3):
+        g._changed()
